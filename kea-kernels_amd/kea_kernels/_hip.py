@@ -1,4 +1,4 @@
-"""ctypes binding of libkea_hip.so (the C ABI of include/kea_lowbit.h).
+"""ctypes binding of libkea_hip.so (the C ABI of include/kea_lowbit.h, kea_encoder.h and kea_block.h).
 
 This replaces the reference's NVRTC loader and launcher (kk/_nvrtc.py): every kernel is compiled ahead of time
 for gfx950 by kea-kernels_amd/build.py, so there is no runtime compilation, no kernel cache and nothing to refuse
@@ -11,6 +11,7 @@ a RuntimeError: there is no fallback path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import importlib.util
 import threading
@@ -27,6 +28,19 @@ DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 # (name, restype, argtypes) of every exported function
 _i32, _i64, _vp, _f32, _cp = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float, ctypes.c_char_p
+
+
+class Norm(ctypes.Structure):
+    """kea_norm of include/kea_block.h."""
+    _fields_ = [("kind", _i32), ("dtype", _i32), ("w", _vp), ("b", _vp), ("eps", _f32)]
+
+
+class Heads(ctypes.Structure):
+    """kea_heads of include/kea_block.h."""
+    _fields_ = [("data", _vp), ("batch_stride", _i64), ("t_stride", _i64), ("head_stride", _i64)]
+
+
+_norm, _heads = ctypes.POINTER(Norm), ctypes.POINTER(Heads)
 
 SIGNATURES = {
     "kea_b1_native_words": (_i64, [_i64, _i64]),
@@ -88,6 +102,14 @@ SIGNATURES = {
     "kea_subsample_out_workspace": (_i64, [_i64, _i64]),
     "kea_subsample_out": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _f32, _vp, _vp, _vp, _i64, _vp]),
     "kea_dwconv_quantize": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _vp, _vp]),
+    "kea_int8_gemm_workspace": (_i64, [_i64, _i64, _i64]),
+    "kea_int8_gemm": (_i32, [_vp, _i64, _vp, _i32, _vp, _i64, _vp, _i32, _vp, _i32, _vp, _i32, _i64, _vp, _i64, _f32,
+                             _i64, _i64, _i64, _i32, _vp, _i64, _vp]),
+    "kea_block_norm": (_i32, [_vp, _i32, _i64, _vp, _i32, _i64, _i64, _i64, _norm, _vp, _i64, _i64, _i32, _f32, _vp, _i64,
+                              _norm, _vp, _i64, _vp, _i64, _vp, _vp]),
+    "kea_window_attention_workspace": (_i64, [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "kea_window_attention": (_i32, [_heads, _heads, _heads, _heads, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                    _i64, _f32, _vp, _vp, _vp, _i64, _vp]),
     "kea_last_error": (_cp, []),
     "kea_version": (_i32, []),
 }
@@ -157,6 +179,20 @@ def dtype_code(dtype: torch.dtype) -> int:
         return DTYPES[dtype]
     except KeyError:
         raise ValueError(f"unsupported dtype {dtype}") from None
+
+
+def refuse_grad(what: str, *tensors: torch.Tensor | None) -> None:
+    """RuntimeError where autograd would have to record a call: the kernels have no backward."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} is inference only: an input requires grad")
+
+
+def on_device(device: torch.device):
+    """A context in which `device` is the current one: the default stream's handle names the current device's stream, so a
+    launch on tensors of another GPU has to be made from that GPU."""
+    if device.type != "cuda" or device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -1,0 +1,285 @@
+"""window.attention (kea_window_attention) against a dense softmax in 64 bits.
+
+Bounds, u = 2^-24: a score is a dot product of d terms in FP32 scaled once, off by at most es = (d + 3) u scale sum |q k| + 3 u |s|;
+a weight exp(s - max) by 2 es + 8 u of itself; the sums over n keys take n + 16 additions and rescalings of u each; for the
+16-bit types the weights are rounded to the type (half a step h of themselves, and 2^-25 where FP16 has no smaller number, the
+largest weight of a row being 1 or more before the division), in the sum as well as in the product at most; the output takes half
+a step of its type. All of it applies to sum_j p_j |v_j|."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from kea_kernels import _hip, window
+
+DEV = "cuda"
+U = 2.0**-24
+HALF_STEP = {torch.float32: 2.0**-24, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+TYPES = [F32, F16, BF16]
+
+
+def expected(q, k, v, left, right, sinks, lengths=None, starts=None, scale=None):
+    """(the output in 64 bits, how far the kernel's may be from it), on the CPU; unseen keys are left out altogether."""
+    dtype = q.dtype
+    q, k, v = (t.detach().cpu().double() for t in (q, k, v))
+    b, tq, h, d = q.shape
+    tk, hk = k.shape[1:3]
+    scale = 1 / math.sqrt(d) if scale is None else scale
+    out, err = torch.zeros(b, tq, h, d, dtype=torch.float64), torch.zeros(b, tq, h, d, dtype=torch.float64)
+    hs = HALF_STEP[dtype]
+    rounded = 0.0 if dtype == F32 else hs
+    for i in range(b):
+        n = tk if lengths is None else min(max(int(lengths[i]), 0), tk)
+        at = n - tq if starts is None else int(starts[i])
+        p = torch.arange(tq)[:, None] + at
+        j = torch.arange(n)
+        seen = torch.ones(tq, n, dtype=torch.bool)
+        if right is not None:
+            seen &= j <= p + right
+        if left is not None:
+            seen &= (j >= p - left) | (j < sinks)
+        seen &= (p >= 0) & (p < n)
+        used = seen.any(0)
+        kk, vv, seen = k[i, :n][used], v[i, :n][used], seen[:, used]
+        if not seen.any():
+            continue
+        for x in range(h):
+            kx, vx = kk[:, x * hk // h], vv[:, x * hk // h]
+            s = (q[i, :, x] @ kx.t()) * scale
+            mag = (q[i, :, x].abs() @ kx.abs().t()) * abs(scale)
+            w = torch.where(seen, s, torch.tensor(-math.inf, dtype=torch.float64))
+            w = torch.nan_to_num(torch.softmax(w, 1))  # (rows that see nothing)
+            es = torch.where(seen, (d + 3) * U * mag + 3 * U * s.abs(), torch.zeros(1, dtype=torch.float64)).amax(1, keepdim=True)
+            o, a = w @ vx, w @ vx.abs()
+            e = a * (2 * es + (len(kx) + 24) * U + 2 * rounded) * 1.05
+            if dtype == F16:
+                e = e + 2.0**-25 * (seen.double() @ vx.abs())
+            out[i, :, x], err[i, :, x] = o, e + (o.abs() + e) * hs + (2.0**-25 if dtype == F16 else 1e-37) * seen.any(1, keepdim=True)
+    return out, err
+
+
+def check(got, want, err):
+    got = got.cpu().double()
+    assert torch.isfinite(got).all()
+    off = (got - want).abs()
+    assert (off[err == 0] == 0).all()
+    worst = (off / err.clamp_min(1e-300))[err > 0].max().item() if (err > 0).any() else 0.0
+    assert worst <= 1, f"{worst:.3g} times the bound"
+
+
+def heads(b, t, h, d, dtype, g, size=1.0):
+    return (size * torch.randn(b, t, h, d, generator=g)).to(dtype).to(DEV)
+
+
+WINDOWS = [(None, 0, 0), (None, None, 0), (0, 0, 0), (5, 0, 2), (16, 16, 1), (63, 0, 4), (64, 7, 70), (100, None, 3), (200, 3, 0), (0, 0, 1), (31, 40, 33)]
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t", [1, 2, 31, 33, 64, 65, 130, 300])
+def test_whole_sequences(t, dtype):
+    g = torch.Generator().manual_seed(t)
+    for i, (left, right, sinks) in enumerate(WINDOWS):
+        h, hk, d = [(2, 2, 64), (4, 1, 128), (6, 2, 80), (1, 1, 8), (3, 3, 256), (2, 1, 40)][(i + t) % 6]
+        q, k, v = heads(2, t, h, d, dtype, g), heads(2, t, hk, d, dtype, g), heads(2, t, hk, d, dtype, g)
+        got = window.attention(q, k, v, left=left, right=right, sinks=sinks)
+        assert got.shape == q.shape and got.dtype == dtype
+        check(got, *expected(q, k, v, left, right, sinks))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tq,tk,h,hk,d", [(1, 1, 4, 4, 64), (1, 77, 8, 2, 128), (1, 1000, 8, 1, 128), (3, 600, 4, 2, 64), (4, 4100, 4, 4, 128), (1, 5000, 2, 1, 256),
+                                          (7, 333, 6, 3, 96), (20, 900, 16, 2, 64), (2, 3000, 33, 1, 32), (150, 1200, 4, 2, 128)])
+def test_tokens_against_a_cache(tq, tk, h, hk, d, dtype):
+    """Sequences of their own lengths (none, one, some, all), queries the last tokens; what the cache holds behind them is NaN."""
+    g = torch.Generator().manual_seed(tq + tk)
+    lengths = torch.tensor([0, 1, tk // 2 + 1, tk, max(1, tk - 3)], dtype=torch.int32)
+    q, k, v = heads(5, tq, h, d, dtype, g), heads(5, tk, hk, d, dtype, g), heads(5, tk, hk, d, dtype, g)
+    for i, n in enumerate(lengths.tolist()):
+        k[i, n:] = float("nan")
+        v[i, n:] = float("nan")
+    for left, right, sinks in ((None, 0, 0), (255, 0, 4), (9, 0, 0), (2000, 0, 65), (0, 0, 1), (None, None, 0)):
+        got = window.attention(q, k, v, left=left, right=right, sinks=sinks, kv_lengths=lengths.to(DEV))
+        check(got, *expected(q, k, v, left, right, sinks, lengths))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+def test_padded_clips_and_positions(dtype):
+    """Padded clips (starts of zero), pieces in the middle of a sequence, queries partly or wholly outside it, lengths past the
+    tensor: rows outside are zeros."""
+    g = torch.Generator().manual_seed(1)
+    q, k, v = heads(4, 90, 4, 64, dtype, g), heads(4, 150, 2, 64, dtype, g), heads(4, 150, 2, 64, dtype, g)
+    for lengths, starts in (([90, 1, 0, 37], [0, 0, 0, 0]), ([150, 100, 120, 60], [10, 60, -40, 200]), ([1000, -5, 150, 150], [60, 0, -89, 149]),
+                            ([150, 150, 150, 150], [2**31 - 1, -(2**31), -90, 150])):
+        ln, st = torch.tensor(lengths, dtype=torch.int32), torch.tensor(starts, dtype=torch.int32)
+        for left, right, sinks in ((40, 0, 2), (16, 16, 0), (None, None, 0)):
+            got = window.attention(q, k, v, left=left, right=right, sinks=sinks, kv_lengths=ln.to(DEV), q_starts=st.to(DEV))
+            check(got, *expected(q, k, v, left, right, sinks, lengths, starts))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t,tq", [(200, 200), (700, 1), (300, 5)])
+def test_unseen_keys_have_no_part(t, tq, dtype):
+    """NaN and infinities in keys and values reach the queries that see them and no others; the type's lowest and highest
+    values among the seen ones are numbers like others."""
+    g = torch.Generator().manual_seed(2)
+    clean = [heads(1, n, 2, 64, dtype, g) for n in (tq, t, t)]
+    q, k, v = (x.clone() for x in clean)
+    bad = t - 60  # seen by positions bad .. bad + 20
+    k[0, bad], v[0, bad] = float("nan"), float("inf")
+    v[0, bad - 1, 0] = float("-inf")
+    got = window.attention(q, k, v, left=20, right=0, sinks=1)[0].cpu()
+    want, err = expected(*clean, 20, 0, 1)
+    want, err = want[0], err[0]
+    p = torch.arange(tq) + t - tq
+    sees = ((p >= bad - 1) & (p <= bad + 20))
+    assert got[~sees].isfinite().all() and ((got[~sees].double() - want[~sees]).abs() <= err[~sees]).all()
+    if tq == t:
+        assert got[(p >= bad) & (p <= bad + 20)].isnan().all() and (got[bad - 1, 0] == float("-inf")).all()
+        assert got[bad - 1, 1].isfinite().all()
+    v = clean[2].clone()
+    v[0, bad] = torch.finfo(dtype).max
+    v[0, bad + 1] = torch.finfo(dtype).min
+    got = window.attention(q, clean[1], v, left=20, right=0, sinks=1)
+    want, err = expected(clean[0], clean[1], v, 20, 0, 1)
+    inside = want[0].abs().amax((1, 2)) < torch.finfo(dtype).max / 2
+    assert ((got[0].cpu().double() - want[0]).abs() <= err[0])[inside].all()
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_scores(dtype):
+    """Scores in the thousands (one key takes all), equal scores, a negative and a zero scale."""
+    g = torch.Generator().manual_seed(3)
+    q, k, v = heads(1, 140, 2, 64, dtype, g, 20), heads(1, 140, 2, 64, dtype, g, 20), heads(1, 140, 2, 64, dtype, g)
+    for scale in (None, 0.0, -0.01, 3.0):
+        for left, right, sinks in ((None, None, 0), (30, 0, 2)):
+            check(window.attention(q, k, v, left=left, right=right, sinks=sinks, scale=scale),
+                  *expected(q, k, v, left, right, sinks, scale=scale))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layouts(dtype):
+    """Slices of a fused projection, heads in front of tokens, keys shared by the batch (stride 0), an out of its own strides."""
+    g = torch.Generator().manual_seed(4)
+    b, t, h, d = 3, 70, 2, 64
+    fused = torch.randn(b, t, 3 * h * d + 16, generator=g).to(dtype).to(DEV)
+    q, k, v = (fused[..., i * h * d:(i + 1) * h * d].view(b, t, h, d) for i in range(3))
+    check(window.attention(q, k, v, left=10, right=3, sinks=1), *expected(q, k, v, 10, 3, 1))
+    q, k, v = (torch.randn(b, h, t, d, generator=g).to(dtype).to(DEV).transpose(1, 2) for _ in range(3))
+    check(window.attention(q, k, v, left=10, sinks=1), *expected(q, k, v, 10, 0, 1))
+    k, v = (x[:1].expand(b, t, h, d) for x in (k, v))
+    base = torch.full((b, t + 1, h, d + 8), 3.0, dtype=dtype, device=DEV)
+    out = base[:, :t, :, :d]
+    got = window.attention(q, k, v, left=10, sinks=1, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    check(out, *expected(q, k, v, 10, 0, 1))
+    assert (base[:, t] == 3).all() and (base[..., d:] == 3).all()
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+def test_offsets_past_32_bits():
+    """Keys and values further apart than 2^31 bytes within a sequence, sequences more than 2^32 bytes apart."""
+    g = torch.Generator().manual_seed(5)
+    step, tk, d = 1 << 24, 150, 64  # 150 tokens 32 MiB apart: 4.9 GB
+    base = torch.zeros(2 * tk * step + 64, dtype=F16, device=DEV)
+    k, v = (base[o:].as_strided((2, tk, 1, d), (tk * step, step, d, 1)) for o in (0, 128))
+    k.copy_(torch.randn(2, tk, 1, d, generator=g))
+    v.copy_(torch.randn(2, tk, 1, d, generator=g))
+    for tq in (1, 150):
+        q = heads(2, tq, 2, d, F16, g)
+        check(window.attention(q, k, v, left=70, sinks=3), *expected(q, k, v, 70, 0, 3))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("tq,tk", [(1, 2000), (130, 130)])
+def test_captured_calls_replay(tq, tk):
+    """Graphs on two streams at once with eager calls between them (each has a workspace of its own), lengths that move on
+    between replays; the same bits every time."""
+    g = torch.Generator().manual_seed(6)
+    k, v = heads(2, tk, 2, 64, BF16, g), heads(2, tk, 2, 64, BF16, g)
+    qs = [heads(2, tq, 8, 64, BF16, g) for _ in range(2)]
+    lengths = torch.tensor([tk - 20, tk // 2], dtype=torch.int32, device=DEV)
+    call = lambda q: window.attention(q, k, v, left=700, sinks=4, kv_lengths=lengths)  # noqa: E731
+    call(qs[0])
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for q, stream in zip(qs, streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+            outs.append(call(q))
+        graphs.append(graph)
+    for _ in range(4):
+        want = [call(q).clone() for q in qs]
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        again = call(qs[0])
+        torch.cuda.synchronize()
+        assert torch.equal(again, want[0]) and torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+        check(again, *expected(qs[0], k, v, 700, 0, 4, lengths.tolist()))
+        lengths += 5
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+def test_empty():
+    q, k = torch.empty(0, 3, 2, 64, device=DEV), torch.empty(0, 3, 2, 64, device=DEV)
+    assert window.attention(q, k, k).shape == (0, 3, 2, 64)
+    q, k = torch.ones(2, 0, 2, 64, device=DEV), torch.ones(2, 3, 2, 64, device=DEV)
+    assert window.attention(q, k, k).shape == (2, 0, 2, 64)
+    q, k = torch.ones(2, 3, 2, 64, device=DEV), torch.ones(2, 0, 2, 64, device=DEV)
+    assert not window.attention(q, k, k, left=4).any()
+
+
+# ---- without a GPU -----------------------------------------------------------------------------------------------------------
+
+def test_refusals():
+    q, k = torch.zeros(2, 5, 4, 64), torch.zeros(2, 9, 2, 64)
+    lengths = torch.zeros(2, dtype=torch.int32)
+    for args, kw, message in [
+        ((q[0], k, k), {}, "q must be"), ((q.double(), k, k), {}, "q must be"), ((q, k.half(), k), {}, "k must be"), ((q, k, k[:, :8]), {}, "v"),
+        ((q, k[:1], k[:1]), {}, "k must be"), ((q, k[..., :32], k[..., :32]), {}, "k must be"), ((q[:, :, :3], k, k), {}, "multiple"),
+        ((q[..., :60], k[..., :60], k[..., :60]), {}, "head size"), ((torch.zeros(1, 1, 1, 264),) * 3, {}, "head size"),
+        ((torch.zeros(2, 5, 4, 66)[..., :64], k, k), {}, "16 bytes"), ((torch.zeros(2, 5, 64, 4).transpose(2, 3), k, k), {}, "16 bytes"),
+        ((torch.zeros(2, 64, 4, 5).transpose(1, 3), k, k), {}, "16 bytes"), ((q, k, k), dict(left=-1), "left"), ((q, k, k), dict(right=1.5), "right"),
+        ((q, k, k), dict(sinks=-2), "sinks"), ((q, k, k), dict(kv_lengths=lengths.long()), "kv_lengths"),
+        ((q, k, k), dict(q_starts=lengths[:1]), "q_starts"), ((q, k, k), dict(out=torch.zeros(2, 5, 4, 64).half()), "out must be"),
+        ((q, k, k), dict(out=torch.zeros(2, 1, 4, 64).expand(2, 5, 4, 64)), "share memory"), ((q, k, k), dict(out=q), "overlaps"),
+        ((q, k, k), {}, "GPU"),
+    ]:
+        with pytest.raises(ValueError, match=message):
+            window.attention(*args, **kw)
+    with pytest.raises(RuntimeError, match="inference only"):
+        window.attention(q.requires_grad_(), k, k)
+
+
+def test_library_refusals():
+    L = _hip.lib()
+    buf = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    t = _hip.Heads(p, 64, 64, 64)
+    good = dict(q=t, k=t, v=t, o=t, dt=0, b=1, tq=1, tk=1, h=2, hk=1, d=64, left=0, right=0, sinks=0, scale=1.0, ln=None, st=None, ws=None, wb=0,
+                stream=None)
+    for change, rc in [(dict(dt=3), -1), (dict(b=-1), -1), (dict(tk=(1 << 30) + 1), -1), (dict(h=3, hk=2), -1), (dict(hk=0), -1), (dict(d=12), -1),
+                       (dict(d=264), -1), (dict(left=-1), -1), (dict(sinks=-1), -1), (dict(k=_hip.Heads(p + 4, 64, 64, 64)), -2),
+                       (dict(o=_hip.Heads(p, 64, 66, 64)), -2), (dict(ln=p + 2), -2), (dict(q=_hip.Heads(None, 64, 64, 64)), -1), (dict(b=0), 0)]:
+        assert L.kea_window_attention(*(good | change).values()) == rc, change
+    assert L.kea_window_attention_workspace(0, 1, 1, 1, 3, 2, 64, 0, 0, 0) < 0
