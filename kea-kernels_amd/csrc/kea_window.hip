@@ -1,70 +1,542 @@
-// Attention within a sliding window and to the first tokens (include/kea_block.h): one wave per query and head, key by key
-// with a running maximum and sum, each lane holding up to four of the head's elements.
+// Attention within a sliding window and to the first tokens (include/kea_block.h).
+//
+// The query heads that share a key head are rows of one problem: row r of a sequence and key head is query r / group, head
+// r % group of the group, so that a tile of rows stands at few positions and their keys are read once. A workgroup takes
+// 32 WQ rows and walks the keys that any of them sees, first those of the first tokens that lie before the window, then the
+// window, in tiles that it copies straight to LDS one ahead. Per tile and wave:
+//   S^T = K Q^T        keys are the matrix instruction's rows, queries its columns: a lane holds 16 keys' scores of one
+//                      query (its column), and the maximum over keys is 15 steps in the lane and one across its halves
+//   p = 2^(s - m)      base 2 with the scale folded into one fma; the reference m is raised, and the sums rescaled, only
+//                      when a score passes it by more than 8, so most tiles leave the output's accumulators alone
+//   O^T += V^T P^T     the scores' layout is the second operand's of this product up to the order of keys, which the sum does
+//                      not depend on: V's columns are read in that order (ds_read_b64_tr_b16, which transposes on the way;
+//                      single words for FP32), and probabilities never leave the registers
+// WQ waves share out the rows (many queries), or WK waves the keys of each tile (few queries), whose parts meet in LDS. Where
+// that still leaves few workgroups the keys are split over several, whose parts a second launch joins.
+//
+// Keys outside the tile's range are read from its last key and masked. A masked score is -infinity whatever K holds, but a
+// product with its weight of 0 is NaN where V is infinite or NaN. Such a sum shows in the output: a workgroup that ends up
+// with a value that is not finite does its work a second time with those elements of V taken out of the product and added to
+// the queries that see them, and (FP32 and BF16) with weights of at most 2^-32, whose sums with V's largest numbers are finite.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
 #include <string>
 
 #include "kea_internal.h"
-#include "kea_wave.h"
 #include "../../include/kea_block.h"
 
 namespace {
 
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(1))) const void *gptr_t;
+typedef __attribute__((address_space(3))) void *lptr_t;
+typedef __attribute__((address_space(3))) v4s *ltr_t;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.0f;  // scores may pass the reference by this much (base 2) before it is raised
+
+constexpr float kRoom = 16.0f;  // parts are joined at 2^-16 of their size, so that finite parts have a finite sum
+
 struct Args {
     kea_heads q, k, v, out;
     const int32_t *lengths, *starts;
-    long long rows;
-    int tq, tk, heads, group, d, left, right, sinks, dtype;
+    float *part, *stats;  // splits > 1: [splits][sequences and key heads][rows][d], [..][rows][2]
+    int batch, tq, tk, kv_heads, group, d, left, right, sinks;
+    int rows, row_tiles, splits;
     float scale;
 };
 
-__device__ __forceinline__ float load(const void *p, int dtype, long long i) {
-    if (dtype == KEA_F32) return ((const float *)p)[i];
-    if (dtype == KEA_F16) return (float)((const _Float16 *)p)[i];
-    return (float)((const __bf16 *)p)[i];
+template <typename T, int DP, int WQ, int WK>
+struct Shape {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int NW = WQ * WK, NT = 64 * NW;
+    // 32-key blocks of a tile: the waves' one each where they share out the keys, otherwise what 32 KB hold, two at most
+    static constexpr int KB = WK > 1 ? WK : (2 * 2 * 32 * DP * (int)sizeof(T) <= 32768 ? 2 : 1);
+    static constexpr int NB = KB / WK, KT = 32 * KB;
+    static constexpr int ROW = DP * (int)sizeof(T), UNITS = ROW / 16, BUF = 2 * KT * ROW;
+    static constexpr int MERGE = WK > 1 ? NW * 32 * (DP + 2) * 4 : 0;
+    static constexpr int LDS = (2 * BUF > MERGE ? 2 * BUF : MERGE) + 64;
+};
+
+// The place of 16-byte unit c of a key's row in LDS, so that rows read together lie in different banks. K: eight (16) rows at
+// one unit. V of 16-bit types: four rows at two neighbouring pairs of units, which stay pairs.
+template <bool F32, int UNITS>
+__device__ __forceinline__ int place_k(int key, int c) {
+    return c ^ (F32 ? key & 7 : UNITS == 8 ? key >> 1 & 7 : key & 15);
+}
+template <bool F32, int UNITS>
+__device__ __forceinline__ int place_v(int key, int c) {
+    return c ^ (F32 ? key & 7 : UNITS == 8 ? (key >> 1 & 1) * 4 : (key & 3) * 4);
 }
 
-__global__ void __launch_bounds__(256) window_kernel(Args a) {
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.rows) return;
-    const int lane = threadIdx.x & 63;
-    const int h = (int)(row % a.heads), t = (int)(row / a.heads % a.tq);
-    const long long b = row / a.heads / a.tq;
+// A lane's value and that of the lane 32 away, the lower half's first. (The components are read before they are cast:
+// hipcc's __builtin_bit_cast of a component access gives component 0.)
+__device__ __forceinline__ float2 halves(float v) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, v);
+    const auto s = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+    const uint32_t lower = s[0], upper = s[1];
+    return make_float2(__builtin_bit_cast(float, lower), __builtin_bit_cast(float, upper));
+}
+__device__ __forceinline__ float other_half_max(float v) {
+    const float2 s = halves(v);
+    return fmaxf(s.x, s.y);
+}
+__device__ __forceinline__ float both_halves(float v) {
+    const float2 s = halves(v);
+    return s.x + s.y;
+}
+
+template <typename T>
+__device__ __forceinline__ v16f mma(v8s a, v8s b, v16f c) {
+    if constexpr (__is_same(T, _Float16)) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ bool finite(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) != 0x7F800000u; }
+// Whether an element of 16 or 32 bits is an infinity or NaN, and a unit of eight or four without such elements.
+template <typename T>
+__device__ __forceinline__ bool finite_bits(T v) {
+    return finite((float)v);
+}
+
+// RAGGED: d < DP, rows of K and V end before DP elements and go through registers, zeros behind them.
+template <typename T, int DP, int WQ, int WK, bool RAGGED>
+__global__ void __launch_bounds__(64 * WQ *WK) window_kernel(Args a) {
+    using S = Shape<T, DP, WQ, WK>;
+    constexpr bool F32 = S::F32;
+    constexpr int NB = S::NB, KT = S::KT, UNITS = S::UNITS, NT = S::NT, ROW = S::ROW, EPU = 16 / (int)sizeof(T);
+    constexpr int QF = DP / 16, DB = DP / 32;  // steps of 16 elements, blocks of 32 output elements
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    uint32_t *const flags = (uint32_t *)(lds + S::LDS - 64);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, h = lane >> 5, wq = wave / WK, wk = wave % WK;
+
+    // Workgroups go to the eight XCDs in turn; each XCD takes a run of its own, so that tiles of neighbouring rows and splits
+    // of one sequence and key head share keys in its L2.
+    const int total = gridDim.x, per = total / 8, rest = total % 8, x = blockIdx.x % 8;
+    const int id = x * per + min(x, rest) + blockIdx.x / 8;
+    const int tile = id % a.row_tiles, split = id / a.row_tiles % a.splits, bh = id / a.row_tiles / a.splits;
+    const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.tk) : a.tk;
     const int start = a.starts ? min(max(a.starts[b], -(1 << 30)), 1 << 30) : len - a.tq;
-    const int p = start + t;
-    const long long qo = b * a.q.batch_stride + t * a.q.t_stride + h * a.q.head_stride;
-    const long long ko = b * a.k.batch_stride + h / a.group * a.k.head_stride;
-    const long long vo = b * a.v.batch_stride + h / a.group * a.v.head_stride;
-    float q[4], o[4] = {0, 0, 0, 0}, top = -INFINITY, sum = 0.0f;
-    for (int e = 0; e < 4; ++e) q[e] = lane + 64 * e < a.d ? load(a.q.data_dev, a.dtype, qo + lane + 64 * e) * a.scale : 0.0f;
-    if (p >= 0 && p < len) {
-        const int low = max(0, p - a.left), high = min(len - 1, (int)min((long long)p + a.right, 1LL << 30));
-        const int first = min(min(a.sinks, low), high + 1);
-        for (int i = 0; i < first + (high - low + 1); ++i) {
-            const int j = i < first ? i : low + (i - first);
-            float s = 0.0f;
-            for (int e = 0; e < 4; ++e)
-                if (lane + 64 * e < a.d) s += q[e] * load(a.k.data_dev, a.dtype, ko + j * a.k.t_stride + lane + 64 * e);
-            s = kea::wave_sum(s);
-            const float next = fmaxf(top, s), old = top == -INFINITY ? 0.0f : expf(top - next);
-            const float w = s == -INFINITY ? 0.0f : expf(s - next);
-            top = next;
-            sum = sum * old + w;
-            for (int e = 0; e < 4; ++e)
-                o[e] = o[e] * old + (lane + 64 * e < a.d ? w * load(a.v.data_dev, a.dtype, vo + j * a.v.t_stride + lane + 64 * e) : 0.0f);
+
+    // this lane's query
+    const int r0 = tile * 32 * WQ, row = r0 + 32 * wq + n;
+    const bool real = row < a.rows;
+    const int t = min(row, a.rows - 1) / a.group, head = hk * a.group + min(row, a.rows - 1) % a.group, p = start + t;
+    const bool inside = real && p >= 0 && p < len;
+    // positions of the tile's and of the wave's rows, those inside the sequence
+    auto first_of = [&](int from) { return max(start + min(from, a.rows - 1) / a.group, 0); };
+    auto last_of = [&](int from, int rows) { return min(start + (min(from + rows, a.rows) - 1) / a.group, len - 1); };
+    const int p0 = first_of(r0), p1 = last_of(r0, 32 * WQ);
+    const int w0 = first_of(r0 + 32 * wq), w1 = r0 + 32 * wq < a.rows ? last_of(r0 + 32 * wq, 32) : -1;
+    int low = max(0, p0 - a.left), first = min(a.sinks, low);
+    const int high = (int)min((long long)len - 1, (long long)p1 + a.right);
+    if (first == low) first = low = 0;  // one range
+    int first_tiles = 0, tiles = 0;
+    if (p0 <= p1) {
+        first_tiles = (first + KT - 1) / KT;
+        tiles = first_tiles + (high - low + KT) / KT;
+    }
+    const int from = (int)((long long)tiles * split / a.splits), to = (int)((long long)tiles * (split + 1) / a.splits);
+
+    const T *const kp = (const T *)a.k.data_dev + b * a.k.batch_stride + hk * a.k.head_stride;
+    const T *const vp = (const T *)a.v.data_dev + b * a.v.batch_stride + hk * a.v.head_stride;
+    auto stage = [&](int ti, int buf) {
+        const int j0 = ti < first_tiles ? ti * KT : low + (ti - first_tiles) * KT, end = ti < first_tiles ? first : high + 1;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int u = 0; u < KT * UNITS / NT; ++u) {
+                const int at = u * NT + tid, key = at / UNITS;
+                const int c = kv ? place_v<F32, UNITS>(key, at % UNITS) : place_k<F32, UNITS>(key, at % UNITS);
+                const long long j = min(j0 + key, end - 1);
+                const T *src = kv ? vp + j * a.v.t_stride + c * EPU : kp + j * a.k.t_stride + c * EPU;
+                char *dst = lds + buf * S::BUF + kv * KT * ROW;
+                if constexpr (RAGGED) {
+                    const v4f zero = {0, 0, 0, 0};
+                    *(v4f *)(dst + at * 16) = c * EPU < a.d ? *(const v4f *)src : zero;
+                } else {
+                    __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(dst + (u * NT + wave * 64) * 16), 16, 0, 0);
+                }
+            }
+    };
+    auto landed = [&]() {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
+    // the query as the product's second operand: elements 16 c + 8 h .. of its row (FP32: 8 c + 4 h ..)
+    v8s qf[F32 ? 1 : QF];
+    v4f qx[F32 ? 2 * QF : 1];
+    {
+        const T *qp = (const T *)a.q.data_dev + b * a.q.batch_stride + (long long)t * a.q.t_stride + head * a.q.head_stride;
+        if constexpr (F32) {
+#pragma unroll
+            for (int c = 0; c < 2 * QF; ++c) {
+                qx[c] = v4f{0, 0, 0, 0};
+                if (inside && 8 * c + 4 * h < a.d) qx[c] = *(const v4f *)(qp + 8 * c + 4 * h);
+                if (a.scale < 0) qx[c] = -qx[c];
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < QF; ++c) {
+                qf[c] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
+                if (inside && 16 * c + 8 * h < a.d) qf[c] = *(const v8s *)(qp + 16 * c + 8 * h);
+                if (a.scale < 0) qf[c] ^= (short)0x8000;
+            }
         }
     }
-    const long long oo = b * a.out.batch_stride + t * a.out.t_stride + h * a.out.head_stride;
-    for (int e = 0; e < 4; ++e) {
-        if (lane + 64 * e >= a.d) break;
-        const float v = sum != 0.0f ? o[e] / sum : 0.0f;
-        const long long at = oo + lane + 64 * e;
-        if (a.dtype == KEA_F32) ((float *)a.out.data_dev)[at] = v;
-        else if (a.dtype == KEA_F16) ((_Float16 *)a.out.data_dev)[at] = (_Float16)v;
-        else ((__bf16 *)a.out.data_dev)[at] = (__bf16)v;
+    const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);  // (0 would make a masked score's -infinity NaN)
+
+    v16f o[DB];
+    float m = -INFINITY, l = 0.0f;  // l: this half's keys
+    bool careful = false;
+    constexpr float kDown = __is_same(T, _Float16) ? 0.0f : 40.0f;
+
+    auto work = [&](int ti, int buf) {
+        const bool in_first = ti < first_tiles;
+        const int j0 = in_first ? ti * KT : low + (ti - first_tiles) * KT, end = in_first ? first : high + 1;
+        // a tile that none of the wave's rows sees (the whole of it lies outside their windows)
+        if (w0 > w1) return;
+        if (!in_first && ((long long)j0 > (long long)w1 + a.right || (j0 + KT <= w0 - a.left && j0 >= a.sinks))) return;
+        const char *const kt = lds + buf * S::BUF, *const vt = kt + KT * ROW;
+        v16f s[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int key = 32 * (i * WK + wk) + n;
+            s[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+            if constexpr (F32) {
+#pragma unroll
+                for (int c = 0; c < 2 * QF; ++c) {
+                    const v4f kx = *(const v4f *)(kt + key * ROW + place_k<F32, UNITS>(key, 2 * c + h) * 16);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(kx[e], qx[c][e], s[i], 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < QF; ++c)
+                    s[i] = mma<T>(*(const v8s *)(kt + key * ROW + place_k<F32, UNITS>(key, 2 * c + h) * 16), qf[c], s[i]);
+            }
+        }
+        // masks, where the tile is not seen as a whole by every row of the wave
+        const bool whole = j0 + KT <= end && (in_first || ((long long)j0 + KT - 1 <= (long long)w0 + a.right && (j0 >= w1 - a.left || j0 + KT <= a.sinks)));
+        if (!whole) {
+            const int hi = (int)min((long long)end - 1, (long long)p + a.right) - j0 - 4 * h;
+            const int lo = in_first ? -KT : max(max(p, 0) - a.left - j0, -KT) - 4 * h, sink = min(a.sinks - j0, KT) - 4 * h;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int at = 32 * (i * WK + wk) + 8 * (e / 4) + e % 4;
+                    if (!(at <= hi && (at >= lo || at < sink))) s[i][e] = -INFINITY;
+                }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, s[i][e]);
+        top = other_half_max(top) * scale;
+        if (__any(top > m + kLazy)) {
+            const float next = fmaxf(m, top);
+            const float by = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+            m = next;
+            l *= by;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= by;
+        }
+        const float ref = (m == -INFINITY ? 0.0f : m) + (careful ? kDown : 0.0f);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], scale, -ref));
+                sum += s[i][e];
+            }
+        l += sum;
+        if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int key = 32 * (i * WK + wk) + 8 * (e / 4) + e % 4 + 4 * h;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        const float vx = *(const float *)(vt + key * ROW + place_v<F32, UNITS>(key, 8 * d + n / 4) * 16 + n % 4 * 4);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vx, s[i][e], o[d], 0, 0, 0);
+                    }
+                }
+        } else {
+            // Each weight is rounded to the type that the product takes (half a step, relative to itself; below the smallest
+            // normal FP16 number 2^-25): as accurate as the values it weighs.
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int k16 = 0; k16 < 2; ++k16) {
+                    T w[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = (T)s[i][8 * k16 + e];
+                    const v8s pf = *(const v8s *)w;
+                    const int key = 32 * (i * WK + wk) + 16 * k16 + 4 * h + (lane & 15) / 4;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        const int c = 4 * d + 2 * (lane >> 4 & 1) + (lane & 3) / 2;
+                        v4s part[2];
+#pragma unroll
+                        for (int y = 0; y < 2; ++y)
+                            part[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)(vt + (key + 8 * y) * ROW + place_v<F32, UNITS>(key + 8 * y, c) * 16 + (lane & 1) * 8));
+                        o[d] = mma<T>(v8s{part[0][0], part[0][1], part[0][2], part[0][3], part[1][0], part[1][1], part[1][2], part[1][3]}, pf, o[d]);
+                    }
+                }
+        }
+        if (__builtin_expect(careful, 0)) {
+            for (int i = 0; i < NB; ++i) {
+                uint32_t left = __builtin_amdgcn_readfirstlane(flags[i * WK + wk]);
+                while (left) {
+                    const int j = j0 + 32 * (i * WK + wk) + __builtin_ctz(left);
+                    left &= left - 1;
+                    const bool seen = j < end && (in_first || ((long long)j <= (long long)p + a.right && (j >= p - a.left || j < a.sinks)));
+                    if (j >= end || !seen) continue;
+                    const T *src = vp + (long long)j * a.v.t_stride;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int at = 32 * d + 8 * (e / 4) + 4 * h + e % 4;
+                            if (at < a.d && !finite_bits(src[at])) o[d][e] += (float)src[at];
+                        }
+                }
+            }
+        }
+    };
+    // V's elements that are no numbers become zeros in LDS, and their keys' flags are set.
+    auto take_out = [&](int buf) {
+        if (tid < S::KB) flags[tid] = 0;
+        __syncthreads();
+        for (int at = tid; at < KT * UNITS; at += NT) {
+            T *unit = (T *)(lds + buf * S::BUF + KT * ROW + at * 16);
+            bool any = false;
+            for (int e = 0; e < EPU; ++e)
+                if (!finite_bits(unit[e])) unit[e] = (T)0.0f, any = true;
+            if (any) atomicOr(&flags[at / UNITS / 32], 1u << (at / UNITS % 32));
+        }
+        __syncthreads();
+    };
+
+    for (int round = 0; round < 2; ++round) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        m = -INFINITY;
+        l = 0.0f;
+        if (from < to) stage(from, 0);
+        for (int ti = from; ti < to; ++ti) {
+            const int buf = ti - from & 1;
+            landed();
+            if (careful) take_out(buf);
+            if (ti + 1 < to) stage(ti + 1, buf ^ 1);
+            work(ti, buf);
+        }
+        bool bad = false;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            float z = 0.0f;  // (an infinity or NaN times 0 is NaN)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) z = __builtin_fmaf(o[d][e], 0.0f, z);
+            bad |= z != z;
+        }
+        if (careful || !__syncthreads_or(bad)) break;
+        careful = true;
     }
+
+    l = both_halves(l);
+    if (careful) m += kDown;  // what the weights and sums refer to
+    T *const out = (T *)a.out.data_dev + b * a.out.batch_stride + (long long)t * a.out.t_stride + head * a.out.head_stride;
+    if constexpr (WK == 1) {
+        if (!real) return;
+        if (a.splits > 1) {
+            const long long at = ((long long)split * (gridDim.x / a.row_tiles / a.splits) + bh) * a.rows + row;
+            float *const part = a.part + at * a.d;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    if (32 * d + 2 * e + 4 * h < a.d) *(v4f *)(part + 32 * d + 2 * e + 4 * h) = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+            if (h == 0) a.stats[2 * at] = m, a.stats[2 * at + 1] = l;
+            return;
+        }
+        const float by = inside && l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int at = 32 * d + 2 * e + 4 * h;
+                if (at >= a.d) continue;
+                T v[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) v[y] = (T)(by == 0.0f ? 0.0f : o[d][e + y] * by);
+                if constexpr (F32) *(v4f *)(out + at) = *(const v4f *)v;
+                else *(v4s *)(out + at) = *(const v4s *)v;
+            }
+    } else {
+        // the waves' parts of each row meet in LDS: [wave][32][DP] outputs, then [wave][32][2] maxima and sums
+        static_assert(WQ == 1, "one group of rows");
+        float *const po = (float *)lds, *const ps = po + S::NW * 32 * DP;
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                // (units of four elements, swizzled by the row: 32 rows are written at once)
+                const int c = 8 * d + e / 2 + h;
+                *(v4f *)(po + ((wave * 32 + n) * (DP / 4) + (c ^ (n & 7))) * 4) = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+            }
+        if (h == 0) ps[2 * (wave * 32 + n)] = m, ps[2 * (wave * 32 + n) + 1] = l;
+        __syncthreads();
+        const int rows = min(32, a.rows - r0);
+        for (int at = tid; at < rows * (DP / 4); at += NT) {
+            const int r = at / (DP / 4), c = at % (DP / 4);
+            if (4 * c >= a.d) continue;
+            float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) top = fmaxf(top, ps[2 * (w * 32 + r)]);
+            v4f v = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < WK; ++w) {
+                const float mw = ps[2 * (w * 32 + r)], by = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - top - kRoom);
+                sum += ps[2 * (w * 32 + r) + 1] * by;
+                if (by != 0.0f) v += *(const v4f *)(po + ((w * 32 + r) * (DP / 4) + (c ^ (r & 7))) * 4) * by;
+            }
+            const int rr = r0 + r, tt = rr / a.group, pp = start + tt;
+            if (a.splits > 1) {
+                const long long slot = ((long long)split * (gridDim.x / a.row_tiles / a.splits) + bh) * a.rows + rr;
+                *(v4f *)(a.part + slot * a.d + 4 * c) = v;
+                if (c == 0) a.stats[2 * slot] = top + kRoom, a.stats[2 * slot + 1] = sum;
+                continue;
+            }
+            const float by = pp >= 0 && pp < len && sum != 0.0f ? 1.0f / sum : 0.0f;
+            T *const y = (T *)a.out.data_dev + b * a.out.batch_stride + (long long)tt * a.out.t_stride + (hk * a.group + rr % a.group) * a.out.head_stride + 4 * c;
+            T res[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) res[e] = (T)(by == 0.0f ? 0.0f : v[e] * by);
+            if constexpr (F32) *(v4f *)y = *(const v4f *)res;
+            else *(v4s *)y = *(const v4s *)res;
+        }
+    }
+}
+
+// Joins the splits: out = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m), four elements a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(Args a, long long units) {
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= units) return;
+    const int per = a.d / 4, c = (int)(at % per);
+    const long long row = at / per, all = (long long)a.batch * a.kv_heads * a.rows;  // row: of all
+    float top = -INFINITY, sum = 0.0f;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.stats[2 * (s * all + row)]);
+    v4f v = {0, 0, 0, 0};
+    for (int s = 0; s < a.splits; ++s) {
+        const float m = a.stats[2 * (s * all + row)], by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top - kRoom);
+        sum += a.stats[2 * (s * all + row) + 1] * by;
+        if (by != 0.0f) v += *(const v4f *)(a.part + (s * all + row) * a.d + 4 * c) * by;
+    }
+    const long long bh = row / a.rows;
+    const int r = (int)(row % a.rows), t = r / a.group, b = (int)(bh / a.kv_heads), hk = (int)(bh % a.kv_heads);
+    const int len = a.lengths ? min(max(a.lengths[b], 0), a.tk) : a.tk;
+    const int p = (a.starts ? min(max(a.starts[b], -(1 << 30)), 1 << 30) : len - a.tq) + t;
+    const float by = p >= 0 && p < len && sum != 0.0f ? 1.0f / sum : 0.0f;
+    T res[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) res[e] = (T)(by == 0.0f ? 0.0f : v[e] * by);
+    T *const y = (T *)a.out.data_dev + b * a.out.batch_stride + (long long)t * a.out.t_stride + (hk * a.group + r % a.group) * a.out.head_stride + 4 * c;
+    if constexpr (sizeof(T) == 4) *(v4f *)y = *(const v4f *)res;
+    else *(v4s *)y = *(const v4s *)res;
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------
+
+struct Plan {
+    bool few;            // waves share out the keys of 32 rows, not the rows
+    int dp, row_tiles, splits;
+    int64_t rows, part_bytes, stats_bytes;
+};
+
+int plan_of(int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads, int64_t d, int64_t left, int64_t right,
+            int64_t sinks, Plan *out) {
+    Plan p{};
+    p.dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+    p.rows = tq * (heads / kv_heads);
+    const int64_t groups = batch * kv_heads;
+    if (p.rows > INT32_MAX / 2 || groups > INT32_MAX / 2) return -1;
+    p.few = p.rows <= 64 || (p.rows + 127) / 128 * groups < 256;
+    const int64_t per = p.few ? 32 : 128;
+    p.row_tiles = (int)((p.rows + per - 1) / per);
+    const int64_t wgs = p.row_tiles * groups;
+    // the keys that a tile of rows can meet
+    const int64_t most = 1 << 30, span = per / (heads / kv_heads) + 2;
+    const int64_t window = left >= most || right >= most ? tk : left + right + span + sinks;
+    const int64_t keys = window < tk ? window : tk;
+    const int64_t blocks = (keys + 127) / 128;
+    p.splits = 1;
+    if (wgs < 256 && blocks > 1) {
+        int64_t s = (512 + wgs - 1) / (wgs > 0 ? wgs : 1);
+        s = s < blocks ? s : blocks;
+        p.splits = (int)(s < 64 ? s : 64);
+    }
+    if (p.splits > 1) {
+        p.part_bytes = p.splits * groups * p.rows * d * 4;
+        p.stats_bytes = p.splits * groups * p.rows * 8;
+    }
+    *out = p;
+    return 0;
+}
+
+int launched() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? KEA_OK : kea::fail((int)e, std::string("kea_window_attention: ") + hipGetErrorString(e));
+}
+
+template <typename T, int DP, int WQ, int WK, bool RAGGED>
+int run_shape(const Args &a, int64_t groups, hipStream_t stream) {
+    using S = Shape<T, DP, WQ, WK>;
+    static_assert(S::LDS <= 160 * 1024 && S::KT * S::UNITS % S::NT == 0 && S::KB <= 16, "tiles and flags");
+    const int64_t blocks = groups * a.row_tiles * a.splits;
+    if (blocks > INT32_MAX / 2 || !kea::fits_dispatch(blocks, S::NT)) return kea::fail(KEA_EINVAL, "kea_window_attention: too large for one launch");
+    const auto kernel = window_kernel<T, DP, WQ, WK, RAGGED>;
+    if (S::LDS > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
+        if (e != hipSuccess) return kea::fail((int)e, std::string("kea_window_attention: ") + hipGetErrorString(e));
+    }
+    kernel<<<dim3((unsigned)blocks), S::NT, S::LDS, stream>>>(a);
+    const int rc = launched();
+    if (rc || a.splits == 1) return rc;
+    const int64_t units = groups * a.rows * (a.d / 4);
+    if (!kea::fits_dispatch((units + 255) / 256, 256)) return kea::fail(KEA_EINVAL, "kea_window_attention: too large for one launch");
+    join_kernel<T><<<dim3((unsigned)((units + 255) / 256)), 256, 0, stream>>>(a, units);
+    return launched();
+}
+
+template <typename T, int DP>
+int run_heads(const Args &a, bool few, int64_t groups, hipStream_t stream) {
+    // waves that share out keys: four of them where two buffers of their blocks fit LDS
+    constexpr int WK = 2 * 2 * 4 * 32 * DP * (int)sizeof(T) <= 131072 ? 4 : 2 * 2 * 2 * 32 * DP * (int)sizeof(T) <= 131072 ? 2 : 1;
+    if (a.d == DP) return few ? run_shape<T, DP, 1, WK, false>(a, groups, stream) : run_shape<T, DP, 4, 1, false>(a, groups, stream);
+    return few ? run_shape<T, DP, 1, WK, true>(a, groups, stream) : run_shape<T, DP, 4, 1, true>(a, groups, stream);
+}
+
+template <typename T>
+int run_type(const Args &a, const Plan &p, int64_t groups, hipStream_t stream) {
+    return p.dp == 64 ? run_heads<T, 64>(a, p.few, groups, stream) : p.dp == 128 ? run_heads<T, 128>(a, p.few, groups, stream)
+                                                                                 : run_heads<T, 256>(a, p.few, groups, stream);
 }
 
 bool heads_ok(const kea_heads *t, int64_t unit) {
@@ -72,12 +544,13 @@ bool heads_ok(const kea_heads *t, int64_t unit) {
 }
 
 int check_sizes(const char *what, int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads, int64_t d,
-                int64_t left, int64_t right, int64_t sinks) {
+                int64_t left, int64_t right, int64_t sinks, Plan *p) {
     if (dtype != KEA_F32 && dtype != KEA_F16 && dtype != KEA_BF16) return kea::fail(KEA_EINVAL, std::string(what) + ": f32, f16 or bf16");
-    if (batch < 0 || tq < 0 || tk < 0 || tq > (1 << 30) || tk > (1 << 30) || heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 65535)
+    if (batch < 0 || tq < 0 || tk < 0 || tq > (1 << 30) || tk > (1 << 30) || heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 65535 || batch > (1 << 30))
         return kea::fail(KEA_EINVAL, std::string(what) + ": batch >= 0, 0 <= tq, tk <= 2^30 and heads a multiple of kv_heads are needed");
     if (d < 8 || d > 256 || d % 8) return kea::fail(KEA_EINVAL, std::string(what) + ": d is a multiple of 8 from 8 to 256");
     if (left < 0 || right < 0 || sinks < 0) return kea::fail(KEA_EINVAL, std::string(what) + ": left, right and sinks are >= 0");
+    if (plan_of(dtype, batch, tq, tk, heads, kv_heads, d, left, right, sinks, p)) return kea::fail(KEA_EINVAL, std::string(what) + ": too large for one launch");
     return KEA_OK;
 }
 
@@ -87,27 +560,32 @@ extern "C" {
 
 int64_t kea_window_attention_workspace(int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads, int64_t d,
                                        int64_t left, int64_t right, int64_t sinks) {
-    return check_sizes("kea_window_attention_workspace", dtype, batch, tq, tk, heads, kv_heads, d, left, right, sinks);
+    Plan p;
+    const int rc = check_sizes("kea_window_attention_workspace", dtype, batch, tq, tk, heads, kv_heads, d, left, right, sinks, &p);
+    return rc ? rc : p.part_bytes + p.stats_bytes;
 }
 
 int kea_window_attention(const kea_heads *q, const kea_heads *k, const kea_heads *v, const kea_heads *out, int dtype, int64_t batch,
                          int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads, int64_t d, int64_t left, int64_t right,
                          int64_t sinks, float scale, const int32_t *kv_lengths, const int32_t *q_starts, void *workspace,
                          int64_t workspace_bytes, void *stream) {
-    const int rc = check_sizes("kea_window_attention", dtype, batch, tq, tk, heads, kv_heads, d, left, right, sinks);
+    Plan p;
+    const int rc = check_sizes("kea_window_attention", dtype, batch, tq, tk, heads, kv_heads, d, left, right, sinks, &p);
     if (rc) return rc;
     const int64_t unit = dtype == KEA_F32 ? 4 : 8;
     if (!heads_ok(q, unit) || !heads_ok(k, unit) || !heads_ok(v, unit) || !heads_ok(out, unit) || (uintptr_t)kv_lengths % 4 || (uintptr_t)q_starts % 4)
         return kea::fail(KEA_EALIGN, "kea_window_attention: pointers and strides are multiples of 16 bytes");
     if (batch == 0 || tq == 0) return KEA_OK;
     if (!q->data_dev || !out->data_dev || (tk > 0 && (!k->data_dev || !v->data_dev))) return kea::fail(KEA_EINVAL, "kea_window_attention: a pointer is missing");
-    const int64_t most = 1 << 30, rows = batch * tq * heads;
-    Args a{*q, *k, *v, *out, kv_lengths, q_starts, rows, (int)tq, (int)tk, (int)heads, (int)(heads / kv_heads), (int)d,
-           (int)(left < most ? left : most), (int)(right < most ? right : most), (int)(sinks < most ? sinks : most), dtype, scale};
-    if (batch > most || !kea::fits_dispatch((rows + 3) / 4, 256)) return kea::fail(KEA_EINVAL, "kea_window_attention: too large for one launch");
-    window_kernel<<<dim3((unsigned)((rows + 3) / 4)), 256, 0, (hipStream_t)stream>>>(a);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? KEA_OK : kea::fail((int)e, std::string("kea_window_attention: ") + hipGetErrorString(e));
+    if (workspace_bytes < p.part_bytes + p.stats_bytes || (p.splits > 1 && !workspace)) return kea::fail(KEA_ESPACE, "kea_window_attention: the workspace is too small");
+    if ((uintptr_t)workspace % 16) return kea::fail(KEA_EALIGN, "kea_window_attention: the workspace is aligned to 16 bytes");
+    const int64_t most = 1 << 30;
+    const Args a{*q, *k, *v, *out, kv_lengths, q_starts, (float *)workspace, workspace ? (float *)((char *)workspace + p.part_bytes) : nullptr,
+                 (int)batch, (int)tq, (int)tk, (int)kv_heads, (int)(heads / kv_heads), (int)d, (int)(left < most ? left : most),
+                 (int)(right < most ? right : most), (int)(sinks < most ? sinks : most), (int)p.rows, p.row_tiles, p.splits, scale};
+    const int64_t groups = batch * kv_heads;
+    const hipStream_t s = (hipStream_t)stream;
+    return dtype == KEA_F32 ? run_type<float>(a, p, groups, s) : dtype == KEA_F16 ? run_type<_Float16>(a, p, groups, s) : run_type<__bf16>(a, p, groups, s);
 }
 
 }  // extern "C"
