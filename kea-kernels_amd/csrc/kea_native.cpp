@@ -17,10 +17,12 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include <cmath>
 #include <cstdint>
 #include <list>
 #include <unordered_map>
 
+#include "../../include/kea_block.h"
 #include "../../include/kea_lowbit.h"
 
 namespace {
@@ -31,6 +33,11 @@ struct Library {
     decltype(&kea_lowbit_gemm) gemm = nullptr;
     decltype(&kea_lowbit_gemm_residual) gemm_residual = nullptr;
     decltype(&kea_quantize) quantize = nullptr;
+    decltype(&kea_int8_gemm) int8_gemm = nullptr;
+    decltype(&kea_int8_gemm_workspace) int8_workspace = nullptr;
+    decltype(&kea_block_norm) block_norm = nullptr;
+    decltype(&kea_window_attention) window = nullptr;
+    decltype(&kea_window_attention_workspace) window_workspace = nullptr;
 } lib;
 
 // The tensor behind an exact torch.Tensor whose memory a kernel may read as it is: on a GPU, strided, no transform
@@ -375,6 +382,227 @@ PyObject *native_gemm(PyObject *, PyObject *const *args, Py_ssize_t count) {
     Py_RETURN_FALSE;
 }
 
+// ---- int8.gemm, norms.block_norm, window.attention ----
+
+// Whether launches on `d` can be made from here: the default stream's handle names the current device's.
+bool current(c10::Device d) { return d.index() == c10::hip::current_device(); }
+
+bool as_float(PyObject *o, double *v) {
+    *v = PyFloat_AsDouble(o);
+    if (!PyErr_Occurred()) return true;
+    PyErr_Clear();
+    return false;
+}
+
+// The first dimensions of t as rows of its last one with one stride (of rows: 1 row, any stride), without a copy.
+bool rows_of(const at::Tensor &t, int64_t *rows, int64_t *stride) {
+    const int64_t dim = t.dim();
+    if (dim < 1 || t.size(dim - 1) < 1 || (t.size(dim - 1) > 1 && t.stride(dim - 1) != 1)) return false;
+    *rows = 1;
+    *stride = t.size(dim - 1);
+    for (int64_t i = dim - 2; i >= 0; --i) {
+        const int64_t n = t.size(i);
+        if (n == 0) return false;
+        if (n == 1) continue;
+        if (*rows == 1) *stride = t.stride(i);
+        else if (t.stride(i) != *stride * *rows) return false;
+        *rows *= n;
+    }
+    return true;
+}
+
+// int8 rows [.., k] that start at multiples of 16 bytes, the last one readable to a multiple of 16 of `k` elements.
+bool rows8(const at::Tensor &t, int64_t dim, int64_t k, int64_t *ld) {
+    const int64_t m = t.size(dim), w = t.size(dim + 1);
+    if (t.scalar_type() != at::kChar || (w > 1 && t.stride(dim + 1) != 1) || (uintptr_t)t.const_data_ptr() % 16) return false;
+    *ld = m > 1 ? t.stride(dim) : (w + 15) / 16 * 16;
+    return m >= 1 && *ld % 16 == 0 && *ld >= w && t.storage_offset() + (m - 1) * *ld + (k + 15) / 16 * 16 <= (int64_t)t.storage().nbytes();
+}
+
+// int8_gemm(q, qs, weight, wscale, bias, out, out_dtype, silu, residual, factor) -> the output, or None
+PyObject *native_int8_gemm(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    if (count != 10) Py_RETURN_NONE;
+    const at::Tensor *q = plain(args[0]);
+    if (!q || modes_active()) Py_RETURN_NONE;
+    const auto device = q->device();
+    const at::Tensor *qs, *w, *ws, *bias, *out, *res;
+    int64_t silu;
+    double factor;
+    if (!current(device) || !optional(args[1], device, &qs) || !optional(args[2], device, &w) || !optional(args[3], device, &ws) ||
+        !optional(args[4], device, &bias) || !optional(args[5], device, &out) || !optional(args[8], device, &res) ||
+        !as_int(args[7], &silu) || !as_float(args[9], &factor) || !THPDtype_Check(args[6]) || !qs || !w || !ws)
+        Py_RETURN_NONE;
+    const auto type = out ? out->scalar_type() : ((THPDtype *)args[6])->scalar_type;
+    const int yc = code_of(type), sc = code_of(qs->scalar_type()), wc = code_of(ws->scalar_type()), bc = bias ? code_of(bias->scalar_type()) : KEA_F32;
+    auto scale = [](int c) { return c == KEA_F32 || c == KEA_F16; };
+    const int64_t qd = q->dim() - 2;
+    if (yc < 0 || !scale(sc) || !scale(wc) || !scale(bc) || (qd != 0 && (qd != 1 || q->size(0) != 1)) || w->dim() != 2) Py_RETURN_NONE;
+    const int64_t m = q->size(qd), n = w->size(0), k = w->size(1);
+    int64_t ldq, ldw;
+    if (m < 1 || n < 1 || k < 1 || k > 131071 || q->size(qd + 1) < k || !rows8(*q, qd, k, &ldq) || !rows8(*w, 0, k, &ldw) ||
+        !qs->is_contiguous() || qs->numel() != m || !ws->is_contiguous() || ws->numel() != n ||
+        (bias && (!bias->is_contiguous() || bias->numel() != n)) ||
+        (res && (res->scalar_type() != at::kFloat || res->dim() != 2 || res->size(0) != m || res->size(1) != n || (n > 1 && res->stride(1) != 1))) ||
+        (out && (out->dim() != 2 || out->size(0) != m || out->size(1) != n || (n > 1 && out->stride(1) != 1) || (m > 1 && out->stride(0) < n))))
+        Py_RETURN_NONE;
+    try {
+        at::Tensor y = out ? *out : at::empty({m, n}, at::TensorOptions().device(device).dtype(type));
+        const int64_t need = lib.int8_workspace(m, n, k);
+        at::Tensor space;
+        if (need > 0) space = at::empty({need}, at::TensorOptions().device(device).dtype(at::kByte));
+        const int rc = lib.int8_gemm((const int8_t *)q->const_data_ptr(), ldq, qs->const_data_ptr(), sc, (const int8_t *)w->const_data_ptr(), ldw,
+                                     ws->const_data_ptr(), wc, bias ? bias->const_data_ptr() : nullptr, bc, y.mutable_data_ptr(), yc,
+                                     m > 1 ? y.stride(0) : n, res ? (const float *)res->const_data_ptr() : nullptr, res && m > 1 ? res->stride(0) : n,
+                                     (float)factor, m, n, k, silu ? KEA_FLAG_SILU : 0, need > 0 ? space.mutable_data_ptr() : nullptr,
+                                     need > 0 ? need : 0, stream_of(device));
+        if (rc == 0) return THPVariable_Wrap(std::move(y));
+    } catch (const std::exception &) {
+    }
+    Py_RETURN_NONE;
+}
+
+// A norm given as (kind, weight, bias, eps) in four arguments; its parameters are read as they are, detached.
+bool norm_of(PyObject *const *args, int64_t d, c10::Device device, kea_norm *n) {
+    int64_t kind;
+    double eps;
+    if (!as_int(args[0], &kind) || !as_float(args[3], &eps)) return false;
+    *n = kea_norm{(int)kind, KEA_F32, nullptr, nullptr, (float)eps};
+    int type = -1;
+    for (int i = 0; i < 2; ++i) {
+        if (args[1 + i] == Py_None) continue;
+        if (!THPVariable_Check(args[1 + i])) return false;
+        const at::Tensor &t = THPVariable_Unpack(args[1 + i]);
+        if (!t.defined() || t.device() != device || t.layout() != at::kStrided || !t.has_storage() || !t.is_contiguous() || t.numel() != d ||
+            t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
+                                                     c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Negative})))
+            return false;
+        const int c = code_of(t.scalar_type());
+        if (c < 0 || (type >= 0 && c != type)) return false;
+        type = c;
+        (i ? n->b_dev : n->w_dev) = t.const_data_ptr();
+    }
+    if (type >= 0) n->dtype = type;
+    return true;
+}
+
+// block_norm(x, block, post x 4, gate, act, factor, pre x 4, quantize, out) -> (y, z) or (y, q, qs), or None. See norm_of.
+PyObject *native_block_norm(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    if (count != 15) Py_RETURN_NONE;
+    const at::Tensor *x = plain(args[0]);
+    if (!x || modes_active()) Py_RETURN_NONE;
+    const auto device = x->device();
+    const at::Tensor *block, *gate, *out;
+    int64_t act, quantize, m, ldx, mb, ldb, ldg = 0, gates = 1, my, ldy;
+    double factor;
+    kea_norm post, pre;
+    if (!current(device) || !optional(args[1], device, &block) || !block || !optional(args[6], device, &gate) || !as_int(args[7], &act) ||
+        !as_float(args[8], &factor) || !as_int(args[13], &quantize) || !optional(args[14], device, &out) || x->dim() < 1)
+        Py_RETURN_NONE;
+    const int64_t d = x->size(x->dim() - 1);
+    const int xc = code_of(x->scalar_type()), bc = code_of(block->scalar_type());
+    if (xc < 0 || bc < 0 || block->sizes() != x->sizes() || d < 1 || d > 32768 || !rows_of(*x, &m, &ldx) || !rows_of(*block, &mb, &ldb) ||
+        !norm_of(args + 2, d, device, &post) || !norm_of(args + 9, d, device, &pre) || act < 0 || act > 2)
+        Py_RETURN_NONE;
+    if (gate && (gate->scalar_type() != block->scalar_type() || gate->dim() < 1 || gate->size(gate->dim() - 1) != d ||
+                 !rows_of(*gate, &gates, &ldg) || m % gates))
+        Py_RETURN_NONE;
+    if (out && (out->scalar_type() != x->scalar_type() || out->sizes() != x->sizes() || !rows_of(*out, &my, &ldy) || ldy < d)) Py_RETURN_NONE;
+    try {
+        const auto options = at::TensorOptions().device(device);
+        at::Tensor y = out ? *out : at::empty(x->sizes(), options.dtype(x->scalar_type())), z, q, qs;
+        if (!out) ldy = d;
+        const int64_t ldq = (d + 15) / 16 * 16;
+        const bool values = !quantize && pre.kind != KEA_NORM_NONE;
+        if (values) z = at::empty(x->sizes(), options.dtype(block->scalar_type()));
+        if (quantize) {
+            q = at::empty({1, m, ldq}, options.dtype(at::kChar));
+            qs = at::empty({1, m}, options.dtype(at::kFloat));
+        }
+        const int rc = lib.block_norm(x->const_data_ptr(), xc, ldx, block->const_data_ptr(), bc, ldb, m, d, &post,
+                                      gate ? gate->const_data_ptr() : nullptr, ldg, m / gates, gate ? (int)act : 0, (float)factor,
+                                      y.mutable_data_ptr(), ldy, &pre, values ? z.mutable_data_ptr() : nullptr, d,
+                                      quantize ? (int8_t *)q.mutable_data_ptr() : nullptr, ldq,
+                                      quantize ? (float *)qs.mutable_data_ptr() : nullptr, stream_of(device));
+        if (rc != 0) Py_RETURN_NONE;
+        const THPObjectPtr yo(THPVariable_Wrap(std::move(y)));
+        if (quantize) {
+            const THPObjectPtr qo(THPVariable_Wrap(std::move(q))), so(THPVariable_Wrap(std::move(qs)));
+            return PyTuple_Pack(3, yo.get(), qo.get(), so.get());
+        }
+        const THPObjectPtr zo(values ? THPVariable_Wrap(std::move(z)) : Py_NewRef(Py_None));
+        return PyTuple_Pack(2, yo.get(), zo.get());
+    } catch (const std::exception &) {
+        Py_RETURN_NONE;
+    }
+}
+
+bool heads_of(const at::Tensor &t, at::ScalarType type, int64_t b, int64_t d, kea_heads *h) {
+    if (t.scalar_type() != type || t.dim() != 4 || t.size(0) != b || t.size(3) != d || t.stride(3) != 1 || (uintptr_t)t.const_data_ptr() % 16 ||
+        t.size(1) > (1 << 30))
+        return false;
+    const int64_t unit = 16 / (int64_t)t.element_size();
+    int64_t s[3];
+    for (int i = 0; i < 3; ++i) {
+        s[i] = t.size(i) > 1 ? t.stride(i) : 0;
+        if (s[i] % unit) return false;
+    }
+    *h = kea_heads{const_cast<void *>(t.const_data_ptr()), s[0], s[1], s[2]};
+    return true;
+}
+
+// window_attention(q, k, v, left, right, sinks, scale, kv_lengths, q_starts) -> the output, or None. left, right: None or int.
+PyObject *native_window(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    if (count != 9) Py_RETURN_NONE;
+    const at::Tensor *q = plain(args[0]);
+    if (!q || modes_active()) Py_RETURN_NONE;
+    const auto device = q->device();
+    const at::Tensor *k, *v, *lengths, *starts;
+    int64_t left = 1 << 30, right = 1 << 30, sinks;
+    double scale;
+    if (!current(device) || !optional(args[1], device, &k) || !optional(args[2], device, &v) || !k || !v || !PyLong_CheckExact(args[5]) ||
+        !as_int(args[5], &sinks) || (args[3] != Py_None && (!PyLong_CheckExact(args[3]) || !as_int(args[3], &left))) ||
+        (args[4] != Py_None && (!PyLong_CheckExact(args[4]) || !as_int(args[4], &right))) || !optional(args[7], device, &lengths) ||
+        !optional(args[8], device, &starts) || q->dim() != 4 || k->dim() != 4)
+        Py_RETURN_NONE;
+    const int64_t b = q->size(0), tq = q->size(1), h = q->size(2), d = q->size(3), tk = k->size(1), hk = k->size(2);
+    const int code = code_of(q->scalar_type());
+    kea_heads qh, kh, vh;
+    if (code < 0 || d < 8 || d % 8 || d > 256 || h < 1 || hk < 1 || h % hk || b < 1 || tq < 1 || left < 0 || right < 0 || sinks < 0 ||
+        v->sizes() != k->sizes() || !heads_of(*q, q->scalar_type(), b, d, &qh) || !heads_of(*k, q->scalar_type(), b, d, &kh) ||
+        !heads_of(*v, q->scalar_type(), b, d, &vh))
+        Py_RETURN_NONE;
+    for (const at::Tensor *t : {lengths, starts})
+        if (t && (t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) != b || !t->is_contiguous())) Py_RETURN_NONE;
+    if (args[6] == Py_None) scale = 1.0 / std::sqrt((double)d);
+    else if (!as_float(args[6], &scale)) Py_RETURN_NONE;
+    try {
+        at::Tensor y = at::empty({b, tq, h, d}, at::TensorOptions().device(device).dtype(q->scalar_type())), space;
+        const kea_heads yh{y.mutable_data_ptr(), tq * h * d, h * d, d};
+        const int64_t need = lib.window_workspace(code, b, tq, tk, h, hk, d, left, right, sinks);
+        if (need < 0) Py_RETURN_NONE;
+        if (need > 0) space = at::empty({need}, at::TensorOptions().device(device).dtype(at::kByte));
+        const int rc = lib.window(&qh, &kh, &vh, &yh, code, b, tq, tk, h, hk, d, left, right, sinks, (float)scale,
+                                  lengths ? (const int32_t *)lengths->const_data_ptr() : nullptr,
+                                  starts ? (const int32_t *)starts->const_data_ptr() : nullptr, need > 0 ? space.mutable_data_ptr() : nullptr, need,
+                                  stream_of(device));
+        if (rc == 0) return THPVariable_Wrap(std::move(y));
+    } catch (const std::exception &) {
+    }
+    Py_RETURN_NONE;
+}
+
+// bind_block(int8_gemm, int8_gemm_workspace, block_norm, window_attention, window_attention_workspace)
+PyObject *native_bind_block(PyObject *, PyObject *args) {
+    unsigned long long g, gw, n, w, ww;
+    if (!PyArg_ParseTuple(args, "KKKKK", &g, &gw, &n, &w, &ww)) return nullptr;
+    lib.int8_gemm = (decltype(lib.int8_gemm))g;
+    lib.int8_workspace = (decltype(lib.int8_workspace))gw;
+    lib.block_norm = (decltype(lib.block_norm))n;
+    lib.window = (decltype(lib.window))w;
+    lib.window_workspace = (decltype(lib.window_workspace))ww;
+    Py_RETURN_NONE;
+}
+
 // bind(project_launch, gemm, gemm_residual, quantize): the library's entry points as integers
 PyObject *native_bind(PyObject *, PyObject *args) {
     unsigned long long p, g, r, q;
@@ -388,6 +616,10 @@ PyObject *native_bind(PyObject *, PyObject *args) {
 
 PyMethodDef module_methods[] = {
     {"bind", native_bind, METH_VARARGS, nullptr},
+    {"bind_block", native_bind_block, METH_VARARGS, nullptr},
+    {"int8_gemm", (PyCFunction)(void (*)())native_int8_gemm, METH_FASTCALL, nullptr},
+    {"block_norm", (PyCFunction)(void (*)())native_block_norm, METH_FASTCALL, nullptr},
+    {"window_attention", (PyCFunction)(void (*)())native_window, METH_FASTCALL, nullptr},
     {"quantize", (PyCFunction)(void (*)())native_quantize, METH_FASTCALL, nullptr},
     {"gemm", (PyCFunction)(void (*)())native_gemm, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -153,6 +153,9 @@ def native():
                 spec.loader.exec_module(module)
                 module.bind(*(ctypes.cast(getattr(library, name), ctypes.c_void_p).value for name in (
                     "kea_lowbit_project_launch", "kea_lowbit_gemm", "kea_lowbit_gemm_residual", "kea_quantize")))
+                module.bind_block(*(ctypes.cast(getattr(library, name), ctypes.c_void_p).value for name in (
+                    "kea_int8_gemm", "kea_int8_gemm_workspace", "kea_block_norm", "kea_window_attention",
+                    "kea_window_attention_workspace")))
                 _native = module
     return _native
 

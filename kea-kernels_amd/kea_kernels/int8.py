@@ -48,6 +48,15 @@ def pad_rows(weight: Tensor) -> Tensor:
     return rows[:, :k]
 
 
+def _native_gemm(*args) -> Tensor | None:
+    """gemm() in one native call (the same checks on the tensors' fields); None, having launched nothing, where an argument is
+    not what it takes: the Python path then checks again and raises or launches."""
+    try:
+        return _hip.native().int8_gemm(*args)
+    except (AttributeError, TypeError, ValueError):
+        return None
+
+
 def gemm(q: Tensor, qs: Tensor | None, weight: Tensor, wscale: Tensor | None, bias: Tensor | None = None, *,
          out: Tensor | None = None, out_dtype: torch.dtype = torch.float32, silu: bool = False,
          residual: Tensor | None = None, residual_factor: float = 1.0) -> Tensor:
@@ -58,6 +67,8 @@ def gemm(q: Tensor, qs: Tensor | None, weight: Tensor, wscale: Tensor | None, bi
     and bias f32 / f16 [N]; residual FP32 [M, N]. silu: act(r) = r * sigmoid(r), the identity otherwise. out (or a new
     tensor of out_dtype: f32, f16, bf16) receives the result, `out` may be the residual itself. out_dtype torch.int32 (or
     an int32 out) gives the sums alone: qs and wscale may then be None, and there is no bias, activation or residual."""
+    if (hit := _native_gemm(q, qs, weight, wscale, bias, out, out_dtype, silu, residual, residual_factor)) is not None:
+        return hit
     if q.dim() == 3:
         if q.shape[0] != 1:
             raise ValueError(f"q must hold one activation part, got {q.shape[0]}")

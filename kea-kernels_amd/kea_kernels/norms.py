@@ -49,6 +49,31 @@ def _stride(t: Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+_NO_PARAMETERS = (0, None, None, 0.0)
+
+
+def _parameters(norm, d: int) -> tuple:
+    """(kind, weight, bias, eps) of a torch.nn norm of d elements whose parameters are its own (LookupError otherwise)."""
+    if norm is None:
+        return _NO_PARAMETERS
+    own = norm.__dict__["_parameters"]
+    if tuple(norm.normalized_shape) != (d,):
+        raise LookupError
+    eps = norm.eps
+    return 1 if "bias" in own else 2, own["weight"], own.get("bias"), torch.finfo(torch.float32).eps if eps is None else eps
+
+
+def _native(x, block, post, gate, act, factor, pre, quantize, out) -> tuple | None:
+    """block_norm() in one native call (the same checks on the tensors' fields); None, having launched nothing, where an
+    argument is not what it takes: the Python path then checks again and raises or launches."""
+    try:
+        d = x.shape[-1]
+        return _hip.native().block_norm(x, block, *_parameters(post, d), gate, _ACTS[act], factor, *_parameters(pre, d),
+                                        bool(quantize), out)
+    except (AttributeError, LookupError, TypeError, ValueError):
+        return None
+
+
 def block_norm(x: Tensor, block: Tensor | None, *, post=None, gate: Tensor | None = None, gate_activation: str = "",
                factor: float = 1.0, pre=None, quantize: bool = False, out: Tensor | None = None) -> tuple:
     """y = x + factor * act(gate) * post(block) and z = pre(y): (y, z), (y, None) without `pre`, and with `quantize`
@@ -64,6 +89,8 @@ def block_norm(x: Tensor, block: Tensor | None, *, post=None, gate: Tensor | Non
     gate, post and factor): y is x itself and z = pre(x) in x's type."""
     if gate_activation not in _ACTS:
         raise ValueError(f"unsupported gate activation {gate_activation!r}")
+    if block is not None and (hit := _native(x, block, post, gate, gate_activation, factor, pre, quantize, out)) is not None:
+        return hit
     xr, device, d = _rows("x", x), x.device, x.shape[-1] if x.dim() else 0
     m = xr.shape[0]
     if d > 32768:

@@ -44,6 +44,15 @@ def _bound(name: str, v) -> int:
     return min(int(v), _NO_BOUND)
 
 
+def _native(*args) -> Tensor | None:
+    """attention() in one native call (the same checks on the tensors' fields); None, having launched nothing, where an
+    argument is not what it takes: the Python path then checks again and raises or launches."""
+    try:
+        return _hip.native().window_attention(*args)
+    except (AttributeError, TypeError, ValueError):
+        return None
+
+
 def attention(q: Tensor, k: Tensor, v: Tensor, *, left: int | None = None, right: int | None = 0, sinks: int = 0,
               scale: float | None = None, kv_lengths: Tensor | None = None, q_starts: Tensor | None = None,
               out: Tensor | None = None) -> Tensor:
@@ -57,6 +66,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, left: int | None = None, right
     kv_lengths the clips' lengths; for tokens against a cache kv_lengths counts them too. Queries that see nothing, or stand
     outside 0 .. len - 1 (padding), give zeros. What a query does not see has no part in its output, whatever it holds.
     scale: 1 / sqrt(D) unless given. out must not overlap q, k or v."""
+    if out is None and (hit := _native(q, k, v, left, right, sinks, scale, kv_lengths, q_starts)) is not None:
+        return hit
     if q.dim() != 4 or k.dim() != 4 or q.dtype not in _hip.DTYPES:
         raise ValueError(f"q must be f32, f16 or bf16 [B, Tq, H, D] and k, v [B, Tk, Hkv, D], got {q.dtype} "
                          f"{tuple(q.shape)}, {tuple(k.shape)}")
