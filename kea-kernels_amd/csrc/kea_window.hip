@@ -48,7 +48,7 @@ struct Args {
     const int32_t *lengths, *starts;
     float *part, *stats;  // splits > 1: [splits][sequences and key heads][rows][d], [..][rows][2]
     int batch, tq, tk, kv_heads, group, d, left, right, sinks;
-    int rows, row_tiles, splits;
+    int rows, row_tiles, splits, buffers;
     float scale;
 };
 
@@ -61,18 +61,21 @@ struct Shape {
     static constexpr int NB = KB / WK, KT = 32 * KB;
     static constexpr int ROW = DP * (int)sizeof(T), UNITS = ROW / 16, BUF = 2 * KT * ROW;
     static constexpr int MERGE = WK > 1 ? NW * 32 * (DP + 2) * 4 : 0;
-    static constexpr int LDS = (2 * BUF > MERGE ? 2 * BUF : MERGE) + 64;
+    // two buffers where two workgroups of a CU have room for them, otherwise one: the other workgroup works meanwhile
+    static constexpr int BUFFERS = 2 * BUF <= 65536 ? 2 : 1;
+    static constexpr int lds(int buffers) { return (buffers * BUF > MERGE ? buffers * BUF : MERGE) + 64; }
 };
 
-// The place of 16-byte unit c of a key's row in LDS, so that rows read together lie in different banks. K: eight (16) rows at
-// one unit. V of 16-bit types: four rows at two neighbouring pairs of units, which stay pairs.
+// The place of 16-byte unit c of a key's row in LDS is c ^ swizzle(key), so that rows read together lie in different banks.
+// K: eight (16) rows at one unit. V of 16-bit types: four rows at two neighbouring pairs of units, which stay pairs. Either
+// depends on key % 32 alone.
 template <bool F32, int UNITS>
-__device__ __forceinline__ int place_k(int key, int c) {
-    return c ^ (F32 ? key & 7 : UNITS == 8 ? key >> 1 & 7 : key & 15);
+__device__ __forceinline__ int swizzle_k(int key) {
+    return F32 ? key & 7 : UNITS == 8 ? key >> 1 & 7 : key & 15;
 }
 template <bool F32, int UNITS>
-__device__ __forceinline__ int place_v(int key, int c) {
-    return c ^ (F32 ? key & 7 : UNITS == 8 ? (key >> 1 & 1) * 4 : (key & 3) * 4);
+__device__ __forceinline__ int swizzle_v(int key) {
+    return F32 ? key & 7 : UNITS == 8 ? (key >> 1 & 1) * 4 : (key & 3) * 4;
 }
 
 // A lane's value and that of the lane 32 away, the lower half's first. (The components are read before they are cast:
@@ -107,13 +110,13 @@ __device__ __forceinline__ bool finite_bits(T v) {
 
 // RAGGED: d < DP, rows of K and V end before DP elements and go through registers, zeros behind them.
 template <typename T, int DP, int WQ, int WK, bool RAGGED>
-__global__ void __launch_bounds__(64 * WQ *WK) window_kernel(Args a) {
+__global__ void __launch_bounds__(64 * WQ *WK, DP * sizeof(T) <= 512 ? 2 : 1) window_kernel(Args a) {
     using S = Shape<T, DP, WQ, WK>;
     constexpr bool F32 = S::F32;
     constexpr int NB = S::NB, KT = S::KT, UNITS = S::UNITS, NT = S::NT, ROW = S::ROW, EPU = 16 / (int)sizeof(T);
     constexpr int QF = DP / 16, DB = DP / 32;  // steps of 16 elements, blocks of 32 output elements
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    uint32_t *const flags = (uint32_t *)(lds + S::LDS - 64);
+    uint32_t *const flags = (uint32_t *)(lds + S::lds(a.buffers) - 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5, wq = wave / WK, wk = wave % WK;
 
@@ -134,38 +137,53 @@ __global__ void __launch_bounds__(64 * WQ *WK) window_kernel(Args a) {
     // positions of the tile's and of the wave's rows, those inside the sequence
     auto first_of = [&](int from) { return max(start + min(from, a.rows - 1) / a.group, 0); };
     auto last_of = [&](int from, int rows) { return min(start + (min(from + rows, a.rows) - 1) / a.group, len - 1); };
+    auto reach = [&](int from) { return (int)min((long long)len - 1, (long long)from + a.right); };  // the last key seen from there
     const int p0 = first_of(r0), p1 = last_of(r0, 32 * WQ);
     const int w0 = first_of(r0 + 32 * wq), w1 = r0 + 32 * wq < a.rows ? last_of(r0 + 32 * wq, 32) : -1;
-    int low = max(0, p0 - a.left), first = min(a.sinks, low);
-    const int high = (int)min((long long)len - 1, (long long)p1 + a.right);
-    if (first == low) first = low = 0;  // one range
-    int first_tiles = 0, tiles = 0;
-    if (p0 <= p1) {
-        first_tiles = (first + KT - 1) / KT;
-        tiles = first_tiles + (high - low + KT) / KT;
-    }
-    const int from = (int)((long long)tiles * split / a.splits), to = (int)((long long)tiles * (split + 1) / a.splits);
+
+    // The keys that some row of the tile sees, numbered on: v < first is key v, others key v + shift.
+    int low = max(0, p0 - a.left), first = min(a.sinks, low), keys = 0;
+    if (first == low) first = low = 0;
+    const int shift = low - first, sinks = shift ? first : a.sinks;
+    if (p0 <= p1) keys = reach(p1) + 1 - shift;
+    auto cut = [&](int s) { return min(keys, (int)((long long)keys * s / a.splits + 31) & ~31); };
+    const int from = cut(split), to = cut(split + 1), tiles = (to - from + KT - 1) / KT;
+    // per lane and wave, in these numbers: the last key seen and the first of the window
+    const int hi = reach(max(p, 0)) - shift, lo = max(p, 0) - a.left - shift;
+    const int hi0 = reach(w0) - shift, hi1 = reach(w1) - shift, lo0 = w0 - a.left - shift, lo1 = w1 - a.left - shift;
 
     const T *const kp = (const T *)a.k.data_dev + b * a.k.batch_stride + hk * a.k.head_stride;
     const T *const vp = (const T *)a.v.data_dev + b * a.v.batch_stride + hk * a.v.head_stride;
-    auto stage = [&](int ti, int buf) {
-        const int j0 = ti < first_tiles ? ti * KT : low + (ti - first_tiles) * KT, end = ti < first_tiles ? first : high + 1;
+    // the copies of this thread: unit tid + u NT of a tile of K and of V, rows STEP apart at one place
+    constexpr int STEP = NT / UNITS, COPIES = KT / STEP;
+    static_assert(NT % UNITS == 0 && (STEP % 16 == 0 || STEP == 8 || STEP == 4 || STEP == 2 || STEP == 1), "copies");
+    const int key0 = tid / UNITS;
+    auto unit = [&](int kv, int key) { return (tid % UNITS ^ (kv ? swizzle_v<F32, UNITS>(key) : swizzle_k<F32, UNITS>(key))) * EPU; };
+    auto stage = [&](int v0, int buf) {
+        const bool plain = v0 >= first && v0 + KT <= to;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv)
+        for (int kv = 0; kv < 2; ++kv) {
+            const long long stride = kv ? a.v.t_stride : a.k.t_stride;
+            const T *const base = kv ? vp : kp;
+            char *const dst = lds + buf * S::BUF + kv * KT * ROW;
 #pragma unroll
-            for (int u = 0; u < KT * UNITS / NT; ++u) {
-                const int at = u * NT + tid, key = at / UNITS;
-                const int c = kv ? place_v<F32, UNITS>(key, at % UNITS) : place_k<F32, UNITS>(key, at % UNITS);
-                const long long j = min(j0 + key, end - 1);
-                const T *src = kv ? vp + j * a.v.t_stride + c * EPU : kp + j * a.k.t_stride + c * EPU;
-                char *dst = lds + buf * S::BUF + kv * KT * ROW;
+            for (int u = 0; u < COPIES; ++u) {
+                const int key = key0 + u * STEP, c = unit(kv, STEP % 16 ? key : key0);
+                const T *src;
+                if (plain) {
+                    src = base + (long long)key0 * stride + c + (long long)(v0 + shift + u * STEP) * stride;
+                } else {
+                    const int v = min(v0 + key, to - 1);
+                    src = base + (long long)(v + (v >= first ? shift : 0)) * stride + c;
+                }
                 if constexpr (RAGGED) {
                     const v4f zero = {0, 0, 0, 0};
-                    *(v4f *)(dst + at * 16) = c * EPU < a.d ? *(const v4f *)src : zero;
+                    *(v4f *)(dst + (u * NT + tid) * 16) = c < a.d ? *(const v4f *)src : zero;
                 } else {
                     __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(dst + (u * NT + wave * 64) * 16), 16, 0, 0);
                 }
             }
+        }
     };
     auto landed = [&]() {
         asm volatile("" ::: "memory");
@@ -202,42 +220,49 @@ __global__ void __launch_bounds__(64 * WQ *WK) window_kernel(Args a) {
     bool careful = false;
     constexpr float kDown = __is_same(T, _Float16) ? 0.0f : 40.0f;
 
-    auto work = [&](int ti, int buf) {
-        const bool in_first = ti < first_tiles;
-        const int j0 = in_first ? ti * KT : low + (ti - first_tiles) * KT, end = in_first ? first : high + 1;
+    // operand addresses in a tile, as offsets: K unit 2 c + h of row n is at ka ^ 32 c, V units 4 d .. of its rows at va ^ 64 d
+    // (FP32: word n of units 8 d .. at va ^ 128 d)
+    int ka = n * ROW + (h ^ swizzle_k<F32, UNITS>(n)) * 16 + 32 * wk * ROW;
+    int va;
+    if constexpr (F32) {
+        va = 4 * h * ROW + n % 4 * 4 + 32 * wk * ROW;
+    } else {
+        const int key = 4 * h + (lane & 15) / 4;
+        va = key * ROW + ((2 * (lane >> 4 & 1) + (lane & 3) / 2) ^ swizzle_v<F32, UNITS>(key)) * 16 + (lane & 1) * 8 + 32 * wk * ROW;
+    }
+
+    auto work = [&](int v0, int buf) {
         // a tile that none of the wave's rows sees (the whole of it lies outside their windows)
-        if (w0 > w1) return;
-        if (!in_first && ((long long)j0 > (long long)w1 + a.right || (j0 + KT <= w0 - a.left && j0 >= a.sinks))) return;
+        if (w0 > w1 || v0 > hi1 || (v0 + KT <= lo0 && v0 >= sinks)) return;
         const char *const kt = lds + buf * S::BUF, *const vt = kt + KT * ROW;
+        asm volatile("" : "+v"(ka), "+v"(va));  // (the addresses made from them are made anew, not kept for every use)
         v16f s[NB];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int key = 32 * (i * WK + wk) + n;
-            s[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-            if constexpr (F32) {
+        for (int i = 0; i < NB; ++i) s[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-                for (int c = 0; c < 2 * QF; ++c) {
-                    const v4f kx = *(const v4f *)(kt + key * ROW + place_k<F32, UNITS>(key, 2 * c + h) * 16);
+        for (int c = 0; c < (F32 ? 2 * QF : QF); ++c) {
+            const char *const row = kt + (ka ^ 32 * c);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                if constexpr (F32) {
+                    const v4f kx = *(const v4f *)(row + 32 * i * WK * ROW);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(kx[e], qx[c][e], s[i], 0, 0, 0);
+                } else {
+                    s[i] = mma<T>(*(const v8s *)(row + 32 * i * WK * ROW), qf[c], s[i]);
                 }
-            } else {
-#pragma unroll
-                for (int c = 0; c < QF; ++c)
-                    s[i] = mma<T>(*(const v8s *)(kt + key * ROW + place_k<F32, UNITS>(key, 2 * c + h) * 16), qf[c], s[i]);
             }
         }
         // masks, where the tile is not seen as a whole by every row of the wave
-        const bool whole = j0 + KT <= end && (in_first || ((long long)j0 + KT - 1 <= (long long)w0 + a.right && (j0 >= w1 - a.left || j0 + KT <= a.sinks)));
+        const bool whole = v0 + KT <= to && v0 + KT - 1 <= hi0 && (v0 >= lo1 || v0 + KT <= sinks);
         if (!whole) {
-            const int hi = (int)min((long long)end - 1, (long long)p + a.right) - j0 - 4 * h;
-            const int lo = in_first ? -KT : max(max(p, 0) - a.left - j0, -KT) - 4 * h, sink = min(a.sinks - j0, KT) - 4 * h;
+            const int off = v0 + 32 * wk + 4 * h, hx = min(to - 1, hi) - off, lx = max(lo, v0 - KT) - off, sx = min(sinks, v0 + KT) - off;
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const int at = 32 * (i * WK + wk) + 8 * (e / 4) + e % 4;
-                    if (!(at <= hi && (at >= lo || at < sink))) s[i][e] = -INFINITY;
+                    const int at = 32 * i * WK + 8 * (e / 4) + e % 4;
+                    if (!(at <= hx && (at >= lx || at < sx))) s[i][e] = -INFINITY;
                 }
         }
         float top = s[0][0];
@@ -269,10 +294,11 @@ __global__ void __launch_bounds__(64 * WQ *WK) window_kernel(Args a) {
             for (int i = 0; i < NB; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const int key = 32 * (i * WK + wk) + 8 * (e / 4) + e % 4 + 4 * h;
+                    // V[8 (e / 4) + e % 4 + 4 h][32 d + n]: unit 8 d + n / 4 at its place
+                    const int key = 8 * (e / 4) + e % 4;
 #pragma unroll
                     for (int d = 0; d < DB; ++d) {
-                        const float vx = *(const float *)(vt + key * ROW + place_v<F32, UNITS>(key, 8 * d + n / 4) * 16 + n % 4 * 4);
+                        const float vx = *(const float *)(vt + va + (32 * i * WK + key) * ROW + ((n / 4) ^ ((key + 4 * h) & 7)) * 16 + 128 * d);
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vx, s[i][e], o[d], 0, 0, 0);
                     }
                 }
@@ -287,15 +313,11 @@ __global__ void __launch_bounds__(64 * WQ *WK) window_kernel(Args a) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) w[e] = (T)s[i][8 * k16 + e];
                     const v8s pf = *(const v8s *)w;
-                    const int key = 32 * (i * WK + wk) + 16 * k16 + 4 * h + (lane & 15) / 4;
 #pragma unroll
                     for (int d = 0; d < DB; ++d) {
-                        const int c = 4 * d + 2 * (lane >> 4 & 1) + (lane & 3) / 2;
-                        v4s part[2];
-#pragma unroll
-                        for (int y = 0; y < 2; ++y)
-                            part[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)(vt + (key + 8 * y) * ROW + place_v<F32, UNITS>(key + 8 * y, c) * 16 + (lane & 1) * 8));
-                        o[d] = mma<T>(v8s{part[0][0], part[0][1], part[0][2], part[0][3], part[1][0], part[1][1], part[1][2], part[1][3]}, pf, o[d]);
+                        const char *const at = vt + (va ^ 64 * d) + (32 * i * WK + 16 * k16) * ROW;
+                        const v4s x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)at), x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)(at + 8 * ROW));
+                        o[d] = mma<T>(v8s{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]}, pf, o[d]);
                     }
                 }
         }
@@ -303,14 +325,12 @@ __global__ void __launch_bounds__(64 * WQ *WK) window_kernel(Args a) {
             for (int i = 0; i < NB; ++i) {
                 uint32_t left = __builtin_amdgcn_readfirstlane(flags[i * WK + wk]);
                 while (left) {
-                    const int j = j0 + 32 * (i * WK + wk) + __builtin_ctz(left);
+                    const int v = v0 + 32 * (i * WK + wk) + __builtin_ctz(left);
                     left &= left - 1;
-                    const bool seen = j < end && (in_first || ((long long)j <= (long long)p + a.right && (j >= p - a.left || j < a.sinks)));
-                    if (j >= end || !seen) continue;
-                    const T *src = vp + (long long)j * a.v.t_stride;
+                    if (!(v <= min(to - 1, hi) && (v >= lo || v < sinks))) continue;
+                    const T *src = vp + (long long)(v + (v >= first ? shift : 0)) * a.v.t_stride;
 #pragma unroll
                     for (int d = 0; d < DB; ++d)
-#pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const int at = 32 * d + 8 * (e / 4) + 4 * h + e % 4;
                             if (at < a.d && !finite_bits(src[at])) o[d][e] += (float)src[at];
@@ -338,13 +358,17 @@ __global__ void __launch_bounds__(64 * WQ *WK) window_kernel(Args a) {
         for (int d = 0; d < DB; ++d) o[d] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
         m = -INFINITY;
         l = 0.0f;
-        if (from < to) stage(from, 0);
-        for (int ti = from; ti < to; ++ti) {
-            const int buf = ti - from & 1;
+        if (tiles) stage(from, 0);
+        for (int i = 0; i < tiles; ++i) {
+            const int v0 = from + i * KT, buf = a.buffers == 2 ? i & 1 : 0;
             landed();
             if (careful) take_out(buf);
-            if (ti + 1 < to) stage(ti + 1, buf ^ 1);
-            work(ti, buf);
+            if (a.buffers == 2 && i + 1 < tiles) stage(v0 + KT, buf ^ 1);
+            work(v0, buf);
+            if (a.buffers == 1 && i + 1 < tiles) {
+                landed();  // (this wave's reads; then all waves')
+                stage(v0 + KT, 0);
+            }
         }
         bool bad = false;
 #pragma unroll
@@ -434,25 +458,41 @@ __global__ void __launch_bounds__(64 * WQ *WK) window_kernel(Args a) {
     }
 }
 
-// Joins the splits: out = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m), four elements a thread.
+// Joins the splits: out = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m), four elements a thread, eight splits at a time.
 template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(Args a, long long units) {
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+__global__ void __launch_bounds__(64) join_kernel(Args a, int units) {
+    const int at = blockIdx.x * 64 + threadIdx.x;
     if (at >= units) return;
-    const int per = a.d / 4, c = (int)(at % per);
-    const long long row = at / per, all = (long long)a.batch * a.kv_heads * a.rows;  // row: of all
-    float top = -INFINITY, sum = 0.0f;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.stats[2 * (s * all + row)]);
-    v4f v = {0, 0, 0, 0};
-    for (int s = 0; s < a.splits; ++s) {
-        const float m = a.stats[2 * (s * all + row)], by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top - kRoom);
-        sum += a.stats[2 * (s * all + row) + 1] * by;
-        if (by != 0.0f) v += *(const v4f *)(a.part + (s * all + row) * a.d + 4 * c) * by;
-    }
-    const long long bh = row / a.rows;
-    const int r = (int)(row % a.rows), t = r / a.group, b = (int)(bh / a.kv_heads), hk = (int)(bh % a.kv_heads);
+    const int per = a.d / 4, c = at % per, row = at / per, all = a.batch * a.kv_heads * a.rows;  // row: of all
+    const int bh = row / a.rows, r = row % a.rows, t = r / a.group, b = bh / a.kv_heads, hk = bh % a.kv_heads;
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.tk) : a.tk;
     const int p = (a.starts ? min(max(a.starts[b], -(1 << 30)), 1 << 30) : len - a.tq) + t;
+    float m = -INFINITY, sum = 0.0f;
+    v4f v = {0, 0, 0, 0};
+    for (int s0 = 0; s0 < a.splits; s0 += 8) {
+        float2 stat[8];
+        v4f part[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const long long slot = (long long)min(s0 + s, a.splits - 1) * all + row;
+            stat[s] = *(const float2 *)(a.stats + 2 * slot);
+            part[s] = *(const v4f *)(a.part + slot * a.d + 4 * c);
+        }
+        float top = m;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) top = s0 + s < a.splits ? fmaxf(top, stat[s].x + kRoom) : top;
+        const float old = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        sum *= old;
+        v *= old;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            if (s0 + s >= a.splits || stat[s].x == -INFINITY) continue;
+            const float by = __builtin_amdgcn_exp2f(stat[s].x - top);
+            sum += stat[s].y * by;
+            v += part[s] * by;
+        }
+    }
     const float by = p >= 0 && p < len && sum != 0.0f ? 1.0f / sum : 0.0f;
     T res[4];
 #pragma unroll
@@ -485,10 +525,11 @@ int plan_of(int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int
     const int64_t most = 1 << 30, span = per / (heads / kv_heads) + 2;
     const int64_t window = left >= most || right >= most ? tk : left + right + span + sinks;
     const int64_t keys = window < tk ? window : tk;
-    const int64_t blocks = (keys + 127) / 128;
+    const int64_t tile = dtype == KEA_F32 ? (p.dp == 64 ? 128 : p.dp == 128 ? 64 : 32) : p.dp == 256 ? 64 : 128;
+    const int64_t blocks = (keys + tile - 1) / tile;
     p.splits = 1;
-    if (wgs < 256 && blocks > 1) {
-        int64_t s = (512 + wgs - 1) / (wgs > 0 ? wgs : 1);
+    if (wgs > 0 && wgs < 256 && blocks > 1) {  // up to two workgroups a CU, a tile of keys each at least
+        int64_t s = 512 / wgs;
         s = s < blocks ? s : blocks;
         p.splits = (int)(s < 64 ? s : 64);
     }
@@ -506,22 +547,23 @@ int launched() {
 }
 
 template <typename T, int DP, int WQ, int WK, bool RAGGED>
-int run_shape(const Args &a, int64_t groups, hipStream_t stream) {
+int run_shape(Args a, int64_t groups, hipStream_t stream) {
     using S = Shape<T, DP, WQ, WK>;
-    static_assert(S::LDS <= 160 * 1024 && S::KT * S::UNITS % S::NT == 0 && S::KB <= 16, "tiles and flags");
+    static_assert(S::lds(S::BUFFERS) <= 160 * 1024 && S::KT * S::UNITS % S::NT == 0 && S::KB <= 16, "tiles and flags");
     const int64_t blocks = groups * a.row_tiles * a.splits;
     if (blocks > INT32_MAX / 2 || !kea::fits_dispatch(blocks, S::NT)) return kea::fail(KEA_EINVAL, "kea_window_attention: too large for one launch");
     const auto kernel = window_kernel<T, DP, WQ, WK, RAGGED>;
-    if (S::LDS > 65536) {
-        const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
+    a.buffers = S::BUFFERS;
+    const int lds = S::lds(a.buffers);
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return kea::fail((int)e, std::string("kea_window_attention: ") + hipGetErrorString(e));
     }
-    kernel<<<dim3((unsigned)blocks), S::NT, S::LDS, stream>>>(a);
+    kernel<<<dim3((unsigned)blocks), S::NT, lds, stream>>>(a);
     const int rc = launched();
     if (rc || a.splits == 1) return rc;
-    const int64_t units = groups * a.rows * (a.d / 4);
-    if (!kea::fits_dispatch((units + 255) / 256, 256)) return kea::fail(KEA_EINVAL, "kea_window_attention: too large for one launch");
-    join_kernel<T><<<dim3((unsigned)((units + 255) / 256)), 256, 0, stream>>>(a, units);
+    const int64_t units = groups * a.rows * (a.d / 4);  // (fewer than 2^23: splits > 1 only for few rows)
+    join_kernel<T><<<dim3((unsigned)((units + 63) / 64)), 64, 0, stream>>>(a, (int)units);
     return launched();
 }
 
@@ -582,7 +624,7 @@ int kea_window_attention(const kea_heads *q, const kea_heads *k, const kea_heads
     const int64_t most = 1 << 30;
     const Args a{*q, *k, *v, *out, kv_lengths, q_starts, (float *)workspace, workspace ? (float *)((char *)workspace + p.part_bytes) : nullptr,
                  (int)batch, (int)tq, (int)tk, (int)kv_heads, (int)(heads / kv_heads), (int)d, (int)(left < most ? left : most),
-                 (int)(right < most ? right : most), (int)(sinks < most ? sinks : most), (int)p.rows, p.row_tiles, p.splits, scale};
+                 (int)(right < most ? right : most), (int)(sinks < most ? sinks : most), (int)p.rows, p.row_tiles, p.splits, 1, scale};
     const int64_t groups = batch * kv_heads;
     const hipStream_t s = (hipStream_t)stream;
     return dtype == KEA_F32 ? run_type<float>(a, p, groups, s) : dtype == KEA_F16 ? run_type<_Float16>(a, p, groups, s) : run_type<__bf16>(a, p, groups, s);
