@@ -34,7 +34,6 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(1))) const void *gptr_t;
 typedef __attribute__((address_space(3))) void *lptr_t;
 typedef __attribute__((address_space(3))) v4s *ltr_t;
 
@@ -93,6 +92,13 @@ __device__ __forceinline__ float other_half_max(float v) {
 __device__ __forceinline__ float both_halves(float v) {
     const float2 s = halves(v);
     return s.x + s.y;
+}
+
+// 16 bytes a lane from global memory straight to LDS, at the wave's base address plus 16 a lane; done when vmcnt says so. In
+// place of the builtin, after which the compiler waits for all of a wave's copies before its next transposing read, those for
+// the tile ahead among them. (Nothing else here uses m0.)
+__device__ __forceinline__ void copy16(const void *src, uint32_t base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(src) : "memory");
 }
 
 template <typename T>
@@ -160,29 +166,33 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP * sizeof(T) <= 512 ? 2 : 1) wi
     const int key0 = tid / UNITS;
     auto unit = [&](int kv, int key) { return (tid % UNITS ^ (kv ? swizzle_v<F32, UNITS>(key) : swizzle_k<F32, UNITS>(key))) * EPU; };
     auto stage = [&](int v0, int buf) {
-        const bool plain = v0 >= first && v0 + KT <= to;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            const long long stride = kv ? a.v.t_stride : a.k.t_stride;
-            const T *const base = kv ? vp : kp;
+        auto put = [&](int kv, int u, const T *src, int c) {
             char *const dst = lds + buf * S::BUF + kv * KT * ROW;
+            if constexpr (RAGGED) {
+                const v4f zero = {0, 0, 0, 0};
+                *(v4f *)(dst + (u * NT + tid) * 16) = c < a.d ? *(const v4f *)src : zero;
+            } else {
+                copy16(src, (uint32_t)(uintptr_t)(lptr_t)(dst + (u * NT + wave * 64) * 16));
+            }
+        };
+        if (v0 >= first && v0 + KT <= to) {
 #pragma unroll
-            for (int u = 0; u < COPIES; ++u) {
-                const int key = key0 + u * STEP, c = unit(kv, STEP % 16 ? key : key0);
-                const T *src;
-                if (plain) {
-                    src = base + (long long)key0 * stride + c + (long long)(v0 + shift + u * STEP) * stride;
-                } else {
-                    const int v = min(v0 + key, to - 1);
-                    src = base + (long long)(v + (v >= first ? shift : 0)) * stride + c;
-                }
-                if constexpr (RAGGED) {
-                    const v4f zero = {0, 0, 0, 0};
-                    *(v4f *)(dst + (u * NT + tid) * 16) = c < a.d ? *(const v4f *)src : zero;
-                } else {
-                    __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(dst + (u * NT + wave * 64) * 16), 16, 0, 0);
+            for (int kv = 0; kv < 2; ++kv) {
+                const long long stride = kv ? a.v.t_stride : a.k.t_stride;
+                const T *const base = (kv ? vp : kp) + (long long)(v0 + shift) * stride;
+#pragma unroll
+                for (int u = 0; u < COPIES; ++u) {
+                    const int c = unit(kv, STEP % 16 ? key0 + u * STEP : key0);
+                    put(kv, u, base + u * STEP * stride + ((long long)key0 * stride + c), c);
                 }
             }
+        } else {  // the tile holds keys on both sides of the gap, or the range's end: each key by itself
+            for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+                for (int u = 0; u < COPIES; ++u) {
+                    const int key = key0 + u * STEP, v = min(v0 + key, to - 1), c = unit(kv, key);
+                    put(kv, u, (kv ? vp : kp) + (long long)(v + (v >= first ? shift : 0)) * (kv ? a.v.t_stride : a.k.t_stride) + c, c);
+                }
         }
     };
     auto landed = [&]() {
@@ -236,23 +246,58 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP * sizeof(T) <= 512 ? 2 : 1) wi
         if (w0 > w1 || v0 > hi1 || (v0 + KT <= lo0 && v0 >= sinks)) return;
         const char *const kt = lds + buf * S::BUF, *const vt = kt + KT * ROW;
         asm volatile("" : "+v"(ka), "+v"(va));  // (the addresses made from them are made anew, not kept for every use)
+        // Operands are read a step ahead of the matrix instructions that take them, into one of two register sets.
+        constexpr int KSTEPS = F32 ? 2 * QF : QF / 2;  // steps of eight elements (FP32) or 32
         v16f s[NB];
 #pragma unroll
         for (int i = 0; i < NB; ++i) s[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        v4f kx[2][NB][F32 ? 1 : 2];
+        auto read_k = [&](int c) {
 #pragma unroll
-        for (int c = 0; c < (F32 ? 2 * QF : QF); ++c) {
-            const char *const row = kt + (ka ^ 32 * c);
+            for (int y = 0; y < (F32 ? 1 : 2); ++y)
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                if constexpr (F32) {
-                    const v4f kx = *(const v4f *)(row + 32 * i * WK * ROW);
+                for (int i = 0; i < NB; ++i) kx[c & 1][i][y] = *(const v4f *)(kt + (ka ^ 32 * (F32 ? c : 2 * c + y)) + 32 * i * WK * ROW);
+        };
+        read_k(0);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(kx[e], qx[c][e], s[i], 0, 0, 0);
-                } else {
-                    s[i] = mma<T>(*(const v8s *)(row + 32 * i * WK * ROW), qf[c], s[i]);
+        for (int c = 0; c < KSTEPS; ++c) {
+            if (c + 1 < KSTEPS) read_k(c + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (F32) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) s[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(kx[c & 1][i][0][e], qx[c][e], s[i], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) s[i] = mma<T>(__builtin_bit_cast(v8s, kx[c & 1][i][y]), qf[2 * c + y], s[i]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // V: steps of one key of each half (FP32) or 16 keys, the first read while the softmax runs
+        constexpr int VSTEPS = NB * (F32 ? 16 : 2);
+        float vx[2][F32 ? DB : 1];
+        v4s vh[2][F32 ? 1 : DB][2];
+        auto read_v = [&](int j) {
+            if constexpr (F32) {
+                // V[8 (e / 4) + e % 4 + 4 h][32 d + n]: unit 8 d + n / 4 at its place
+                const int i = j / 16, key = 8 * (j % 16 / 4) + j % 4;
+                const char *const at = vt + va + (32 * i * WK + key) * ROW + ((n / 4) ^ ((key + 4 * h) & 7)) * 16;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) vx[j & 1][d] = *(const float *)(at + 128 * d);
+            } else {
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    const char *const at = vt + (va ^ 64 * d) + (32 * (j / 2) * WK + 16 * (j % 2)) * ROW;
+                    vh[j & 1][d][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)at);
+                    vh[j & 1][d][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)(at + 8 * ROW));
                 }
             }
-        }
+        };
+        read_v(0);
+        __builtin_amdgcn_sched_barrier(0);
         // masks, where the tile is not seen as a whole by every row of the wave
         const bool whole = v0 + KT <= to && v0 + KT - 1 <= hi0 && (v0 >= lo1 || v0 + KT <= sinks);
         if (!whole) {
@@ -289,37 +334,27 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP * sizeof(T) <= 512 ? 2 : 1) wi
                 sum += s[i][e];
             }
         l += sum;
-        if constexpr (F32) {
+        // The 16-bit types' weights are rounded to what the product takes (half a step, relative to themselves; below the
+        // smallest normal FP16 number 2^-25): as accurate as the values they weigh.
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
+        for (int j = 0; j < VSTEPS; ++j) {
+            if (j + 1 < VSTEPS) read_v(j + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (F32) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    // V[8 (e / 4) + e % 4 + 4 h][32 d + n]: unit 8 d + n / 4 at its place
-                    const int key = 8 * (e / 4) + e % 4;
+                for (int d = 0; d < DB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vx[j & 1][d], s[j / 16][j % 16], o[d], 0, 0, 0);
+            } else {
+                T w[8];
 #pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        const float vx = *(const float *)(vt + va + (32 * i * WK + key) * ROW + ((n / 4) ^ ((key + 4 * h) & 7)) * 16 + 128 * d);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vx, s[i][e], o[d], 0, 0, 0);
-                    }
+                for (int e = 0; e < 8; ++e) w[e] = (T)s[j / 2][8 * (j % 2) + e];
+                const v8s pf = *(const v8s *)w;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    const v4s x0 = vh[j & 1][d][0], x1 = vh[j & 1][d][1];
+                    o[d] = mma<T>(v8s{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]}, pf, o[d]);
                 }
-        } else {
-            // Each weight is rounded to the type that the product takes (half a step, relative to itself; below the smallest
-            // normal FP16 number 2^-25): as accurate as the values it weighs.
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int k16 = 0; k16 < 2; ++k16) {
-                    T w[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e] = (T)s[i][8 * k16 + e];
-                    const v8s pf = *(const v8s *)w;
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        const char *const at = vt + (va ^ 64 * d) + (32 * i * WK + 16 * k16) * ROW;
-                        const v4s x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)at), x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)(at + 8 * ROW));
-                        o[d] = mma<T>(v8s{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]}, pf, o[d]);
-                    }
-                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         if (__builtin_expect(careful, 0)) {
             for (int i = 0; i < NB; ++i) {
