@@ -96,9 +96,12 @@ __device__ __forceinline__ float both_halves(float v) {
 
 // 16 bytes a lane from global memory straight to LDS, at the wave's base address plus 16 a lane; done when vmcnt says so. In
 // place of the builtin, after which the compiler waits for all of a wave's copies before its next transposing read, those for
-// the tile ahead among them. (Nothing else here uses m0.)
+// the tile ahead among them. (Nothing else here uses m0.) The second form reads at a uniform address plus an offset.
 __device__ __forceinline__ void copy16(const void *src, uint32_t base) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(src) : "memory");
+}
+__device__ __forceinline__ void copy16(const void *src, uint32_t offset, uint32_t base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(offset), "s"(src) : "memory");
 }
 
 template <typename T>
@@ -116,7 +119,7 @@ __device__ __forceinline__ bool finite_bits(T v) {
 
 // RAGGED: d < DP, rows of K and V end before DP elements and go through registers, zeros behind them.
 template <typename T, int DP, int WQ, int WK, bool RAGGED>
-__global__ void __launch_bounds__(64 * WQ *WK, DP * sizeof(T) <= 512 ? 2 : 1) window_kernel(Args a) {
+__global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) window_kernel(Args a) {
     using S = Shape<T, DP, WQ, WK>;
     constexpr bool F32 = S::F32;
     constexpr int NB = S::NB, KT = S::KT, UNITS = S::UNITS, NT = S::NT, ROW = S::ROW, EPU = 16 / (int)sizeof(T);
@@ -165,35 +168,35 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP * sizeof(T) <= 512 ? 2 : 1) wi
     static_assert(NT % UNITS == 0 && (STEP % 16 == 0 || STEP == 8 || STEP == 4 || STEP == 2 || STEP == 1), "copies");
     const int key0 = tid / UNITS;
     auto unit = [&](int kv, int key) { return (tid % UNITS ^ (kv ? swizzle_v<F32, UNITS>(key) : swizzle_k<F32, UNITS>(key))) * EPU; };
+    // a tile of neighbouring keys is copied from a uniform address, each thread's rows at 32-bit offsets from it, where those
+    // suffice (of 16-bit types and the copies' rows a multiple of 16 apart: others have more swizzles)
+    constexpr bool NEAR = !RAGGED && STEP % 16 == 0;
+    const bool near_k = (long long)KT * a.k.t_stride < 1 << 29, near_v = (long long)KT * a.v.t_stride < 1 << 29;
+    const uint32_t off_k = ((uint32_t)(key0 * (int)a.k.t_stride) + unit(0, key0)) * (uint32_t)sizeof(T);
+    const uint32_t off_v = ((uint32_t)(key0 * (int)a.v.t_stride) + unit(1, key0)) * (uint32_t)sizeof(T);
     auto stage = [&](int v0, int buf) {
-        auto put = [&](int kv, int u, const T *src, int c) {
-            char *const dst = lds + buf * S::BUF + kv * KT * ROW;
-            if constexpr (RAGGED) {
-                const v4f zero = {0, 0, 0, 0};
-                *(v4f *)(dst + (u * NT + tid) * 16) = c < a.d ? *(const v4f *)src : zero;
-            } else {
-                copy16(src, (uint32_t)(uintptr_t)(lptr_t)(dst + (u * NT + wave * 64) * 16));
-            }
-        };
-        if (v0 >= first && v0 + KT <= to) {
+        char *const dst = lds + buf * S::BUF + wave * 1024;
+        if (NEAR && near_k && near_v && v0 >= first && v0 + KT <= to) {
+            const T *k0 = kp + (long long)(v0 + shift) * a.k.t_stride, *w0 = vp + (long long)(v0 + shift) * a.v.t_stride;
 #pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-                const long long stride = kv ? a.v.t_stride : a.k.t_stride;
-                const T *const base = (kv ? vp : kp) + (long long)(v0 + shift) * stride;
+            for (int u = 0; u < COPIES; ++u) copy16(k0 + u * (STEP * a.k.t_stride), off_k, (uint32_t)(uintptr_t)(lptr_t)(dst + u * NT * 16));
 #pragma unroll
-                for (int u = 0; u < COPIES; ++u) {
-                    const int c = unit(kv, STEP % 16 ? key0 + u * STEP : key0);
-                    put(kv, u, base + u * STEP * stride + ((long long)key0 * stride + c), c);
-                }
-            }
-        } else {  // the tile holds keys on both sides of the gap, or the range's end: each key by itself
-            for (int kv = 0; kv < 2; ++kv)
-#pragma unroll
-                for (int u = 0; u < COPIES; ++u) {
-                    const int key = key0 + u * STEP, v = min(v0 + key, to - 1), c = unit(kv, key);
-                    put(kv, u, (kv ? vp : kp) + (long long)(v + (v >= first ? shift : 0)) * (kv ? a.v.t_stride : a.k.t_stride) + c, c);
-                }
+            for (int u = 0; u < COPIES; ++u) copy16(w0 + u * (STEP * a.v.t_stride), off_v, (uint32_t)(uintptr_t)(lptr_t)(dst + (KT * ROW + u * NT * 16)));
+            return;
         }
+        for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int u = 0; u < COPIES; ++u) {
+                const int key = key0 + u * STEP, v = min(v0 + key, to - 1), c = unit(kv, key);
+                const T *src = (kv ? vp : kp) + (long long)(v + (v >= first ? shift : 0)) * (kv ? a.v.t_stride : a.k.t_stride) + c;
+                char *const to_lds = dst + kv * KT * ROW + u * NT * 16;
+                if constexpr (RAGGED) {
+                    const v4f zero = {0, 0, 0, 0};
+                    *(v4f *)(to_lds + lane * 16) = c < a.d ? *(const v4f *)src : zero;
+                } else {
+                    copy16(src, (uint32_t)(uintptr_t)(lptr_t)to_lds);
+                }
+            }
     };
     auto landed = [&]() {
         asm volatile("" ::: "memory");
@@ -302,13 +305,22 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP * sizeof(T) <= 512 ? 2 : 1) wi
         const bool whole = v0 + KT <= to && v0 + KT - 1 <= hi0 && (v0 >= lo1 || v0 + KT <= sinks);
         if (!whole) {
             const int off = v0 + 32 * wk + 4 * h, hx = min(to - 1, hi) - off, lx = max(lo, v0 - KT) - off, sx = min(sinks, v0 + KT) - off;
+            const uint32_t width = (uint32_t)max(hx - lx + 1, 0);
+            if (v0 >= sinks) {
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
+                for (int i = 0; i < NB; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int at = 32 * i * WK + 8 * (e / 4) + e % 4;
-                    if (!(at <= hx && (at >= lx || at < sx))) s[i][e] = -INFINITY;
-                }
+                    for (int e = 0; e < 16; ++e)
+                        if ((uint32_t)(32 * i * WK + 8 * (e / 4) + e % 4 - lx) >= width) s[i][e] = -INFINITY;
+            } else {
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int at = 32 * i * WK + 8 * (e / 4) + e % 4;
+                        if (!(at <= hx && (at >= lx || at < sx))) s[i][e] = -INFINITY;
+                    }
+            }
         }
         float top = s[0][0];
 #pragma unroll
