@@ -47,8 +47,17 @@ struct Args {
     const int32_t *lengths, *starts;
     float *part, *stats;  // splits > 1: [splits][sequences and key heads][rows][d], [..][rows][2]
     int batch, tq, tk, kv_heads, group, d, left, right, sinks;
-    int rows, row_tiles, splits, buffers;
+    int rows, row_tiles, tiles8, splits;
+    uint32_t group_mul, group_shift;
     float scale;
+
+    // row / group, for rows below 2^31: group_mul = 2^(31 + s) / group + 1 with 2^s >= group
+    __device__ __forceinline__ int token(int row) const { return (int)(__umulhi(2u * (uint32_t)row, group_mul) >> group_shift); }
+};
+
+template <int N>
+struct Count {
+    static constexpr int value = N;
 };
 
 template <typename T, int DP, int WQ, int WK>
@@ -62,7 +71,7 @@ struct Shape {
     static constexpr int MERGE = WK > 1 ? NW * 32 * (DP + 2) * 4 : 0;
     // two buffers where two workgroups of a CU have room for them, otherwise one: the other workgroup works meanwhile
     static constexpr int BUFFERS = 2 * BUF <= 65536 ? 2 : 1;
-    static constexpr int lds(int buffers) { return (buffers * BUF > MERGE ? buffers * BUF : MERGE) + 64; }
+    static constexpr int LDS = (BUFFERS * BUF > MERGE ? BUFFERS * BUF : MERGE) + 64;
 };
 
 // The place of 16-byte unit c of a key's row in LDS is c ^ swizzle(key), so that rows read together lie in different banks.
@@ -125,27 +134,27 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
     constexpr int NB = S::NB, KT = S::KT, UNITS = S::UNITS, NT = S::NT, ROW = S::ROW, EPU = 16 / (int)sizeof(T);
     constexpr int QF = DP / 16, DB = DP / 32;  // steps of 16 elements, blocks of 32 output elements
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    uint32_t *const flags = (uint32_t *)(lds + S::lds(a.buffers) - 64);
+    uint32_t *const flags = (uint32_t *)(lds + S::LDS - 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5, wq = wave / WK, wk = wave % WK;
 
-    // Workgroups go to the eight XCDs in turn; each XCD takes a run of its own, so that tiles of neighbouring rows and splits
-    // of one sequence and key head share keys in its L2.
-    const int total = gridDim.x, per = total / 8, rest = total % 8, x = blockIdx.x % 8;
-    const int id = x * per + min(x, rest) + blockIdx.x / 8;
-    const int tile = id % a.row_tiles, split = id / a.row_tiles % a.splits, bh = id / a.row_tiles / a.splits;
-    const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+    // Workgroups go to the eight XCDs in turn: where there are eight tiles of rows or more, each XCD takes a run of its own,
+    // so that neighbours share keys in its L2. (Of the last up to seven workgroups some have no tile.)
+    const int split = a.splits > 1 ? (int)blockIdx.x / a.tiles8 : 0, x = (int)blockIdx.x - split * a.tiles8;
+    const int tile = a.tiles8 == a.row_tiles && a.tiles8 < 8 ? x : x % 8 * (a.tiles8 / 8) + x / 8;
+    if (tile >= a.row_tiles) return;
+    const int hk = blockIdx.y, b = blockIdx.z;
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.tk) : a.tk;
     const int start = a.starts ? min(max(a.starts[b], -(1 << 30)), 1 << 30) : len - a.tq;
 
     // this lane's query
     const int r0 = tile * 32 * WQ, row = r0 + 32 * wq + n;
     const bool real = row < a.rows;
-    const int t = min(row, a.rows - 1) / a.group, head = hk * a.group + min(row, a.rows - 1) % a.group, p = start + t;
+    const int t = a.token(min(row, a.rows - 1)), head = hk * a.group + min(row, a.rows - 1) - t * a.group, p = start + t;
     const bool inside = real && p >= 0 && p < len;
     // positions of the tile's and of the wave's rows, those inside the sequence
-    auto first_of = [&](int from) { return max(start + min(from, a.rows - 1) / a.group, 0); };
-    auto last_of = [&](int from, int rows) { return min(start + (min(from + rows, a.rows) - 1) / a.group, len - 1); };
+    auto first_of = [&](int from) { return max(start + a.token(min(from, a.rows - 1)), 0); };
+    auto last_of = [&](int from, int rows) { return min(start + a.token(min(from + rows, a.rows) - 1), len - 1); };
     auto reach = [&](int from) { return (int)min((long long)len - 1, (long long)from + a.right); };  // the last key seen from there
     const int p0 = first_of(r0), p1 = last_of(r0, 32 * WQ);
     const int w0 = first_of(r0 + 32 * wq), w1 = r0 + 32 * wq < a.rows ? last_of(r0 + 32 * wq, 32) : -1;
@@ -155,8 +164,13 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
     if (first == low) first = low = 0;
     const int shift = low - first, sinks = shift ? first : a.sinks;
     if (p0 <= p1) keys = reach(p1) + 1 - shift;
-    auto cut = [&](int s) { return min(keys, (int)((long long)keys * s / a.splits + 31) & ~31); };
-    const int from = cut(split), to = cut(split + 1), tiles = (to - from + KT - 1) / KT;
+    int from = 0, to = keys;
+    if (a.splits > 1) {
+        const int share = ((keys + 31) / 32 + a.splits - 1) / a.splits * 32;
+        from = min(keys, split * share);
+        to = min(keys, from + share);
+    }
+    const int tiles = (to - from + KT - 1) / KT;
     // per lane and wave, in these numbers: the last key seen and the first of the window
     const int hi = reach(max(p, 0)) - shift, lo = max(p, 0) - a.left - shift;
     const int hi0 = reach(w0) - shift, hi1 = reach(w1) - shift, lo0 = w0 - a.left - shift, lo1 = w1 - a.left - shift;
@@ -174,17 +188,19 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
     const bool near_k = (long long)KT * a.k.t_stride < 1 << 29, near_v = (long long)KT * a.v.t_stride < 1 << 29;
     const uint32_t off_k = ((uint32_t)(key0 * (int)a.k.t_stride) + unit(0, key0)) * (uint32_t)sizeof(T);
     const uint32_t off_v = ((uint32_t)(key0 * (int)a.v.t_stride) + unit(1, key0)) * (uint32_t)sizeof(T);
-    auto stage = [&](int v0, int buf) {
+    auto stage = [&](int v0, int buf, bool of_k, bool of_v) {
         char *const dst = lds + buf * S::BUF + wave * 1024;
         if (NEAR && near_k && near_v && v0 >= first && v0 + KT <= to) {
             const T *k0 = kp + (long long)(v0 + shift) * a.k.t_stride, *w0 = vp + (long long)(v0 + shift) * a.v.t_stride;
+            if (of_k)
 #pragma unroll
-            for (int u = 0; u < COPIES; ++u) copy16(k0 + u * (STEP * a.k.t_stride), off_k, (uint32_t)(uintptr_t)(lptr_t)(dst + u * NT * 16));
+                for (int u = 0; u < COPIES; ++u) copy16(k0 + u * (STEP * a.k.t_stride), off_k, (uint32_t)(uintptr_t)(lptr_t)(dst + u * NT * 16));
+            if (of_v)
 #pragma unroll
-            for (int u = 0; u < COPIES; ++u) copy16(w0 + u * (STEP * a.v.t_stride), off_v, (uint32_t)(uintptr_t)(lptr_t)(dst + (KT * ROW + u * NT * 16)));
+                for (int u = 0; u < COPIES; ++u) copy16(w0 + u * (STEP * a.v.t_stride), off_v, (uint32_t)(uintptr_t)(lptr_t)(dst + (KT * ROW + u * NT * 16)));
             return;
         }
-        for (int kv = 0; kv < 2; ++kv)
+        for (int kv = of_k ? 0 : 1; kv < (of_v ? 2 : 1); ++kv)
 #pragma unroll
             for (int u = 0; u < COPIES; ++u) {
                 const int key = key0 + u * STEP, v = min(v0 + key, to - 1), c = unit(kv, key);
@@ -198,9 +214,11 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
                 }
             }
     };
-    auto landed = [&]() {
+    // All but the last LEFT of this wave's copies have landed and its LDS reads are done; then all waves'.
+    auto landed = [&](auto left) {
+        constexpr int LEFT = RAGGED ? 0 : decltype(left)::value;
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+        __builtin_amdgcn_s_waitcnt((LEFT & 15) | ((LEFT >> 4) << 14) | (7 << 4));  // vmcnt(LEFT) lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
@@ -212,18 +230,24 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
         const T *qp = (const T *)a.q.data_dev + b * a.q.batch_stride + (long long)t * a.q.t_stride + head * a.q.head_stride;
         if constexpr (F32) {
 #pragma unroll
-            for (int c = 0; c < 2 * QF; ++c) {
-                qx[c] = v4f{0, 0, 0, 0};
-                if (inside && 8 * c + 4 * h < a.d) qx[c] = *(const v4f *)(qp + 8 * c + 4 * h);
-                if (a.scale < 0) qx[c] = -qx[c];
-            }
+            for (int c = 0; c < 2 * QF; ++c) qx[c] = v4f{0, 0, 0, 0};
+            if (inside)
+#pragma unroll
+                for (int c = 0; c < 2 * QF; ++c)
+                    if (!RAGGED || 8 * c + 4 * h < a.d) qx[c] = *(const v4f *)(qp + 8 * c + 4 * h);
+            if (a.scale < 0)
+#pragma unroll
+                for (int c = 0; c < 2 * QF; ++c) qx[c] = -qx[c];
         } else {
 #pragma unroll
-            for (int c = 0; c < QF; ++c) {
-                qf[c] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
-                if (inside && 16 * c + 8 * h < a.d) qf[c] = *(const v8s *)(qp + 16 * c + 8 * h);
-                if (a.scale < 0) qf[c] ^= (short)0x8000;
-            }
+            for (int c = 0; c < QF; ++c) qf[c] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
+            if (inside)
+#pragma unroll
+                for (int c = 0; c < QF; ++c)
+                    if (!RAGGED || 16 * c + 8 * h < a.d) qf[c] = *(const v8s *)(qp + 16 * c + 8 * h);
+            if (a.scale < 0)
+#pragma unroll
+                for (int c = 0; c < QF; ++c) qf[c] ^= (short)0x8000;
         }
     }
     const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);  // (0 would make a masked score's -infinity NaN)
@@ -244,14 +268,15 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
         va = key * ROW + ((2 * (lane >> 4 & 1) + (lane & 3) / 2) ^ swizzle_v<F32, UNITS>(key)) * 16 + (lane & 1) * 8 + 32 * wk * ROW;
     }
 
-    auto work = [&](int v0, int buf) {
-        // a tile that none of the wave's rows sees (the whole of it lies outside their windows)
-        if (w0 > w1 || v0 > hi1 || (v0 + KT <= lo0 && v0 >= sinks)) return;
-        const char *const kt = lds + buf * S::BUF, *const vt = kt + KT * ROW;
-        asm volatile("" : "+v"(ka), "+v"(va));  // (the addresses made from them are made anew, not kept for every use)
+    // a tile that none of the wave's rows sees (the whole of it lies outside their windows)
+    auto unseen = [&](int v0) { return w0 > w1 || v0 > hi1 || (v0 + KT <= lo0 && v0 >= sinks); };
+    v16f s[NB];
+    auto scores = [&](int v0, int buf) {
+        if (unseen(v0)) return;
+        const char *const kt = lds + buf * S::BUF;
+        asm volatile("" : "+v"(ka));  // (the addresses made from it are made anew, not kept for every use; va likewise)
         // Operands are read a step ahead of the matrix instructions that take them, into one of two register sets.
         constexpr int KSTEPS = F32 ? 2 * QF : QF / 2;  // steps of eight elements (FP32) or 32
-        v16f s[NB];
 #pragma unroll
         for (int i = 0; i < NB; ++i) s[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
         v4f kx[2][NB][F32 ? 1 : 2];
@@ -279,6 +304,11 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    auto output = [&](int v0, int buf) {
+        if (unseen(v0)) return;
+        const char *const vt = lds + buf * S::BUF + KT * ROW;
+        asm volatile("" : "+v"(va));
         // V: steps of one key of each half (FP32) or 16 keys, the first read while the softmax runs
         constexpr int VSTEPS = NB * (F32 ? 16 : 2);
         float vx[2][F32 ? DB : 1];
@@ -330,11 +360,13 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
         top = other_half_max(top) * scale;
         if (__any(top > m + kLazy)) {
             const float next = fmaxf(m, top);
-            const float by = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
-            m = next;
-            l *= by;
+            if (__any(m != -INFINITY)) {  // (nothing is there to rescale at first)
+                const float by = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+                l *= by;
 #pragma unroll
-            for (int d = 0; d < DB; ++d) o[d] *= by;
+                for (int d = 0; d < DB; ++d) o[d] *= by;
+            }
+            m = next;
         }
         const float ref = (m == -INFINITY ? 0.0f : m) + (careful ? kDown : 0.0f);
         float sum = 0.0f;
@@ -400,105 +432,140 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
         __syncthreads();
     };
 
+    constexpr int PER = WK > 1 ? 32 * (DP / 4) / NT : 1;  // units of four outputs that each thread joins
+    const int rows = min(32 * WQ, a.rows - r0);
+    v4f joined[PER];
+    float2 refs[PER];
     for (int round = 0; round < 2; ++round) {
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
         m = -INFINITY;
         l = 0.0f;
-        if (tiles) stage(from, 0);
-        for (int i = 0; i < tiles; ++i) {
-            const int v0 = from + i * KT, buf = a.buffers == 2 ? i & 1 : 0;
-            landed();
-            if (careful) take_out(buf);
-            if (a.buffers == 2 && i + 1 < tiles) stage(v0 + KT, buf ^ 1);
-            work(v0, buf);
-            if (a.buffers == 1 && i + 1 < tiles) {
-                landed();  // (this wave's reads; then all waves')
-                stage(v0 + KT, 0);
+        if (tiles) stage(from, 0, true, true);
+        if constexpr (S::BUFFERS == 2) {
+            for (int i = 0; i < tiles; ++i) {
+                const int v0 = from + i * KT, buf = i & 1;
+                landed(Count<0>());
+                if (careful) take_out(buf);
+                if (i + 1 < tiles) stage(v0 + KT, buf ^ 1, true, true);
+                scores(v0, buf);
+                output(v0, buf);
+            }
+        } else {
+            // one buffer of K and one of V: a tile's V is on its way during its scores, the next tile's K during its outputs
+            for (int i = 0; i < tiles; ++i) {
+                const int v0 = from + i * KT;
+                if (i == 0) landed(Count<COPIES>());
+                else landed(Count<0>());
+                if (i) stage(v0, 0, false, true);
+                scores(v0, 0);
+                landed(Count<0>());
+                if (i + 1 < tiles) stage(v0 + KT, 0, true, false);
+                if (careful) take_out(0);
+                output(v0, 0);
             }
         }
+        l = both_halves(l);
+        if (careful) m += kDown;  // what the weights and sums refer to
         bool bad = false;
+        if constexpr (WK == 1) {
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-            float z = 0.0f;  // (an infinity or NaN times 0 is NaN)
+            for (int d = 0; d < DB; ++d) {
+                float z = 0.0f;  // (an infinity or NaN times 0 is NaN)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) z = __builtin_fmaf(o[d][e], 0.0f, z);
-            bad |= z != z;
+                for (int e = 0; e < 16; ++e) z = __builtin_fmaf(o[d][e], 0.0f, z);
+                bad |= z != z;
+            }
+        } else {
+            // the waves' parts of each row meet in LDS: [wave][32][DP] outputs, then [wave][32][2] maxima and sums
+            float *const po = (float *)lds, *const ps = po + S::NW * 32 * DP;
+            __syncthreads();
+            if (n < rows) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        // (units of four elements, swizzled by the row: 32 rows are written at once)
+                        const int c = 8 * d + e / 2 + h;
+                        *(v4f *)(po + ((wave * 32 + n) * (DP / 4) + (c ^ (n & 7))) * 4) = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+                    }
+                if (h == 0) *(float2 *)(ps + 2 * (wave * 32 + n)) = make_float2(m, l);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < PER; ++u) {
+                if (u * NT >= rows * (DP / 4)) break;
+                const int at = u * NT + tid, r = min(at / (DP / 4), rows - 1), c = at % (DP / 4);
+                float2 part[WK];
+                float top = -INFINITY, all = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WK; ++w) {
+                    part[w] = *(const float2 *)(ps + 2 * (w * 32 + r));
+                    top = fmaxf(top, part[w].x);
+                }
+                v4f v = {0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < WK; ++w) {
+                    const float by = part[w].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part[w].x - top - kRoom);
+                    all += part[w].y * by;
+                    if (by != 0.0f) v += *(const v4f *)(po + ((w * 32 + r) * (DP / 4) + (c ^ (r & 7))) * 4) * by;
+                }
+                joined[u] = v;
+                refs[u] = make_float2(top + kRoom, all);
+                bad |= !finite(v[0]) || !finite(v[1]) || !finite(v[2]) || !finite(v[3]);
+            }
         }
         if (careful || !__syncthreads_or(bad)) break;
         careful = true;
     }
 
-    l = both_halves(l);
-    if (careful) m += kDown;  // what the weights and sums refer to
-    T *const out = (T *)a.out.data_dev + b * a.out.batch_stride + (long long)t * a.out.t_stride + head * a.out.head_stride;
+    const long long slot0 = (((long long)split * a.batch + b) * a.kv_heads + hk) * a.rows;
+    T *const out = (T *)a.out.data_dev + b * a.out.batch_stride;
     if constexpr (WK == 1) {
         if (!real) return;
         if (a.splits > 1) {
-            const long long at = ((long long)split * (gridDim.x / a.row_tiles / a.splits) + bh) * a.rows + row;
-            float *const part = a.part + at * a.d;
+            float *const part = a.part + (slot0 + row) * a.d;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int e = 0; e < 16; e += 4)
-                    if (32 * d + 2 * e + 4 * h < a.d) *(v4f *)(part + 32 * d + 2 * e + 4 * h) = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
-            if (h == 0) a.stats[2 * at] = m, a.stats[2 * at + 1] = l;
+                    if (!RAGGED || 32 * d + 2 * e + 4 * h < a.d) *(v4f *)(part + 32 * d + 2 * e + 4 * h) = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+            if (h == 0) *(float2 *)(a.stats + 2 * (slot0 + row)) = make_float2(m, l);
             return;
         }
-        const float by = inside && l != 0.0f ? 1.0f / l : 0.0f;
+        T *const y = out + (long long)t * a.out.t_stride + head * a.out.head_stride + 4 * h;
+        const float by = l != 0.0f ? 1.0f / l : 0.0f;
+        const bool some = inside && l != 0.0f;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
-                const int at = 32 * d + 2 * e + 4 * h;
-                if (at >= a.d) continue;
+                if (RAGGED && 32 * d + 2 * e + 4 * h >= a.d) continue;
                 T v[4];
 #pragma unroll
-                for (int y = 0; y < 4; ++y) v[y] = (T)(by == 0.0f ? 0.0f : o[d][e + y] * by);
-                if constexpr (F32) *(v4f *)(out + at) = *(const v4f *)v;
-                else *(v4s *)(out + at) = *(const v4s *)v;
+                for (int z = 0; z < 4; ++z) v[z] = (T)(some ? o[d][e + z] * by : 0.0f);
+                if constexpr (F32) *(v4f *)(y + 32 * d + 2 * e) = *(const v4f *)v;
+                else *(v4s *)(y + 32 * d + 2 * e) = *(const v4s *)v;
             }
     } else {
-        // the waves' parts of each row meet in LDS: [wave][32][DP] outputs, then [wave][32][2] maxima and sums
         static_assert(WQ == 1, "one group of rows");
-        float *const po = (float *)lds, *const ps = po + S::NW * 32 * DP;
-        __syncthreads();
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                // (units of four elements, swizzled by the row: 32 rows are written at once)
-                const int c = 8 * d + e / 2 + h;
-                *(v4f *)(po + ((wave * 32 + n) * (DP / 4) + (c ^ (n & 7))) * 4) = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
-            }
-        if (h == 0) ps[2 * (wave * 32 + n)] = m, ps[2 * (wave * 32 + n) + 1] = l;
-        __syncthreads();
-        const int rows = min(32, a.rows - r0);
-        for (int at = tid; at < rows * (DP / 4); at += NT) {
-            const int r = at / (DP / 4), c = at % (DP / 4);
-            if (4 * c >= a.d) continue;
-            float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WK; ++w) top = fmaxf(top, ps[2 * (w * 32 + r)]);
-            v4f v = {0, 0, 0, 0};
-#pragma unroll
-            for (int w = 0; w < WK; ++w) {
-                const float mw = ps[2 * (w * 32 + r)], by = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - top - kRoom);
-                sum += ps[2 * (w * 32 + r) + 1] * by;
-                if (by != 0.0f) v += *(const v4f *)(po + ((w * 32 + r) * (DP / 4) + (c ^ (r & 7))) * 4) * by;
-            }
-            const int rr = r0 + r, tt = rr / a.group, pp = start + tt;
+        for (int u = 0; u < PER; ++u) {
+            const int at = u * NT + tid, r = at / (DP / 4), c = at % (DP / 4);
+            if (r >= rows || (RAGGED && 4 * c >= a.d)) break;
+            const int rr = r0 + r;
             if (a.splits > 1) {
-                const long long slot = ((long long)split * (gridDim.x / a.row_tiles / a.splits) + bh) * a.rows + rr;
-                *(v4f *)(a.part + slot * a.d + 4 * c) = v;
-                if (c == 0) a.stats[2 * slot] = top + kRoom, a.stats[2 * slot + 1] = sum;
+                *(v4f *)(a.part + (slot0 + rr) * a.d + 4 * c) = joined[u];
+                if (c == 0) *(float2 *)(a.stats + 2 * (slot0 + rr)) = refs[u];
                 continue;
             }
-            const float by = pp >= 0 && pp < len && sum != 0.0f ? 1.0f / sum : 0.0f;
-            T *const y = (T *)a.out.data_dev + b * a.out.batch_stride + (long long)tt * a.out.t_stride + (hk * a.group + rr % a.group) * a.out.head_stride + 4 * c;
+            const int tt = a.token(rr), pp = start + tt;
+            const bool some = pp >= 0 && pp < len && refs[u].y != 0.0f;
+            const float by = some ? 1.0f / refs[u].y : 0.0f;
+            T *const y = out + (long long)tt * a.out.t_stride + (hk * a.group + rr - tt * a.group) * a.out.head_stride + 4 * c;
             T res[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) res[e] = (T)(by == 0.0f ? 0.0f : v[e] * by);
+            for (int e = 0; e < 4; ++e) res[e] = (T)(some ? joined[u][e] * by : 0.0f);
             if constexpr (F32) *(v4f *)y = *(const v4f *)res;
             else *(v4s *)y = *(const v4s *)res;
         }
@@ -507,11 +574,10 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
 
 // Joins the splits: out = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m), four elements a thread, eight splits at a time.
 template <typename T>
-__global__ void __launch_bounds__(64) join_kernel(Args a, int units) {
-    const int at = blockIdx.x * 64 + threadIdx.x;
-    if (at >= units) return;
-    const int per = a.d / 4, c = at % per, row = at / per, all = a.batch * a.kv_heads * a.rows;  // row: of all
-    const int bh = row / a.rows, r = row % a.rows, t = r / a.group, b = bh / a.kv_heads, hk = bh % a.kv_heads;
+__global__ void __launch_bounds__(64) join_kernel(Args a) {
+    const int at = blockIdx.x * 64 + threadIdx.x, per = a.d / 4, r = at / per, c = at - r * per, hk = blockIdx.y, b = blockIdx.z;
+    if (r >= a.rows) return;
+    const int row = (b * a.kv_heads + hk) * a.rows + r, all = a.batch * a.kv_heads * a.rows, t = a.token(r);
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.tk) : a.tk;
     const int p = (a.starts ? min(max(a.starts[b], -(1 << 30)), 1 << 30) : len - a.tq) + t;
     float m = -INFINITY, sum = 0.0f;
@@ -544,7 +610,7 @@ __global__ void __launch_bounds__(64) join_kernel(Args a, int units) {
     T res[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) res[e] = (T)(by == 0.0f ? 0.0f : v[e] * by);
-    T *const y = (T *)a.out.data_dev + b * a.out.batch_stride + (long long)t * a.out.t_stride + (hk * a.group + r % a.group) * a.out.head_stride + 4 * c;
+    T *const y = (T *)a.out.data_dev + b * a.out.batch_stride + (long long)t * a.out.t_stride + (hk * a.group + r - t * a.group) * a.out.head_stride + 4 * c;
     if constexpr (sizeof(T) == 4) *(v4f *)y = *(const v4f *)res;
     else *(v4s *)y = *(const v4s *)res;
 }
@@ -553,7 +619,7 @@ __global__ void __launch_bounds__(64) join_kernel(Args a, int units) {
 
 struct Plan {
     bool few;            // waves share out the keys of 32 rows, not the rows
-    int dp, row_tiles, splits;
+    int dp, row_tiles, tiles8, splits;
     int64_t rows, part_bytes, stats_bytes;
 };
 
@@ -563,10 +629,11 @@ int plan_of(int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int
     p.dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
     p.rows = tq * (heads / kv_heads);
     const int64_t groups = batch * kv_heads;
-    if (p.rows > INT32_MAX / 2 || groups > INT32_MAX / 2) return -1;
+    if (p.rows > INT32_MAX / 8 || batch > 65535) return -1;
     p.few = p.rows <= 64 || (p.rows + 127) / 128 * groups < 256;
     const int64_t per = p.few ? 32 : 128;
     p.row_tiles = (int)((p.rows + per - 1) / per);
+    p.tiles8 = p.row_tiles < 8 ? p.row_tiles : (p.row_tiles + 7) / 8 * 8;
     const int64_t wgs = p.row_tiles * groups;
     // the keys that a tile of rows can meet
     const int64_t most = 1 << 30, span = per / (heads / kv_heads) + 2;
@@ -594,42 +661,42 @@ int launched() {
 }
 
 template <typename T, int DP, int WQ, int WK, bool RAGGED>
-int run_shape(Args a, int64_t groups, hipStream_t stream) {
+int run_shape(const Args &a, hipStream_t stream) {
     using S = Shape<T, DP, WQ, WK>;
-    static_assert(S::lds(S::BUFFERS) <= 160 * 1024 && S::KT * S::UNITS % S::NT == 0 && S::KB <= 16, "tiles and flags");
-    const int64_t blocks = groups * a.row_tiles * a.splits;
-    if (blocks > INT32_MAX / 2 || !kea::fits_dispatch(blocks, S::NT)) return kea::fail(KEA_EINVAL, "kea_window_attention: too large for one launch");
+    static_assert(S::LDS <= 160 * 1024 && S::KT * S::UNITS % S::NT == 0 && S::KB <= 16, "tiles and flags");
+    const int64_t along = (int64_t)a.tiles8 * a.splits;
+    if (along > INT32_MAX || !kea::fits_dispatch(along, S::NT) || !kea::fits_dispatch(a.rows * (a.d / 4) / 64 + 1, 64))
+        return kea::fail(KEA_EINVAL, "kea_window_attention: too large for one launch");
+    const dim3 grid((unsigned)along, (unsigned)a.kv_heads, (unsigned)a.batch);
     const auto kernel = window_kernel<T, DP, WQ, WK, RAGGED>;
-    a.buffers = S::BUFFERS;
-    const int lds = S::lds(a.buffers);
+    const int lds = S::LDS;
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return kea::fail((int)e, std::string("kea_window_attention: ") + hipGetErrorString(e));
     }
-    kernel<<<dim3((unsigned)blocks), S::NT, lds, stream>>>(a);
+    kernel<<<grid, S::NT, lds, stream>>>(a);
     const int rc = launched();
     if (rc || a.splits == 1) return rc;
-    const int64_t units = groups * a.rows * (a.d / 4);  // (fewer than 2^23: splits > 1 only for few rows)
-    join_kernel<T><<<dim3((unsigned)((units + 63) / 64)), 64, 0, stream>>>(a, (int)units);
+    join_kernel<T><<<dim3((unsigned)((a.rows * (a.d / 4) + 63) / 64), grid.y, grid.z), 64, 0, stream>>>(a);
     return launched();
 }
 
 template <typename T, int DP>
-int run_heads(const Args &a, bool few, int64_t groups, hipStream_t stream) {
+int run_heads(const Args &a, bool few, hipStream_t stream) {
     // waves that share out keys: four of them where two buffers of their blocks fit LDS
     constexpr int WK = 2 * 2 * 4 * 32 * DP * (int)sizeof(T) <= 131072 ? 4 : 2 * 2 * 2 * 32 * DP * (int)sizeof(T) <= 131072 ? 2 : 1;
-    if (a.d == DP) return few ? run_shape<T, DP, 1, WK, false>(a, groups, stream) : run_shape<T, DP, 4, 1, false>(a, groups, stream);
-    return few ? run_shape<T, DP, 1, WK, true>(a, groups, stream) : run_shape<T, DP, 4, 1, true>(a, groups, stream);
+    if (a.d == DP) return few ? run_shape<T, DP, 1, WK, false>(a, stream) : run_shape<T, DP, 4, 1, false>(a, stream);
+    return few ? run_shape<T, DP, 1, WK, true>(a, stream) : run_shape<T, DP, 4, 1, true>(a, stream);
 }
 
 template <typename T>
-int run_type(const Args &a, const Plan &p, int64_t groups, hipStream_t stream) {
-    return p.dp == 64 ? run_heads<T, 64>(a, p.few, groups, stream) : p.dp == 128 ? run_heads<T, 128>(a, p.few, groups, stream)
-                                                                                 : run_heads<T, 256>(a, p.few, groups, stream);
+int run_type(const Args &a, const Plan &p, hipStream_t stream) {
+    return p.dp == 64 ? run_heads<T, 64>(a, p.few, stream) : p.dp == 128 ? run_heads<T, 128>(a, p.few, stream)
+                                                                                 : run_heads<T, 256>(a, p.few, stream);
 }
 
 bool heads_ok(const kea_heads *t, int64_t unit) {
-    return t && (uintptr_t)t->data_dev % 16 == 0 && t->batch_stride % unit == 0 && t->t_stride % unit == 0 && t->head_stride % unit == 0;
+    return t && t->batch_stride >= 0 && t->t_stride >= 0 && t->head_stride >= 0 && (uintptr_t)t->data_dev % 16 == 0 && t->batch_stride % unit == 0 && t->t_stride % unit == 0 && t->head_stride % unit == 0;
 }
 
 int check_sizes(const char *what, int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads, int64_t d,
@@ -663,18 +730,20 @@ int kea_window_attention(const kea_heads *q, const kea_heads *k, const kea_heads
     if (rc) return rc;
     const int64_t unit = dtype == KEA_F32 ? 4 : 8;
     if (!heads_ok(q, unit) || !heads_ok(k, unit) || !heads_ok(v, unit) || !heads_ok(out, unit) || (uintptr_t)kv_lengths % 4 || (uintptr_t)q_starts % 4)
-        return kea::fail(KEA_EALIGN, "kea_window_attention: pointers and strides are multiples of 16 bytes");
+        return kea::fail(KEA_EALIGN, "kea_window_attention: pointers and strides are multiples of 16 bytes, strides not negative");
     if (batch == 0 || tq == 0) return KEA_OK;
     if (!q->data_dev || !out->data_dev || (tk > 0 && (!k->data_dev || !v->data_dev))) return kea::fail(KEA_EINVAL, "kea_window_attention: a pointer is missing");
     if (workspace_bytes < p.part_bytes + p.stats_bytes || (p.splits > 1 && !workspace)) return kea::fail(KEA_ESPACE, "kea_window_attention: the workspace is too small");
     if ((uintptr_t)workspace % 16) return kea::fail(KEA_EALIGN, "kea_window_attention: the workspace is aligned to 16 bytes");
     const int64_t most = 1 << 30;
+    uint32_t shift = 0;
+    while ((1 << shift) < heads / kv_heads) ++shift;
+    const uint32_t mul = (uint32_t)((1ULL << (31 + shift)) / (uint64_t)(heads / kv_heads) + 1);
     const Args a{*q, *k, *v, *out, kv_lengths, q_starts, (float *)workspace, workspace ? (float *)((char *)workspace + p.part_bytes) : nullptr,
                  (int)batch, (int)tq, (int)tk, (int)kv_heads, (int)(heads / kv_heads), (int)d, (int)(left < most ? left : most),
-                 (int)(right < most ? right : most), (int)(sinks < most ? sinks : most), (int)p.rows, p.row_tiles, p.splits, 1, scale};
-    const int64_t groups = batch * kv_heads;
+                 (int)(right < most ? right : most), (int)(sinks < most ? sinks : most), (int)p.rows, p.row_tiles, p.tiles8, p.splits, mul, shift, scale};
     const hipStream_t s = (hipStream_t)stream;
-    return dtype == KEA_F32 ? run_type<float>(a, p, groups, s) : dtype == KEA_F16 ? run_type<_Float16>(a, p, groups, s) : run_type<__bf16>(a, p, groups, s);
+    return dtype == KEA_F32 ? run_type<float>(a, p, s) : dtype == KEA_F16 ? run_type<_Float16>(a, p, s) : run_type<__bf16>(a, p, s);
 }
 
 }  // extern "C"
