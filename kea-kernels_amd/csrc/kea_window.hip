@@ -110,7 +110,9 @@ __device__ __forceinline__ void copy16(const void *src, uint32_t base) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(src) : "memory");
 }
 __device__ __forceinline__ void copy16(const void *src, uint32_t offset, uint32_t base) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(offset), "s"(src) : "memory");
+    const uint64_t at = (uint64_t)(uintptr_t)src;
+    const uint64_t uniform = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(offset), "s"(uniform) : "memory");
 }
 
 template <typename T>
@@ -144,8 +146,9 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
     const int tile = a.tiles8 == a.row_tiles && a.tiles8 < 8 ? x : x % 8 * (a.tiles8 / 8) + x / 8;
     if (tile >= a.row_tiles) return;
     const int hk = blockIdx.y, b = blockIdx.z;
-    const int len = a.lengths ? min(max(a.lengths[b], 0), a.tk) : a.tk;
-    const int start = a.starts ? min(max(a.starts[b], -(1 << 30)), 1 << 30) : len - a.tq;
+    // (uniform, which the compiler does not see of loaded values)
+    const int len = __builtin_amdgcn_readfirstlane(a.lengths ? min(max(a.lengths[b], 0), a.tk) : a.tk);
+    const int start = __builtin_amdgcn_readfirstlane(a.starts ? min(max(a.starts[b], -(1 << 30)), 1 << 30) : len - a.tq);
 
     // this lane's query
     const int r0 = tile * 32 * WQ, row = r0 + 32 * wq + n;
@@ -183,36 +186,51 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
     const int key0 = tid / UNITS;
     auto unit = [&](int kv, int key) { return (tid % UNITS ^ (kv ? swizzle_v<F32, UNITS>(key) : swizzle_k<F32, UNITS>(key))) * EPU; };
     // a tile of neighbouring keys is copied from a uniform address, each thread's rows at 32-bit offsets from it, where those
-    // suffice (of 16-bit types and the copies' rows a multiple of 16 apart: others have more swizzles)
-    constexpr bool NEAR = !RAGGED && STEP % 16 == 0;
+    // suffice: as many offsets as the swizzle has values over the thread's rows
+    constexpr int PERIOD = F32 ? 8 : 16, OFFSETS = STEP < PERIOD ? PERIOD / STEP : 1;
+    constexpr bool NEAR = !RAGGED && OFFSETS <= 4;
     const bool near_k = (long long)KT * a.k.t_stride < 1 << 29, near_v = (long long)KT * a.v.t_stride < 1 << 29;
-    const uint32_t off_k = ((uint32_t)(key0 * (int)a.k.t_stride) + unit(0, key0)) * (uint32_t)sizeof(T);
-    const uint32_t off_v = ((uint32_t)(key0 * (int)a.v.t_stride) + unit(1, key0)) * (uint32_t)sizeof(T);
+    uint32_t off_k[OFFSETS], off_v[OFFSETS];
+#pragma unroll
+    for (int u = 0; u < OFFSETS; ++u) {
+        off_k[u] = ((uint32_t)(key0 * (int)a.k.t_stride) + unit(0, key0 + u * STEP)) * (uint32_t)sizeof(T);
+        off_v[u] = ((uint32_t)(key0 * (int)a.v.t_stride) + unit(1, key0 + u * STEP)) * (uint32_t)sizeof(T);
+    }
     auto stage = [&](int v0, int buf, bool of_k, bool of_v) {
-        char *const dst = lds + buf * S::BUF + wave * 1024;
-        if (NEAR && near_k && near_v && v0 >= first && v0 + KT <= to) {
-            const T *k0 = kp + (long long)(v0 + shift) * a.k.t_stride, *w0 = vp + (long long)(v0 + shift) * a.v.t_stride;
-            if (of_k)
+        // (made anew on every call: kept for all copies of a tile, the addresses would not fit the registers)
+        uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)lds + buf * S::BUF + wave * 1024);
+        int v1 = __builtin_amdgcn_readfirstlane(v0);
+        asm volatile("" : "+s"(dst), "+s"(v1));
+        if (NEAR && near_k && near_v && v1 >= first && v1 + KT <= to) {
+            auto copy = [&](const T *from, long long stride, const uint32_t (&offset)[OFFSETS], uint32_t at) {
+                from += (long long)(v1 + shift) * stride;
 #pragma unroll
-                for (int u = 0; u < COPIES; ++u) copy16(k0 + u * (STEP * a.k.t_stride), off_k, (uint32_t)(uintptr_t)(lptr_t)(dst + u * NT * 16));
-            if (of_v)
-#pragma unroll
-                for (int u = 0; u < COPIES; ++u) copy16(w0 + u * (STEP * a.v.t_stride), off_v, (uint32_t)(uintptr_t)(lptr_t)(dst + (KT * ROW + u * NT * 16)));
+                for (int u = 0; u < COPIES; ++u) {
+                    copy16(from, offset[u % OFFSETS], at);
+                    from += STEP * stride;
+                    at += NT * 16;
+                }
+            };
+            if (of_k) copy(kp, a.k.t_stride, off_k, dst);
+            if (of_v) copy(vp, a.v.t_stride, off_v, dst + KT * ROW);
             return;
         }
-        for (int kv = of_k ? 0 : 1; kv < (of_v ? 2 : 1); ++kv)
+        auto copy = [&](const T *from, long long stride, int kv, uint32_t at) {
 #pragma unroll
             for (int u = 0; u < COPIES; ++u) {
-                const int key = key0 + u * STEP, v = min(v0 + key, to - 1), c = unit(kv, key);
-                const T *src = (kv ? vp : kp) + (long long)(v + (v >= first ? shift : 0)) * (kv ? a.v.t_stride : a.k.t_stride) + c;
-                char *const to_lds = dst + kv * KT * ROW + u * NT * 16;
+                const int key = key0 + u * STEP, v = min(v1 + key, to - 1), c = unit(kv, key);
+                const T *src = from + (long long)(v + (v >= first ? shift : 0)) * stride + c;
                 if constexpr (RAGGED) {
                     const v4f zero = {0, 0, 0, 0};
-                    *(v4f *)(to_lds + lane * 16) = c < a.d ? *(const v4f *)src : zero;
+                    *(v4f *)(lds + buf * S::BUF + kv * KT * ROW + (u * NT + tid) * 16) = c < a.d ? *(const v4f *)src : zero;
                 } else {
-                    copy16(src, (uint32_t)(uintptr_t)(lptr_t)to_lds);
+                    copy16(src, at);
+                    at += NT * 16;
                 }
             }
+        };
+        if (of_k) copy(kp, a.k.t_stride, 0, dst);
+        if (of_v) copy(vp, a.v.t_stride, 1, dst + KT * ROW);
     };
     // All but the last LEFT of this wave's copies have landed and its LDS reads are done; then all waves'.
     auto landed = [&](auto left) {
@@ -492,27 +510,34 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
                 if (h == 0) *(float2 *)(ps + 2 * (wave * 32 + n)) = make_float2(m, l);
             }
             __syncthreads();
+            // (a wave that saw nothing of a row has zeros there and weighs nothing; rows past the last are the last again)
+            float2 part[PER][WK];
+            v4f share[PER][WK];
 #pragma unroll
             for (int u = 0; u < PER; ++u) {
-                if (u * NT >= rows * (DP / 4)) break;
                 const int at = u * NT + tid, r = min(at / (DP / 4), rows - 1), c = at % (DP / 4);
-                float2 part[WK];
-                float top = -INFINITY, all = 0.0f;
 #pragma unroll
                 for (int w = 0; w < WK; ++w) {
-                    part[w] = *(const float2 *)(ps + 2 * (w * 32 + r));
-                    top = fmaxf(top, part[w].x);
+                    part[u][w] = *(const float2 *)(ps + 2 * (w * 32 + r));
+                    share[u][w] = *(const v4f *)(po + ((w * 32 + r) * (DP / 4) + (c ^ (r & 7))) * 4);
                 }
+            }
+#pragma unroll
+            for (int u = 0; u < PER; ++u) {
+                float top = part[u][0].x, all = 0.0f;
+#pragma unroll
+                for (int w = 1; w < WK; ++w) top = fmaxf(top, part[u][w].x);
                 v4f v = {0, 0, 0, 0};
 #pragma unroll
                 for (int w = 0; w < WK; ++w) {
-                    const float by = part[w].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part[w].x - top - kRoom);
-                    all += part[w].y * by;
-                    if (by != 0.0f) v += *(const v4f *)(po + ((w * 32 + r) * (DP / 4) + (c ^ (r & 7))) * 4) * by;
+                    const float by = part[u][w].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part[u][w].x - top - kRoom);
+                    all += part[u][w].y * by;
+                    v += share[u][w] * by;
                 }
                 joined[u] = v;
                 refs[u] = make_float2(top + kRoom, all);
-                bad |= !finite(v[0]) || !finite(v[1]) || !finite(v[2]) || !finite(v[3]);
+                const float z = (v[0] + v[1] + (v[2] + v[3])) * 0.0f;  // (an infinity or NaN times 0 is NaN)
+                bad |= z != z;
             }
         }
         if (careful || !__syncthreads_or(bad)) break;
@@ -549,20 +574,24 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
             }
     } else {
         static_assert(WQ == 1, "one group of rows");
+        if (a.splits > 1) {
+#pragma unroll
+            for (int u = 0; u < PER; ++u) {
+                const int at = u * NT + tid, r = at / (DP / 4), c = at % (DP / 4);
+                if (r >= rows || (RAGGED && 4 * c >= a.d)) continue;
+                *(v4f *)(a.part + (slot0 + r0 + r) * a.d + 4 * c) = joined[u];
+                if (c == 0) *(float2 *)(a.stats + 2 * (slot0 + r0 + r)) = refs[u];
+            }
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < PER; ++u) {
             const int at = u * NT + tid, r = at / (DP / 4), c = at % (DP / 4);
-            if (r >= rows || (RAGGED && 4 * c >= a.d)) break;
-            const int rr = r0 + r;
-            if (a.splits > 1) {
-                *(v4f *)(a.part + (slot0 + rr) * a.d + 4 * c) = joined[u];
-                if (c == 0) *(float2 *)(a.stats + 2 * (slot0 + rr)) = refs[u];
-                continue;
-            }
-            const int tt = a.token(rr), pp = start + tt;
+            if (r >= rows || (RAGGED && 4 * c >= a.d)) continue;
+            const int tt = a.token(r0 + r), pp = start + tt;
             const bool some = pp >= 0 && pp < len && refs[u].y != 0.0f;
-            const float by = some ? 1.0f / refs[u].y : 0.0f;
-            T *const y = out + (long long)tt * a.out.t_stride + (hk * a.group + rr - tt * a.group) * a.out.head_stride + 4 * c;
+            const float by = 1.0f / refs[u].y;
+            T *const y = out + (long long)tt * a.out.t_stride + (hk * a.group + r0 + r - tt * a.group) * a.out.head_stride + 4 * c;
             T res[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) res[e] = (T)(some ? joined[u][e] * by : 0.0f);
@@ -642,8 +671,8 @@ int plan_of(int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int
     const int64_t tile = dtype == KEA_F32 ? (p.dp == 64 ? 128 : p.dp == 128 ? 64 : 32) : p.dp == 256 ? 64 : 128;
     const int64_t blocks = (keys + tile - 1) / tile;
     p.splits = 1;
-    if (wgs > 0 && wgs < 256 && blocks > 1) {  // up to two workgroups a CU, a tile of keys each at least
-        int64_t s = 512 / wgs;
+    if (wgs > 0 && wgs < 256 && blocks > 3) {  // (the second launch takes as long as two or three tiles)
+        int64_t s = 512 / wgs;  // up to two workgroups a CU
         s = s < blocks ? s : blocks;
         p.splits = (int)(s < 64 ? s : 64);
     }
