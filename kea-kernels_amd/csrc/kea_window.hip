@@ -47,12 +47,15 @@ struct Args {
     const int32_t *lengths, *starts;
     float *part, *stats;  // splits > 1: [splits][sequences and key heads][rows][d], [..][rows][2]
     int batch, tq, tk, kv_heads, group, d, left, right, sinks;
-    int rows, row_tiles, tiles8, splits;
-    uint32_t group_mul, group_shift;
+    int rows, row_tiles, splits;
+    int by_group;  // the grid is [sequences and key heads][tiles][splits], or [tiles][sequences and key heads][splits]
+    uint32_t group_mul, group_shift, heads_mul, heads_shift;
     float scale;
 
-    // row / group, for rows below 2^31: group_mul = 2^(31 + s) / group + 1 with 2^s >= group
+    // row / group and (sequence and key head) / kv_heads, for numbers below 2^31: mul = 2^(31 + s) / divisor + 1 with
+    // 2^s >= divisor
     __device__ __forceinline__ int token(int row) const { return (int)(__umulhi(2u * (uint32_t)row, group_mul) >> group_shift); }
+    __device__ __forceinline__ int sequence(int bh) const { return (int)(__umulhi(2u * (uint32_t)bh, heads_mul) >> heads_shift); }
 };
 
 template <int N>
@@ -140,12 +143,18 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5, wq = wave / WK, wk = wave % WK;
 
-    // Workgroups go to the eight XCDs in turn: where there are eight tiles of rows or more, each XCD takes a run of its own,
-    // so that neighbours share keys in its L2. (Of the last up to seven workgroups some have no tile.)
-    const int split = a.splits > 1 ? (int)blockIdx.x / a.tiles8 : 0, x = (int)blockIdx.x - split * a.tiles8;
-    const int tile = a.tiles8 == a.row_tiles && a.tiles8 < 8 ? x : x % 8 * (a.tiles8 / 8) + x / 8;
-    if (tile >= a.row_tiles) return;
-    const int hk = blockIdx.y, b = blockIdx.z;
+    // Workgroups go to the eight XCDs in turn, and the first grid dimension is a multiple of eight (or alone on its row): with
+    // eight sequences and key heads or more, one XCD takes all tiles of each of them; otherwise runs of neighbouring tiles.
+    // Either way what shares keys shares an L2. (Of the last up to seven workgroups of a row some have nothing to do.)
+    int tile, bh;
+    if (a.by_group) {
+        bh = blockIdx.x, tile = blockIdx.y;
+    } else {
+        const int x = blockIdx.x, run = (int)gridDim.x / 8;
+        bh = blockIdx.y, tile = run ? x % 8 * run + x / 8 : x;
+    }
+    if (bh >= a.batch * a.kv_heads || tile >= a.row_tiles) return;
+    const int split = blockIdx.z, b = a.sequence(bh), hk = bh - b * a.kv_heads;
     // (uniform, which the compiler does not see of loaded values)
     const int len = __builtin_amdgcn_readfirstlane(a.lengths ? min(max(a.lengths[b], 0), a.tk) : a.tk);
     const int start = __builtin_amdgcn_readfirstlane(a.starts ? min(max(a.starts[b], -(1 << 30)), 1 << 30) : len - a.tq);
@@ -544,7 +553,7 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
         careful = true;
     }
 
-    const long long slot0 = (((long long)split * a.batch + b) * a.kv_heads + hk) * a.rows;
+    const long long slot0 = ((long long)split * a.batch * a.kv_heads + bh) * a.rows;
     T *const out = (T *)a.out.data_dev + b * a.out.batch_stride;
     if constexpr (WK == 1) {
         if (!real) return;
@@ -604,9 +613,9 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
 // Joins the splits: out = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m), four elements a thread, eight splits at a time.
 template <typename T>
 __global__ void __launch_bounds__(64) join_kernel(Args a) {
-    const int at = blockIdx.x * 64 + threadIdx.x, per = a.d / 4, r = at / per, c = at - r * per, hk = blockIdx.y, b = blockIdx.z;
+    const int at = blockIdx.x * 64 + threadIdx.x, per = a.d / 4, r = at / per, c = at - r * per, bh = blockIdx.y, b = a.sequence(bh), hk = bh - b * a.kv_heads;
     if (r >= a.rows) return;
-    const int row = (b * a.kv_heads + hk) * a.rows + r, all = a.batch * a.kv_heads * a.rows, t = a.token(r);
+    const int row = bh * a.rows + r, all = a.batch * a.kv_heads * a.rows, t = a.token(r);
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.tk) : a.tk;
     const int p = (a.starts ? min(max(a.starts[b], -(1 << 30)), 1 << 30) : len - a.tq) + t;
     float m = -INFINITY, sum = 0.0f;
@@ -648,7 +657,7 @@ __global__ void __launch_bounds__(64) join_kernel(Args a) {
 
 struct Plan {
     bool few;            // waves share out the keys of 32 rows, not the rows
-    int dp, row_tiles, tiles8, splits;
+    int dp, row_tiles, splits;
     int64_t rows, part_bytes, stats_bytes;
 };
 
@@ -658,11 +667,10 @@ int plan_of(int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int
     p.dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
     p.rows = tq * (heads / kv_heads);
     const int64_t groups = batch * kv_heads;
-    if (p.rows > INT32_MAX / 8 || batch > 65535) return -1;
+    if (p.rows > INT32_MAX / 8 || groups > INT32_MAX / 8) return -1;
     p.few = p.rows <= 64 || (p.rows + 127) / 128 * groups < 256;
     const int64_t per = p.few ? 32 : 128;
     p.row_tiles = (int)((p.rows + per - 1) / per);
-    p.tiles8 = p.row_tiles < 8 ? p.row_tiles : (p.row_tiles + 7) / 8 * 8;
     const int64_t wgs = p.row_tiles * groups;
     // the keys that a tile of rows can meet
     const int64_t most = 1 << 30, span = per / (heads / kv_heads) + 2;
@@ -693,10 +701,10 @@ template <typename T, int DP, int WQ, int WK, bool RAGGED>
 int run_shape(const Args &a, hipStream_t stream) {
     using S = Shape<T, DP, WQ, WK>;
     static_assert(S::LDS <= 160 * 1024 && S::KT * S::UNITS % S::NT == 0 && S::KB <= 16, "tiles and flags");
-    const int64_t along = (int64_t)a.tiles8 * a.splits;
-    if (along > INT32_MAX || !kea::fits_dispatch(along, S::NT) || !kea::fits_dispatch(a.rows * (a.d / 4) / 64 + 1, 64))
+    const int64_t groups = (int64_t)a.batch * a.kv_heads, padded = a.by_group ? (groups + 7) / 8 * 8 : a.row_tiles < 8 ? a.row_tiles : (a.row_tiles + 7) / 8 * 8;
+    const dim3 grid((unsigned)padded, (unsigned)(a.by_group ? a.row_tiles : groups), (unsigned)a.splits);
+    if (!kea::fits_dispatch(padded, S::NT) || grid.y > 65535 || !kea::fits_dispatch((int64_t)a.rows * (a.d / 4) / 64 + 1, 64))
         return kea::fail(KEA_EINVAL, "kea_window_attention: too large for one launch");
-    const dim3 grid((unsigned)along, (unsigned)a.kv_heads, (unsigned)a.batch);
     const auto kernel = window_kernel<T, DP, WQ, WK, RAGGED>;
     const int lds = S::LDS;
     if (lds > 65536) {
@@ -706,7 +714,7 @@ int run_shape(const Args &a, hipStream_t stream) {
     kernel<<<grid, S::NT, lds, stream>>>(a);
     const int rc = launched();
     if (rc || a.splits == 1) return rc;
-    join_kernel<T><<<dim3((unsigned)((a.rows * (a.d / 4) + 63) / 64), grid.y, grid.z), 64, 0, stream>>>(a);
+    join_kernel<T><<<dim3((unsigned)((a.rows * (a.d / 4) + 63) / 64), (unsigned)groups), 64, 0, stream>>>(a);
     return launched();
 }
 
@@ -765,12 +773,18 @@ int kea_window_attention(const kea_heads *q, const kea_heads *k, const kea_heads
     if (workspace_bytes < p.part_bytes + p.stats_bytes || (p.splits > 1 && !workspace)) return kea::fail(KEA_ESPACE, "kea_window_attention: the workspace is too small");
     if ((uintptr_t)workspace % 16) return kea::fail(KEA_EALIGN, "kea_window_attention: the workspace is aligned to 16 bytes");
     const int64_t most = 1 << 30;
-    uint32_t shift = 0;
-    while ((1 << shift) < heads / kv_heads) ++shift;
-    const uint32_t mul = (uint32_t)((1ULL << (31 + shift)) / (uint64_t)(heads / kv_heads) + 1);
+    auto divide = [](uint64_t by, uint32_t *mul, uint32_t *shift) {
+        for (*shift = 0; (1ULL << *shift) < by;) ++*shift;
+        *mul = (uint32_t)((1ULL << (31 + *shift)) / by + 1);
+    };
+    uint32_t group_mul, group_shift, heads_mul, heads_shift;
+    divide((uint64_t)(heads / kv_heads), &group_mul, &group_shift);
+    divide((uint64_t)kv_heads, &heads_mul, &heads_shift);
+    const int by_group = batch * kv_heads >= 8 && p.row_tiles <= 65535;
     const Args a{*q, *k, *v, *out, kv_lengths, q_starts, (float *)workspace, workspace ? (float *)((char *)workspace + p.part_bytes) : nullptr,
                  (int)batch, (int)tq, (int)tk, (int)kv_heads, (int)(heads / kv_heads), (int)d, (int)(left < most ? left : most),
-                 (int)(right < most ? right : most), (int)(sinks < most ? sinks : most), (int)p.rows, p.row_tiles, p.tiles8, p.splits, mul, shift, scale};
+                 (int)(right < most ? right : most), (int)(sinks < most ? sinks : most), (int)p.rows, p.row_tiles, p.splits, by_group,
+                 group_mul, group_shift, heads_mul, heads_shift, scale};
     const hipStream_t s = (hipStream_t)stream;
     return dtype == KEA_F32 ? run_type<float>(a, p, s) : dtype == KEA_F16 ? run_type<_Float16>(a, p, s) : run_type<__bf16>(a, p, s);
 }
