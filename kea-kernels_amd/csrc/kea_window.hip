@@ -668,7 +668,10 @@ int plan_of(int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int
     p.rows = tq * (heads / kv_heads);
     const int64_t groups = batch * kv_heads;
     if (p.rows > INT32_MAX / 8 || groups > INT32_MAX / 8) return -1;
-    p.few = p.rows <= 64 || (p.rows + 127) / 128 * groups < 256;
+    // Tiles of 32 rows fill the chip with fewer queries, tiles of 128 read keys a quarter as often: BF16, 8 heads of 128, windows
+    // of 128 to both sides, 5 clips of 750 (960 workgroups of 32 rows) 25 against 30 us, 8 clips (1536) 38 against 24. FP32, whose
+    // matrix instructions take longer than the reads, 8 clips 103 against 117, 16 (3072) 183 and 183.
+    p.few = p.rows <= 64 || (p.rows + 31) / 32 * groups <= (dtype == KEA_F32 && p.dp > 64 ? 2560 : 1024);
     const int64_t per = p.few ? 32 : 128;
     p.row_tiles = (int)((p.rows + per - 1) / per);
     const int64_t wgs = p.row_tiles * groups;
