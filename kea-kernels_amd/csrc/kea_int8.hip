@@ -7,9 +7,14 @@
 //
 // Two kernels:
 //   tile_kernel   many output tiles: a workgroup owns BM x BN outputs; stages of 128 k of both operands stream into LDS by
-//                 direct copies, NS stages deep, and every byte is read by several waves.
+//                 direct copies, NS stages deep, and every byte is read by several waves. 16000 x 4096 x 4096 in 256 x 256
+//                 tiles takes 233 us, 2.3 POP/s of the 4.1 that the int8 matrix instruction reaches on such data (a library
+//                 product of that size 255): the matrix cores wait at the barrier of each stage, when all eight waves read
+//                 their next operands at once; reading one tile's operands for all tiles, out of L2, takes as long.
 //   split_kernel  few output tiles (few tokens): a workgroup owns 16 RM x 16 RN outputs, its NW waves share out k, each
-//                 loading its operands straight into registers, and the exact int32 sums meet in LDS.
+//                 loading its operands straight into registers, and the exact int32 sums meet in LDS. 1 x 2560 x 640 takes
+//                 2.9 us, of which an empty launch is 1.6; 16 x 1024 x 4096 5.7, at the rate at which 64 CUs take in the
+//                 128 KB each of them needs.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -225,6 +230,7 @@ __global__ void __launch_bounds__(WM *WN * 64) tile_kernel(Args p, int tiles_m, 
     }
     const int8_t *const q0 = p.q + (long long)m0 * p.ldq, *const w0 = p.w + (long long)n0 * p.ldw;
     const int last = (p.k - 1) & ~15, stages = (p.k + BK - 1) / BK;  // the last unit of a row
+    static_assert(BK == 128, "a stage is two steps of 64");
     auto copy = [&](int s, int buf) {
         // units past the row's end are read from its last one
         const int back_q = min(0, last - (s * BK + unit_q)), back_w = min(0, last - (s * BK + unit_w));
@@ -251,8 +257,6 @@ __global__ void __launch_bounds__(WM *WN * 64) tile_kernel(Args p, int tiles_m, 
         for (int b = 0; b < RN; ++b) acc[a][b] = v4i{0, 0, 0, 0};
 
     const int wrow = 8 * (i >> 2) + (i & 3);
-    constexpr int STEPS = BK / 64;
-    static_assert(STEPS == 1 || STEPS == 2, "operands alternate between two register sets");
     v4i qf[2][RM], wf[2][RN];
     auto fetch = [&](int buf, int h, int set) {
         const char *qa = lds + buf * STAGE + (wm * RM * 16 + i) * BK, *wa = lds + buf * STAGE + (BM + wn * RN * 16 + wrow) * BK;
@@ -268,27 +272,6 @@ __global__ void __launch_bounds__(WM *WN * 64) tile_kernel(Args p, int tiles_m, 
 #pragma unroll
             for (int b = 0; b < RN; ++b) acc[a][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[set][b], qf[set][a], acc[a][b], 0, 0, 0);
     };
-    int buf = 0;
-    // Stage s, whose first operands are in set 0 (or `set` where a stage is one step): the copies of stage s + NS - 1 go into
-    // the buffer that every wave finished before the last barrier (past the end the last stage again: every wave counts the
-    // same copies), and the operands of the next step are read while the matrix cores work on this one's.
-    auto step = [&](int s, int set) {
-        {
-            int next = buf + NS - 1;
-            next = next >= NS ? next - NS : next;
-            copy(min(s + NS - 1, stages - 1), next);
-        }
-        if constexpr (STEPS == 2) {
-            fetch(buf, 1, 1);
-            product(0);
-        }
-        buf = buf + 1 == NS ? 0 : buf + 1;
-        wait_copies<(NS - 2) * COPIES>();
-        barrier();
-        if (s + 2 == stages) clear_tail(s + 1, buf);
-        fetch(buf, 0, STEPS == 2 ? 0 : set ^ 1);
-        product(STEPS == 2 ? 1 : set);
-    };
     // scales and bias of the tile, on their way while the first copies are issued
     constexpr int LR = (BM + NT - 1) / NT, LC = (BN + NT - 1) / NT;
     uint32_t rs[LR], cs[LC], cb[LC];
@@ -299,8 +282,13 @@ __global__ void __launch_bounds__(WM *WN * 64) tile_kernel(Args p, int tiles_m, 
         cs[u] = scalar_word(p.ws, p.ws_dtype, min(n0 + tid + u * NT, p.n - 1));
         cb[u] = scalar_word(p.bias, p.bias_dtype, min(n0 + tid + u * NT, p.n - 1));
     }
+    // With two buffers a stage's copies start as soon as the waves have read what its buffer held, in the middle of a stage;
+    // with more there is time, and they start with the next stage, off the operands' way (NS = 2: 16000 x 4096 x 4096 250 -> 231
+    // us, NS = 4: 1000 x 1024 x 4096 11.2 -> 10.7).
+    constexpr bool MIDDLE = NS == 2;
+    constexpr int AHEAD = MIDDLE ? NS : NS - 1;
 #pragma unroll
-    for (int s = 0; s < NS - 1; ++s) copy(min(s, stages - 1), s);
+    for (int s = 0; s < AHEAD; ++s) copy(min(s, stages - 1), s);
 #pragma unroll
     for (int u = 0; u < LR; ++u)
         if (tid + u * NT < BM) row_scale[tid + u * NT] = scalar_value(rs[u], p.qs, p.qs_dtype, min(m0 + tid + u * NT, p.m - 1));
@@ -310,28 +298,29 @@ __global__ void __launch_bounds__(WM *WN * 64) tile_kernel(Args p, int tiles_m, 
             col_scale[tid + u * NT] = scalar_value(cs[u], p.ws, p.ws_dtype, min(n0 + tid + u * NT, p.n - 1));
             col_bias[tid + u * NT] = p.bias ? scalar_value(cb[u], p.bias, p.bias_dtype, min(n0 + tid + u * NT, p.n - 1)) : kea::kNoBias;
         }
-    wait_copies<(NS - 2) * COPIES>();
+    wait_copies<(AHEAD - 1) * COPIES>();
     barrier();
     if (stages == 1) clear_tail(0, 0);
     fetch(0, 0, 0);
-    if constexpr (STEPS == 2) {
-        for (int s = 0; s + 1 < stages; ++s) step(s, 0);
+    // Stage s, whose first half's operands are in set 0: each half's operands are read while the matrix cores work on the
+    // other's. Between its halves the next stage has landed. (Past the end the last stage is copied again: every wave counts
+    // the same copies.)
+    int buf = 0;
+    for (int s = 0; s + 1 < stages; ++s) {
+        if (!MIDDLE) copy(min(s + AHEAD, stages - 1), buf ? buf - 1 : NS - 1);
         fetch(buf, 1, 1);
         product(0);
+        wait_copies<(NS - 2) * COPIES>();
+        barrier();
+        if (MIDDLE) copy(min(s + AHEAD, stages - 1), buf);
+        buf = buf + 1 == NS ? 0 : buf + 1;
+        if (s + 2 == stages) clear_tail(s + 1, buf);
+        fetch(buf, 0, 0);
         product(1);
-    } else {
-        int s = 0;
-        for (; s + 2 < stages; s += 2) {
-            step(s, 0);
-            step(s + 1, 1);
-        }
-        if (s + 1 < stages) {
-            step(s, 0);
-            product(1);
-        } else {
-            product(0);
-        }
     }
+    fetch(buf, 1, 1);
+    product(0);
+    product(1);
     wait_copies<0>();
 
 #pragma unroll
@@ -465,23 +454,23 @@ int run_split(const Args &a, hipStream_t stream) {
 // The variant of the shortest estimated time. Each tile form's launch takes `base` us and, for every `full` workgroups that
 // run at once, fa us a stage of 128 k and fe besides (ha and he where at most 256 are left, one to a CU); the forms that split
 // k take what the bytes of one workgroup take (they are too few to fill the CU's loads) or, with many workgroups, what all take.
-// The figures are fits to 29 shapes from 1 x 1024 x 1024 to 8000 x 4096 x 4096, hot, as graphs of launches (us; tile forms in
-// the order below, then 32 x 32, 32 x 16 and 16 x 16 split over 4 waves):
-//   8000 x 4096 x 4096   117.2  134.4  153.0  162.6  220.9
-//   2000 x 4096 x 1024    18.8   13.3   14.9   14.9   20.3
-//   1000 x 4096 x 1024    16.8    9.4    8.8    8.9   11.8  31.3
-//   1500 x 1024 x 1024    15.8    7.8    7.4    5.7    6.4  13.5
-//   1000 x 1024 x 1024    15.7    7.7    7.3    5.5    5.0   9.8
-//    125 x 1024 x 1024                           5.2   4.5   4.3   3.7   4.2
-//     64 x 4096 x 1024                                 4.5   4.5   5.1   6.0
-//     16 x 2560 x  640                                 3.7   3.6   3.4   3.2
-//     64 x 1024 x 4096                                       9.3   7.6   6.0
+// The figures are fits to what the forms take on 60 shapes of 1 to 16000 rows, hot, as graphs of launches; some of them (us, the
+// tile forms in the order below, then 32 x 32, 32 x 16 and 16 x 16 split over 4 waves):
+//   8000 x 4096 x 4096   116.7  138.4  159.2  173.6  232.1
+//   2000 x 4096 x 1024    19.4   14.4   15.9   16.6   21.9
+//   1000 x 4096 x 1024    17.2    8.6    8.4    9.1   12.3  31.7
+//   1500 x 1024 x 1024    16.4    7.4    7.3    5.7    6.3  13.5
+//   1000 x 1024 x 1024    16.1    7.2    7.1    5.5    4.9   9.9
+//    125 x 1024 x 1024    15.2    6.9    6.8    5.1    4.5   4.3    3.6    4.0
+//     64 x 4096 x 1024    13.4    6.8    6.8    5.1    4.5   4.4    5.3    5.9
+//     16 x 2560 x  640     9.1    4.7    4.9    3.9    3.7   3.6    3.4    3.2
+//     64 x 1024 x 4096    40.1   17.0   16.1   11.5    9.8   9.4    7.7    5.9
 struct Form {
     int bm, bn, full;
     float base, fa, fe, ha, he;
 };
-constexpr Form kForms[] = {{256, 256, 256, 2.0f, 1.5f, 8.0f, 1.5f, 8.0f},
-                           {128, 128, 512, 2.3f, 0.93f, 3.2f, 0.78f, 0.9f},
+constexpr Form kForms[] = {{256, 256, 256, 2.0f, 1.45f, 8.0f, 1.45f, 8.0f},
+                           {128, 128, 512, 2.3f, 0.93f, 3.2f, 0.62f, 1.3f},
                            {128, 128, 256, 2.0f, 0.48f, 2.9f, 0.48f, 2.9f},
                            {128, 64, 512, 2.0f, 0.55f, 2.7f, 0.36f, 1.3f},
                            {64, 64, 512, 2.0f, 0.37f, 1.9f, 0.23f, 1.1f}};
@@ -520,25 +509,6 @@ int run(int variant, const Args &a, hipStream_t stream) {
         case kSplit32: return run_split<2, 2, 4, 2>(a, stream);
         case kSplit32x16: return run_split<2, 1, 4, 4>(a, stream);
         case kSplit16: return run_split<1, 1, 4, 4>(a, stream);
-#ifdef KEA_INT8_SWEEP
-        case 23: return run_split<1, 1, 8, 8>(a, stream);
-        case 8: return run_split<2, 2, 8, 2>(a, stream);
-        case 9: return run_split<2, 2, 8, 4>(a, stream);
-        case 10: return run_split<1, 1, 16, 4>(a, stream);
-        case 11: return run_split<1, 1, 4, 8>(a, stream);
-        case 12: return run_split<1, 1, 8, 4>(a, stream);
-        case 13: return run_split<1, 2, 8, 4>(a, stream);
-        case 14: return run_split<2, 1, 8, 4>(a, stream);
-        case 15: return run_split<2, 2, 4, 4>(a, stream);
-        case 16: return run_split<1, 2, 4, 4>(a, stream);
-        case 17: return run_tiles<32, 64, 2, 2, 128, 6>(a, stream);
-        case 18: return run_tiles<64, 128, 2, 4, 128, 4>(a, stream);
-        case 19: return run_tiles<64, 64, 2, 2, 128, 3>(a, stream);
-        case 20: return run_tiles<128, 64, 4, 2, 128, 4>(a, stream);
-        case 21: return run_tiles<64, 64, 4, 2, 128, 6>(a, stream);
-        case 22: return run_tiles<64, 32, 4, 1, 128, 6>(a, stream);
-        case 24: return run_split<1, 1, 2, 4>(a, stream);
-#endif
         default: return kea::fail(KEA_EINVAL, "kea_int8_gemm: no such variant");
     }
 }
@@ -552,10 +522,6 @@ int64_t kea_int8_gemm_workspace(int64_t m, int64_t n, int64_t k) {
     return 0;
 }
 
-#ifdef KEA_INT8_SWEEP
-int kea_int8_variant = -1;
-void kea_int8_set_variant(int v) { kea_int8_variant = v; }
-#endif
 
 int kea_int8_gemm(const int8_t *q, int64_t ldq, const void *qs, int qs_dtype, const int8_t *w, int64_t ldw, const void *wscale,
                   int ws_dtype, const void *bias, int bias_dtype, void *y, int y_dtype, int64_t ldy, const float *residual,
@@ -581,9 +547,6 @@ int kea_int8_gemm(const int8_t *q, int64_t ldq, const void *qs, int qs_dtype, co
                  qs_dtype, ws_dtype, bias_dtype, y_dtype, flags};
     // (the tile forms address a tile's rows with 32 bits)
     int v = ldq < (1 << 23) && ldw < (1 << 23) ? choose(a.m, a.n, a.k) : kSplit32;
-#ifdef KEA_INT8_SWEEP
-    if (kea_int8_variant >= 0) v = kea_int8_variant;
-#endif
     return run(v, a, (hipStream_t)stream);
 }
 
