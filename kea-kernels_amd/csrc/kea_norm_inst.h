@@ -1,7 +1,8 @@
 // The row kernel of kea_block_norm and its launch for one stream type; each kea_norm_*.hip defines KEA_NORM_STREAM.
 //
-// A row stays in registers from its loads to its stores: W waves hold it as N vectors of eight elements a thread, so each input
-// is read once, each output written once, and the sums of a norm are a wave's reduction (and, where W > 1, one exchange of
+// y = x + factor * act(gate) * post(block), z = pre(y). A row stays in registers from its loads to its stores: W waves hold it as
+// N vectors of eight elements a thread, so each input is read once, each output written once (memory bounds it: 16000 rows of
+// 4096, BF16, with a gate and two RMS norms, take 102 us, 5.1 TB/s, a large copy's rate), and the sums of a norm are a wave's reduction (and, where W > 1, one exchange of
 // wave totals through LDS). The row's loads are issued together; the norms' parameters, which every row reads, come from the
 // caches when they are used. The variance is the mean of the squared differences from the mean, a second reduction over
 // registers.
@@ -226,14 +227,17 @@ void launch(const NormArgs &a, hipStream_t stream) {
     else block_norm_kernel<XT, BT, N, W, TINY><<<dim3((unsigned)a.m), 64 * W, 0, stream>>>(a);
 }
 
+// As many waves as hold the row in one vector a thread, up to sixteen: one row of 4096 takes 3.8 us so, 4.8 in four waves of two
+// vectors and 6.6 in two of four; 16000 of them (FP32 streams, FP16 blocks) 152, 163 and 161. Rows of 8192 are alike (4.7
+// against 7.0 in four waves of four, 16000 of them 289 and 298, but 1000 of them 22 and 20).
 template <typename XT, typename BT>
 void rows(const NormArgs &a, hipStream_t s) {
     if (a.d < 8) launch<XT, BT, 1, 1, true>(a, s);
     else if (a.d <= 512) launch<XT, BT, 1, 1>(a, s);
-    else if (a.d <= 1024) launch<XT, BT, 2, 1>(a, s);
+    else if (a.d <= 1024) launch<XT, BT, 1, 2>(a, s);
     else if (a.d <= 2048) launch<XT, BT, 1, 4>(a, s);
-    else if (a.d <= 4096) launch<XT, BT, 2, 4>(a, s);
-    else if (a.d <= 8192) launch<XT, BT, 4, 4>(a, s);
+    else if (a.d <= 4096) launch<XT, BT, 1, 8>(a, s);
+    else if (a.d <= 8192) launch<XT, BT, 1, 16>(a, s);
     else if (a.d <= 16384) launch<XT, BT, 2, 16>(a, s);
     else launch<XT, BT, 4, 16>(a, s);
 }
