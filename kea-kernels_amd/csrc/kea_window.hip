@@ -202,8 +202,8 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
     uint32_t off_k[OFFSETS], off_v[OFFSETS];
 #pragma unroll
     for (int u = 0; u < OFFSETS; ++u) {
-        off_k[u] = ((uint32_t)(key0 * (int)a.k.t_stride) + unit(0, key0 + u * STEP)) * (uint32_t)sizeof(T);
-        off_v[u] = ((uint32_t)(key0 * (int)a.v.t_stride) + unit(1, key0 + u * STEP)) * (uint32_t)sizeof(T);
+        off_k[u] = ((uint32_t)key0 * (uint32_t)a.k.t_stride + unit(0, key0 + u * STEP)) * (uint32_t)sizeof(T);
+        off_v[u] = ((uint32_t)key0 * (uint32_t)a.v.t_stride + unit(1, key0 + u * STEP)) * (uint32_t)sizeof(T);
     }
     auto stage = [&](int v0, int buf, bool of_k, bool of_v) {
         // (made anew on every call: kept for all copies of a tile, the addresses would not fit the registers)
@@ -638,8 +638,8 @@ __global__ void __launch_bounds__(64) join_kernel(Args a) {
         v *= old;
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
-            if (s0 + s >= a.splits || stat[s].x == -INFINITY) continue;
-            const float by = __builtin_amdgcn_exp2f(stat[s].x - top);
+            if (s0 + s >= a.splits) continue;
+            const float by = stat[s].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(stat[s].x - top);  // (a NaN stays one)
             sum += stat[s].y * by;
             v += part[s] * by;
         }

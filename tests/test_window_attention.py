@@ -160,6 +160,28 @@ def test_unseen_keys_have_no_part(t, tq, dtype):
 @pytest.mark.gpu
 @torch.inference_mode()
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t,tq", [(90, 90), (3000, 1)])
+def test_seen_nan_scores_show(t, tq, dtype):
+    """Keys of NaN alone (in one of several parts of the keys, too) make the rows that see one NaN, and only those."""
+    g = torch.Generator().manual_seed(8)
+    q, k, v = heads(3, tq, 2, 64, dtype, g), heads(3, t, 2, 64, dtype, g), heads(3, t, 2, 64, dtype, g)
+    k[0, t - 70:t - 1] = float("nan")
+    k[1, :] = float("nan")
+    got = window.attention(q, k, v)
+    assert got[:2, -1].isnan().all() and got[2].isfinite().all()
+    clean = k.clone()
+    clean[:2] = 0
+    want, err = expected(q, clean, v, None, 0, 0)
+    check(got[2:], want[2:], err[2:])
+    if tq > 1:
+        assert got[1].isnan().all()
+        first = t - 70
+        assert got[0, :first].isfinite().all() and got[0, first:].isnan().all()
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
 def test_large_scores(dtype):
     """Scores in the thousands (one key takes all), equal scores, a negative and a zero scale."""
     g = torch.Generator().manual_seed(3)
