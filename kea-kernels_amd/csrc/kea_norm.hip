@@ -34,7 +34,8 @@ extern "C" int kea_block_norm(const void *x, int x_dtype, int64_t ldx, const voi
     if (!x || (block && !y) || (!block && !z && !q)) return kea::fail(KEA_EINVAL, "kea_block_norm: a pointer is missing");
     if (!aligned(x, x_dtype) || !aligned(block, block_dtype) || !aligned(gate, block_dtype) || !aligned(y, x_dtype) || !aligned(z, block_dtype) || (uintptr_t)qs % 4)
         return kea::fail(KEA_EALIGN, "kea_block_norm: a pointer is not aligned to its element size");
-    if (!kea::fits_dispatch(m, 1024)) return kea::fail(KEA_EINVAL, "kea_block_norm: too large for one launch");
+    const unsigned threads = d <= 512 ? 64 : d <= 1024 ? 128 : d <= 2048 ? 256 : d <= 4096 ? 512 : 1024;  // of a row
+    if (m > UINT32_MAX || !kea::fits_dispatch(m + 3, threads)) return kea::fail(KEA_EINVAL, "kea_block_norm: too large for one launch");
     const kea::NormArgs a{x, block, gate, y, z, q, qs, m, ldx, ldb, ldg, ldy, ldz, ldq, gate_rows, *post, *pre, factor, (int)d, block_dtype, gate_act};
     if (x_dtype == KEA_F32) kea::norm_rows<float>(a, stream);
     else if (x_dtype == KEA_F16) kea::norm_rows<_Float16>(a, stream);

@@ -1,11 +1,12 @@
 // The row kernel of kea_block_norm and its launch for one stream type; each kea_norm_*.hip defines KEA_NORM_STREAM.
 //
-// y = x + factor * act(gate) * post(block), z = pre(y). A row stays in registers from its loads to its stores: W waves hold it as
-// N vectors of eight elements a thread, so each input is read once, each output written once (memory bounds it: 16000 rows of
-// 4096, BF16, with a gate and two RMS norms, take 102 us, 5.1 TB/s, a large copy's rate), and the sums of a norm are a wave's reduction (and, where W > 1, one exchange of
-// wave totals through LDS). The row's loads are issued together; the norms' parameters, which every row reads, come from the
-// caches when they are used. The variance is the mean of the squared differences from the mean, a second reduction over
-// registers.
+// y = x + factor * act(gate) * post(block), z = pre(y). A row stays in registers from its loads to its stores: W waves hold
+// it as N vectors of eight elements a thread, so each input is read once and each output written once. Memory bounds it:
+// 16000 rows of 4096, BF16, with a gate and two RMS norms, take 100 us, 5.2 TB/s, a large copy's rate; one such row takes
+// 3.5 us, mostly the launch and the loads' latency. The sums of a norm are a wave's reduction and, where W > 1, one exchange
+// of wave totals through LDS. The row's loads are issued together; the norms' parameters, which every row reads, come from
+// the caches when they are used. The variance is the mean of the squared differences from the mean, a second reduction
+// over registers.
 //
 // Vectors are accessed at any alignment of their elements. Where d is no multiple of 8, the last vector is moved back to end
 // with the row: the elements that it shares with its neighbour are left out of the sums and not stored.

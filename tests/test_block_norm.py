@@ -166,6 +166,18 @@ def test_many_rows():
 
 @pytest.mark.gpu
 @torch.inference_mode()
+def test_millions_of_rows():
+    """More rows than 2^32 / 1024: rows of 8, each normalised to the same values."""
+    x = torch.arange(8, dtype=F32, device=DEV).repeat(5_000_003, 1)
+    pre = module("layer", 8, torch.Generator().manual_seed(1))
+    _, z = norms.block_norm(x, x.half(), factor=0.0, pre=pre)
+    (_, _), (want, err) = expected(x[:1], x[:1].half(), None, None, "", 0.0, pre)
+    check(z[:1], want, err)
+    assert (z == z[0]).all()
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
 @pytest.mark.parametrize("d", [64, 1024, 1031])
 def test_norm_alone_and_rows_of_the_stream(d):
     """Without a block: the norm of x, as values or int8 rows; without a norm: the rows that lowbit.quantize makes, to the bit."""
