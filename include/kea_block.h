@@ -32,14 +32,11 @@ extern "C" {
  *              behind take no part in the sums, whatever they hold; no byte from the last row's k, rounded up to 16, on
  *              is read.
  *   qs, wscale KEA_F32 or KEA_F16; bias NULL or KEA_F32 / KEA_F16; each aligned to its element size.
- *   residual   NULL or FP32 [m][ldr]; y may be the residual itself (y_dtype KEA_F32, ldy == ldr).
- *   workspace  kea_int8_gemm_workspace(m, n, k) bytes, 16-byte aligned (0: may be NULL). It holds int32 sums of parts of k,
- *              written before they are read. */
-int64_t kea_int8_gemm_workspace(int64_t m, int64_t n, int64_t k);
+ *   residual   NULL or FP32 [m][ldr]; y may be the residual itself (y_dtype KEA_F32, ldy == ldr). */
 int kea_int8_gemm(const int8_t *q_dev, int64_t ldq, const void *qs_dev, int qs_dtype, const int8_t *w_dev, int64_t ldw,
                   const void *wscale_dev, int ws_dtype, const void *bias_dev, int bias_dtype, void *y_dev, int y_dtype,
                   int64_t ldy, const float *residual_dev, int64_t ldr, float factor, int64_t m, int64_t n, int64_t k,
-                  int flags, void *workspace_dev, int64_t workspace_bytes, void *stream);
+                  int flags, void *stream);
 
 /* Kinds of norms, and of what a gate passes through. */
 #define KEA_NORM_NONE 0
@@ -65,8 +62,7 @@ typedef struct {
  *   z          NULL, or [m][ldz] of block_dtype (pre.kind must not be KEA_NORM_NONE).
  *   q, qs      NULL, or instead of z its quantization to int8 rows with an FP32 scale each, as kea_quantize makes one part:
  *              s = max(max|z| / 127, 1e-30), q = rint(z / s), zero from d to ldq; q [m][ldq], ldq >= d, qs [m].
- * 1 <= d <= 32768. Pointers are aligned to their element size; rows whose pointers and strides are multiples of 16 bytes,
- * d a multiple of 8, take vector loads. */
+ * 1 <= d <= 32768. Pointers are aligned to their element size. */
 int kea_block_norm(const void *x_dev, int x_dtype, int64_t ldx, const void *block_dev, int block_dtype, int64_t ldb,
                    int64_t m, int64_t d, const kea_norm *post, const void *gate_dev, int64_t ldg, int64_t gate_rows,
                    int gate_act, float factor, void *y_dev, int64_t ldy, const kea_norm *pre, void *z_dev, int64_t ldz,
@@ -81,7 +77,8 @@ typedef struct {
 /* Attention within a sliding window and to the first tokens. Query i (0 <= i < tq) of sequence b stands at position
  * p = q_starts[b] + i among the sequence's keys 0 .. len-1, len = kv_lengths[b] clamped to 0 .. tk, and sees key j < len iff
  *   j <= p + right  and  (j >= p - left  or  j < sinks);
- *   out_i = sum_j softmax_j(scale * q_i . k_j) v_j over the keys it sees, 0 where it sees none or p is outside 0 .. len-1.
+ *   out_i = sum_j softmax_j(scale * q_i . k_j) v_j over the keys it sees, 0 where it sees none (or scores of -infinity
+ *   alone) or p is outside 0 .. len-1.
  * Head h reads key head h / (heads / kv_heads). A key that a query does not see has no part in its output, whatever k and v
  * hold there; k and v at len and behind are not read. Scores, their maximum and sum and the output's sums are FP32; the
  * weights exp(s - max) are rounded to the type for the product with v (KEA_F16, KEA_BF16).

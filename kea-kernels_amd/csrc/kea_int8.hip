@@ -517,16 +517,9 @@ int run(int variant, const Args &a, hipStream_t stream) {
 
 extern "C" {
 
-int64_t kea_int8_gemm_workspace(int64_t m, int64_t n, int64_t k) {
-    if (m < 0 || n < 1 || k < 1) return kea::fail(KEA_EINVAL, "kea_int8_gemm_workspace: m >= 0, n >= 1 and k >= 1 are needed");
-    return 0;
-}
-
-
 int kea_int8_gemm(const int8_t *q, int64_t ldq, const void *qs, int qs_dtype, const int8_t *w, int64_t ldw, const void *wscale,
                   int ws_dtype, const void *bias, int bias_dtype, void *y, int y_dtype, int64_t ldy, const float *residual,
-                  int64_t ldr, float factor, int64_t m, int64_t n, int64_t k, int flags, void *workspace,
-                  int64_t workspace_bytes, void *stream) {
+                  int64_t ldr, float factor, int64_t m, int64_t n, int64_t k, int flags, void *stream) {
     if (m < 0 || n < 1 || k < 1 || k > 131071 || m > INT32_MAX - 4096 || n > INT32_MAX - 4096)
         return kea::fail(KEA_EINVAL, "kea_int8_gemm: sizes m >= 0, n >= 1, 1 <= k <= 131071 below 2^31 are needed");
     if (ldq < k || ldw < k || ldy < n || (residual && ldr < n))
@@ -546,7 +539,7 @@ int kea_int8_gemm(const int8_t *q, int64_t ldq, const void *qs, int qs_dtype, co
     const Args a{q, w, ldq, ldw, qs, wscale, bias, y, ldy, residual, ldr, factor, (int)m, (int)n, (int)k,
                  qs_dtype, ws_dtype, bias_dtype, y_dtype, flags};
     // (the tile forms address a tile's rows with 32 bits)
-    int v = ldq < (1 << 23) && ldw < (1 << 23) ? choose(a.m, a.n, a.k) : kSplit32;
+    const int v = ldq < (1 << 23) && ldw < (1 << 23) ? choose(a.m, a.n, a.k) : kSplit32;
     return run(v, a, (hipStream_t)stream);
 }
 

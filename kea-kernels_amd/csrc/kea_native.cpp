@@ -34,7 +34,6 @@ struct Library {
     decltype(&kea_lowbit_gemm_residual) gemm_residual = nullptr;
     decltype(&kea_quantize) quantize = nullptr;
     decltype(&kea_int8_gemm) int8_gemm = nullptr;
-    decltype(&kea_int8_gemm_workspace) int8_workspace = nullptr;
     decltype(&kea_block_norm) block_norm = nullptr;
     decltype(&kea_window_attention) window = nullptr;
     decltype(&kea_window_attention_workspace) window_workspace = nullptr;
@@ -447,14 +446,10 @@ PyObject *native_int8_gemm(PyObject *, PyObject *const *args, Py_ssize_t count) 
         Py_RETURN_NONE;
     try {
         at::Tensor y = out ? *out : at::empty({m, n}, at::TensorOptions().device(device).dtype(type));
-        const int64_t need = lib.int8_workspace(m, n, k);
-        at::Tensor space;
-        if (need > 0) space = at::empty({need}, at::TensorOptions().device(device).dtype(at::kByte));
         const int rc = lib.int8_gemm((const int8_t *)q->const_data_ptr(), ldq, qs->const_data_ptr(), sc, (const int8_t *)w->const_data_ptr(), ldw,
                                      ws->const_data_ptr(), wc, bias ? bias->const_data_ptr() : nullptr, bc, y.mutable_data_ptr(), yc,
                                      m > 1 ? y.stride(0) : n, res ? (const float *)res->const_data_ptr() : nullptr, res && m > 1 ? res->stride(0) : n,
-                                     (float)factor, m, n, k, silu ? KEA_FLAG_SILU : 0, need > 0 ? space.mutable_data_ptr() : nullptr,
-                                     need > 0 ? need : 0, stream_of(device));
+                                     (float)factor, m, n, k, silu ? KEA_FLAG_SILU : 0, stream_of(device));
         if (rc == 0) return THPVariable_Wrap(std::move(y));
     } catch (const std::exception &) {
     }
@@ -591,12 +586,11 @@ PyObject *native_window(PyObject *, PyObject *const *args, Py_ssize_t count) {
     Py_RETURN_NONE;
 }
 
-// bind_block(int8_gemm, int8_gemm_workspace, block_norm, window_attention, window_attention_workspace)
+// bind_block(int8_gemm, block_norm, window_attention, window_attention_workspace)
 PyObject *native_bind_block(PyObject *, PyObject *args) {
-    unsigned long long g, gw, n, w, ww;
-    if (!PyArg_ParseTuple(args, "KKKKK", &g, &gw, &n, &w, &ww)) return nullptr;
+    unsigned long long g, n, w, ww;
+    if (!PyArg_ParseTuple(args, "KKKK", &g, &n, &w, &ww)) return nullptr;
     lib.int8_gemm = (decltype(lib.int8_gemm))g;
-    lib.int8_workspace = (decltype(lib.int8_workspace))gw;
     lib.block_norm = (decltype(lib.block_norm))n;
     lib.window = (decltype(lib.window))w;
     lib.window_workspace = (decltype(lib.window_workspace))ww;

@@ -102,9 +102,8 @@ SIGNATURES = {
     "kea_subsample_out_workspace": (_i64, [_i64, _i64]),
     "kea_subsample_out": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _f32, _vp, _vp, _vp, _i64, _vp]),
     "kea_dwconv_quantize": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _vp, _vp]),
-    "kea_int8_gemm_workspace": (_i64, [_i64, _i64, _i64]),
     "kea_int8_gemm": (_i32, [_vp, _i64, _vp, _i32, _vp, _i64, _vp, _i32, _vp, _i32, _vp, _i32, _i64, _vp, _i64, _f32,
-                             _i64, _i64, _i64, _i32, _vp, _i64, _vp]),
+                             _i64, _i64, _i64, _i32, _vp]),
     "kea_block_norm": (_i32, [_vp, _i32, _i64, _vp, _i32, _i64, _i64, _i64, _norm, _vp, _i64, _i64, _i32, _f32, _vp, _i64,
                               _norm, _vp, _i64, _vp, _i64, _vp, _vp]),
     "kea_window_attention_workspace": (_i64, [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
@@ -154,8 +153,7 @@ def native():
                 module.bind(*(ctypes.cast(getattr(library, name), ctypes.c_void_p).value for name in (
                     "kea_lowbit_project_launch", "kea_lowbit_gemm", "kea_lowbit_gemm_residual", "kea_quantize")))
                 module.bind_block(*(ctypes.cast(getattr(library, name), ctypes.c_void_p).value for name in (
-                    "kea_int8_gemm", "kea_int8_gemm_workspace", "kea_block_norm", "kea_window_attention",
-                    "kea_window_attention_workspace")))
+                    "kea_int8_gemm", "kea_block_norm", "kea_window_attention", "kea_window_attention_workspace")))
                 _native = module
     return _native
 

@@ -3,8 +3,7 @@
 For the layers of a model that do not stand 1- or 2-bit weights (the first and last ones, a decoder's): `gemm` multiplies the
 int8 rows that lowbit.quantize or norms.block_norm make (one part) with int8 weights [N, K] as they are stored, and applies
 the epilogue of lowbit.gemm: scales, bias, SiLU, residual. `Int8Linear` holds such a weight and takes float rows. Calls run
-on torch's current stream of the tensors' device, never synchronize the host and take their workspace, if the shape needs
-one, from torch's allocator; they can be captured into a graph.
+on torch's current stream of the tensors' device, never synchronize the host and can be captured into a graph.
 """
 from __future__ import annotations
 
@@ -111,16 +110,13 @@ def gemm(q: Tensor, qs: Tensor | None, weight: Tensor, wscale: Tensor | None, bi
         return out
     L = _hip.lib()
     with _hip.on_device(device):
-        need = L.kea_int8_gemm_workspace(m, n, k)
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
         code = lambda t: 0 if t is None else _hip.dtype_code(t.dtype)  # noqa: E731
         rc = L.kea_int8_gemm(q.data_ptr(), max(q.stride(0), lowbit.round_up(ldq, 16)) if m == 1 else q.stride(0),
                              _hip.ptr(qs), code(qs), weight.data_ptr(),
                              lowbit.round_up(k, 16) if n == 1 else weight.stride(0), _hip.ptr(wscale), code(wscale),
                              _hip.ptr(bias), code(bias), out.data_ptr(), _OUT[out_dtype], n if m == 1 else out.stride(0),
                              _hip.ptr(residual), (n if m == 1 else residual.stride(0)) if residual is not None else 0,
-                             float(residual_factor), m, n, k, int(silu), _hip.ptr(ws), max(need, 0),
-                             _hip.stream_handle(device))
+                             float(residual_factor), m, n, k, int(silu), _hip.stream_handle(device))
     _hip.check(rc, "kea_int8_gemm")
     return out
 
@@ -175,6 +171,8 @@ class Int8Linear:
             raise ValueError(f"expected [..., {self.in_features}] input, got {tuple(x.shape)}")
         _hip.refuse_grad("Int8Linear", x)
         lead, m = x.shape[:-1], math.prod(x.shape[:-1])
+        if m == 0:
+            return torch.empty(*lead, self.out_features, device=self.device, dtype=out_dtype)
         xr = x.reshape(-1, x.shape[-2], x.shape[-1]) if x.dim() > 2 else x.view(1, 1, -1) if x.dim() == 1 else x[None]
         with _hip.on_device(x.device):
             q, qs, _ = lowbit.quantize(xr, (xr.stride(0), xr.stride(1), xr.stride(2), max(xr.shape[1], 1)), m,

@@ -128,6 +128,34 @@ def test_views_stay_inside_their_rows(m, n, k):
 
 @pytest.mark.gpu
 @torch.inference_mode()
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(3, 70, 90), (40, 131, 260), (300, 267, 1000), (600, 1031, 128)])
+def test_outputs_at_any_alignment(m, n, k, dtype):
+    """Rows of out and of the residual that start at odd elements and lie an odd number of elements apart."""
+    q, qs, w, ws = make(m, n, k, 5)
+    base = torch.full((m + 1, n + 4), 7.0, device=DEV).to(dtype)[:, :n + 3]
+    base = base.contiguous() if n % 2 == 0 else torch.full((m + 1, n + 2), 7.0, device=DEV).to(dtype)
+    out, res = base[:m, 1:n + 1], torch.randn(m, n + 3, device=DEV)[:, 3:]
+    int8.gemm(q, qs, w, ws, out=out, residual=res, residual_factor=-2.0)
+    want, err = expected(q, qs, w, ws, None, False, res, -2.0, dtype)
+    check(out, want, err.abs() + 4 * U * (want - res.cpu().double()).abs())
+    assert (base[m] == 7).all() and (base[:, 0] == 7).all() and (base[:, n + 1:] == 7).all()
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+def test_rows_far_apart():
+    """Leading dimensions that 32-bit offsets within a tile do not reach."""
+    far = 1 << 24
+    base = torch.zeros(130 * far, dtype=torch.int8, device=DEV)
+    q = base.as_strided((130, 200), (far, 1))
+    q.copy_(torch.randint(-128, 128, (130, 200), dtype=torch.int8))
+    w = torch.randint(-128, 128, (140, 208), dtype=torch.int8).to(DEV)[:, :200]
+    assert torch.equal(int8.gemm(q, None, w, None, out_dtype=torch.int32).cpu().double(), sums(q, w))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
 def test_offsets_past_32_bits():
     """Rows of q and out beyond 2^31 bytes."""
     k, n, m = 4096, 32, 600000
@@ -188,7 +216,8 @@ def test_linear_layer():
             y = layer.linear(x, activation="silu", out_dtype=dtype)
             assert y.shape == (*x.shape[:-1], 130)
             check(y.reshape(-1, 130), *expected(q, qs, layer.weight, layer.scale, layer.bias, True, None, 1.0, dtype))
-    assert layer.linear(torch.empty(0, 271, device=DEV)).shape == (0, 130)
+    for empty in ((0, 271), (2, 0, 271), (0, 3, 271)):
+        assert layer.linear(torch.empty(empty, device=DEV)).shape == (*empty[:-1], 130)
     norm = torch.nn.LayerNorm(271, device=DEV)
     x = torch.randn(4, 271, generator=g).to(DEV)
     q, qs, _ = lowbit.quantize(x[None], (0, 271, 1, 4), 4, 271, 1, norm=norm, input_activation="silu")
@@ -251,13 +280,12 @@ def test_library_refusals():
     buf = (ctypes.c_char * 4096)()
     p = (ctypes.addressof(buf) + 15) // 16 * 16
     good = dict(q=p, ldq=32, qs=p, qd=0, w=p, ldw=32, ws=p, wd=0, b=None, bd=0, y=p, yd=0, ldy=8, r=None, ldr=0, f=1.0, m=4, n=8,
-                k=32, flags=0, space=None, bytes=0, stream=None)
+                k=32, flags=0, stream=None)
     for change, rc in [(dict(k=0), -1), (dict(k=131072), -1), (dict(n=0), -1), (dict(m=-1), -1), (dict(ldq=16), -1), (dict(ldy=7), -1),
                        (dict(yd=4), -1), (dict(yd=3, flags=1), -1), (dict(yd=3, r=p, ldr=8), -1), (dict(flags=2), -1), (dict(qd=2), -1),
                        (dict(b=p, bd=2), -1), (dict(q=None), -1), (dict(qs=None), -1), (dict(q=p + 4), -2), (dict(ldw=40), -2),
                        (dict(y=p + 2), -2), (dict(r=p, ldr=4), -1), (dict(m=0), 0), (dict(n=1 << 31), -1)]:
         assert L.kea_int8_gemm(*(good | change).values()) == rc, change
-    assert L.kea_int8_gemm_workspace(-1, 8, 32) < 0 and L.kea_int8_gemm_workspace(4, 8, 32) >= 0
 
 
 def test_linear_refusals():
