@@ -32,7 +32,8 @@ extern "C" {
  *              behind take no part in the sums, whatever they hold; no byte from the last row's k, rounded up to 16, on
  *              is read.
  *   qs, wscale KEA_F32 or KEA_F16; bias NULL or KEA_F32 / KEA_F16; each aligned to its element size.
- *   residual   NULL or FP32 [m][ldr]; y may be the residual itself (y_dtype KEA_F32, ldy == ldr). */
+ *   residual   NULL or FP32 [m][ldr]; y may be the residual itself (y_dtype KEA_F32, ldy == ldr) and overlaps no other
+ *              operand. */
 int kea_int8_gemm(const int8_t *q_dev, int64_t ldq, const void *qs_dev, int qs_dtype, const int8_t *w_dev, int64_t ldw,
                   const void *wscale_dev, int ws_dtype, const void *bias_dev, int bias_dtype, void *y_dev, int y_dtype,
                   int64_t ldy, const float *residual_dev, int64_t ldr, float factor, int64_t m, int64_t n, int64_t k,
@@ -58,7 +59,8 @@ typedef struct {
  * for rows r = 0 .. m-1 of d elements, every step in FP32 (a row's mean and variance too) and y and z rounded once, each on
  * its own: z is the norm of y before its rounding. x and y are of x_dtype; block, gate and z of block_dtype.
  *   gate       NULL (1), or [ceil(m / gate_rows)][ldg]: gate_rows rows in turn share a gate row.
- *   y          y may be x itself (in place, ldy == ldx). block NULL: y is not written (pass NULL) and z = pre(x).
+ *   y          y may be x itself (in place, ldy == ldx), or the block, and overlaps no other operand. block NULL: y is not
+ *              written (pass NULL) and z = pre(x).
  *   z          NULL, or [m][ldz] of block_dtype (pre.kind must not be KEA_NORM_NONE).
  *   q, qs      NULL, or instead of z its quantization to int8 rows with an FP32 scale each, as kea_quantize makes one part:
  *              s = max(max|z| / 127, 1e-30), q = rint(z / s), zero from d to ldq; q [m][ldq], ldq >= d, qs [m].

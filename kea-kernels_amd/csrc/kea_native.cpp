@@ -410,6 +410,17 @@ bool rows_of(const at::Tensor &t, int64_t *rows, int64_t *stride) {
     return true;
 }
 
+// Whether the bytes from a's first element to its last and from b's meet. (An output that lies between an input's rows meets
+// it too; the Python path sorts that out.)
+bool meet(const at::Tensor &a, const at::Tensor &b) {
+    auto end = [](const at::Tensor &t) {
+        int64_t last = 1;
+        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+        return (uintptr_t)t.const_data_ptr() + last * t.element_size();
+    };
+    return (uintptr_t)a.const_data_ptr() < end(b) && (uintptr_t)b.const_data_ptr() < end(a);
+}
+
 // int8 rows [.., k] that start at multiples of 16 bytes, the last one readable to a multiple of 16 of `k` elements.
 bool rows8(const at::Tensor &t, int64_t dim, int64_t k, int64_t *ld) {
     const int64_t m = t.size(dim), w = t.size(dim + 1);
@@ -444,6 +455,11 @@ PyObject *native_int8_gemm(PyObject *, PyObject *const *args, Py_ssize_t count) 
         (res && (res->scalar_type() != at::kFloat || res->dim() != 2 || res->size(0) != m || res->size(1) != n || (n > 1 && res->stride(1) != 1))) ||
         (out && (out->dim() != 2 || out->size(0) != m || out->size(1) != n || (n > 1 && out->stride(1) != 1) || (m > 1 && out->stride(0) < n))))
         Py_RETURN_NONE;
+    if (out) {
+        const bool same = res && out->const_data_ptr() == res->const_data_ptr() && type == at::kFloat && (m == 1 || out->stride(0) == res->stride(0));
+        for (const at::Tensor *t : {q, qs, w, ws, bias, same ? nullptr : res})
+            if (t && meet(*out, *t)) Py_RETURN_NONE;
+    }
     try {
         at::Tensor y = out ? *out : at::empty({m, n}, at::TensorOptions().device(device).dtype(type));
         const int rc = lib.int8_gemm((const int8_t *)q->const_data_ptr(), ldq, qs->const_data_ptr(), sc, (const int8_t *)w->const_data_ptr(), ldw,
@@ -502,6 +518,12 @@ PyObject *native_block_norm(PyObject *, PyObject *const *args, Py_ssize_t count)
                  !rows_of(*gate, &gates, &ldg) || m % gates))
         Py_RETURN_NONE;
     if (out && (out->scalar_type() != x->scalar_type() || out->sizes() != x->sizes() || !rows_of(*out, &my, &ldy) || ldy < d)) Py_RETURN_NONE;
+    if (out) {
+        auto same = [&](const at::Tensor &t, int64_t ld) {
+            return t.scalar_type() == out->scalar_type() && t.const_data_ptr() == out->const_data_ptr() && (m == 1 || ld == ldy);
+        };
+        if ((!same(*x, ldx) && meet(*out, *x)) || (!same(*block, ldb) && meet(*out, *block)) || (gate && meet(*out, *gate))) Py_RETURN_NONE;
+    }
     try {
         const auto options = at::TensorOptions().device(device);
         at::Tensor y = out ? *out : at::empty(x->sizes(), options.dtype(x->scalar_type())), z, q, qs;

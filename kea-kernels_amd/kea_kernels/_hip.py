@@ -196,6 +196,22 @@ def on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
+def rows_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether rows [M, N] and [M', N'] of contiguous elements share memory."""
+    def span(t):
+        return t.data_ptr(), t.element_size() * t.shape[1], t.element_size() * t.stride(0) if t.shape[0] > 1 else 0
+
+    if not a.numel() or not b.numel():
+        return False
+    (pa, na, la), (pb, nb, lb) = span(a), span(b)
+    if pa >= pb + (b.shape[0] - 1) * lb + nb or pb >= pa + (a.shape[0] - 1) * la + na:
+        return False
+    if la == lb > 0:  # columns of one matrix
+        gap = (pb - pa) % la
+        return gap < na or gap + nb > la
+    return True
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 

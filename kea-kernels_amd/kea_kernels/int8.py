@@ -17,6 +17,7 @@ from kea_kernels import _hip, lowbit
 _SCALES = (torch.float32, torch.float16)
 _OUT = {torch.float32: _hip.F32, torch.float16: _hip.F16, torch.bfloat16: _hip.BF16, torch.int32: 3}
 MAX_K = 131071  # sums of k products of two int8 values fit int32
+MAX_FEATURES = 8192  # of a row that lowbit.quantize takes
 
 
 def _vector(name: str, t: Tensor, n: int, device) -> None:
@@ -101,6 +102,12 @@ def gemm(q: Tensor, qs: Tensor | None, weight: Tensor, wscale: Tensor | None, bi
     if out is not None and (tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or out.device != device
                             or (m > 1 and out.stride(0) < n)):
         raise ValueError(f"out must be [{m}, {n}] rows with unit column stride on {device}")
+    if out is not None:
+        same = residual is not None and out.dtype == residual.dtype and out.data_ptr() == residual.data_ptr() and (
+            m < 2 or out.stride(0) == residual.stride(0))
+        others = [q, weight, *(t.view(1, -1) for t in (qs, wscale, bias) if t is not None)]
+        if any(_hip.rows_meet(out, t) for t in (others if same or residual is None else [*others, residual])):
+            raise ValueError("out shares memory with another operand (it may be the residual itself)")
     if weight.device != device:
         raise ValueError(f"tensor on {weight.device}, expected {device}")
     _hip.refuse_grad("the int8 GEMM", qs, wscale, bias, residual, out)
@@ -111,7 +118,7 @@ def gemm(q: Tensor, qs: Tensor | None, weight: Tensor, wscale: Tensor | None, bi
     L = _hip.lib()
     with _hip.on_device(device):
         code = lambda t: 0 if t is None else _hip.dtype_code(t.dtype)  # noqa: E731
-        rc = L.kea_int8_gemm(q.data_ptr(), max(q.stride(0), lowbit.round_up(ldq, 16)) if m == 1 else q.stride(0),
+        rc = L.kea_int8_gemm(q.data_ptr(), lowbit.round_up(ldq, 16) if m == 1 else q.stride(0),
                              _hip.ptr(qs), code(qs), weight.data_ptr(),
                              lowbit.round_up(k, 16) if n == 1 else weight.stride(0), _hip.ptr(wscale), code(wscale),
                              _hip.ptr(bias), code(bias), out.data_ptr(), _OUT[out_dtype], n if m == 1 else out.stride(0),
@@ -132,19 +139,22 @@ class Int8Linear:
 
     @classmethod
     def prepare(cls, weight: Tensor, scale: Tensor, bias: Tensor | None, device) -> "Int8Linear":
-        """int8 weight [N, K], a scale for each row and an optional bias [N]; makes the only GPU copies."""
+        """int8 weight [N, K], K <= 8192, a scale for each row and an optional bias [N]; makes the only GPU copies."""
         device = torch.device(device)
         if device.type != "cuda":
             raise ValueError("Int8Linear runs on GPU devices only")
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
-        if weight.dtype != torch.int8 or weight.dim() != 2 or not 1 <= weight.shape[1] <= MAX_K or weight.shape[0] < 1:
-            raise ValueError(f"weight must be int8 [N, K], got {weight.dtype} {tuple(weight.shape)}")
+        if weight.dtype != torch.int8 or weight.dim() != 2 or not 1 <= weight.shape[1] <= MAX_FEATURES or weight.shape[0] < 1:
+            raise ValueError(f"weight must be int8 [N, K], K <= {MAX_FEATURES}, got {weight.dtype} {tuple(weight.shape)}")
         for name, t in (("scale", scale), ("bias", bias)):
             if t is not None and (t.numel() != weight.shape[0] or not torch.isfinite(t.float()).all()):
                 raise ValueError(f"{name} must be {weight.shape[0]} finite values")
         with torch.no_grad():
-            return cls(pad_rows(weight.to(device)), scale.to(device=device, dtype=torch.float32, copy=True).contiguous().view(-1),
+            n, k = weight.shape
+            rows = torch.zeros(n, lowbit.round_up(k, 16), dtype=torch.int8, device=device)
+            rows[:, :k] = weight  # (never the caller's memory)
+            return cls(rows[:, :k], scale.to(device=device, dtype=torch.float32, copy=True).contiguous().view(-1),
                        None if bias is None else bias.to(device=device, dtype=torch.float32, copy=True).contiguous().view(-1))
 
     @classmethod

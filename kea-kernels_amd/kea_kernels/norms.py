@@ -81,10 +81,10 @@ def block_norm(x: Tensor, block: Tensor | None, *, post=None, gate: Tensor | Non
     lowbit.quantize makes one part of them.
 
     x [..., d] is the residual stream, block [..., d] the output of the block in the same shape, each f32, f16 or bf16; y
-    has x's type (`out` receives it if given, x itself for in place), z the block's. post and pre: modules with weight, bias
-    and eps (torch.nn.LayerNorm) or weight and eps (torch.nn.RMSNorm). gate: [G, d] in the block's type, any leading
-    dimensions of G elements, M a multiple of G: M / G rows in turn share a gate row (G = 1 a gate for each channel, G = the
-    batch one for each sequence, G = M one for each token), passed through gate_activation ("", "sigmoid", "tanh").
+    has x's type (`out` receives it if given; it may be x or the block itself), z the block's. post and pre: modules with
+    weight, bias and eps (torch.nn.LayerNorm) or weight and eps (torch.nn.RMSNorm). gate: [G, d] in the block's type, any
+    leading dimensions of G elements, M a multiple of G: M / G rows in turn share a gate row (G = 1 a gate for each channel,
+    G = the batch one for each sequence, G = M one for each token), passed through gate_activation ("", "sigmoid", "tanh").
     Everything is FP32 up to one rounding of each output: z is the norm of y before y's rounding. block None (then without
     gate, post and factor): y is x itself and z = pre(x) in x's type."""
     if gate_activation not in _ACTS:
@@ -112,6 +112,10 @@ def block_norm(x: Tensor, block: Tensor | None, *, post=None, gate: Tensor | Non
             yr = _rows("out", out)
             if m > 1 and yr.stride(0) < d:
                 raise ValueError("the rows of out overlap")
+            others = [t for t in (xr, br) if t.dtype != yr.dtype or t.data_ptr() != yr.data_ptr() or (
+                m > 1 and t.stride(0) != yr.stride(0))] + ([] if gate is None else [_rows("gate", gate)])
+            if any(_hip.rows_meet(yr, t) for t in others):
+                raise ValueError("out shares memory with another operand (it may be x or the block itself)")
     if gate is not None:
         gr = _rows("gate", gate)
         if gr.shape[1] != d or gr.shape[0] < 1 and m or (m and m % gr.shape[0]) or gate.dtype != block.dtype:

@@ -64,8 +64,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, left: int | None = None, right
     bound; right = 0 is causal), and the first `sinks` keys. len is kv_lengths[b] (int32 [B] on the device, held to 0 .. Tk;
     None: Tk); q_starts int32 [B] (None: len - Tq, the queries are the last tokens). For padded clips q_starts is zeros and
     kv_lengths the clips' lengths; for tokens against a cache kv_lengths counts them too. Queries that see nothing (or
-    scores of -infinity alone), or stand outside 0 .. len - 1 (padding), give zeros. What a query does not see has no part in its output, whatever it holds.
-    scale: 1 / sqrt(D) unless given. out must not overlap q, k or v."""
+    scores of -infinity alone), or stand outside 0 .. len - 1 (padding), give zeros. What a query does not see has no part in
+    its output, whatever it holds. scale: 1 / sqrt(D) unless given. out must not overlap q, k or v."""
     if out is None and (hit := _native(q, k, v, left, right, sinks, scale, kv_lengths, q_starts)) is not None:
         return hit
     if q.dim() != 4 or k.dim() != 4 or q.dtype not in _hip.DTYPES:

@@ -289,7 +289,45 @@ def test_no_rows():
     assert norms.block_norm(x, x, quantize=True)[1].shape == (1, 0, 16)
 
 
+@pytest.mark.gpu
+@torch.inference_mode()
+def test_small_gates_keep_their_digits():
+    """tanh of gates down to 2^-60, without a stream that hides them. Below 1/4 a series, whose next term is 2^-26 of its value,
+    in three roundings that count; above, at most 8 u from 1 - 2 / (1 + e^(2 g)); two roundings more to the output."""
+    gate = torch.cat([s * 2.0 ** torch.linspace(-60, 4, 1300) for s in (1, -1)] + [torch.tensor([0.0, 0.25, -0.25])]).to(DEV)[None]
+    o = torch.linspace(-3, 3, gate.shape[1], device=DEV)[None]
+    y, _ = norms.block_norm(torch.zeros_like(o), o, gate=gate, gate_activation="tanh")
+    g = gate.cpu().double()
+    want = torch.tanh(g) * o.cpu().double()
+    assert ((y.cpu().double() - want).abs() <= want.abs() * U * torch.where(g.abs() < 0.25, 6.0, 8 / torch.tanh(g).abs() + 2)).all()
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("d", [99, 1024, 4100])
+def test_out_as_the_block_and_beside_the_stream(d):
+    g = torch.Generator().manual_seed(11)
+    x, o, gate = tensors(8, d, BF16, BF16, g, 8)
+    want, _ = norms.block_norm(x, o, gate=gate, factor=0.5)
+    both = torch.empty(8, 2 * d, dtype=BF16, device=DEV)
+    both[:, :d] = x
+    norms.block_norm(both[:, :d], o, gate=gate, factor=0.5, out=both[:, d:])
+    assert torch.equal(both[:, d:], want) and torch.equal(both[:, :d], x)
+    norms.block_norm(x, o, gate=gate, factor=0.5, out=o)
+    assert torch.equal(o, want)
+
+
 # ---- without a GPU -----------------------------------------------------------------------------------------------------------
+
+def test_an_output_that_overlaps_is_refused():
+    x, o, gate = torch.zeros(64, 32), torch.zeros(6, 32), torch.zeros(6, 32)
+    for args in ((x[:6], o, gate, x[1:7]), (x[:6], x[6:12], gate, x[3:9]), (x[:6], o, x[20:26], x[20:26]), (x[:1], o[:1], x[:1], x[:1]),
+                 (x[:6], o, gate, x.view(-1)[16:208].view(6, 32))):
+        with pytest.raises(ValueError, match="shares memory"):
+            norms.block_norm(*args[:2], gate=args[2], out=args[3])
+    with pytest.raises(ValueError, match="GPU"):
+        norms.block_norm(x.view(32, 64)[:, :32], x.view(32, 64)[:, :32], out=x.view(32, 64)[:, 32:])
+
 
 def test_refusals():
     x, o = torch.zeros(6, 32), torch.zeros(6, 32, dtype=F16)

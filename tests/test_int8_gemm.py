@@ -234,7 +234,47 @@ def test_empty_rows_and_unaligned_views_on_the_gpu():
         int8.gemm(flat[1:].view(4, 48), qs, w, ws)
 
 
+@pytest.mark.gpu
+@torch.inference_mode()
+def test_a_layer_owns_its_weight():
+    w = torch.randint(-128, 128, (40, 64), dtype=torch.int8).to(DEV)
+    scale, bias, x = torch.ones(40, device=DEV), torch.zeros(40, device=DEV), torch.randn(3, 64, device=DEV)
+    layer = int8.Int8Linear.prepare(w, scale, bias, DEV)
+    want = layer.linear(x)
+    w.zero_(), scale.zero_(), bias.fill_(1)
+    assert torch.equal(layer.linear(x), want)
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+def test_one_row_of_any_stride_and_out_beside_the_residual():
+    q, qs, w, ws = make(4, 70, 200, 9)
+    want = int8.gemm(q, qs, w, ws)
+    one = torch.as_strided(q, (1, q.shape[2]), (100, 1), 0)
+    assert torch.equal(int8.gemm(one, qs[:, :1], w, ws), want[:1])
+    both = torch.zeros(4, 140, device=DEV)
+    both[:, :70] = 1
+    int8.gemm(q, qs, w, ws, out=both[:, 70:], residual=both[:, :70])
+    assert torch.equal(both[:, 70:], int8.gemm(q, qs, w, ws, residual=torch.ones(4, 70, device=DEV))) and (both[:, :70] == 1).all()
+
+
 # ---- without a GPU -----------------------------------------------------------------------------------------------------------
+
+def test_an_output_that_overlaps_is_refused():
+    q, qs, w, ws = _cpu()
+    far = torch.zeros(64, 8)
+    for out, kw in ((far[:4], dict(residual=far[1:5])), (far.view(32, 16)[:4, :8], dict(residual=far.view(32, 16)[:4, 4:12])),
+                    (far[:1], dict(residual=far.view(-1)[4:12].view(1, 8)))):
+        with pytest.raises(ValueError, match="shares memory"):
+            int8.gemm(q[:, :out.shape[0]], qs[:, :out.shape[0]], w, ws, out=out, **kw)
+    words = torch.zeros(64, dtype=torch.int32)
+    with pytest.raises(ValueError, match="shares memory"):
+        int8.gemm(words.view(torch.int8)[:128].view(4, 32), None, w, None, out=words[16:48].view(4, 8))
+    with pytest.raises(ValueError, match="GPU"):
+        int8.gemm(q, qs, w, ws, out=far[:4], residual=far[:4])
+    with pytest.raises(ValueError, match="8192"):
+        int8.Int8Linear.prepare(torch.zeros(4, 8193, dtype=torch.int8), torch.ones(4), None, "cuda:0")
+
 
 def _cpu(m=4, n=8, k=32):
     return (torch.zeros(1, m, k, dtype=torch.int8), torch.ones(1, m), torch.zeros(n, k, dtype=torch.int8), torch.ones(n))
