@@ -14,6 +14,12 @@
 // WQ waves share out the rows (many queries), or WK waves the keys of each tile (few queries), whose parts meet in LDS. Where
 // that still leaves few workgroups the keys are split over several, whose parts a second launch joins.
 //
+// Measured (heads of 128, BF16, 8 on 4, causal): 32768 tokens with a window of 1023 174 us, 790 TFLOP/s of the pairs that are
+// seen (a large product reaches 1250); 10000 of them 74 to 80 us, in two rounds of workgroups of which the second fills a
+// quarter of the chip. Matrix instructions take half of such a wave's time: its softmax and the LDS reads are in line with
+// them, two waves a SIMD overlap in part, and the clock falls to 1.9 GHz. FP32: the matrix instruction (73 % of a tile's
+// cycles). One token of 16 sequences against 1028 keys each: 13 us in two launches, latency of 64 KB a CU and of the join.
+//
 // Keys outside the tile's range are read from its last key and masked. A masked score is -infinity whatever K holds, but a
 // product with its weight of 0 is NaN where V is infinite or NaN. Such a sum shows in the output: a workgroup that ends up
 // with a value that is not finite does its work a second time with those elements of V taken out of the product and added to
@@ -668,10 +674,12 @@ int plan_of(int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int
     p.rows = tq * (heads / kv_heads);
     const int64_t groups = batch * kv_heads;
     if (p.rows > INT32_MAX / 8 || groups > INT32_MAX / 8) return -1;
-    // Tiles of 32 rows fill the chip with fewer queries, tiles of 128 read keys a quarter as often: BF16, 8 heads of 128, windows
-    // of 128 to both sides, 5 clips of 750 (960 workgroups of 32 rows) 25 against 30 us, 8 clips (1536) 38 against 24. FP32, whose
-    // matrix instructions take longer than the reads, 8 clips 103 against 117, 16 (3072) 183 and 183.
-    p.few = p.rows <= 64 || (p.rows + 31) / 32 * groups <= (dtype == KEA_F32 && p.dp > 64 ? 2560 : 1024);
+    // Tiles of 32 rows fill the chip with fewer queries, tiles of 128 read keys a quarter as often. BF16, heads of 128: 3000 queries
+    // of 8 heads on 4 (752 tiles of 32), a window of 127 behind them 18 against 11 us, of 1023 36 and 32; 2048 queries (512) 11 and
+    // 11, 23 against 31; 4 clips of 750, 128 to both sides (768) 19 and 17, 2 (384) 12 against 16. FP32's matrix instructions take
+    // longer than the reads: heads of 64, 1024 tiles 91 and 86 (1023 behind), heads of 128, 1500 tiles 281 against 337.
+    const int64_t most_few = dtype != KEA_F32 ? 640 : p.dp > 64 ? 2560 : 1024;
+    p.few = p.rows <= 64 || (p.rows + 31) / 32 * groups <= most_few;
     const int64_t per = p.few ? 32 : 128;
     p.row_tiles = (int)((p.rows + per - 1) / per);
     const int64_t wgs = p.row_tiles * groups;
@@ -682,7 +690,11 @@ int plan_of(int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int
     const int64_t tile = dtype == KEA_F32 ? (p.dp == 64 ? 128 : p.dp == 128 ? 64 : 32) : p.dp == 256 ? 64 : 128;
     const int64_t blocks = (keys + tile - 1) / tile;
     p.splits = 1;
-    if (wgs > 0 && wgs < 256 && blocks > 3) {  // (the second launch takes as long as two or three tiles)
+    // Parts, where tiles of 32 rows leave CUs idle (or, of workgroups of one or two waves, SIMDs: FP32, heads of 128, 256 tiles 86 us
+    // whole and 56 in two parts; BF16, four waves, 16 and 20). The second launch takes as long as two or three tiles of keys, and
+    // parts of 128 rows are long: BF16, 240 such tiles 16 us whole, 27 in two parts.
+    const bool two_waves = p.dp >= (dtype == KEA_F32 ? 128 : 256);
+    if (p.few && wgs > 0 && wgs <= (two_waves ? 256 : 255) && blocks > 3) {
         int64_t s = 512 / wgs;  // up to two workgroups a CU
         s = s < blocks ? s : blocks;
         p.splits = (int)(s < 64 ? s : 64);
