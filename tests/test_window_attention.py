@@ -179,6 +179,50 @@ def test_seen_nan_scores_show(t, tq, dtype):
         assert got[0, :first].isfinite().all() and got[0, first:].isnan().all()
 
 
+MANY = [(60, 150, 4, 2, 64), (140, 150, 4, 2, 128), (260, 150, 2, 2, 80), (60, 150, 6, 2, 40), (130, 150, 4, 2, 256), (1, 2600, 8, 4, 64)]
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,t,h,hk,d", MANY)
+def test_many_rows(b, t, h, hk, d, dtype):
+    """Enough rows for the tiles of 128, which end in the middle of one: whole sequences, padded clips with NaN behind them,
+    the last tokens of ragged ones."""
+    g = torch.Generator().manual_seed(b + d)
+    q, k, v = heads(b, t, h, d, dtype, g), heads(b, t, hk, d, dtype, g), heads(b, t, hk, d, dtype, g)
+    check(window.attention(q, k, v, left=70, sinks=5), *expected(q, k, v, 70, 0, 5))
+    lengths = torch.randint(0, t + 1, (b,), generator=g, dtype=torch.int32)
+    lengths[:3] = torch.tensor([t, 0, 1], dtype=torch.int32)[:b]
+    for i, n in enumerate(lengths.tolist()):
+        k[i, n:], v[i, n:] = float("nan"), float("inf")
+    zeros = torch.zeros(b, dtype=torch.int32)
+    for left, right, sinks, starts in ((20, 16, 1, zeros), (None, None, 0, zeros), (31, 0, 2, None)):
+        got = window.attention(q, k, v, left=left, right=right, sinks=sinks, kv_lengths=lengths.to(DEV),
+                               q_starts=None if starts is None else starts.to(DEV))
+        check(got, *expected(q, k, v, left, right, sinks, lengths, starts))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows_and_bad_values(dtype):
+    """Tiles of 128 rows: infinities and NaN of keys and values reach the queries that see them and no others."""
+    g = torch.Generator().manual_seed(12)
+    b, t = 60, 150
+    q, k, v = heads(b, t, 4, 64, dtype, g), heads(b, t, 2, 64, dtype, g), heads(b, t, 2, 64, dtype, g)
+    want, err = expected(q, k, v, 20, 0, 1)
+    bad = 90  # seen by positions 90 .. 110
+    k[::2, bad], v[::2, bad], v[::2, bad - 1, 0] = float("nan"), float("inf"), float("-inf")
+    got = window.attention(q, k, v, left=20, sinks=1).cpu()
+    p = torch.arange(t)
+    sees = (p >= bad - 1) & (p <= bad + 20)
+    check(got[1::2], want[1::2], err[1::2])
+    check(got[::2, ~sees], want[::2, ~sees], err[::2, ~sees])
+    assert got[::2, bad:bad + 21].isnan().all() and (got[::2, bad - 1, :2] == float("-inf")).all()
+    check(got[::2, bad - 1, 2:], want[::2, bad - 1, 2:], err[::2, bad - 1, 2:])
+
+
 @pytest.mark.gpu
 @torch.inference_mode()
 @pytest.mark.parametrize("dtype", TYPES)
