@@ -92,6 +92,22 @@ def test_the_largest_sums_are_exact(m, n, k):
 
 @pytest.mark.gpu
 @torch.inference_mode()
+@pytest.mark.parametrize("m,n,k", [(6000, 2050, 641), (1500, 10243, 641), (2500, 5121, 1000), (1000, 2050, 1500), (8001, 257, 1500), (500, 5121, 1500)])
+def test_the_widest_tiles(m, n, k):
+    """Sizes that take tiles of 256 x 256, or four stages ahead, with ragged edges: the sums, and the epilogue's types."""
+    q, qs, w, ws = make(m, n, k, m)
+    want = sums(q, w)
+    assert torch.equal(int8.gemm(q, None, w, None, out_dtype=torch.int32).cpu().double(), want)
+    bias, residual = torch.linspace(-3, 3, n, device=DEV), torch.linspace(-2, 2, m * n, device=DEV).view(m, n)
+    for b, silu, res, dtype in ((bias, True, None, torch.bfloat16), (None, False, residual, torch.float32), (bias, False, None, torch.float16)):
+        rows = slice(m - 300, m)  # (the first and last rows: all have the sums of above)
+        got = int8.gemm(q, qs, w, ws, b, out_dtype=dtype, silu=silu, residual=res, residual_factor=0.5)
+        check(got[rows], *expected(q[:, rows], qs[:, rows], w, ws, b, silu, None if res is None else res[rows], 0.5, dtype))
+        check(got[:300], *expected(q[:, :300], qs[:, :300], w, ws, b, silu, None if res is None else res[:300], 0.5, dtype))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
 @pytest.mark.parametrize("scales", [torch.float32, torch.float16])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("m,n,k", [(1, 2560, 640), (16, 1024, 4096), (33, 1030, 641), (257, 513, 1025), (1000, 1024, 1024)])
