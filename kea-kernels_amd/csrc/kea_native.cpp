@@ -1,12 +1,14 @@
 // The host side of an operator call in one native call: argument checks on the tensors' own fields, the output and
 // workspace allocations and the library's launch, without the Python objects (shape tuples, dictionary keys, ctypes
-// conversions) that cost a call more than its two kernel launches. The module extends kea_kernels.lowbit: everything it does
+// conversions) that cost a call more than its two kernel launches. The module extends kea_kernels.lowbit, int8, norms and
+// window: everything it does
 // not take (tensor subclasses and transforms, arguments that would raise) it declines by returning None / False, and the
 // caller's Python path, which holds the full checks and their messages, runs instead.
 //
 // Calls in a row, host bound: Int8MmaLayer.linear at M = 128, N = 4096, K = 1024 (fp16 in and out) 13.2 -> 9.3 us, at one
 // row 13.2 -> 9.9, lowbit.quantize + lowbit.gemm with group scales 21.9 -> 12.9, the provider's call on a few rows 18.7 ->
-// 11.7; the two HIP launches are about 6 us of each.
+// 11.7; the two HIP launches are about 6 us of each. int8.gemm on one row 15.5 -> 5.1 (one launch), norms.block_norm 23 -> 6.5,
+// window.attention (two launches) 27 -> 13.
 #include <Python.h>
 
 #include <ATen/ATen.h>

@@ -3,7 +3,8 @@
 Drop-in for the reference package `kea_kernels` on its low-bit GEMM path: the same operator classes
 (binary.layer.Int8MmaLayer, binary.layer_parts, binary.provider), export formats (formats), the package-level
 load / transcribe / close (model) and the `python -m kea_kernels` command line, with the kernels in a prebuilt HIP
-library (lib/libkea_hip.so, C ABI in include/kea_lowbit.h).
+library (lib/libkea_hip.so, C ABI in include/kea_lowbit.h). Beside them the operators of a layer with 8-bit weights:
+int8.gemm, norms.block_norm and window.attention (include/kea_block.h).
 
     import kea_kernels
     model = kea_kernels.load("kea-b-0.1")           # a downloaded model directory; mode = the model's default
