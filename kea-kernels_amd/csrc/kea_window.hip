@@ -690,11 +690,13 @@ int plan_of(int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int
     const int64_t tile = dtype == KEA_F32 ? (p.dp == 64 ? 128 : p.dp == 128 ? 64 : 32) : p.dp == 256 ? 64 : 128;
     const int64_t blocks = (keys + tile - 1) / tile;
     p.splits = 1;
-    // Parts, where tiles of 32 rows leave CUs idle (or, of workgroups of one or two waves, SIMDs: FP32, heads of 128, 256 tiles 86 us
-    // whole and 56 in two parts; BF16, four waves, 16 and 20). The second launch takes as long as two or three tiles of keys, and
-    // parts of 128 rows are long: BF16, 240 such tiles 16 us whole, 27 in two parts.
-    const bool two_waves = p.dp >= (dtype == KEA_F32 ? 128 : 256);
-    if (p.few && wgs > 0 && wgs <= (two_waves ? 256 : 255) && blocks > 3) {
+    // Parts, where tiles of 32 rows leave CUs idle (one part more at 256 workgroups of four waves: BF16, heads of 128, 20 us
+    // against 16), or SIMDs, where a workgroup has one or two waves and no form of four (heads of 129 to 256). FP32, heads of 65
+    // to 128, has one from 129 workgroups on (750 frames of 8 heads, 128 to both sides, 26 us against 31 in two parts of two
+    // waves). The second launch takes as long as two or three tiles of keys, and parts of 128 rows are long: BF16, 240 such
+    // tiles 16 us whole, 27 in two parts.
+    const int64_t most_split = p.dp == 256 ? 256 : p.dp == 128 && dtype == KEA_F32 ? 128 : 255;
+    if (p.few && wgs > 0 && wgs <= most_split && blocks > 3) {
         int64_t s = 512 / wgs;  // up to two workgroups a CU
         s = s < blocks ? s : blocks;
         p.splits = (int)(s < 64 ? s : 64);
@@ -735,6 +737,12 @@ int run_shape(const Args &a, hipStream_t stream) {
 
 template <typename T, int DP>
 int run_heads(const Args &a, bool few, hipStream_t stream) {
+    if constexpr (sizeof(T) == 4 && DP == 128) {
+        // Four waves in place of two, alone on their CU (128 KB of LDS), where all workgroups find one: 750 frames of 8 heads, 16 to
+        // both sides, 14 against 20 us, 4 clips of 125 14 against 17; with 384 workgroups of five tiles 45 against 37.
+        const int64_t wgs = (int64_t)a.row_tiles * a.batch * a.kv_heads;
+        if (few && a.splits == 1 && wgs <= 256) return a.d == DP ? run_shape<T, DP, 1, 4, false>(a, stream) : run_shape<T, DP, 1, 4, true>(a, stream);
+    }
     // waves that share out keys: four of them where two buffers of their blocks fit LDS
     constexpr int WK = 2 * 2 * 4 * 32 * DP * (int)sizeof(T) <= 131072 ? 4 : 2 * 2 * 2 * 32 * DP * (int)sizeof(T) <= 131072 ? 2 : 1;
     if (a.d == DP) return few ? run_shape<T, DP, 1, WK, false>(a, stream) : run_shape<T, DP, 4, 1, false>(a, stream);
