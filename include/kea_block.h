@@ -85,7 +85,7 @@ typedef struct {
  * hold there; k and v at len and behind are not read. Scores, their maximum and sum and the output's sums are FP32; the
  * weights exp(s - max) are rounded to the type for the product with v (KEA_F16, KEA_BF16).
  *   dtype        of q, k, v and out: KEA_F32, KEA_F16 or KEA_BF16. d a multiple of 8, at most 256; every pointer and stride
- *                a multiple of 16 bytes.
+ *                a multiple of 16 bytes, strides not negative. out overlaps no input.
  *   kv_lengths   int32 [batch], NULL: tk for each.  q_starts: int32 [batch], NULL: len - tq (the last tokens).
  *   left, right  >= 0; 2^30 and above: without bound.  sinks >= 0.  tq, tk <= 2^30.
  *   workspace    kea_window_attention_workspace bytes, 16-byte aligned (0: may be NULL): the unnormalised outputs, maxima and

@@ -13,7 +13,7 @@
 //                 their next operands at once; reading one tile's operands for all tiles, out of L2, takes as long.
 //   split_kernel  few output tiles (few tokens): a workgroup owns 16 RM x 16 RN outputs, its NW waves share out k, each
 //                 loading its operands straight into registers, and the exact int32 sums meet in LDS. 1 x 2560 x 640 takes
-//                 2.9 us, of which an empty launch is 1.6; 16 x 1024 x 4096 5.7, at the rate at which 64 CUs take in the
+//                 3.8 us, of which an empty launch is 1.6; 16 x 1024 x 4096 6.6, at the rate at which 64 CUs take in the
 //                 128 KB each of them needs.
 #include <hip/hip_runtime.h>
 
