@@ -56,11 +56,16 @@ def _parameters(norm, d: int) -> tuple:
     """(kind, weight, bias, eps) of a torch.nn norm of d elements whose parameters are its own (LookupError otherwise)."""
     if norm is None:
         return _NO_PARAMETERS
-    own = norm.__dict__["_parameters"]
+    fields = norm.__dict__
+    own = fields["_parameters"]
     if tuple(norm.normalized_shape) != (d,):
         raise LookupError
+    kind = 1 if "bias" in own else 2
+    # (a bias kept elsewhere makes a LayerNorm too; hasattr on a plain RMSNorm would cost a microsecond)
+    if kind == 2 and ("bias" in fields or "bias" in fields["_buffers"] if type(norm) is torch.nn.RMSNorm else hasattr(norm, "bias")):
+        raise LookupError
     eps = norm.eps
-    return 1 if "bias" in own else 2, own["weight"], own.get("bias"), torch.finfo(torch.float32).eps if eps is None else eps
+    return kind, own["weight"], own.get("bias"), torch.finfo(torch.float32).eps if eps is None else eps
 
 
 def _native(x, block, post, gate, act, factor, pre, quantize, out) -> tuple | None:

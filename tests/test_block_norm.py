@@ -11,6 +11,8 @@ from types import SimpleNamespace
 
 import pytest
 import torch
+import torch.nn.utils.parametrize
+import torch.nn.utils.prune
 
 from kea_kernels import _hip, lowbit, norms
 
@@ -364,3 +366,26 @@ def test_library_refusals():
                        (dict(z=None, q=p, ldq=32), -1), (dict(b=None), -1), (dict(x=p + 2), -2), (dict(z=p + 1), -2), (dict(x=None), -1),
                        (dict(pre=_hip.Norm(3, 0, None, None, 0.0)), -1), (dict(pre=_hip.Norm(1, 0, p + 2, None, 0.0)), -1), (dict(m=0), 0)]:
         assert L.kea_block_norm(*(good | change).values()) == rc, change
+
+
+def test_a_bias_that_is_no_parameter_makes_a_layer_norm():
+    """The native call takes a module's own parameters; a bias that a LayerNorm keeps elsewhere (pruned, parametrized, as a
+    buffer, an attribute) is not taken for the bias that an RMSNorm lacks."""
+    class Shifted(torch.nn.Module):
+        def forward(self, b):
+            return b + 1
+
+    pruned, parametrized, buffered, plain = (torch.nn.LayerNorm(8) for _ in range(4))
+    torch.nn.utils.prune.identity(pruned, "bias")
+    torch.nn.utils.parametrize.register_parametrization(parametrized, "bias", Shifted())
+    del buffered.bias, plain.bias
+    buffered.register_buffer("bias", torch.ones(8))
+    plain.bias = torch.ones(8)
+    odd = torch.nn.RMSNorm(8)
+    odd.bias = torch.ones(8)
+    for m in (pruned, parametrized, buffered, plain, odd):
+        with pytest.raises(LookupError):
+            norms._parameters(m, 8)
+        assert norms._norm("pre", m, 8, torch.device("cpu"))[0].kind == 1
+    assert [norms._parameters(m, 8)[0] for m in (None, torch.nn.LayerNorm(8), torch.nn.LayerNorm(8, bias=False), torch.nn.RMSNorm(8))] == [0, 1, 1, 2]
+    assert norms._parameters(type("Own", (torch.nn.RMSNorm,), {})(8), 8)[0] == 2
