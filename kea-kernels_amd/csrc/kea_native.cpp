@@ -474,7 +474,7 @@ PyObject *native_int8_gemm(PyObject *, PyObject *const *args, Py_ssize_t count) 
     Py_RETURN_NONE;
 }
 
-// A norm given as (kind, weight, bias, eps) in four arguments; its parameters are read as they are, detached.
+// A norm given as (kind, weight, bias, eps) in four arguments; false where autograd would have to record its parameters.
 bool norm_of(PyObject *const *args, int64_t d, c10::Device device, kea_norm *n) {
     int64_t kind;
     double eps;
@@ -486,7 +486,7 @@ bool norm_of(PyObject *const *args, int64_t d, c10::Device device, kea_norm *n) 
         if (!THPVariable_Check(args[1 + i])) return false;
         const at::Tensor &t = THPVariable_Unpack(args[1 + i]);
         if (!t.defined() || t.device() != device || t.layout() != at::kStrided || !t.has_storage() || !t.is_contiguous() || t.numel() != d ||
-            t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
+            (t.requires_grad() && c10::GradMode::is_enabled()) || t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
                                                      c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Negative})))
             return false;
         const int c = code_of(t.scalar_type());

@@ -179,7 +179,7 @@ class Int8Linear:
             raise ValueError(f"input on {x.device}, layer on {self.device}")
         if x.dim() < 1 or x.shape[-1] != self.in_features:
             raise ValueError(f"expected [..., {self.in_features}] input, got {tuple(x.shape)}")
-        _hip.refuse_grad("Int8Linear", x)
+        _hip.refuse_grad("Int8Linear", x, getattr(norm, "weight", None), getattr(norm, "bias", None))
         lead, m = x.shape[:-1], math.prod(x.shape[:-1])
         if m == 0:
             return torch.empty(*lead, self.out_features, device=self.device, dtype=out_dtype)

@@ -14,7 +14,7 @@ _ACTS = {"": 0, "sigmoid": 1, "tanh": 2}
 
 
 def _norm(name: str, norm, d: int, device) -> tuple:
-    """(the C description, the tensors to keep until the launch) of a norm: a LayerNorm has a `bias` (which may be None), an
+    """(the C description, the parameters, to keep until the launch) of a norm: a LayerNorm has a `bias` (which may be None), an
     RMSNorm has none; `weight` may be None, `eps` None stands for FP32's epsilon as in torch.nn.RMSNorm."""
     if norm is None:
         return _NO_NORM, ()
@@ -23,7 +23,6 @@ def _norm(name: str, norm, d: int, device) -> tuple:
     if tuple(shape) != (d,):
         raise ValueError(f"{name} normalizes {tuple(shape)}, the rows have {d} elements")
     w, b = norm.weight, getattr(norm, "bias", None)
-    w, b = (None if t is None else t.detach() for t in (w, b))
     for what, t in (("weight", w), ("bias", b)):
         if t is not None and (t.numel() != d or t.device != device or not t.is_contiguous() or t.dtype not in _hip.DTYPES):
             raise ValueError(f"{name}.{what} must be a contiguous f32, f16 or bf16 tensor of {d} elements on {device}")
@@ -87,7 +86,8 @@ def block_norm(x: Tensor, block: Tensor | None, *, post=None, gate: Tensor | Non
 
     x [..., d] is the residual stream, block [..., d] the output of the block in the same shape, each f32, f16 or bf16; y
     has x's type (`out` receives it if given; it may be x or the block itself), z the block's. post and pre: modules with
-    weight, bias and eps (torch.nn.LayerNorm) or weight and eps (torch.nn.RMSNorm). gate: [G, d] in the block's type, any
+    weight, bias and eps (torch.nn.LayerNorm) or weight and eps (torch.nn.RMSNorm); there is no backward, so like the tensors
+    their parameters must not require grad while autograd records. gate: [G, d] in the block's type, any
     leading dimensions of G elements, M a multiple of G: M / G rows in turn share a gate row (G = 1 a gate for each channel,
     G = the batch one for each sequence, G = M one for each token), passed through gate_activation ("", "sigmoid", "tanh").
     Everything is FP32 up to one rounding of each output: z is the norm of y before y's rounding. block None (then without
@@ -131,6 +131,8 @@ def block_norm(x: Tensor, block: Tensor | None, *, post=None, gate: Tensor | Non
     _hip.refuse_grad("block_norm", x, block, gate, out)
     pn, keep0 = _norm("post", post, d, device)
     nn, keep1 = _norm("pre", pre, d, device)
+    stream = _hip.stream_handle(device) if m else 0
+    _hip.refuse_grad("block_norm", *keep0, *keep1)
     y = x if block is None else torch.empty(x.shape, dtype=x.dtype, device=device) if out is None else out
     if block is not None and yr is None:
         yr = y.view(-1, d) if y.numel() else y.new_empty(0, d)
@@ -148,7 +150,7 @@ def block_norm(x: Tensor, block: Tensor | None, *, post=None, gate: Tensor | Non
                 _stride(br) if br is not None else 0, m, d, pn, _hip.ptr(gr), _stride(gr) if gr is not None else 0,
                 m // gr.shape[0] if gr is not None else 1, _ACTS[gate_activation], float(factor),
                 _hip.ptr(yr), _stride(yr) if yr is not None else 0, nn, _hip.ptr(z), d, _hip.ptr(q), ldq, _hip.ptr(qs),
-                _hip.stream_handle(device))
+                stream)
         _hip.check(rc, "kea_block_norm")
     del keep0, keep1
     return (y, q, qs) if quantize else (y, z)

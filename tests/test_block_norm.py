@@ -389,3 +389,32 @@ def test_a_bias_that_is_no_parameter_makes_a_layer_norm():
         assert norms._norm("pre", m, 8, torch.device("cpu"))[0].kind == 1
     assert [norms._parameters(m, 8)[0] for m in (None, torch.nn.LayerNorm(8), torch.nn.LayerNorm(8, bias=False), torch.nn.RMSNorm(8))] == [0, 1, 1, 2]
     assert norms._parameters(type("Own", (torch.nn.RMSNorm,), {})(8), 8)[0] == 2
+
+
+def test_parameters_that_require_grad_are_refused():
+    """Without rows, so that the refusal is all that can happen."""
+    x = torch.zeros(0, 8)
+    fresh, frozen = torch.nn.LayerNorm(8), torch.nn.RMSNorm(8).requires_grad_(False)
+    half = torch.nn.LayerNorm(8).requires_grad_(False)
+    half.bias.requires_grad_()
+    for kw in (dict(pre=fresh), dict(post=fresh, pre=frozen), dict(pre=half)):
+        with pytest.raises(RuntimeError, match="inference only"):
+            norms.block_norm(x, x, **kw)
+        with torch.no_grad():
+            norms.block_norm(x, x, **kw)
+    with pytest.raises(RuntimeError, match="inference only"):
+        norms.block_norm(x, None, pre=fresh)
+    norms.block_norm(x, x, post=frozen, pre=frozen)
+
+
+@pytest.mark.gpu
+def test_parameters_that_require_grad_are_refused_on_the_gpu():
+    x = torch.randn(4, 64, device=DEV)
+    fresh = torch.nn.LayerNorm(64, device=DEV)
+    frozen = torch.nn.LayerNorm(64, device=DEV).requires_grad_(False)
+    want = norms.block_norm(x, x, pre=frozen)
+    for kw in (dict(pre=fresh), dict(post=fresh, pre=frozen), dict(pre=fresh, quantize=True)):
+        with pytest.raises(RuntimeError, match="inference only"):
+            norms.block_norm(x, x, **kw)
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(norms.block_norm(x, x, pre=fresh), want))

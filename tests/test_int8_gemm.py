@@ -379,3 +379,12 @@ def test_launches_are_made_from_the_tensors_device(monkeypatch):
         assert entered == [1]
     with _hip.on_device(torch.device("cuda", 0)):
         assert entered == [1]
+
+
+def test_a_norm_that_requires_grad_is_refused():
+    layer = int8.Int8Linear(torch.zeros(4, 16, dtype=torch.int8), torch.ones(4), None)
+    with pytest.raises(RuntimeError, match="inference only"):
+        layer.linear(torch.zeros(2, 16), norm=torch.nn.LayerNorm(16))
+    with pytest.raises(RuntimeError, match="inference only"):
+        layer.linear(torch.zeros(0, 16), norm=torch.nn.LayerNorm(16))
+    assert layer.linear(torch.zeros(0, 16), norm=torch.nn.LayerNorm(16).requires_grad_(False)).shape == (0, 4)
