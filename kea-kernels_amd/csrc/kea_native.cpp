@@ -42,7 +42,7 @@ struct Library {
 } lib;
 
 // The tensor behind an exact torch.Tensor whose memory a kernel may read as it is: on a GPU, strided, no transform
-// (functorch, lazy negation or conjugation), nothing that autograd would have to record. nullptr otherwise.
+// (functorch, lazy negation or conjugation), nothing that autograd would have to record or carry on. nullptr otherwise.
 const at::Tensor *plain(PyObject *o) {
     if (!THPVariable_CheckExact(o)) return nullptr;
     const at::Tensor &t = THPVariable_Unpack(o);
@@ -52,7 +52,7 @@ const at::Tensor *plain(PyObject *o) {
                                               c10::DispatchKey::Negative, c10::DispatchKey::Conjugate,
                                               c10::DispatchKey::ZeroTensor});
     if (t.key_set().has_any(transforms)) return nullptr;
-    if (t.requires_grad() && c10::GradMode::is_enabled()) return nullptr;
+    if ((t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined()) return nullptr;
     return &t;
 }
 
@@ -486,7 +486,7 @@ bool norm_of(PyObject *const *args, int64_t d, c10::Device device, kea_norm *n) 
         if (!THPVariable_Check(args[1 + i])) return false;
         const at::Tensor &t = THPVariable_Unpack(args[1 + i]);
         if (!t.defined() || t.device() != device || t.layout() != at::kStrided || !t.has_storage() || !t.is_contiguous() || t.numel() != d ||
-            (t.requires_grad() && c10::GradMode::is_enabled()) || t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
+            (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined() || t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
                                                      c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Negative})))
             return false;
         const int c = code_of(t.scalar_type());

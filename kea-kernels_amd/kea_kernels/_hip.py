@@ -18,6 +18,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libkea_hip.so"
 NATIVE_PATH = LIB_PATH.with_name("kea_native.so")
@@ -183,9 +184,12 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 
 def refuse_grad(what: str, *tensors: torch.Tensor | None) -> None:
-    """RuntimeError where autograd would have to record a call: the kernels have no backward."""
+    """RuntimeError where autograd would have to record a call, or to carry a tangent through it (forward mode): the kernels
+    have no derivatives."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} is inference only: an input requires grad")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} is inference only: an input carries a forward-mode tangent")
 
 
 def on_device(device: torch.device):

@@ -4,9 +4,11 @@ a model would, against the same layer in 64 bits."""
 from __future__ import annotations
 
 import math
+from types import SimpleNamespace
 
 import pytest
 import torch
+import torch.autograd.forward_ad
 
 from kea_kernels import _hip, int8, lowbit, norms, window
 
@@ -184,3 +186,40 @@ def test_a_missing_native_library_is_an_error(monkeypatch):
     monkeypatch.setattr(_hip, "native", missing)
     with pytest.raises(RuntimeError, match="missing"):
         window.attention(*(torch.zeros(1, 1, 1, 64),) * 3)
+
+
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor requires no grad, but its tangent would be lost all the same."""
+    x, q, qs = torch.zeros(0, 16), torch.zeros(0, 16, dtype=torch.int8), torch.ones(0)
+    w, ws, bias, heads = torch.zeros(4, 16, dtype=torch.int8), torch.ones(4), torch.zeros(4), torch.zeros(1, 0, 1, 8)
+    norm = torch.nn.RMSNorm(16).requires_grad_(False)
+    layer = int8.Int8Linear(w, ws, None)
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        moving = SimpleNamespace(weight=dual(torch.ones(16)), eps=1e-5)
+        calls = [lambda: norms.block_norm(dual(x), x), lambda: norms.block_norm(x, dual(x), pre=norm), lambda: norms.block_norm(x, x, pre=moving),
+                 lambda: int8.gemm(q, qs, w, ws, dual(bias)), lambda: int8.gemm(q, dual(qs), w, ws), lambda: layer.linear(dual(x)),
+                 lambda: window.attention(dual(heads), heads, heads), lambda: window.attention(heads, heads, dual(heads))]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="inference only"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="inference only"):  # (which leaves forward mode on)
+                call()
+            with torch.inference_mode():
+                call()
+        norms.block_norm(x, x, pre=norm)
+        window.attention(heads, heads, heads)
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_are_refused_on_the_gpu():
+    x, norm, moving = torch.randn(3, 64, device=DEV), *(torch.nn.RMSNorm(64, device=DEV).requires_grad_(False) for _ in range(2))
+    q, qs, w, ws = torch.zeros(3, 64, dtype=torch.int8, device=DEV), torch.ones(3, device=DEV), torch.zeros(4, 64, dtype=torch.int8, device=DEV), torch.ones(4, device=DEV)
+    heads = torch.randn(1, 5, 2, 64, device=DEV)
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        moving._parameters["weight"] = dual(moving.weight)  # (as torch.func.functional_call leaves it)
+        for call in (lambda: norms.block_norm(x, dual(x), pre=norm), lambda: norms.block_norm(x, x, pre=moving), lambda: int8.gemm(q, dual(qs), w, ws), lambda: window.attention(heads, dual(heads), heads)):
+            with pytest.raises(RuntimeError, match="inference only"):
+                call()
+        norms.block_norm(x, x, pre=norm), int8.gemm(q, qs, w, ws), window.attention(heads, heads, heads)
