@@ -41,7 +41,8 @@ def pad_rows(weight: Tensor) -> Tensor:
     n, k = weight.shape
     if weight.data_ptr() % 16 == 0 and (k <= 1 or weight.stride(1) == 1) and (n <= 1 or (
             weight.stride(0) % 16 == 0 and weight.stride(0) >= lowbit.round_up(k, 16))):
-        if n > 1 or weight.untyped_storage().nbytes() - weight.storage_offset() >= lowbit.round_up(k, 16):
+        end = weight.storage_offset() + (n - 1) * (weight.stride(0) if n > 1 else 0) + lowbit.round_up(k, 16)
+        if end <= weight.untyped_storage().nbytes():  # (the last row is read to a multiple of 16 bytes)
             return weight
     rows = torch.zeros(n, lowbit.round_up(k, 16), dtype=torch.int8, device=weight.device)
     rows[:, :k] = weight

@@ -388,3 +388,16 @@ def test_a_norm_that_requires_grad_is_refused():
     with pytest.raises(RuntimeError, match="inference only"):
         layer.linear(torch.zeros(0, 16), norm=torch.nn.LayerNorm(16))
     assert layer.linear(torch.zeros(0, 16), norm=torch.nn.LayerNorm(16).requires_grad_(False)).shape == (0, 4)
+
+
+@pytest.mark.parametrize("n,k,ld,offset", [(2, 10, 16, 0), (5, 20, 32, 0), (3, 1, 16, 0), (2, 16, 32, 16), (1, 10, 16, 0), (4, 31, 48, 32)])
+def test_pad_rows_gives_what_gemm_takes(n, k, ld, offset):
+    """Rows whose storage ends with the last one's elements, short of 16 bytes, are copied; with the bytes there they are not."""
+    for tail, kept in ((0, k % 16 == 0), (lowbit.round_up(k, 16) - k, True)):
+        flat = torch.arange(offset + (n - 1) * ld + k + tail).to(torch.int8)
+        w = flat.as_strided((n, k), (ld, 1), offset)
+        rows = int8.pad_rows(w)
+        assert torch.equal(rows, w) and (rows.data_ptr() == w.data_ptr()) == kept
+        q, qs, _, ws = _cpu(k=lowbit.round_up(k, 16), n=n)
+        with pytest.raises(ValueError, match="GPU"):  # all that is left to refuse
+            int8.gemm(q, qs, rows, ws)
