@@ -87,7 +87,7 @@ typedef struct {
  *   dtype        of q, k, v and out: KEA_F32, KEA_F16 or KEA_BF16. d a multiple of 8, at most 256; every pointer and stride
  *                a multiple of 16 bytes, strides not negative. out overlaps no input.
  *   kv_lengths   int32 [batch], NULL: tk for each.  q_starts: int32 [batch], NULL: len - tq (the last tokens).
- *   left, right  >= 0; 2^30 and above: without bound.  sinks >= 0.  tq, tk <= 2^30.
+ *   left, right  >= 0; 2^30 and above: without bound.  sinks >= 0.  tq, tk <= 2^30.  scale: finite.
  *   workspace    kea_window_attention_workspace bytes, 16-byte aligned (0: may be NULL): the unnormalised outputs, maxima and
  *                sums of parts of the keys where few queries meet many, written before they are read. */
 int64_t kea_window_attention_workspace(int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads,

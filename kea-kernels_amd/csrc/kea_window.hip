@@ -26,6 +26,7 @@
 // the queries that see them, and (FP32 and BF16) with weights of at most 2^-32, whose sums with V's largest numbers are finite.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 #include <string>
 
@@ -271,6 +272,9 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
             if (a.scale < 0)
 #pragma unroll
                 for (int c = 0; c < 2 * QF; ++c) qx[c] = -qx[c];
+            if (a.scale == 0)
+#pragma unroll
+                for (int c = 0; c < 2 * QF; ++c) qx[c] *= 0.0f;
         } else {
 #pragma unroll
             for (int c = 0; c < QF; ++c) qf[c] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
@@ -281,9 +285,15 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
             if (a.scale < 0)
 #pragma unroll
                 for (int c = 0; c < QF; ++c) qf[c] ^= (short)0x8000;
+            if (a.scale == 0)
+#pragma unroll
+                for (int c = 0; c < QF; ++c)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) qf[c][e] = __builtin_bit_cast(short, (T)((float)__builtin_bit_cast(T, (short)qf[c][e]) * 0.0f));
         }
     }
-    const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);  // (0 would make a masked score's -infinity NaN)
+    // (a scale of 0 would make a masked score's -infinity NaN: it is in the queries then)
+    const float scale = a.scale != 0 ? fabsf(a.scale) * kLog2e : 1.0f;
 
     v16f o[DB];
     float m = -INFINITY, l = 0.0f;  // l: this half's keys
@@ -791,6 +801,7 @@ int kea_window_attention(const kea_heads *q, const kea_heads *k, const kea_heads
     const int64_t unit = dtype == KEA_F32 ? 4 : 8;
     if (!heads_ok(q, unit) || !heads_ok(k, unit) || !heads_ok(v, unit) || !heads_ok(out, unit) || (uintptr_t)kv_lengths % 4 || (uintptr_t)q_starts % 4)
         return kea::fail(KEA_EALIGN, "kea_window_attention: pointers and strides are multiples of 16 bytes, strides not negative");
+    if (!std::isfinite(scale)) return kea::fail(KEA_EINVAL, "kea_window_attention: the scale is not finite");
     if (batch == 0 || tq == 0) return KEA_OK;
     if (!q->data_dev || !out->data_dev || (tk > 0 && (!k->data_dev || !v->data_dev))) return kea::fail(KEA_EINVAL, "kea_window_attention: a pointer is missing");
     if (workspace_bytes < p.part_bytes + p.stats_bytes || (p.splits > 1 && !workspace)) return kea::fail(KEA_ESPACE, "kea_window_attention: the workspace is too small");

@@ -5,6 +5,7 @@ captured into a graph.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -80,6 +81,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, left: int | None = None, right
         _heads(name, t, b, None, d, q.dtype, device)
     if v.shape != k.shape:
         raise ValueError(f"k is {tuple(k.shape)}, v {tuple(v.shape)}")
+    scale = 1 / math.sqrt(d) if scale is None else ctypes.c_float(scale).value
+    if not math.isfinite(scale):
+        raise ValueError("scale is not a finite FP32 number")
     left, right, sinks = _bound("left", left), _bound("right", right), _bound("sinks", 0 if sinks is None else sinks)
     for name, t in (("kv_lengths", kv_lengths), ("q_starts", q_starts)):
         if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (b,) or not t.is_contiguous() or t.device != device):
@@ -103,7 +107,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, left: int | None = None, right
         need = L.kea_window_attention_workspace(code, b, tq, tk, h, hk, d, left, right, sinks)
         ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
         rc = L.kea_window_attention(_describe(q), _describe(k), _describe(v), _describe(out), code, b, tq, tk, h, hk, d,
-                                    left, right, sinks, 1 / math.sqrt(d) if scale is None else float(scale),
+                                    left, right, sinks, scale,
                                     _hip.ptr(kv_lengths), _hip.ptr(q_starts), _hip.ptr(ws), max(need, 0),
                                     _hip.stream_handle(device))
     _hip.check(rc, "kea_window_attention")

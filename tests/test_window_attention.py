@@ -349,3 +349,42 @@ def test_library_refusals():
                        (dict(o=_hip.Heads(p, 64, 66, 64)), -2), (dict(ln=p + 2), -2), (dict(q=_hip.Heads(None, 64, 64, 64)), -1), (dict(b=0), 0)]:
         assert L.kea_window_attention(*(good | change).values()) == rc, change
     assert L.kea_window_attention_workspace(0, 1, 1, 1, 3, 2, 64, 0, 0, 0) < 0
+
+
+def test_a_scale_that_is_no_number_is_refused():
+    q = torch.zeros(1, 0, 2, 64)
+    for scale in (float("nan"), float("inf"), -float("inf"), 1e300):
+        with pytest.raises(ValueError, match="scale"):
+            window.attention(q, q, q, scale=scale)
+    t, L = _hip.Heads(16, 64, 64, 64), _hip.lib()
+    for scale in (float("nan"), float("inf")):
+        assert L.kea_window_attention(t, t, t, t, 0, 0, 1, 1, 2, 1, 64, 0, 0, 0, scale, None, None, None, 0, None) == -1
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("tq", [1, 60])
+def test_scales_at_the_end_of_the_range(tq):
+    """A scale of zero weighs all keys alike whatever their products, one of 2^-126 and below is taken as it is. (Its product with
+    log2(e) is off by at most 2^-150, 1.5 u of 2^-127, where a bound of u is counted: the sum of d products has 4 u to spare.)"""
+    g = torch.Generator().manual_seed(21)
+    q, k, v = heads(2, tq, 2, 64, F32, g, 2.0**60), heads(2, 70, 2, 64, F32, g, 2.0**60), heads(2, 70, 2, 64, F32, g)
+    for scale in (0.0, 1.25 * 2.0**-126, -2.0**-127):
+        want, err = expected(q, k, v, 30, 0, 1, scale=scale)
+        check(window.attention(q, k, v, left=30, sinks=1, scale=scale), want, err)
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_scale_of_zero(dtype):
+    """The mean of what is seen, and NaN for a query that is no number."""
+    g = torch.Generator().manual_seed(22)
+    q, k, v = heads(2, 40, 2, 64, dtype, g, 100), heads(2, 40, 2, 64, dtype, g, 100), heads(2, 40, 2, 64, dtype, g)
+    want, err = expected(q, k, v, 9, 0, 1, scale=0.0)
+    q[0, 5, 1, 7], q[1, 9, 0, 3] = float("nan"), float("inf")
+    got = window.attention(q, k, v, left=9, sinks=1, scale=0.0)
+    bad = torch.zeros(2, 40, 2, dtype=torch.bool)
+    bad[0, 5, 1] = bad[1, 9, 0] = True
+    assert got[bad].isnan().all()
+    check(got[~bad], want[~bad], err[~bad])
