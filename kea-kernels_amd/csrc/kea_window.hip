@@ -695,7 +695,7 @@ int plan_of(int dtype, int64_t batch, int64_t tq, int64_t tk, int64_t heads, int
     const int64_t wgs = p.row_tiles * groups;
     // the keys that a tile of rows can meet
     const int64_t most = 1 << 30, span = per / (heads / kv_heads) + 2;
-    const int64_t window = left >= most || right >= most ? tk : left + right + span + sinks;
+    const int64_t window = left >= most || right >= most ? tk : left + right + span + (sinks < tk ? sinks : tk);
     const int64_t keys = window < tk ? window : tk;
     const int64_t tile = dtype == KEA_F32 ? (p.dp == 64 ? 128 : p.dp == 128 ? 64 : 32) : p.dp == 256 ? 64 : 128;
     const int64_t blocks = (keys + tile - 1) / tile;

@@ -388,3 +388,11 @@ def test_a_scale_of_zero(dtype):
     bad[0, 5, 1] = bad[1, 9, 0] = True
     assert got[bad].isnan().all()
     check(got[~bad], want[~bad], err[~bad])
+
+
+def test_any_number_of_first_tokens():
+    """As many first tokens as an int64 says: the parts of the keys are those of all keys seen."""
+    L = _hip.lib()
+    want = L.kea_window_attention_workspace(2, 1, 1, 5000, 2, 2, 64, 10, 0, 5000)
+    for sinks in (1 << 30, (1 << 63) - 1):
+        assert L.kea_window_attention_workspace(2, 1, 1, 5000, 2, 2, 64, 10, 0, sinks) == want > 0
