@@ -66,7 +66,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, left: int | None = None, right
     None: Tk); q_starts int32 [B] (None: len - Tq, the queries are the last tokens). For padded clips q_starts is zeros and
     kv_lengths the clips' lengths; for tokens against a cache kv_lengths counts them too. Queries that see nothing (or
     scores of -infinity alone), or stand outside 0 .. len - 1 (padding), give zeros. What a query does not see has no part in
-    its output, whatever it holds. scale: 1 / sqrt(D) unless given. out must not overlap q, k or v."""
+    its output, whatever it holds. scale: 1 / sqrt(D) unless given. out must not overlap an
+    input."""
     if out is None and (hit := _native(q, k, v, left, right, sinks, scale, kv_lengths, q_starts)) is not None:
         return hit
     if q.dim() != 4 or k.dim() != 4 or q.dtype not in _hip.DTYPES:
@@ -95,8 +96,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, left: int | None = None, right
         steps = sorted((out.stride(i), out.shape[i]) for i in range(4) if out.shape[i] > 1)
         if any(s < reach for (s, _), reach in zip(steps[1:], (a * n for a, n in steps))) or any(s < 1 for s, _ in steps):
             raise ValueError(f"out has elements that share memory: strides {out.stride()}")
-        if out.numel() and any(t.numel() and _span(out)[0] < _span(t)[1] and _span(t)[0] < _span(out)[1] for t in (q, k, v)):
-            raise ValueError("out overlaps q, k or v")
+        others = [t for t in (q, k, v, kv_lengths, q_starts) if t is not None and t.numel()]
+        if out.numel() and any(_span(out)[0] < _span(t)[1] and _span(t)[0] < _span(out)[1] for t in others):
+            raise ValueError("out overlaps q, k or v, or the lengths or starts")
     _hip.refuse_grad("window.attention", q, k, v, out)
     if out is None:
         out = torch.empty(b, tq, h, d, dtype=q.dtype, device=device)

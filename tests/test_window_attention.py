@@ -396,3 +396,13 @@ def test_any_number_of_first_tokens():
     want = L.kea_window_attention_workspace(2, 1, 1, 5000, 2, 2, 64, 10, 0, 5000)
     for sinks in (1 << 30, (1 << 63) - 1):
         assert L.kea_window_attention_workspace(2, 1, 1, 5000, 2, 2, 64, 10, 0, sinks) == want > 0
+
+
+def test_an_out_over_the_lengths_is_refused():
+    q, words = torch.zeros(2, 5, 4, 8), torch.zeros(400, dtype=torch.int32)
+    out = words[:320].view(torch.float32).view(2, 5, 4, 8)
+    for kw in (dict(kv_lengths=words[318:320]), dict(q_starts=words[:2])):
+        with pytest.raises(ValueError, match="overlaps"):
+            window.attention(q, q, q, out=out, **kw)
+    with pytest.raises(ValueError, match="GPU"):
+        window.attention(q, q, q, out=out, kv_lengths=words[320:322])
