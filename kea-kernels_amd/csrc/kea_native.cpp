@@ -412,16 +412,18 @@ bool rows_of(const at::Tensor &t, int64_t *rows, int64_t *stride) {
     return true;
 }
 
-// Whether the bytes from a's first element to its last and from b's meet. (An output that lies between an input's rows meets
-// it too; the Python path sorts that out.)
-bool meet(const at::Tensor &a, const at::Tensor &b) {
-    auto end = [](const at::Tensor &t) {
-        int64_t last = 1;
-        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
-        return (uintptr_t)t.const_data_ptr() + last * t.element_size();
-    };
-    return (uintptr_t)a.const_data_ptr() < end(b) && (uintptr_t)b.const_data_ptr() < end(a);
+// Whether the bytes from a's first element to its last meet b's (or `bytes` at b). (An output that lies between an input's
+// rows meets it too; the Python path sorts that out.)
+int64_t reach(const at::Tensor &t) {
+    int64_t last = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return last * (int64_t)t.element_size();
 }
+bool meet(const at::Tensor &a, const void *b, int64_t bytes) {
+    const uintptr_t from = (uintptr_t)a.const_data_ptr(), other = (uintptr_t)b;
+    return b && from < other + bytes && other < from + reach(a);
+}
+bool meet(const at::Tensor &a, const at::Tensor &b) { return meet(a, b.const_data_ptr(), reach(b)); }
 
 // int8 rows [.., k] that start at multiples of 16 bytes, the last one readable to a multiple of 16 of `k` elements.
 bool rows8(const at::Tensor &t, int64_t dim, int64_t k, int64_t *ld) {
@@ -525,6 +527,10 @@ PyObject *native_block_norm(PyObject *, PyObject *const *args, Py_ssize_t count)
             return t.scalar_type() == out->scalar_type() && t.const_data_ptr() == out->const_data_ptr() && (m == 1 || ld == ldy);
         };
         if ((!same(*x, ldx) && meet(*out, *x)) || (!same(*block, ldb) && meet(*out, *block)) || (gate && meet(*out, *gate))) Py_RETURN_NONE;
+        for (const kea_norm *n : {&post, &pre}) {
+            const int64_t bytes = d * (n->dtype == KEA_F32 ? 4 : 2);
+            if (meet(*out, n->w_dev, bytes) || meet(*out, n->b_dev, bytes)) Py_RETURN_NONE;
+        }
     }
     try {
         const auto options = at::TensorOptions().device(device);

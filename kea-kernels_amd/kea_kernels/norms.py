@@ -131,6 +131,8 @@ def block_norm(x: Tensor, block: Tensor | None, *, post=None, gate: Tensor | Non
     _hip.refuse_grad("block_norm", x, block, gate, out)
     pn, keep0 = _norm("post", post, d, device)
     nn, keep1 = _norm("pre", pre, d, device)
+    if yr is not None and any(_hip.rows_meet(yr, t.view(1, d)) for t in (*keep0, *keep1) if t is not None):
+        raise ValueError("out shares memory with a norm's parameters")
     stream = _hip.stream_handle(device) if m else 0
     _hip.refuse_grad("block_norm", *keep0, *keep1)
     y = x if block is None else torch.empty(x.shape, dtype=x.dtype, device=device) if out is None else out

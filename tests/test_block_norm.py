@@ -418,3 +418,25 @@ def test_parameters_that_require_grad_are_refused_on_the_gpu():
             norms.block_norm(x, x, **kw)
     with torch.no_grad():
         assert all(torch.equal(a, b) for a, b in zip(norms.block_norm(x, x, pre=fresh), want))
+
+
+def test_an_out_over_a_norms_parameters_is_refused():
+    x, norm, flat = torch.zeros(2, 8), torch.nn.LayerNorm(8).requires_grad_(False), torch.zeros(40)
+    for name in ("weight", "bias"):
+        for which in ("post", "pre"):
+            setattr(norm, name, torch.nn.Parameter(flat[12:20], requires_grad=False))
+            with pytest.raises(ValueError, match="shares memory"):
+                norms.block_norm(x, x, out=flat[:16].view(2, 8), **{which: norm})
+            with pytest.raises(ValueError, match="GPU"):
+                norms.block_norm(x, x, out=flat[20:36].view(2, 8), **{which: norm})
+            setattr(norm, name, torch.nn.Parameter(torch.ones(8), requires_grad=False))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+def test_an_out_over_a_norms_parameters_is_refused_on_the_gpu():
+    x, norm = torch.randn(1, 64, device=DEV), torch.nn.LayerNorm(64, device=DEV)
+    for out in (norm.weight.view(1, 64), norm.bias.view(1, 64)):
+        for kw in (dict(post=norm), dict(pre=norm)):
+            with pytest.raises(ValueError, match="shares memory"):
+                norms.block_norm(x, x, out=out, **kw)
