@@ -47,7 +47,9 @@ typedef __attribute__((address_space(3))) v4s *ltr_t;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.0f;  // scores may pass the reference by this much (base 2) before it is raised
 
-constexpr float kRoom = 16.0f;  // parts are joined at 2^-16 of their size, so that finite parts have a finite sum
+// Parts are joined at 2^-16 of their size, so that finite parts have a finite sum. A factor of the weights: in their exponent it
+// would round the difference of the maxima.
+constexpr float kRoom = 0x1p-16f;
 
 struct Args {
     kea_heads q, k, v, out;
@@ -555,12 +557,12 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
                 v4f v = {0, 0, 0, 0};
 #pragma unroll
                 for (int w = 0; w < WK; ++w) {
-                    const float by = part[u][w].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part[u][w].x - top - kRoom);
+                    const float by = part[u][w].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part[u][w].x - top) * kRoom;
                     all += part[u][w].y * by;
                     v += share[u][w] * by;
                 }
                 joined[u] = v;
-                refs[u] = make_float2(top + kRoom, all);
+                refs[u] = make_float2(top, all);
                 const float z = (v[0] + v[1] + (v[2] + v[3])) * 0.0f;  // (an infinity or NaN times 0 is NaN)
                 bad |= z != z;
             }
@@ -647,7 +649,7 @@ __global__ void __launch_bounds__(64) join_kernel(Args a) {
         }
         float top = m;
 #pragma unroll
-        for (int s = 0; s < 8; ++s) top = s0 + s < a.splits ? fmaxf(top, stat[s].x + kRoom) : top;
+        for (int s = 0; s < 8; ++s) top = s0 + s < a.splits ? fmaxf(top, stat[s].x) : top;
         const float old = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
         m = top;
         sum *= old;
@@ -655,7 +657,7 @@ __global__ void __launch_bounds__(64) join_kernel(Args a) {
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
             if (s0 + s >= a.splits) continue;
-            const float by = stat[s].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(stat[s].x - top);  // (a NaN stays one)
+            const float by = stat[s].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(stat[s].x - top) * kRoom;  // (a NaN stays one)
             sum += stat[s].y * by;
             v += part[s] * by;
         }

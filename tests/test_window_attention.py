@@ -406,3 +406,31 @@ def test_an_out_over_the_lengths_is_refused():
             window.attention(q, q, q, out=out, **kw)
     with pytest.raises(ValueError, match="GPU"):
         window.attention(q, q, q, out=out, kv_lengths=words[320:322])
+
+
+LN2 = 0.693147182464599609375  # in FP32; its FP32 product with log2(e) is 1, so that weights are 2^(s - max)
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("d", [64, 80, 128, 256])
+@pytest.mark.parametrize("tk,a,b", [(128, 3, 40), (128, 33, 100), (5000, 7, 4000), (5000, 2500, 33), (50000, 100, 49000)])
+def test_parts_join_without_loss(tk, a, b, d):
+    """Two keys count, in the parts of two waves or workgroups, the rest weigh 2^-200. Key a's score is 0 and key b's -x, so that the
+    output is 1 for v = (1 at a, 0 at b) over 1 + 2^-x, and 2^-x over that for the reverse. x is a multiple of 2^-21 below 4: in FP32
+    every difference of scores is exact, weights and the factor of a part are one exp2 of 2 u each, their products and sums u each:
+    2^-x is off by 5 u, 1 + 2^-x by a third of that and u at most (x >= 1), then come three products or quotients of u, and u for
+    2.7e-9 x in the exponent: 11 u. (Exponents rounded behind 2^4 or 2^5 would add 11 or 22.)"""
+    g = torch.Generator().manual_seed(tk + a)
+    h = d  # head i reads element i of the keys
+    x = 1 + torch.randint(0, 3 * 2**21, (d,), generator=g) / 2**21
+    q = torch.eye(h).view(1, 1, h, d).to(DEV)
+    k = torch.full((1, tk, 1, d), -200.0)
+    k[0, a], k[0, b] = 0, -x
+    v = torch.zeros(1, tk, 1, d)
+    v[0, a, 0, ::2], v[0, b, 0, 1::2] = 1, 1
+    got = window.attention(q, k.to(DEV), v.to(DEV), scale=LN2)[0, 0].cpu().double()
+    w = torch.exp2(-x.double())[:, None]
+    want = torch.cat([1 / (1 + w), w / (1 + w)], 1).repeat(1, d // 2)
+    worst = ((got - want).abs() / want).max().item() / U
+    assert worst <= 11, f"{worst:.3g} u"
