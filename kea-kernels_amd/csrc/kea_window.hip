@@ -47,14 +47,13 @@ typedef __attribute__((address_space(3))) v4s *ltr_t;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.0f;  // scores may pass the reference by this much (base 2) before it is raised
 
-// Parts are joined at 2^-16 of their size, so that finite parts have a finite sum. A factor of the weights: in their exponent it
-// would round the difference of the maxima.
-constexpr float kRoom = 0x1p-16f;
+// The exponent e with 2^(e - 1) <= v < 2^e; 0 for 0, infinities and NaN.
+__device__ __forceinline__ int exponent(float v) { return __builtin_amdgcn_frexp_expf(v); }
 
 struct Args {
     kea_heads q, k, v, out;
     const int32_t *lengths, *starts;
-    float *part, *stats;  // splits > 1: [splits][sequences and key heads][rows][d], [..][rows][2]
+    float *part, *stats;  // splits > 1: [splits][sequences and key heads][rows][d], [..][rows][2] (see join_kernel)
     int batch, tq, tk, kv_heads, group, d, left, right, sinks;
     int rows, row_tiles, splits;
     int by_group;  // the grid is [sequences and key heads][tiles][splits], or [tiles][sequences and key heads][splits]
@@ -557,7 +556,7 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
                 v4f v = {0, 0, 0, 0};
 #pragma unroll
                 for (int w = 0; w < WK; ++w) {
-                    const float by = part[u][w].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part[u][w].x - top) * kRoom;
+                    const float by = part[u][w].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part[u][w].x - top);
                     all += part[u][w].y * by;
                     v += share[u][w] * by;
                 }
@@ -577,11 +576,12 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
         if (!real) return;
         if (a.splits > 1) {
             float *const part = a.part + (slot0 + row) * a.d;
+            const float unit = __builtin_amdgcn_ldexpf(1.0f, -exponent(l));
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int e = 0; e < 16; e += 4)
-                    if (!RAGGED || 32 * d + 2 * e + 4 * h < a.d) *(v4f *)(part + 32 * d + 2 * e + 4 * h) = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+                    if (!RAGGED || 32 * d + 2 * e + 4 * h < a.d) *(v4f *)(part + 32 * d + 2 * e + 4 * h) = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]} * unit;
             if (h == 0) *(float2 *)(a.stats + 2 * (slot0 + row)) = make_float2(m, l);
             return;
         }
@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
             for (int u = 0; u < PER; ++u) {
                 const int at = u * NT + tid, r = at / (DP / 4), c = at % (DP / 4);
                 if (r >= rows || (RAGGED && 4 * c >= a.d)) continue;
-                *(v4f *)(a.part + (slot0 + r0 + r) * a.d + 4 * c) = joined[u];
+                *(v4f *)(a.part + (slot0 + r0 + r) * a.d + 4 * c) = joined[u] * __builtin_amdgcn_ldexpf(1.0f, -exponent(refs[u].y));
                 if (c == 0) *(float2 *)(a.stats + 2 * (slot0 + r0 + r)) = refs[u];
             }
             return;
@@ -628,7 +628,9 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
     }
 }
 
-// Joins the splits: out = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m), four elements a thread, eight splits at a time.
+// Joins the splits: out = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m), four elements a thread, eight splits at a time. The parts
+// hold O_s 2^-e_s and the sum so far is kept at 2^-e of its size, e_s and e the exponents of l_s and of the sum of weights: that is
+// below the largest value and a half or more of the weighted mean, so it neither overflows nor loses digits that the mean has.
 template <typename T>
 __global__ void __launch_bounds__(64) join_kernel(Args a) {
     const int at = blockIdx.x * 64 + threadIdx.x, per = a.d / 4, r = at / per, c = at - r * per, bh = blockIdx.y, b = a.sequence(bh), hk = bh - b * a.kv_heads;
@@ -637,6 +639,7 @@ __global__ void __launch_bounds__(64) join_kernel(Args a) {
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.tk) : a.tk;
     const int p = (a.starts ? min(max(a.starts[b], -(1 << 30)), 1 << 30) : len - a.tq) + t;
     float m = -INFINITY, sum = 0.0f;
+    int e = 0;
     v4f v = {0, 0, 0, 0};
     for (int s0 = 0; s0 < a.splits; s0 += 8) {
         float2 stat[8];
@@ -653,19 +656,23 @@ __global__ void __launch_bounds__(64) join_kernel(Args a) {
         const float old = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
         m = top;
         sum *= old;
-        v *= old;
+        float by[8];
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
-            if (s0 + s >= a.splits) continue;
-            const float by = stat[s].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(stat[s].x - top) * kRoom;  // (a NaN stays one)
-            sum += stat[s].y * by;
-            v += part[s] * by;
+            by[s] = stat[s].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(stat[s].x - top);  // (a NaN stays one)
+            if (s0 + s < a.splits) sum += stat[s].y * by[s];
         }
+        const int next = exponent(sum);
+        v *= __builtin_amdgcn_ldexpf(old, e - next);
+        e = next;
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+            if (s0 + s < a.splits) v += part[s] * __builtin_amdgcn_ldexpf(by[s], exponent(stat[s].y) - e);
     }
-    const float by = p >= 0 && p < len && sum != 0.0f ? 1.0f / sum : 0.0f;
+    const float by = p >= 0 && p < len && sum != 0.0f ? __builtin_amdgcn_ldexpf(1.0f / sum, e) : 0.0f;
     T res[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) res[e] = (T)(by == 0.0f ? 0.0f : v[e] * by);
+    for (int i = 0; i < 4; ++i) res[i] = (T)(by == 0.0f ? 0.0f : v[i] * by);
     T *const y = (T *)a.out.data_dev + b * a.out.batch_stride + (long long)t * a.out.t_stride + (hk * a.group + r - t * a.group) * a.out.head_stride + 4 * c;
     if constexpr (sizeof(T) == 4) *(v4f *)y = *(const v4f *)res;
     else *(v4s *)y = *(const v4s *)res;

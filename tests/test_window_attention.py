@@ -434,3 +434,17 @@ def test_parts_join_without_loss(tk, a, b, d):
     want = torch.cat([1 / (1 + w), w / (1 + w)], 1).repeat(1, d // 2)
     worst = ((got - want).abs() / want).max().item() / U
     assert worst <= 11, f"{worst:.3g} u"
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [64, 40, 128, 256])
+@pytest.mark.parametrize("tq,tk", [(1, 100), (1, 6000), (30, 700), (300, 300)])
+def test_small_values_keep_their_digits(tq, tk, d, dtype):
+    """Values 2^100 smaller give an output 2^100 smaller to the bit: the scores are small, so that no weight is below 2^-10, and
+    every product and sum stays a normal number."""
+    g = torch.Generator().manual_seed(tk + d)
+    q, k, v = heads(1, tq, 2, d, dtype, g, 0.25), heads(1, tk, 1, d, dtype, g), heads(1, tk, 1, d, dtype, g)
+    want = window.attention(q, k, v)
+    assert torch.equal(window.attention(q, k, v * 2.0**-100), want * 2.0**-100)
