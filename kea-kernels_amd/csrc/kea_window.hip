@@ -23,7 +23,9 @@
 // Keys outside the tile's range are read from its last key and masked. A masked score is -infinity whatever K holds, but a
 // product with its weight of 0 is NaN where V is infinite or NaN. Such a sum shows in the output: a workgroup that ends up
 // with a value that is not finite does its work a second time with those elements of V taken out of the product and added to
-// the queries that see them, and (FP32 and BF16) with weights of at most 2^-32, whose sums with V's largest numbers are finite.
+// the queries that see them, and (FP32 and BF16) a third time for rows that are still not finite, with values of 2^-40 of their
+// size, whose sums are finite. (In such rows, and there alone, elements of values below 2^-86 lose digits.) A row's bits depend on
+// the keys that it sees alone: its maximum, sums and passes are decided by its own scores and sums.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -298,8 +300,9 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
 
     v16f o[DB];
     float m = -INFINITY, l = 0.0f;  // l: this half's keys
-    bool careful = false;
-    constexpr float kDown = __is_same(T, _Float16) ? 0.0f : 40.0f;
+    int pass = 0;
+    uint32_t small = 0;  // the wave's rows that the third pass is for
+    constexpr int kDown = 40;  // 2^30 keys of weights up to 2^8
 
     // operand addresses in a tile, as offsets: K unit 2 c + h of row n is at ka ^ 32 c, V units 4 d .. of its rows at va ^ 64 d
     // (FP32: word n of units 8 d .. at va ^ 128 d)
@@ -403,7 +406,7 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
             for (int e = 0; e < 16; ++e) top = fmaxf(top, s[i][e]);
         top = other_half_max(top) * scale;
         if (__any(top > m + kLazy)) {
-            const float next = fmaxf(m, top);
+            const float next = top > m + kLazy ? top : m;
             if (__any(m != -INFINITY)) {  // (nothing is there to rescale at first)
                 const float by = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
                 l *= by;
@@ -412,7 +415,7 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
             }
             m = next;
         }
-        const float ref = (m == -INFINITY ? 0.0f : m) + (careful ? kDown : 0.0f);
+        const float ref = m == -INFINITY ? 0.0f : m;
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < NB; ++i)
@@ -444,7 +447,7 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (__builtin_expect(careful, 0)) {
+        if (__builtin_expect(pass > 0, 0)) {
             for (int i = 0; i < NB; ++i) {
                 uint32_t left = __builtin_amdgcn_readfirstlane(flags[i * WK + wk]);
                 while (left) {
@@ -462,15 +465,18 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
             }
         }
     };
-    // V's elements that are no numbers become zeros in LDS, and their keys' flags are set.
+    // V's elements that are no numbers become zeros in LDS, and their keys' flags are set; in the third pass the others are scaled.
     auto take_out = [&](int buf) {
+        const float by = pass == 2 ? __builtin_amdgcn_ldexpf(1.0f, -kDown) : 1.0f;
         if (tid < S::KB) flags[tid] = 0;
         __syncthreads();
         for (int at = tid; at < KT * UNITS; at += NT) {
             T *unit = (T *)(lds + buf * S::BUF + KT * ROW + at * 16);
             bool any = false;
-            for (int e = 0; e < EPU; ++e)
+            for (int e = 0; e < EPU; ++e) {
                 if (!finite_bits(unit[e])) unit[e] = (T)0.0f, any = true;
+                else if (pass == 2) unit[e] = (T)((float)unit[e] * by);
+            }
             if (any) atomicOr(&flags[at / UNITS / 32], 1u << (at / UNITS % 32));
         }
         __syncthreads();
@@ -480,7 +486,65 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
     const int rows = min(32 * WQ, a.rows - r0);
     v4f joined[PER];
     float2 refs[PER];
-    for (int round = 0; round < 2; ++round) {
+    const long long slot0 = ((long long)split * a.batch * a.kv_heads + bh) * a.rows;
+    T *const out = (T *)a.out.data_dev + b * a.out.batch_stride;
+    // Stores the rows of `done`, whose sums are 2^-up of their size.
+    auto store = [&](uint32_t done, int up) {
+        // (addresses made here, not kept through the passes for both calls)
+        int thread = tid, of = row;
+        asm volatile("" : "+v"(thread), "+v"(of));
+        if constexpr (WK == 1) {
+            if (real && (done >> n & 1)) {
+                if (a.splits > 1) {
+                    float *const part = a.part + (slot0 + of) * a.d;
+                    const float unit = __builtin_amdgcn_ldexpf(1.0f, up - exponent(l));
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4)
+                            if (!RAGGED || 32 * d + 2 * e + 4 * h < a.d) *(v4f *)(part + 32 * d + 2 * e + 4 * h) = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]} * unit;
+                    if (h == 0) *(float2 *)(a.stats + 2 * (slot0 + of)) = make_float2(m, l);
+                } else {
+                    T *const y = out + (long long)t * a.out.t_stride + head * a.out.head_stride + 4 * h;
+                    const float by = l != 0.0f ? __builtin_amdgcn_ldexpf(1.0f / l, up) : 0.0f;
+                    const bool some = inside && l != 0.0f;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) {
+                            if (RAGGED && 32 * d + 2 * e + 4 * h >= a.d) continue;
+                            T v[4];
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) v[z] = (T)(some ? o[d][e + z] * by : 0.0f);
+                            if constexpr (F32) *(v4f *)(y + 32 * d + 2 * e) = *(const v4f *)v;
+                            else *(v4s *)(y + 32 * d + 2 * e) = *(const v4s *)v;
+                        }
+                }
+            }
+        } else {
+            static_assert(WQ == 1, "one group of rows");
+#pragma unroll
+            for (int u = 0; u < PER; ++u) {
+                const int at = u * NT + thread, r = at / (DP / 4), c = at % (DP / 4);
+                if (r >= rows || (RAGGED && 4 * c >= a.d) || !(done >> r & 1)) continue;
+                if (a.splits > 1) {
+                    *(v4f *)(a.part + (slot0 + r0 + r) * a.d + 4 * c) = joined[u] * __builtin_amdgcn_ldexpf(1.0f, up - exponent(refs[u].y));
+                    if (c == 0) *(float2 *)(a.stats + 2 * (slot0 + r0 + r)) = refs[u];
+                    continue;
+                }
+                const int tt = a.token(r0 + r), pp = start + tt;
+                const bool some = pp >= 0 && pp < len && refs[u].y != 0.0f;
+                const float by = __builtin_amdgcn_ldexpf(1.0f / refs[u].y, up);
+                T *const y = out + (long long)tt * a.out.t_stride + (hk * a.group + r0 + r - tt * a.group) * a.out.head_stride + 4 * c;
+                T res[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) res[e] = (T)(some ? joined[u][e] * by : 0.0f);
+                if constexpr (F32) *(v4f *)y = *(const v4f *)res;
+                else *(v4s *)y = *(const v4s *)res;
+            }
+        }
+    };
+    for (;; ++pass) {
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
         m = -INFINITY;
@@ -490,7 +554,7 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
             for (int i = 0; i < tiles; ++i) {
                 const int v0 = from + i * KT, buf = i & 1;
                 landed(Count<0>());
-                if (careful) take_out(buf);
+                if (pass) take_out(buf);
                 if (i + 1 < tiles) stage(v0 + KT, buf ^ 1, true, true);
                 scores(v0, buf);
                 output(v0, buf);
@@ -505,13 +569,13 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
                 scores(v0, 0);
                 landed(Count<0>());
                 if (i + 1 < tiles) stage(v0 + KT, 0, true, false);
-                if (careful) take_out(0);
+                if (pass) take_out(0);
                 output(v0, 0);
             }
         }
         l = both_halves(l);
-        if (careful) m += kDown;  // what the weights and sums refer to
         bool bad = false;
+        uint32_t bad_rows = 0;
         if constexpr (WK == 1) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
@@ -562,70 +626,26 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
                 }
                 joined[u] = v;
                 refs[u] = make_float2(top, all);
-                const float z = (v[0] + v[1] + (v[2] + v[3])) * 0.0f;  // (an infinity or NaN times 0 is NaN)
-                bad |= z != z;
+                const float z = (v[0] * 0.0f + v[1] * 0.0f) + (v[2] * 0.0f + v[3] * 0.0f);  // (an infinity or NaN times 0 is NaN)
+                if (z != z) bad = true, bad_rows |= 1u << min((u * NT + tid) / (DP / 4), rows - 1);
             }
         }
-        if (careful || !__syncthreads_or(bad)) break;
-        careful = true;
-    }
-
-    const long long slot0 = ((long long)split * a.batch * a.kv_heads + bh) * a.rows;
-    T *const out = (T *)a.out.data_dev + b * a.out.batch_stride;
-    if constexpr (WK == 1) {
-        if (!real) return;
-        if (a.splits > 1) {
-            float *const part = a.part + (slot0 + row) * a.d;
-            const float unit = __builtin_amdgcn_ldexpf(1.0f, -exponent(l));
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                    if (!RAGGED || 32 * d + 2 * e + 4 * h < a.d) *(v4f *)(part + 32 * d + 2 * e + 4 * h) = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]} * unit;
-            if (h == 0) *(float2 *)(a.stats + 2 * (slot0 + row)) = make_float2(m, l);
-            return;
-        }
-        T *const y = out + (long long)t * a.out.t_stride + head * a.out.head_stride + 4 * h;
-        const float by = l != 0.0f ? 1.0f / l : 0.0f;
-        const bool some = inside && l != 0.0f;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                if (RAGGED && 32 * d + 2 * e + 4 * h >= a.d) continue;
-                T v[4];
-#pragma unroll
-                for (int z = 0; z < 4; ++z) v[z] = (T)(some ? o[d][e + z] * by : 0.0f);
-                if constexpr (F32) *(v4f *)(y + 32 * d + 2 * e) = *(const v4f *)v;
-                else *(v4s *)(y + 32 * d + 2 * e) = *(const v4s *)v;
+        if (pass == (__is_same(T, _Float16) ? 1 : 2) || !__syncthreads_or(bad)) break;
+        if (__builtin_expect(pass == 1, 0)) {
+            if constexpr (WK == 1) {
+                const uint64_t lanes = __ballot(bad);
+                small = (uint32_t)lanes | (uint32_t)(lanes >> 32);
+            } else {
+                if (tid == 0) flags[8] = 0;
+                __syncthreads();
+                if (bad_rows) atomicOr(&flags[8], bad_rows);
+                __syncthreads();
+                small = __builtin_amdgcn_readfirstlane(flags[8]);
             }
-    } else {
-        static_assert(WQ == 1, "one group of rows");
-        if (a.splits > 1) {
-#pragma unroll
-            for (int u = 0; u < PER; ++u) {
-                const int at = u * NT + tid, r = at / (DP / 4), c = at % (DP / 4);
-                if (r >= rows || (RAGGED && 4 * c >= a.d)) continue;
-                *(v4f *)(a.part + (slot0 + r0 + r) * a.d + 4 * c) = joined[u] * __builtin_amdgcn_ldexpf(1.0f, -exponent(refs[u].y));
-                if (c == 0) *(float2 *)(a.stats + 2 * (slot0 + r0 + r)) = refs[u];
-            }
-            return;
-        }
-#pragma unroll
-        for (int u = 0; u < PER; ++u) {
-            const int at = u * NT + tid, r = at / (DP / 4), c = at % (DP / 4);
-            if (r >= rows || (RAGGED && 4 * c >= a.d)) continue;
-            const int tt = a.token(r0 + r), pp = start + tt;
-            const bool some = pp >= 0 && pp < len && refs[u].y != 0.0f;
-            const float by = 1.0f / refs[u].y;
-            T *const y = out + (long long)tt * a.out.t_stride + (hk * a.group + r0 + r - tt * a.group) * a.out.head_stride + 4 * c;
-            T res[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) res[e] = (T)(some ? joined[u][e] * by : 0.0f);
-            if constexpr (F32) *(v4f *)y = *(const v4f *)res;
-            else *(v4s *)y = *(const v4s *)res;
+            store(~small, 0);
         }
     }
+    store(pass == 2 ? small : ~0u, pass == 2 ? kDown : 0);
 }
 
 // Joins the splits: out = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m), four elements a thread, eight splits at a time. The parts
@@ -736,7 +756,7 @@ int launched() {
 template <typename T, int DP, int WQ, int WK, bool RAGGED>
 int run_shape(const Args &a, hipStream_t stream) {
     using S = Shape<T, DP, WQ, WK>;
-    static_assert(S::LDS <= 160 * 1024 && S::KT * S::UNITS % S::NT == 0 && S::KB <= 16, "tiles and flags");
+    static_assert(S::LDS <= 160 * 1024 && S::KT * S::UNITS % S::NT == 0 && S::KB <= 8, "tiles and flags");
     const int64_t groups = (int64_t)a.batch * a.kv_heads, padded = a.by_group ? (groups + 7) / 8 * 8 : a.row_tiles < 8 ? a.row_tiles : (a.row_tiles + 7) / 8 * 8;
     const dim3 grid((unsigned)padded, (unsigned)(a.by_group ? a.row_tiles : groups), (unsigned)a.splits);
     if (!kea::fits_dispatch(padded, S::NT) || grid.y > 65535 || !kea::fits_dispatch((int64_t)a.rows * (a.d / 4) / 64 + 1, 64))

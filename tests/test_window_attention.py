@@ -448,3 +448,38 @@ def test_small_values_keep_their_digits(tq, tk, d, dtype):
     q, k, v = heads(1, tq, 2, d, dtype, g, 0.25), heads(1, tk, 1, d, dtype, g), heads(1, tk, 1, d, dtype, g)
     want = window.attention(q, k, v)
     assert torch.equal(window.attention(q, k, v * 2.0**-100), want * 2.0**-100)
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 40, 80, 128, 200, 256])
+@pytest.mark.parametrize("b,t,tq", [(1, 300, 300), (1, 3000, 4), (2, 130, 130), (1, 100, 3), (40, 150, 150)])
+def test_unseen_keys_leave_the_bits(b, t, tq, d, dtype):
+    """NaN, infinities and the type's largest values in keys and values: who does not see them has the same bits as without them,
+    in every form (tiles of 32 rows whose keys are shared out or split, of 128 rows, ragged heads); who does has their sum."""
+    g = torch.Generator().manual_seed(t + d)
+    q, k, v = heads(b, tq, 4, d, dtype, g), heads(b, t, 2, d, dtype, g), heads(b, t, 2, d, dtype, g)
+    lengths = torch.full((b,), t - 10, dtype=torch.int32, device=DEV)
+    starts = torch.full((b,), t - 10 - tq, dtype=torch.int32, device=DEV) if tq < t else torch.zeros(b, dtype=torch.int32, device=DEV)
+    call = lambda k, v: window.attention(q, k, v, left=20, right=0, sinks=1, kv_lengths=lengths, q_starts=starts)  # noqa: E731
+    want = call(k, v)
+    p = torch.arange(tq) + int(starts[0])
+    real = p < t - 10
+    bad = t - 42 if tq == t else t - 33  # seen by positions bad .. bad + 20 (tq < t: the middle of the queries is the first)
+    for at_k, at_v in ((float("nan"), float("inf")), (0.0, torch.finfo(dtype).max), (float("inf"), float("nan")), (0.0, -float("inf"))):
+        k1, v1 = k.clone(), v.clone()
+        k1[:, bad], v1[:, bad], v1[:, bad + 1] = at_k, at_v, at_v
+        k1[:, t - 10:], v1[:, t - 10:] = float("nan"), float("inf")
+        got = call(k1, v1)
+        sees = (p >= bad) & (p <= bad + 21) & real
+        assert torch.equal(got[:, ~sees], want[:, ~sees]), (at_k, at_v)
+        if at_k == 0 and at_v > 0:  # two of the largest value: finite sums, within the bounds but for the last binade
+            x, e = expected(q, k1[:, :t - 10], v1[:, :t - 10], 20, 0, 1, starts=starts.tolist())
+            off = (got[:, sees].cpu().double() - x[:, sees]).abs() <= e[:, sees]
+            assert (off | (x[:, sees].abs() > torch.finfo(dtype).max / 2)).all()
+        elif at_k == 0:
+            assert (got[:, sees] == at_v).all()
+        else:
+            first = sees & (p <= bad + 20)
+            assert got[:, first].isnan().all()
