@@ -82,8 +82,8 @@ typedef struct {
  *   out_i = sum_j softmax_j(scale * q_i . k_j) v_j over the keys it sees, 0 where it sees none (or scores of -infinity
  *   alone) or p is outside 0 .. len-1.
  * Head h reads key head h / (heads / kv_heads). A key that a query does not see has no part in its output, whatever k and v
- * hold there; k and v at len and behind are not read. Scores, their maximum and sum and the output's sums are FP32; the
- * weights exp(s - max) are rounded to the type for the product with v (KEA_F16, KEA_BF16).
+ * hold there; k and v at len and behind are not read. Scores, their maximum and sum and the output's sums are FP32; with
+ * KEA_F16 and KEA_BF16 the weights exp(s - max) are rounded to the type, in their sum as in the product with v.
  *   dtype        of q, k, v and out: KEA_F32, KEA_F16 or KEA_BF16. d a multiple of 8, at most 256; every pointer and stride
  *                a multiple of 16 bytes, strides not negative. out overlaps no input.
  *   kv_lengths   int32 [batch], NULL: tk for each.  q_starts: int32 [batch], NULL: len - tq (the last tokens).

@@ -134,6 +134,15 @@ __device__ __forceinline__ v16f mma(v8s a, v8s b, v16f c) {
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
 }
 
+// c + the two weights of a pair: FP32, to 2.7 u of it (measured), where two additions would be off by 2 u. (T: the pair's type.)
+template <typename T>
+__device__ __forceinline__ float add_pair(const T *w, float c) {
+    typedef T pair __attribute__((ext_vector_type(2)));
+    const pair ones = {(T)1.0f, (T)1.0f};
+    if constexpr (__is_same(T, _Float16)) return __builtin_amdgcn_fdot2(*(const pair *)w, ones, c, false);
+    else return __builtin_amdgcn_fdot2_f32_bf16(*(const pair *)w, ones, c, false);
+}
+
 __device__ __forceinline__ bool finite(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) != 0x7F800000u; }
 // Whether an element of 16 or 32 bits is an infinity or NaN, and a unit of eight or four without such elements.
 template <typename T>
@@ -422,11 +431,11 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 s[i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], scale, -ref));
-                sum += s[i][e];
+                if constexpr (F32) sum += s[i][e];
             }
-        l += sum;
         // The 16-bit types' weights are rounded to what the product takes (half a step, relative to themselves; below the
-        // smallest normal FP16 number 2^-25): as accurate as the values they weigh.
+        // smallest normal FP16 number 2^-25): as accurate as the values they weigh. Their sum is of the rounded ones, so that they
+        // add up to one and the output stays among the values.
 #pragma unroll
         for (int j = 0; j < VSTEPS; ++j) {
             if (j + 1 < VSTEPS) read_v(j + 1);
@@ -438,6 +447,8 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
                 T w[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) w[e] = (T)s[j / 2][8 * (j % 2) + e];
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) sum = add_pair<T>(w + e, sum);
                 const v8s pf = *(const v8s *)w;
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
@@ -447,6 +458,7 @@ __global__ void __launch_bounds__(64 * WQ *WK, DP *sizeof(T) <= 256 ? 2 : 1) win
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        l += sum;
         if (__builtin_expect(pass > 0, 0)) {
             for (int i = 0; i < NB; ++i) {
                 uint32_t left = __builtin_amdgcn_readfirstlane(flags[i * WK + wk]);

@@ -483,3 +483,25 @@ def test_unseen_keys_leave_the_bits(b, t, tq, d, dtype):
         else:
             first = sees & (p <= bad + 20)
             assert got[:, first].isnan().all()
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,t,tq,h,hk,d", [(2, 33, 1, 2, 1, 64), (2, 200, 200, 2, 2, 128), (2, 3000, 2, 2, 1, 64), (2, 2600, 2600, 8, 4, 80), (2, 90, 90, 2, 1, 256)])
+def test_weights_add_up_to_one(b, t, tq, h, hk, d, dtype):
+    """Values that are all c give c: the weights that the product takes are the ones that are summed. Every sixteenth key weighs 1,
+    the others just less than halfway from 1/2 to the 16-bit type's next number: rounded to 1/2, all sums are exact (fewer than 2^12
+    keys, c of 11 bits at most), and the quotient is off by 2 u. (The weights as they were would add up to 2^-8.2 more in BF16, and
+    c is just below 2.) In FP32 either sum is off by t + 16 roundings of u at most."""
+    x = {BF16: 0.50194, F16: 0.50024, F32: 0.3}[dtype]
+    q, k = torch.zeros(b, tq, h, d), torch.zeros(b, t, hk, d)
+    q[..., 0], k[..., 0] = 1, -1
+    k[:, ::16, :, 0] = 0
+    for c in (2 - torch.finfo(dtype).eps, 1.0, -3.96875):
+        v = torch.full((b, t, hk, d), c)
+        got = window.attention(q.to(dtype).to(DEV), k.to(dtype).to(DEV), v.to(dtype).to(DEV), scale=-math.log(x), right=None)
+        if dtype == F32:
+            assert ((got - c).abs() <= abs(c) * 2 * (t + 20) * U).all()
+        else:
+            assert (got == c).all()
