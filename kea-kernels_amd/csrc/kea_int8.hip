@@ -13,8 +13,8 @@
 //                 their next operands at once; reading one tile's operands for all tiles, out of L2, takes as long.
 //   split_kernel  few output tiles (few tokens): a workgroup owns 16 RM x 16 RN outputs, its NW waves share out k, each
 //                 loading its operands straight into registers, and the exact int32 sums meet in LDS. 1 x 2560 x 640 takes
-//                 3.8 us, of which an empty launch is 1.6; 16 x 1024 x 4096 6.6, at the rate at which 64 CUs take in the
-//                 128 KB each of them needs.
+//                 3.8 us, of which an empty launch is 1.6; 16 x 1024 x 4096 6.6, the time in which one workgroup takes in the
+//                 128 KB that it needs, be they 64 of them or 256 (64 x 1024 x 4096: 5.9).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

@@ -7,8 +7,8 @@
 //
 // Calls in a row, host bound: Int8MmaLayer.linear at M = 128, N = 4096, K = 1024 (fp16 in and out) 13.2 -> 9.3 us, at one
 // row 13.2 -> 9.9, lowbit.quantize + lowbit.gemm with group scales 21.9 -> 12.9, the provider's call on a few rows 18.7 ->
-// 11.7; the two HIP launches are about 6 us of each. int8.gemm on one row 15.5 -> 5.1 (one launch), norms.block_norm 23 -> 6.5,
-// window.attention (two launches) 27 -> 13.
+// 11.7; the two HIP launches are about 6 us of each. int8.gemm on one row 15.5 -> 5.1 (one launch), norms.block_norm 23 -> 6.8,
+// window.attention (two launches) 27 -> 13.7.
 #include <Python.h>
 
 #include <ATen/ATen.h>

@@ -66,8 +66,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, left: int | None = None, right
     None: Tk); q_starts int32 [B] (None: len - Tq, the queries are the last tokens). For padded clips q_starts is zeros and
     kv_lengths the clips' lengths; for tokens against a cache kv_lengths counts them too. Queries that see nothing (or
     scores of -infinity alone), or stand outside 0 .. len - 1 (padding), give zeros. What a query does not see has no part in
-    its output, whatever it holds. scale: 1 / sqrt(D) unless given. out must not overlap an
-    input."""
+    its output, whatever it holds. scale: 1 / sqrt(D) unless given, any finite FP32 number. out must not overlap an input.
+    Everything is FP32 up to the output's rounding, but for the softmax's weights of f16 and bf16 inputs, which are rounded to
+    their type; the same values as f32 keep them whole."""
     if out is None and (hit := _native(q, k, v, left, right, sinks, scale, kv_lengths, q_starts)) is not None:
         return hit
     if q.dim() != 4 or k.dim() != 4 or q.dtype not in _hip.DTYPES:

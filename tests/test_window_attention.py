@@ -486,6 +486,13 @@ def test_unseen_keys_leave_the_bits(b, t, tq, d, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [128, 120, 256])
+def test_unseen_keys_leave_the_bits_of_many_fp32_rows(d):
+    """As above, with enough FP32 rows for the tiles of 128 (2560 of 32 rows, for heads over 64)."""
+    test_unseen_keys_leave_the_bits(140, 150, 150, d, F32)
+
+
+@pytest.mark.gpu
 @torch.inference_mode()
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("b,t,tq,h,hk,d", [(2, 33, 1, 2, 1, 64), (2, 200, 200, 2, 2, 128), (2, 3000, 2, 2, 1, 64), (2, 2600, 2600, 8, 4, 80), (2, 90, 90, 2, 1, 256)])
