@@ -25,6 +25,7 @@
 #include <unordered_map>
 
 #include "../../include/kea_block.h"
+#include "../../include/kea_decode.h"
 #include "../../include/kea_lowbit.h"
 
 namespace {
@@ -39,6 +40,7 @@ struct Library {
     decltype(&kea_block_norm) block_norm = nullptr;
     decltype(&kea_window_attention) window = nullptr;
     decltype(&kea_window_attention_workspace) window_workspace = nullptr;
+    decltype(&kea_int4_gemm) int4_gemm = nullptr;
 } lib;
 
 // The tensor behind an exact torch.Tensor whose memory a kernel may read as it is: on a GPU, strided, no transform
@@ -616,6 +618,61 @@ PyObject *native_window(PyObject *, PyObject *const *args, Py_ssize_t count) {
     Py_RETURN_NONE;
 }
 
+// int4_gemm(q, qs, words, scales, n, k, group, bias, out, out_dtype, silu, residual, factor) -> the output, or None
+PyObject *native_int4_gemm(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    if (count != 13) Py_RETURN_NONE;
+    const at::Tensor *q = plain(args[0]);
+    if (!q || modes_active()) Py_RETURN_NONE;
+    const auto device = q->device();
+    const at::Tensor *qs, *w, *ws, *bias, *out, *res;
+    int64_t n, k, group, silu;
+    double factor;
+    if (!current(device) || !optional(args[1], device, &qs) || !optional(args[2], device, &w) || !optional(args[3], device, &ws) ||
+        !as_int(args[4], &n) || !as_int(args[5], &k) || !as_int(args[6], &group) || !optional(args[7], device, &bias) ||
+        !optional(args[8], device, &out) || !THPDtype_Check(args[9]) || !as_int(args[10], &silu) || !optional(args[11], device, &res) ||
+        !as_float(args[12], &factor) || !qs || !w || !ws)
+        Py_RETURN_NONE;
+    const auto type = out ? out->scalar_type() : ((THPDtype *)args[9])->scalar_type;
+    const int yc = code_of(type), sc = code_of(qs->scalar_type()), wc = code_of(ws->scalar_type()), bc = bias ? code_of(bias->scalar_type()) : KEA_F32;
+    auto scale = [](int c) { return c == KEA_F32 || c == KEA_F16; };
+    const int64_t qd = q->dim() - 2;
+    if (yc < 0 || !scale(sc) || !scale(wc) || !scale(bc) || (qd != 0 && (qd != 1 || q->size(0) != 1)) || n < 1 || n > INT32_MAX || k < 1 || k > (1 << 20) ||
+        group < 32 || group > (1 << 30) || (group & (group - 1)))
+        Py_RETURN_NONE;
+    const int64_t m = q->size(qd), tiles = (n + 15) / 16, blocks = (k + 127) / 128, groups = (k + group - 1) / group;
+    int64_t ldq;
+    if (m < 1 || q->size(qd + 1) < k || !rows8(*q, qd, k, &ldq) || !qs->is_contiguous() || qs->numel() != m ||
+        w->scalar_type() != at::kInt || !w->is_contiguous() || w->numel() != tiles * blocks * 256 || (uintptr_t)w->const_data_ptr() % 16 ||
+        ws->dim() != 3 || ws->size(0) != tiles || ws->size(1) != groups || ws->size(2) != 16 || !ws->is_contiguous() || (uintptr_t)ws->const_data_ptr() % 16 ||
+        (bias && (!bias->is_contiguous() || bias->numel() != n)) ||
+        (res && (res->scalar_type() != at::kFloat || res->dim() != 2 || res->size(0) != m || res->size(1) != n || (n > 1 && res->stride(1) != 1) || (m > 1 && res->stride(0) < n))) ||
+        (out && (out->dim() != 2 || out->size(0) != m || out->size(1) != n || (n > 1 && out->stride(1) != 1) || (m > 1 && out->stride(0) < n))))
+        Py_RETURN_NONE;
+    if (out) {
+        const bool same = res && out->const_data_ptr() == res->const_data_ptr() && type == at::kFloat && (m == 1 || out->stride(0) == res->stride(0));
+        for (const at::Tensor *t : {q, qs, w, ws, bias, same ? nullptr : res})
+            if (t && meet(*out, *t)) Py_RETURN_NONE;
+    }
+    try {
+        at::Tensor y = out ? *out : at::empty({m, n}, at::TensorOptions().device(device).dtype(type));
+        const int rc = lib.int4_gemm((const int8_t *)q->const_data_ptr(), ldq, qs->const_data_ptr(), sc, (const uint32_t *)w->const_data_ptr(),
+                                     ws->const_data_ptr(), wc, group, bias ? bias->const_data_ptr() : nullptr, bc, y.mutable_data_ptr(), yc,
+                                     m > 1 ? y.stride(0) : n, res ? (const float *)res->const_data_ptr() : nullptr, res && m > 1 ? res->stride(0) : n,
+                                     (float)factor, m, n, k, silu ? KEA_FLAG_SILU : 0, stream_of(device));
+        if (rc == 0) return THPVariable_Wrap(std::move(y));
+    } catch (const std::exception &) {
+    }
+    Py_RETURN_NONE;
+}
+
+// bind_decode(int4_gemm)
+PyObject *native_bind_decode(PyObject *, PyObject *args) {
+    unsigned long long g;
+    if (!PyArg_ParseTuple(args, "K", &g)) return nullptr;
+    lib.int4_gemm = (decltype(lib.int4_gemm))g;
+    Py_RETURN_NONE;
+}
+
 // bind_block(int8_gemm, block_norm, window_attention, window_attention_workspace)
 PyObject *native_bind_block(PyObject *, PyObject *args) {
     unsigned long long g, n, w, ww;
@@ -641,6 +698,8 @@ PyObject *native_bind(PyObject *, PyObject *args) {
 PyMethodDef module_methods[] = {
     {"bind", native_bind, METH_VARARGS, nullptr},
     {"bind_block", native_bind_block, METH_VARARGS, nullptr},
+    {"bind_decode", native_bind_decode, METH_VARARGS, nullptr},
+    {"int4_gemm", (PyCFunction)(void (*)())native_int4_gemm, METH_FASTCALL, nullptr},
     {"int8_gemm", (PyCFunction)(void (*)())native_int8_gemm, METH_FASTCALL, nullptr},
     {"block_norm", (PyCFunction)(void (*)())native_block_norm, METH_FASTCALL, nullptr},
     {"window_attention", (PyCFunction)(void (*)())native_window, METH_FASTCALL, nullptr},

@@ -1,4 +1,4 @@
-"""ctypes binding of libkea_hip.so (the C ABI of include/kea_lowbit.h, kea_encoder.h and kea_block.h).
+"""ctypes binding of libkea_hip.so (the C ABI of include/kea_lowbit.h, kea_encoder.h, kea_block.h and kea_decode.h).
 
 This replaces the reference's NVRTC loader and launcher (kk/_nvrtc.py): every kernel is compiled ahead of time
 for gfx950 by kea-kernels_amd/build.py, so there is no runtime compilation, no kernel cache and nothing to refuse
@@ -110,6 +110,8 @@ SIGNATURES = {
     "kea_window_attention_workspace": (_i64, [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     "kea_window_attention": (_i32, [_heads, _heads, _heads, _heads, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                     _i64, _f32, _vp, _vp, _vp, _i64, _vp]),
+    "kea_int4_gemm": (_i32, [_vp, _i64, _vp, _i32, _vp, _vp, _i32, _i64, _vp, _i32, _vp, _i32, _i64, _vp, _i64, _f32, _i64, _i64,
+                             _i64, _i32, _vp]),
     "kea_last_error": (_cp, []),
     "kea_version": (_i32, []),
 }
@@ -155,6 +157,8 @@ def native():
                     "kea_lowbit_project_launch", "kea_lowbit_gemm", "kea_lowbit_gemm_residual", "kea_quantize")))
                 module.bind_block(*(ctypes.cast(getattr(library, name), ctypes.c_void_p).value for name in (
                     "kea_int8_gemm", "kea_block_norm", "kea_window_attention", "kea_window_attention_workspace")))
+                module.bind_decode(*(ctypes.cast(getattr(library, name), ctypes.c_void_p).value for name in (
+                    "kea_int4_gemm",)))
                 _native = module
     return _native
 
