@@ -37,6 +37,42 @@ int kea_int4_gemm(const int8_t *q_dev, int64_t ldq, const void *qs_dev, int qs_d
                   int y_dtype, int64_t ldy, const float *residual_dev, int64_t ldr, float factor, int64_t m, int64_t n, int64_t k,
                   int flags, void *stream);
 
+/* An int8 key or value cache in pages: row r (0 <= r < page_size) of head h of page i is d bytes at data_dev + i * page_stride +
+ * h * head_stride + r * row_stride and one scale at scale_dev + i * scale_page_stride + h * scale_head_stride + r *
+ * scale_row_stride; element e stands for data[e] * scale. data_dev and its strides are multiples of 16; no strides are negative;
+ * no two rows share memory. */
+typedef struct {
+    int8_t *data_dev;
+    float *scale_dev;
+    int64_t page_stride, head_stride, row_stride, scale_page_stride, scale_head_stride, scale_row_stride;
+} kea_pages;
+
+/* Where the tokens of `batch` sequences stand. Position p of sequence b is row p % page_size of page table_dev[b * table_stride +
+ * p / page_size]; an entry outside 0 .. pages-1 names no page. Sequence b holds len = kv_lengths_dev[b] positions, clamped to
+ * 0 .. table_width * page_size, its new tokens among them. The new tokens of a call, `tokens` rows, are packed: sequence b has rows
+ * q_offsets_dev[b] .. q_offsets_dev[b + 1] - 1 (ascending, held to 0 .. tokens), or, where q_offsets_dev is NULL, n = tokens / batch
+ * rows from b * n on. The n rows of a sequence stand at its last positions: the i-th at len - n + i.
+ * page_size: a power of two from 8 to 1024; table_width * page_size <= 2^30; tokens and batch below 2^30. Pointers are aligned to
+ * four bytes. Everything is read on the device: lengths, offsets and table entries may change between replays. */
+typedef struct {
+    const int32_t *table_dev, *kv_lengths_dev, *q_offsets_dev;
+    int64_t table_stride, table_width, batch, pages, page_size, tokens;
+} kea_paging;
+
+/* Writes new tokens' keys and values, [tokens][kv_heads][d] of `dtype` (KEA_F32, KEA_F16, KEA_BF16; batch_stride is not used), to
+ * their places: a row x becomes s = max(max|x| / 127, 1e-30) and rint(x / s), as kea_quantize makes one part (s is held to the
+ * largest number of which 127 s is finite); a row with an infinity or NaN becomes s = NaN and zeros. Tokens that stand at no position (rows of no sequence, positions below 0, entries that name no
+ * page) are left out; nothing else is written. Tokens of one call that stand at the same place are not ordered: what is written
+ * there is not defined. d: a multiple of 16 up to 256; k, v and their strides multiples of 16 bytes, not negative. */
+int kea_paged_write(const kea_heads *k, const kea_heads *v, int dtype, int64_t kv_heads, int64_t d, const kea_pages *k_pages,
+                    const kea_pages *v_pages, const kea_paging *paging, void *stream);
+
+/* Reads positions starts_dev[b] + i (starts_dev NULL: i), 0 <= i < length, of every sequence as values: k_dev, v_dev
+ * [batch][length][kv_heads][d] of `dtype`, contiguous and 16-byte aligned, data * scale rounded once; zeros for positions
+ * outside 0 .. len-1 and for entries that name no page. paging->tokens and q_offsets_dev are not used. */
+int kea_paged_read(const kea_pages *k_pages, const kea_pages *v_pages, const kea_paging *paging, const int32_t *starts_dev,
+                   int64_t length, int64_t kv_heads, int64_t d, void *k_dev, void *v_dev, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -41,7 +41,20 @@ class Heads(ctypes.Structure):
     _fields_ = [("data", _vp), ("batch_stride", _i64), ("t_stride", _i64), ("head_stride", _i64)]
 
 
+class Pages(ctypes.Structure):
+    """kea_pages of include/kea_decode.h."""
+    _fields_ = [("data", _vp), ("scale", _vp), ("page_stride", _i64), ("head_stride", _i64), ("row_stride", _i64),
+                ("scale_page_stride", _i64), ("scale_head_stride", _i64), ("scale_row_stride", _i64)]
+
+
+class Paging(ctypes.Structure):
+    """kea_paging of include/kea_decode.h."""
+    _fields_ = [("table", _vp), ("kv_lengths", _vp), ("q_offsets", _vp), ("table_stride", _i64), ("table_width", _i64),
+                ("batch", _i64), ("pages", _i64), ("page_size", _i64), ("tokens", _i64)]
+
+
 _norm, _heads = ctypes.POINTER(Norm), ctypes.POINTER(Heads)
+_pages, _paging = ctypes.POINTER(Pages), ctypes.POINTER(Paging)
 
 SIGNATURES = {
     "kea_b1_native_words": (_i64, [_i64, _i64]),
@@ -112,6 +125,8 @@ SIGNATURES = {
                                     _i64, _f32, _vp, _vp, _vp, _i64, _vp]),
     "kea_int4_gemm": (_i32, [_vp, _i64, _vp, _i32, _vp, _vp, _i32, _i64, _vp, _i32, _vp, _i32, _i64, _vp, _i64, _f32, _i64, _i64,
                              _i64, _i32, _vp]),
+    "kea_paged_write": (_i32, [_heads, _heads, _i32, _i64, _i64, _pages, _pages, _paging, _vp]),
+    "kea_paged_read": (_i32, [_pages, _pages, _paging, _vp, _i64, _i64, _i64, _vp, _vp, _i32, _vp]),
     "kea_last_error": (_cp, []),
     "kea_version": (_i32, []),
 }
