@@ -52,7 +52,7 @@ typedef struct {
  * 0 .. table_width * page_size, its new tokens among them. The new tokens of a call, `tokens` rows, are packed: sequence b has rows
  * q_offsets_dev[b] .. q_offsets_dev[b + 1] - 1 (ascending, held to 0 .. tokens), or, where q_offsets_dev is NULL, n = tokens / batch
  * rows from b * n on. The n rows of a sequence stand at its last positions: the i-th at len - n + i.
- * page_size: a power of two from 8 to 1024; table_width * page_size <= 2^30; tokens and batch below 2^30. Pointers are aligned to
+ * page_size: a power of two from 16 to 1024; table_width * page_size <= 2^30; tokens and batch below 2^30. Pointers are aligned to
  * four bytes. Everything is read on the device: lengths, offsets and table entries may change between replays. */
 typedef struct {
     const int32_t *table_dev, *kv_lengths_dev, *q_offsets_dev;
@@ -72,6 +72,24 @@ int kea_paged_write(const kea_heads *k, const kea_heads *v, int dtype, int64_t k
  * outside 0 .. len-1 and for entries that name no page. paging->tokens and q_offsets_dev are not used. */
 int kea_paged_read(const kea_pages *k_pages, const kea_pages *v_pages, const kea_paging *paging, const int32_t *starts_dev,
                    int64_t length, int64_t kv_heads, int64_t d, void *k_dev, void *v_dev, int dtype, void *stream);
+
+/* Attention of the new tokens q [tokens][heads][d] to the positions of their sequences (the new tokens' own keys and values are in
+ * the cache): the token at position p sees position j iff p - left <= j <= p and the table names a page for j;
+ *   out = sum_j softmax_j(scale * q . k_j) v_j over what it sees, zeros where it sees nothing or p is below 0.
+ * Head h reads key head h / (heads / kv_heads). A position that a token does not see has no part in its output, whatever its scales
+ * and codes are. Sums, maxima and scores are FP32; the weights exp(s - max) v_scale are rounded to FP16 (to two parts of it, 22
+ * bits, with KEA_F32), and the elements of a row of q, with KEA_BF16 and KEA_F32, to 2^-28 of the row's largest (KEA_F32: 22 bits).
+ *   dtype        of q and out: KEA_F32, KEA_F16 or KEA_BF16; pointers and strides multiples of 16 bytes, strides not negative
+ *                (batch_stride is not used). out overlaps no input, and no two of its rows share memory.
+ *   left         >= 0; 2^30 and above: without bound.  scale: finite.  Rows of a page less than 2^26 bytes apart.
+ *   fill         0: rows of no sequence are left as they are; otherwise they become zeros.
+ *   workspace    kea_paged_attention_workspace bytes (positions = table_width * page_size; offsets: whether q_offsets_dev is given),
+ *                16-byte aligned (0: may be NULL): means, references and sums of parts of the keys, written before they are read. */
+int64_t kea_paged_attention_workspace(int dtype, int64_t batch, int64_t tokens, int64_t positions, int64_t heads, int64_t kv_heads, int64_t d,
+                                      int64_t left, int offsets);
+int kea_paged_attention(const kea_heads *q, const kea_heads *out, int dtype, int64_t heads, int64_t kv_heads, int64_t d, const kea_pages *k_pages,
+                        const kea_pages *v_pages, const kea_paging *paging, int64_t left, float scale, int fill, void *workspace_dev,
+                        int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,657 @@
+// Attention of new tokens over an int8 cache in pages (include/kea_decode.h).
+//
+// The query heads that share a key head are rows of one problem: row r of a sequence and key head is its new token r / group, head
+// r % group of the group. Keys are walked once, 32 at a time, in products of 16-bit floats on whole numbers:
+//   S^T = K Q^T        keys are the matrix instruction's rows, queries its columns, keys and values their codes -127 .. 127, exact in
+//                      FP16: a lane holds 16 keys' sums of one query (its column)
+//   s = S^T a          a = scale log2(e) k_scale, a number for each key
+//   p = 2^(s - ref)    l += p;   w = p v_scale, rounded to FP16;   O^T += V^T w^T;   out = O / l
+// The queries are FP16 numbers: F16 as they are, BF16 by a power of two of their row (an element below 2^-28 of the row's largest is
+// rounded to a multiple of 2^-28 of it), F32 the same in two parts, 22 bits of each element. The weights of F32 are in two parts too.
+// The reference is such that w is at most 2^15: it is raised, and l and O rescaled, only where a block's largest s, with the
+// exponent of the block's largest v_scale, passes it by more than 8 (base 2). Weights below 2^-14 lose digits of FP16: they are
+// 2^-21 and less of the largest at that time.
+//
+// Keys that a query does not see have p = 0, whatever scales they have: a scale of a key that no query sees is taken as 0, one that is
+// no number makes the scores of its key NaN, for the queries that see it.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "kea_attend.h"
+#include "kea_internal.h"
+#include "kea_pages.h"
+#include "../../include/kea_decode.h"
+
+namespace {
+
+using kea::both_halves;
+using kea::lptr_t;
+using kea::other_half_max;
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) v2i *ltr8_t;
+typedef __attribute__((address_space(3))) v4s *ltr16_t;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.0f;   // what a block may pass the reference by (base 2) before it is raised
+constexpr int kTop = 7;         // the exponent of the largest weight where the reference has just been raised
+constexpr int kLeast = -85;     // scales of values below 2^-85 count as that for the reference, so that sums of 2^33 weights are finite
+
+struct Args {
+    kea_heads q, out;
+    kea_pages kp, vp;
+    kea::Paging at;
+    float *part, *stats;  // splits > 1: [splits][tokens][heads][d], [splits][tokens][heads][2]
+    int kv_heads, group, d, left, splits, tiles_each, tiles;  // tiles_each: of a sequence, without offsets; tiles: the most there can be
+    int fill;  // rows of no sequence become zeros
+    float scale;
+};
+
+// ---- what both kernels do --------------------------------------------------------------------------------------------------------
+
+// A tile: rows r0 .. r0 + count - 1 of sequence b, whose first new token is row `first` of q and stands at position `start`.
+struct Tile {
+    int b, r0, rows, first, start, len;
+};
+
+// Tile `at` of PER rows; false where there are no more. All values are uniform.
+template <int PER>
+__device__ __forceinline__ bool find_tile(const Args &a, int at, Tile *t) {
+    int tile;
+    if (!a.at.offsets) {
+        t->b = at / a.tiles_each;
+        tile = at - t->b * a.tiles_each;
+        if (t->b >= a.at.batch) return false;
+    } else {
+        const int lane = __lane_id();
+        int before = 0, found = -1;
+        for (int j = 0; j < a.at.batch; j += 64) {
+            int2 r = make_int2(0, 0);
+            if (j + lane < a.at.batch) r = a.at.rows(j + lane);
+            const int own = ((r.y - r.x) * a.group + PER - 1) / PER;
+            int sum = own;
+#pragma unroll
+            for (int o = 1; o < 64; o *= 2) {
+                const int other = __shfl_up(sum, o);
+                sum += lane >= o ? other : 0;
+            }
+            const uint64_t past = __ballot(before + sum > at);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                found = j + l;
+                tile = at - (before + __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(own, l));
+                break;
+            }
+            before += __builtin_amdgcn_readlane(sum, 63);
+        }
+        if (found < 0) return false;
+        t->b = found;
+    }
+    t->b = __builtin_amdgcn_readfirstlane(t->b);
+    const int2 r = a.at.rows(t->b);
+    t->first = __builtin_amdgcn_readfirstlane(r.x);
+    const int n = __builtin_amdgcn_readfirstlane(r.y - r.x);
+    t->rows = n * a.group;
+    // the last tiles of a sequence see the most keys: they come first
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    t->r0 = ((t->rows + PER - 1) / PER - 1 - tile) * PER;
+    t->len = __builtin_amdgcn_readfirstlane(a.at.length(t->b));
+    t->start = t->len - n;
+    return true;
+}
+
+// Zeros for the rows of no sequence, of the heads of one key head.
+template <typename T>
+__device__ void fill_rest(const Args &a, int hk, int threads) {
+    const int from = min(max(a.at.offsets[0], 0), a.at.tokens), to = min(max(a.at.offsets[a.at.batch], from), a.at.tokens);
+    const int per = a.group * a.d;
+    const long long all = (long long)(a.at.tokens - (to - from)) * per;
+    for (long long i = threadIdx.x; i < all; i += threads) {
+        const int row = (int)(i / per), e = (int)(i - (long long)row * per), t = row < from ? row : row + (to - from);
+        ((T *)a.out.data_dev)[(long long)t * a.out.t_stride + (long long)(hk * a.group + e / a.d) * a.out.head_stride + e % a.d] = (T)0.0f;
+    }
+}
+
+// Eight codes as FP16 numbers: 0x6400 + u is 1024 + u, u = code + 128.
+__device__ __forceinline__ v8h numbers(uint32_t a, uint32_t b) {
+    a ^= 0x80808080u, b ^= 0x80808080u;
+    v4u w;
+    w[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
+    w[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
+    w[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+    w[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+    const _Float16 less = (_Float16)1152.0f;
+    return __builtin_bit_cast(v8h, w) - v8h{less, less, less, less, less, less, less, less};
+}
+
+__device__ __forceinline__ v16f mma(v8h a, v8h b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// The exponent e with 2^(e - 1) <= |v| < 2^e; 0 for 0, infinities and NaN.
+__device__ __forceinline__ int exponent(float v) { return __builtin_amdgcn_frexp_expf(v); }
+__device__ __forceinline__ bool finite(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) != 0x7F800000u; }
+
+// The largest of 32 lanes' numbers (both halves of the wave hold the same ones).
+__device__ __forceinline__ int max32(int v) {
+    auto dpp = [](int v, auto ctrl) { return __builtin_amdgcn_update_dpp(v, v, decltype(ctrl)::value, 0xF, 0xF, false); };
+    v = max(v, dpp(v, std::integral_constant<int, 0xB1>{}));
+    v = max(v, dpp(v, std::integral_constant<int, 0x4E>{}));
+    v = max(v, dpp(v, std::integral_constant<int, 0x141>{}));
+    v = max(v, dpp(v, std::integral_constant<int, 0x140>{}));
+    return max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
+}
+
+// A row of queries as the product's second operand, eight elements at a time; `at(i)` is the first element of operand i of this
+// lane. *by: what a sum with it is multiplied by (a power of two).
+template <typename T, int N, typename At>
+__device__ __forceinline__ void load_queries(const T *row, int d, bool inside, At at, v8h (&q)[N * (sizeof(T) == 4 ? 2 : 1)], float *by) {
+    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
+    auto load = [&](int i, float *v) {
+        typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+        constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+        for (int u = 0; u < 8 / E; ++u) {
+            const vec x = *(const vec *)(row + at(i) + u * E);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[u * E + e] = (float)x[e];
+        }
+    };
+    *by = 1.0f;
+    int less = 0;
+    if constexpr (!__is_same(T, _Float16)) {
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (!inside || at(i) >= d) continue;
+            float v[8];
+            load(i, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, finite(v[e]) ? fabsf(v[e]) : 0.0f);
+        }
+        less = exponent(other_half_max(most)) - 5;
+        *by = __builtin_amdgcn_ldexpf(1.0f, max(less, -126));
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (!inside || at(i) >= d) {
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) q[i * PARTS + p] = v8h{0, 0, 0, 0, 0, 0, 0, 0};
+            continue;
+        }
+        if constexpr (__is_same(T, _Float16)) {
+            q[i] = *(const v8h *)(row + at(i));
+        } else {
+            float v[8];
+            load(i, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = __builtin_amdgcn_ldexpf(v[e], -less);
+                q[i * PARTS][e] = (_Float16)x;
+                if constexpr (PARTS == 2) q[i * PARTS + 1][e] = (_Float16)(finite(x) ? x - (float)q[i * PARTS][e] : 0.0f);
+            }
+        }
+    }
+}
+
+// The running sums of a lane's query: the weights' reference and sum (of this half's keys).
+struct Sums {
+    float ref, l;
+};
+
+// A block's scores s (16 keys of one query) become weights: p in the sum, w = p v as operands of the second product. v: the keys'
+// value scales, v_exponent: the exponent of the largest of them; by: what the scores are multiplied by.
+template <int PARTS, int DB>
+__device__ __forceinline__ void weigh(v16f s, const v4f *v, float by, int v_exponent, Sums *m, v16f (&o)[DB], v8h (&w)[2 * PARTS]) {
+    float top = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+    top = other_half_max(top) * by + (float)(v_exponent - kTop);
+    if (__any(top > m->ref + kLazy)) {
+        const float next = top > m->ref + kLazy ? top : m->ref;
+        if (__any(m->ref != -INFINITY)) {  // (nothing is there to rescale at first)
+            const float half = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m->ref - next) * 0.5f), all = half * half;
+            m->l = m->l * half * half;  // (the sum may be as large as 2^100 where the values are small)
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= all;
+        }
+        m->ref = next;
+    }
+    const float ref = m->ref == -INFINITY ? 0.0f : m->ref;
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], by, -ref));
+        float x = p * v[e / 4][e % 4];
+        // (of two parts both are made from the FP32 product: the compiler may round the exact one to FP16 for the first)
+        if constexpr (PARTS == 2) asm("" : "+v"(x));
+        sum += p;
+        const _Float16 hi = (_Float16)x;
+        w[e / 8 * PARTS][e % 8] = hi;
+        if constexpr (PARTS == 2) w[e / 8 * PARTS + 1][e % 8] = (_Float16)(x - (float)hi);
+    }
+    m->l += sum;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T *y, v4f v) {
+    T t[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = (T)v[e];
+    if constexpr (sizeof(T) == 4) *(v4f *)y = *(const v4f *)t;
+    else *(v2u *)y = *(const v2u *)t;
+}
+
+// ---- few rows --------------------------------------------------------------------------------------------------------------------
+
+// A workgroup takes up to 32 rows; its four waves take every fourth block of 32 keys each, on their own: a wave copies its blocks'
+// codes and scales straight to LDS, NS - 1 blocks ahead, and no wave waits for another before the end, where their parts meet.
+//
+// A slot holds a block's keys, values (rows of DP bytes) and 32 scales of either. Unit u of 16 bytes of a row lies at u ^ f(key), so
+// that neither the eight keys at one unit that eight lanes read as scores' operands, nor the eight keys at one unit that a
+// transposing read takes, share banks.
+template <int UNITS>
+__device__ __forceinline__ int place(int key) {
+    return UNITS == 4 ? (key >> 1 & 1) | ((key >> 2 ^ key >> 3) & 1) << 1 : (key & 7) ^ (key >> 3 & 1) << 2;
+}
+
+template <int DP, int NS>
+struct Ring {
+    static constexpr int UNITS = DP / 16, COPIES = UNITS / 2, KEYS = 32 * DP, SLOT = 2 * KEYS + 256, WAVE = NS * SLOT;
+    static constexpr int MERGE = 4 * 32 * (DP + 2) * 4;
+    static constexpr int LDS = 4 * WAVE > MERGE ? 4 * WAVE : MERGE;
+};
+
+template <typename T, int DP, int NS>
+__global__ void __launch_bounds__(256, 1) token_kernel(Args a) {
+    using R = Ring<DP, NS>;
+    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, UNITS = R::UNITS, COPIES = R::COPIES, DB = DP / 32, QN = DP / 16;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, h = lane >> 5;
+    const int hk = blockIdx.x % a.kv_heads, split = blockIdx.y;
+    Tile t;
+    if (!find_tile<32>(a, blockIdx.x / a.kv_heads, &t)) {
+        if (a.fill && split == 0 && (int)blockIdx.x / a.kv_heads == a.tiles) fill_rest<T>(a, hk, 256);
+        return;
+    }
+    const int count = min(32, t.rows - t.r0), row = min(t.r0 + n, t.rows - 1), token = row / a.group, head = hk * a.group + row - token * a.group;
+    const int p = t.start + token, p0 = t.start + t.r0 / a.group, p1 = t.start + (t.r0 + count - 1) / a.group;
+    const int hi = p, lo = max(0, p - a.left);
+
+    // the blocks of 32 keys that some row sees, this split's and this wave's share of them
+    const int first_key = max(0, p0 - a.left), block0 = first_key / 32, blocks = p1 < 0 ? 0 : p1 / 32 + 1 - block0;
+    const int share = ((blocks + a.splits - 1) / a.splits + 3) / 4 * 4;
+    const int from = min(blocks, split * share), to = min(blocks, from + share);
+    const int steps = from + wave < to ? (to - from - wave + 3) / 4 : 0;
+    if (to <= from && a.splits > 1) {  // nothing for this split
+        if (tid < count) {
+            const long long slot = ((long long)split * a.at.tokens + t.first + (t.r0 + tid) / a.group) * (a.kv_heads * a.group) + hk * a.group + (t.r0 + tid) % a.group;
+            *(float2 *)(a.stats + 2 * slot) = make_float2(-INFINITY, 0.0f);
+        }
+        return;
+    }
+
+    // a lane's row and unit in the rows of one copy; the places of the units repeat every 16 keys
+    constexpr int ROWS = 64 / UNITS, VARIANTS = 16 / ROWS;
+    const uint32_t ring = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)lds + wave * R::WAVE);
+    char *const own = lds + wave * R::WAVE;
+    uint32_t off_k[VARIANTS], off_v[VARIANTS];
+    bool some[VARIANTS];
+#pragma unroll
+    for (int u = 0; u < VARIANTS; ++u) {
+        const int in = lane / UNITS, unit = (lane % UNITS) ^ place<UNITS>(u * ROWS + in);
+        off_k[u] = (uint32_t)in * (uint32_t)a.kp.row_stride + 16 * unit;
+        off_v[u] = (uint32_t)in * (uint32_t)a.vp.row_stride + 16 * unit;
+        some[u] = 16 * unit < a.d;
+    }
+    const int8_t *const kd = a.kp.data_dev + (long long)hk * a.kp.head_stride, *const vd = a.vp.data_dev + (long long)hk * a.vp.head_stride;
+    const float *const ks = a.kp.scale_dev + (long long)hk * a.kp.scale_head_stride, *const vs = a.vp.scale_dev + (long long)hk * a.vp.scale_head_stride;
+    const int32_t *const table = a.at.table + (long long)t.b * a.at.table_stride;
+    const int last_entry = a.at.width - 1, page_mask = (1 << a.at.shift) - 1;
+    // the pages of the two halves of a block (uniform: read through the scalar cache)
+    auto entries = [&](int step) {
+        const int k0 = 32 * (block0 + from + wave + 4 * step);
+        typedef const __attribute__((address_space(4))) int32_t *uniform_t;
+        const uniform_t u = (uniform_t)(uintptr_t)table;
+        return make_int2(u[min(k0 >> a.at.shift, last_entry)], u[min((k0 + 16) >> a.at.shift, last_entry)]);
+    };
+    auto stage = [&](int step, int2 page) {
+        const int k0 = 32 * (block0 + from + wave + 4 * step);
+        const uint32_t dst = ring + step % NS * R::SLOT;
+        // (a half without a page is read from page 0, and masked)
+        const int2 at = make_int2((unsigned)page.x < (unsigned)a.at.pages ? page.x : 0, (unsigned)page.y < (unsigned)a.at.pages ? page.y : 0);
+        const int r0 = k0 & page_mask, r1 = (k0 + 16) & page_mask;
+        const int8_t *const k_half[2] = {kd + at.x * a.kp.page_stride + r0 * a.kp.row_stride, kd + at.y * a.kp.page_stride + r1 * a.kp.row_stride};
+        const int8_t *const v_half[2] = {vd + at.x * a.vp.page_stride + r0 * a.vp.row_stride, vd + at.y * a.vp.page_stride + r1 * a.vp.row_stride};
+#pragma unroll
+        for (int c = 0; c < COPIES; ++c) {
+            const int key = c * ROWS;
+            if (!some[c % VARIANTS]) continue;  // (units behind the row's end)
+            kea::copy16(k_half[key / 16] + (key & 15) * a.kp.row_stride, off_k[c % VARIANTS], dst + c * 1024);
+            kea::copy16(v_half[key / 16] + (key & 15) * a.vp.row_stride, off_v[c % VARIANTS], dst + R::KEYS + c * 1024);
+        }
+        const bool upper = n >= 16;
+        const long long in_page = n & 15;
+        const float *const k_from = ks + (upper ? at.y : at.x) * a.kp.scale_page_stride + ((upper ? r1 : r0) + in_page) * a.kp.scale_row_stride;
+        const float *const v_from = vs + (upper ? at.y : at.x) * a.vp.scale_page_stride + ((upper ? r1 : r0) + in_page) * a.vp.scale_row_stride;
+        kea::copy4(h ? v_from : k_from, dst + 2 * R::KEYS);
+    };
+    constexpr int COUNT = 2 * COPIES + 1;  // copies of a block
+    static_assert(COUNT * (NS - 1) < 64, "vmcnt");
+    auto landed = [&](int behind) {  // all copies but those of the last `behind` blocks
+        asm volatile("" ::: "memory");
+        auto wait = [&](auto left) {
+            constexpr int LEFT = decltype(left)::value * COUNT;
+            __builtin_amdgcn_s_waitcnt((LEFT & 15) | ((LEFT >> 4) << 14) | (15 << 8) | (7 << 4));
+        };
+        if (NS > 3 && behind >= 3) wait(std::integral_constant<int, (NS > 3 ? 3 : 0)>{});
+        else if (NS > 2 && behind == 2) wait(std::integral_constant<int, (NS > 2 ? 2 : 0)>{});
+        else if (behind == 1) wait(std::integral_constant<int, 1>{});
+        else wait(std::integral_constant<int, 0>{});
+        asm volatile("" ::: "memory");
+    };
+
+    int2 page[NS];  // of the blocks on their way, the next one to be computed first
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        page[s] = make_int2(-1, -1);
+        if (s < NS - 1 && s < steps) {
+            page[s] = entries(s);
+            stage(s, page[s]);
+        }
+    }
+    int2 next_page = NS - 1 < steps ? entries(NS - 1) : make_int2(-1, -1);
+
+    v8h q[QN * PARTS];
+    float by;
+    load_queries<T, QN>((const T *)a.q.data_dev + (long long)(t.first + token) * a.q.t_stride + (long long)head * a.q.head_stride, a.d, p >= 0,
+                        [&](int i) { return 16 * (2 * (i / 2) + h) + 8 * (i % 2); }, q, &by);
+    const float scale = a.scale * kLog2e;
+
+    v16f o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    Sums m{-INFINITY, 0.0f};
+    // operand addresses: unit 2 c + h of key n at ka ^ 32 c; eight keys' values of unit 2 d + (lane / 16) % 2, for the lanes' d
+    const int ka = n * DP + (h ^ place<UNITS>(n)) * 16;
+    const int vr = (lane & 15) >> 1, vkey = vr % 4 + 8 * (vr / 4) + 4 * h;
+    const int va = vkey * DP + ((lane >> 4 & 1) ^ place<UNITS>(vkey)) * 16 + (lane & 1) * 8;
+
+    for (int i = 0; i < steps; ++i) {
+        // the block that follows those on their way, into the slot that has been read
+        if (i + NS - 1 < steps) {
+            page[NS - 1] = next_page;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            stage(i + NS - 1, next_page);
+            if (i + NS < steps) next_page = entries(i + NS);
+        }
+        landed(min(NS - 1, steps - 1 - i));
+        const int k0 = 32 * (block0 + from + wave + 4 * i);
+        char *const slot = own + i % NS * R::SLOT;
+        float *const scales = (float *)(slot + 2 * R::KEYS);
+
+        // the scales: of keys that some row may see and that have a page, others 0; both rows are rewritten in place
+        const uint32_t paged = ((unsigned)page[0].x < (unsigned)a.at.pages ? 0xFFFFu : 0u) | ((unsigned)page[0].y < (unsigned)a.at.pages ? 0xFFFF0000u : 0u);
+        const int ahead = p1 - k0, behind = first_key - k0;  // the last and first key seen, in the block
+        const uint32_t valid = paged & (ahead >= 31 ? ~0u : (2u << ahead) - 1u) & (behind > 0 ? ~0u << behind : ~0u);
+        const float k_scale = scales[n], v_scale = scales[32 + n];
+        const bool there = valid >> n & 1, number = finite(v_scale);
+        const float x = !there ? 0.0f : number ? k_scale * scale : __builtin_nanf(""), y = there && number ? v_scale : 0.0f;
+        int v_exponent = max32(y != 0.0f ? max(exponent(y), kLeast) : kLeast);
+        asm volatile("" ::: "memory");
+        scales[lane] = h ? y : x;
+
+        v16f s = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < QN / 2; ++c) {
+            const v4u codes = *(const v4u *)(slot + (ka ^ 32 * c));
+            const v8h k_lo = numbers(codes[0], codes[1]), k_hi = numbers(codes[2], codes[3]);
+#pragma unroll
+            for (int u = 0; u < PARTS; ++u) {
+                s = mma(k_lo, q[2 * c * PARTS + u], s);
+                s = mma(k_hi, q[(2 * c + 1) * PARTS + u], s);
+            }
+        }
+        asm volatile("" ::: "memory");
+        v4f kx[4], vx[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kx[e] = *(const v4f *)(scales + 8 * e + 4 * h), vx[e] = *(const v4f *)(scales + 32 + 8 * e + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] *= kx[e / 4][e % 4];
+        if (!(valid == 0xFFFFFFFFu && k0 + 31 <= p0 && k0 >= p1 - a.left)) {  // not seen as a whole by every row
+            const int hx = hi - k0 - 4 * h, lx = lo - k0 - 4 * h;
+            const uint32_t bits = valid >> (4 * h);
+            float most = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int at = 8 * (e / 4) + e % 4;
+                const bool seen = at <= hx && at >= lx && (bits >> at & 1);
+                if (!seen) s[e] = -INFINITY;
+                most = fmaxf(most, seen ? fabsf(vx[e / 4][e % 4]) : 0.0f);
+            }
+            most = other_half_max(most);
+            v_exponent = most != 0.0f ? max(exponent(most), kLeast) : kLeast;  // (of what this query sees)
+        }
+        v8h w[2 * PARTS];
+        weigh<PARTS, DB>(s, vx, by, v_exponent, &m, o, w);
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const v2i codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32((ltr8_t)(slot + R::KEYS + (va ^ 32 * d) + 16 * z * DP));
+                const v8h v = numbers((uint32_t)codes[0], (uint32_t)codes[1]);
+#pragma unroll
+                for (int u = 0; u < PARTS; ++u) o[d] = mma(v, w[z * PARTS + u], o[d]);
+            }
+#pragma unroll
+        for (int s1 = 0; s1 + 1 < NS; ++s1) page[s1] = page[s1 + 1];
+    }
+    m.l = both_halves(m.l);
+
+    // the waves' means, references and sums meet in LDS: [wave][32][DP], then [wave][32][2]
+    float *const po = (float *)lds, *const ps = po + 4 * 32 * DP;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (n < count) {
+        const float inv = m.l != 0.0f ? 1.0f / m.l : 0.0f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int c = 8 * d + e / 2 + h;  // (units of four elements, moved by the row: 32 rows are written at once)
+                *(v4f *)(po + ((wave * 32 + n) * (DP / 4) + (c ^ (n & 7))) * 4) = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]} * inv;
+            }
+        if (h == 0) *(float2 *)(ps + 2 * (wave * 32 + n)) = make_float2(m.ref, m.l);
+    }
+    __syncthreads();
+    for (int at = tid; at < count * (DP / 4); at += 256) {
+        const int r = at / (DP / 4), c = at % (DP / 4);
+        if (4 * c >= a.d) continue;
+        float2 st[4];
+        float top = -INFINITY, all = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) st[w] = *(const float2 *)(ps + 2 * (w * 32 + r)), top = fmaxf(top, st[w].x);
+        v4f v = {0, 0, 0, 0};
+        float part[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            part[w] = st[w].y * (st[w].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st[w].x - top));  // (a NaN stays one)
+            all += part[w];
+        }
+        const float inv = all != 0.0f ? 1.0f / all : 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v += *(const v4f *)(po + ((w * 32 + r) * (DP / 4) + (c ^ (r & 7))) * 4) * (part[w] * inv);
+        const int tt = (t.r0 + r) / a.group, hh = hk * a.group + (t.r0 + r) - tt * a.group;
+        if (a.splits > 1) {
+            const long long slot = ((long long)split * a.at.tokens + t.first + tt) * (a.kv_heads * a.group) + hh;
+            *(v4f *)(a.part + slot * a.d + 4 * c) = v;
+            if (c == 0) *(float2 *)(a.stats + 2 * slot) = make_float2(top, all);
+        } else {
+            store4((T *)a.out.data_dev + (long long)(t.first + tt) * a.out.t_stride + (long long)hh * a.out.head_stride + 4 * c, v);
+        }
+    }
+}
+
+// Joins the splits: out = sum_s f_s mean_s, f_s = l_s 2^(ref_s - ref) over their sum; four elements a thread, eight splits at a time.
+template <typename T>
+__global__ void __launch_bounds__(64) join_kernel(Args a) {
+    const int heads = a.kv_heads * a.group, per = a.d / 4;
+    const long long at = (long long)blockIdx.x * 64 + threadIdx.x, slot0 = at / per, all_rows = (long long)a.at.tokens * heads;
+    if (slot0 >= all_rows) return;
+    const int c = (int)(at - slot0 * per), t = (int)(slot0 / heads), head = (int)(slot0 - (long long)t * heads);
+    if (a.at.offsets && !(t >= a.at.offsets[0] && t < a.at.offsets[a.at.batch])) return;
+    float ref = -INFINITY, all = 0.0f;
+    v4f v = {0, 0, 0, 0};
+    for (int s0 = 0; s0 < a.splits; s0 += 8) {
+        float2 st[8];
+        v4f part[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const long long slot = min(s0 + s, a.splits - 1) * all_rows + slot0;
+            st[s] = *(const float2 *)(a.stats + 2 * slot);
+            part[s] = *(const v4f *)(a.part + slot * a.d + 4 * c);
+        }
+        float top = ref;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) top = fmaxf(top, st[s].x);
+        const float old = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - top);
+        ref = top;
+        float f[8], sum = all * old;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            f[s] = s0 + s < a.splits ? st[s].y * (st[s].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st[s].x - top)) : 0.0f;
+            sum += f[s];
+        }
+        // (the sum so far is kept as a mean: it neither overflows nor loses digits that the mean has)
+        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+        v *= all * old * inv;
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+            if (f[s] != 0.0f) v += part[s] * (f[s] * inv);  // (a part that saw nothing was not written)
+        all = sum;
+    }
+    store4((T *)a.out.data_dev + (long long)t * a.out.t_stride + (long long)head * a.out.head_stride + 4 * c, v);
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------
+
+struct Plan {
+    int64_t tiles, tiles_each, splits, part_bytes, stats_bytes;
+};
+
+int plan_of(int64_t batch, int64_t tokens, int64_t positions, int64_t heads, int64_t kv_heads, int64_t d, int64_t left, bool offsets, Plan *out) {
+    const int64_t group = heads / kv_heads;
+    Plan p{};
+    const int64_t each = batch > 0 ? tokens / batch : 0;
+    p.tiles_each = (each * group + 31) / 32;
+    p.tiles = offsets ? tokens * group / 32 + batch : p.tiles_each * batch;
+    if (tokens * group > INT32_MAX / 4 || p.tiles > INT32_MAX / 4) return -1;
+    const int64_t wgs = p.tiles * kv_heads;
+    const int64_t span = left < positions ? left + 32 / group + 64 : positions, keys = span < positions ? span : positions;
+    p.splits = 1;
+    if (wgs > 0 && wgs < 512) {
+        int64_t s = 1024 / wgs;
+        const int64_t most = (keys + 255) / 256;
+        s = s < most ? s : most;
+        p.splits = s < 1 ? 1 : s < 64 ? s : 64;
+    }
+    if (p.splits > 1) {
+        p.part_bytes = p.splits * tokens * heads * d * 4;
+        p.stats_bytes = p.splits * tokens * heads * 8;
+    }
+    *out = p;
+    return 0;
+}
+
+int launched() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? KEA_OK : kea::fail((int)e, std::string("kea_paged_attention: ") + hipGetErrorString(e));
+}
+
+template <typename T, int DP, int NS>
+int run_shape(const Args &a, hipStream_t stream) {
+    using R = Ring<DP, NS>;
+    static_assert(R::LDS <= 160 * 1024, "LDS");
+    const int64_t tiles = ((int64_t)a.tiles + a.fill) * a.kv_heads;
+    const int64_t join = ((int64_t)a.at.tokens * a.kv_heads * a.group * (a.d / 4) + 63) / 64;
+    if (!kea::fits_dispatch(tiles, 256) || !kea::fits_dispatch(join, 64)) return kea::fail(KEA_EINVAL, "kea_paged_attention: too large for one launch");
+    const auto kernel = token_kernel<T, DP, NS>;
+    if (R::LDS > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, R::LDS);
+        if (e != hipSuccess) return kea::fail((int)e, std::string("kea_paged_attention: ") + hipGetErrorString(e));
+    }
+    kernel<<<dim3((unsigned)tiles, (unsigned)a.splits), 256, R::LDS, stream>>>(a);
+    const int rc = launched();
+    if (rc || a.splits == 1) return rc;
+    join_kernel<T><<<dim3((unsigned)join), 64, 0, stream>>>(a);
+    return launched();
+}
+
+template <typename T>
+int run(const Args &a, hipStream_t stream) {
+    return a.d <= 64 ? run_shape<T, 64, 4>(a, stream) : a.d <= 128 ? run_shape<T, 128, 3>(a, stream) : run_shape<T, 256, 2>(a, stream);
+}
+
+bool rows_ok(const kea_heads *t, int64_t unit) {
+    return t && t->t_stride >= 0 && t->head_stride >= 0 && (uintptr_t)t->data_dev % 16 == 0 && t->t_stride % unit == 0 && t->head_stride % unit == 0;
+}
+
+int check_sizes(const char *what, int dtype, int64_t batch, int64_t tokens, int64_t positions, int64_t heads, int64_t kv_heads, int64_t d,
+                int64_t left, bool offsets, Plan *p) {
+    const std::string name(what);
+    if (dtype != KEA_F32 && dtype != KEA_F16 && dtype != KEA_BF16) return kea::fail(KEA_EINVAL, name + ": f32, f16 or bf16");
+    if (batch < 0 || tokens < 0 || positions < 0 || batch >= (1 << 30) || tokens >= (1 << 30) || positions > (1 << 30) || heads < 1 || kv_heads < 1 || heads % kv_heads ||
+        heads > 65535 || left < 0)
+        return kea::fail(KEA_EINVAL, name + ": sizes are not negative and below 2^30, heads a multiple of kv_heads");
+    if (d < 16 || d > 256 || d % 16) return kea::fail(KEA_EINVAL, name + ": d is a multiple of 16 from 16 to 256");
+    if (plan_of(batch, tokens, positions, heads, kv_heads, d, left, offsets, p)) return kea::fail(KEA_EINVAL, name + ": too large for one launch");
+    return KEA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t kea_paged_attention_workspace(int dtype, int64_t batch, int64_t tokens, int64_t positions, int64_t heads, int64_t kv_heads, int64_t d,
+                                      int64_t left, int offsets) {
+    Plan p;
+    const int rc = check_sizes("kea_paged_attention_workspace", dtype, batch, tokens, positions, heads, kv_heads, d, left, offsets != 0, &p);
+    return rc ? rc : p.part_bytes + p.stats_bytes;
+}
+
+int kea_paged_attention(const kea_heads *q, const kea_heads *out, int dtype, int64_t heads, int64_t kv_heads, int64_t d, const kea_pages *k_pages,
+                        const kea_pages *v_pages, const kea_paging *paging, int64_t left, float scale, int fill, void *workspace,
+                        int64_t workspace_bytes, void *stream) {
+    Args a{};
+    const int bad = kea::check_paging("kea_paged_attention", k_pages, v_pages, paging, kv_heads, d, &a.at);
+    if (bad) return bad;
+    Plan p;
+    const int rc = check_sizes("kea_paged_attention", dtype, paging->batch, paging->tokens, paging->table_width * paging->page_size, heads, kv_heads, d,
+                               left, paging->q_offsets_dev != nullptr, &p);
+    if (rc) return rc;
+    const int64_t unit = dtype == KEA_F32 ? 4 : 8;
+    if (!rows_ok(q, unit) || !rows_ok(out, unit)) return kea::fail(KEA_EALIGN, "kea_paged_attention: rows and their strides are multiples of 16 bytes, strides not negative");
+    if (!std::isfinite(scale)) return kea::fail(KEA_EINVAL, "kea_paged_attention: the scale is not finite");
+    if (k_pages->row_stride >= (1 << 26) || v_pages->row_stride >= (1 << 26)) return kea::fail(KEA_EINVAL, "kea_paged_attention: rows of a page 2^26 bytes and more apart");
+    if (paging->tokens == 0) return KEA_OK;
+    if (!q->data_dev || !out->data_dev) return kea::fail(KEA_EINVAL, "kea_paged_attention: a pointer is missing");
+    if (workspace_bytes < p.part_bytes + p.stats_bytes || (p.splits > 1 && !workspace)) return kea::fail(KEA_ESPACE, "kea_paged_attention: the workspace is too small");
+    if ((uintptr_t)workspace % 16) return kea::fail(KEA_EALIGN, "kea_paged_attention: the workspace is aligned to 16 bytes");
+    a.q = *q, a.out = *out, a.kp = *k_pages, a.vp = *v_pages;
+    a.part = (float *)workspace, a.stats = workspace ? (float *)((char *)workspace + p.part_bytes) : nullptr;
+    a.kv_heads = (int)kv_heads, a.group = (int)(heads / kv_heads), a.d = (int)d, a.left = (int)(left < (1 << 30) ? left : 1 << 30);
+    a.splits = (int)p.splits, a.tiles_each = (int)p.tiles_each, a.tiles = (int)p.tiles, a.scale = scale;
+    a.fill = fill && paging->q_offsets_dev ? 1 : 0;
+    const hipStream_t s = (hipStream_t)stream;
+    return dtype == KEA_F32 ? run<float>(a, s) : dtype == KEA_F16 ? run<_Float16>(a, s) : run<__bf16>(a, s);
+}
+
+}  // extern "C"

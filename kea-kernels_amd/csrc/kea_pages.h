@@ -54,7 +54,7 @@ inline int check_paging(const char *what, const kea_pages *k, const kea_pages *v
     const std::string name(what);
     if (!g || g->batch < 0 || g->batch >= (1 << 30) || g->tokens < 0 || g->tokens >= (1 << 30) || g->pages < 0 || g->pages > INT32_MAX || g->table_width < 0 || g->table_stride < 0)
         return fail(KEA_EINVAL, name + ": batch, tokens, pages and the table's width are >= 0 and below 2^30");
-    if (g->page_size < 8 || g->page_size > 1024 || (g->page_size & (g->page_size - 1))) return fail(KEA_EINVAL, name + ": a page holds a power of two of 8 to 1024 positions");
+    if (g->page_size < 16 || g->page_size > 1024 || (g->page_size & (g->page_size - 1))) return fail(KEA_EINVAL, name + ": a page holds a power of two of 16 to 1024 positions");
     if (g->table_width > (1 << 30) / g->page_size) return fail(KEA_EINVAL, name + ": more than 2^30 positions");
     if (kv_heads < 1 || kv_heads > 65535 || d < 16 || d > 256 || d % 16) return fail(KEA_EINVAL, name + ": 1 to 65535 heads of a multiple of 16, 16 to 256, elements");
     if (!g->q_offsets_dev && g->batch > 0 && g->tokens % g->batch) return fail(KEA_EINVAL, name + ": without offsets every sequence has as many tokens");

@@ -32,6 +32,7 @@
 #include <cstdint>
 #include <string>
 
+#include "kea_attend.h"
 #include "kea_internal.h"
 #include "../../include/kea_block.h"
 
@@ -43,7 +44,7 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(3))) void *lptr_t;
+using kea::lptr_t;
 typedef __attribute__((address_space(3))) v4s *ltr_t;
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -99,34 +100,10 @@ __device__ __forceinline__ int swizzle_v(int key) {
     return F32 ? key & 7 : UNITS == 8 ? (key >> 1 & 1) * 4 : (key & 3) * 4;
 }
 
-// A lane's value and that of the lane 32 away, the lower half's first. (The components are read before they are cast:
-// hipcc's __builtin_bit_cast of a component access gives component 0.)
-__device__ __forceinline__ float2 halves(float v) {
-    const uint32_t bits = __builtin_bit_cast(uint32_t, v);
-    const auto s = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
-    const uint32_t lower = s[0], upper = s[1];
-    return make_float2(__builtin_bit_cast(float, lower), __builtin_bit_cast(float, upper));
-}
-__device__ __forceinline__ float other_half_max(float v) {
-    const float2 s = halves(v);
-    return fmaxf(s.x, s.y);
-}
-__device__ __forceinline__ float both_halves(float v) {
-    const float2 s = halves(v);
-    return s.x + s.y;
-}
-
-// 16 bytes a lane from global memory straight to LDS, at the wave's base address plus 16 a lane; done when vmcnt says so. In
-// place of the builtin, after which the compiler waits for all of a wave's copies before its next transposing read, those for
-// the tile ahead among them. (Nothing else here uses m0.) The second form reads at a uniform address plus an offset.
-__device__ __forceinline__ void copy16(const void *src, uint32_t base) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(src) : "memory");
-}
-__device__ __forceinline__ void copy16(const void *src, uint32_t offset, uint32_t base) {
-    const uint64_t at = (uint64_t)(uintptr_t)src;
-    const uint64_t uniform = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(base)), "v"(offset), "s"(uniform) : "memory");
-}
+using kea::both_halves;
+using kea::copy16;
+using kea::halves;
+using kea::other_half_max;
 
 template <typename T>
 __device__ __forceinline__ v16f mma(v8s a, v8s b, v16f c) {

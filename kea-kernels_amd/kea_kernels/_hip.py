@@ -127,6 +127,8 @@ SIGNATURES = {
                              _i64, _i32, _vp]),
     "kea_paged_write": (_i32, [_heads, _heads, _i32, _i64, _i64, _pages, _pages, _paging, _vp]),
     "kea_paged_read": (_i32, [_pages, _pages, _paging, _vp, _i64, _i64, _i64, _vp, _vp, _i32, _vp]),
+    "kea_paged_attention_workspace": (_i64, [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32]),
+    "kea_paged_attention": (_i32, [_heads, _heads, _i32, _i64, _i64, _i64, _pages, _pages, _paging, _i64, _f32, _i32, _vp, _i64, _vp]),
     "kea_last_error": (_cp, []),
     "kea_version": (_i32, []),
 }

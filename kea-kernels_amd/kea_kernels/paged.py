@@ -9,11 +9,14 @@ current stream of the tensors' device and never synchronize the host.
 """
 from __future__ import annotations
 
+import ctypes
+import math
+
 import torch
 from torch import Tensor
 
 from kea_kernels import _hip
-from kea_kernels.window import _span
+from kea_kernels.window import _bound, _span
 
 _MOST = 1 << 30  # positions of a sequence, tokens of a call
 
@@ -27,7 +30,7 @@ def _distinct(name: str, t: Tensor) -> None:
 
 class Cache:
     """Keys and values as int8 `k`, `v` [pages, kv_heads, page_size, D] with FP32 scales `k_scale`, `v_scale` [pages, kv_heads,
-    page_size]: element e of a row stands for k[..., e] * k_scale[...]. page_size is a power of two from 8 to 1024, D a multiple of 16
+    page_size]: element e of a row stands for k[..., e] * k_scale[...]. page_size is a power of two from 16 to 1024, D a multiple of 16
     up to 256; rows of D are contiguous and start at multiples of 16 bytes, the other dimensions may have any order in memory. The
     tensors are the caller's (no copies are made); pages need no initial values."""
 
@@ -35,8 +38,8 @@ class Cache:
         if k.dim() != 4 or k.dtype != torch.int8 or k.shape != v.shape or v.dtype != torch.int8:
             raise ValueError(f"k and v must be int8 [pages, kv_heads, page_size, D], got {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}")
         pages, heads, size, d = k.shape
-        if size < 8 or size > 1024 or size & (size - 1):
-            raise ValueError(f"page size {size}: a power of two from 8 to 1024")
+        if size < 16 or size > 1024 or size & (size - 1):
+            raise ValueError(f"page size {size}: a power of two from 16 to 1024")
         if d < 16 or d > 256 or d % 16 or not 1 <= heads <= 65535:
             raise ValueError(f"{heads} heads of {d}: at least one, of a multiple of 16 from 16 to 256")
         for name, t in (("k", k), ("v", v)):
@@ -180,6 +183,51 @@ def read(cache: Cache, table: Tensor, kv_lengths: Tensor, length: int, *, starts
                                            _hip.stream_handle(cache.device))
         _hip.check(rc, "kea_paged_read")
     return k, v
+
+
+def attention(q: Tensor, cache: Cache, table: Tensor, kv_lengths: Tensor, q_offsets: Tensor | None = None, *, left: int | None = None,
+              scale: float | None = None, out: Tensor | None = None) -> Tensor:
+    """out [T, H, D] = attention of the new tokens q [T, H, D] (f32, f16 or bf16; H a multiple of kv_heads, query head h reads key head
+    h // (H / kv_heads)) to their sequences' positions in the cache, their own among them: `write` comes first. table, kv_lengths and
+    q_offsets as there: the n rows of a sequence of len positions stand at len - n .. len - 1, and the token at position p sees
+    position j iff p - left <= j <= p (left None: all before) and the table names a page for it. A token that sees nothing gives
+    zeros, and so do rows of no sequence, but in `out`, where those stay as they are. What a token does not see has no part in its
+    output, whatever it holds. scale: 1 / sqrt(D) unless given, any finite FP32 number. out must not overlap an input.
+
+    Scores, maxima and sums are FP32 and the codes enter the products exactly; the softmax's weights times the values' scales are
+    rounded to FP16 (f32: to two parts, 22 bits), and so are bf16 and f32 queries, after a power of two of each row's own (what is
+    below 2^-28 of a row's largest element is lost; f32 keeps 22 bits)."""
+    if out is None and (hit := _native("paged_attention", cache, q, table, kv_lengths, q_offsets, left, scale)) is not None:
+        return hit
+    rows = _rows("q", q, cache, None)
+    (tokens, h, d), hk, device = q.shape, cache.kv_heads, cache.device
+    if h < 1 or h % hk or h > 65535:
+        raise ValueError(f"{h} query heads are no multiple of {hk} key heads")
+    paging = _paging(cache, table, kv_lengths, q_offsets, tokens)
+    scale = 1 / math.sqrt(d) if scale is None else ctypes.c_float(scale).value
+    if not math.isfinite(scale):
+        raise ValueError("scale is not a finite FP32 number")
+    left = _bound("left", left)
+    fill = out is None
+    if out is not None:
+        _rows("out", out, cache, h)
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, q {q.dtype} {tuple(q.shape)}")
+        _distinct("out", out)
+        _apart("out", (out,), (q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, kv_lengths, q_offsets))
+    _hip.refuse_grad("paged.attention", q, cache.k_scale, cache.v_scale, out)
+    if out is None:
+        out = torch.empty(tokens, h, d, dtype=q.dtype, device=device)
+    if not tokens:
+        return out
+    L, code, batch, width = _hip.lib(), _hip.dtype_code(q.dtype), *table.shape
+    with _hip.on_device(device):
+        need = L.kea_paged_attention_workspace(code, batch, tokens, width * cache.page_size, h, hk, d, left, q_offsets is not None)
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+        rc = L.kea_paged_attention(rows, _rows("out", out, cache, h), code, h, hk, d, _pages(cache.k, cache.k_scale),
+                                   _pages(cache.v, cache.v_scale), paging, left, scale, fill, _hip.ptr(ws), max(need, 0), _hip.stream_handle(device))
+    _hip.check(rc, "kea_paged_attention")
+    return out
 
 
 def _native(name: str, cache: Cache, *args):

@@ -57,8 +57,8 @@ def plain(t):
     return t.detach().cpu().clone()
 
 
-CASES = [([1], [1], 1, 64, 16), ([1, 1, 1], [5, 16, 33], 4, 128, 16), ([7, 0, 40, 1], [40, 9, 40, 100], 2, 80, 32), ([3, 3], [3, 260], 5, 16, 8),
-         ([130], [130], 3, 256, 64), ([65, 64, 63], [200, 64, 70], 8, 96, 128), ([2] * 70, [9] * 70, 2, 48, 8)]
+CASES = [([1], [1], 1, 64, 16), ([1, 1, 1], [5, 16, 33], 4, 128, 16), ([7, 0, 40, 1], [40, 9, 40, 100], 2, 80, 32), ([3, 3], [3, 260], 5, 16, 16),
+         ([130], [130], 3, 256, 64), ([65, 64, 63], [200, 64, 70], 8, 96, 128), ([2] * 70, [9] * 70, 2, 48, 16)]
 
 
 @pytest.mark.gpu
@@ -124,26 +124,26 @@ def test_read_gives_the_values(news, lengths, heads, d, size, dtype):
 def test_bad_entries_lengths_and_offsets_are_left_out():
     """Entries that name no page, lengths past the table or below the new tokens, rows in front of and behind all sequences."""
     g = torch.Generator().manual_seed(4)
-    cache = make_cache(6, 2, 8, 32, g)
+    cache = make_cache(6, 2, 16, 32, g)
     want = [plain(t) for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
     table = torch.tensor([[0, -1, 3], [6, 1, 2**31 - 1], [4, -(2**31), 5]], dtype=torch.int32)
-    lengths, offsets = torch.tensor([20, 14, 1000], dtype=torch.int32), torch.tensor([2, 22, 42, 50], dtype=torch.int32)
+    lengths, offsets = torch.tensor([40, 14, 1000], dtype=torch.int32), torch.tensor([2, 22, 42, 50], dtype=torch.int32)
     k, v = (torch.randn(60, 2, 32, generator=g) for _ in range(2))
-    for b, (n, lo, hi) in enumerate(((20, 2, 22), (14, 22, 42), (24, 42, 50))):
+    for b, (n, lo, hi) in enumerate(((40, 2, 22), (14, 22, 42), (48, 42, 50))):
         for t in range(lo, hi):
             p = n - hi + t
-            if p >= 0 and 0 <= int(table[b, p // 8]) < 6:
-                page, row = int(table[b, p // 8]), p % 8
+            if p >= 0 and 0 <= int(table[b, p // 16]) < 6:
+                page, row = int(table[b, p // 16]), p % 16
                 want[0][page, :, row], want[2][page, :, row] = rows8(k[t])
                 want[1][page, :, row], want[3][page, :, row] = rows8(v[t])
     paged.write(cache, k.to(DEV), v.to(DEV), table.to(DEV), lengths.to(DEV), offsets.to(DEV))
     for got, w in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), want):
         assert torch.equal(got.cpu(), w)
-    values = paged.read(cache, table.to(DEV), lengths.to(DEV), 30)
-    for b, n in enumerate((20, 14, 24)):
-        for p in range(30):
-            page = int(table[b, p // 8]) if p < n else -1
-            w = want[0][page, :, p % 8].float() * want[2][page, :, p % 8][:, None] if 0 <= page < 6 else torch.zeros(2, 32)
+    values = paged.read(cache, table.to(DEV), lengths.to(DEV), 60)
+    for b, n in enumerate((40, 14, 48)):
+        for p in range(60):
+            page = int(table[b, p // 16]) if p < n else -1
+            w = want[0][page, :, p % 16].float() * want[2][page, :, p % 16][:, None] if 0 <= page < 6 else torch.zeros(2, 32)
             assert torch.equal(values[0][b, p].cpu(), w)
     # lengths below zero, a table without columns, no sequences, no tokens
     before = [plain(t) for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
@@ -169,12 +169,12 @@ def test_values_that_are_no_numbers_and_of_any_size(dtype):
     x[4] = (x[4].float().clamp(-1, 1) * big).to(dtype)
     x[5] = (x[5].float() * small).to(dtype)
     x[6, 0, 1:] = 0.0
-    cache = paged.Cache.empty(1, 8, 1, 64, DEV)
+    cache = paged.Cache.empty(1, 16, 1, 64, DEV)
     table, lengths = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.tensor([8], dtype=torch.int32, device=DEV)
     paged.write(cache, x.to(DEV), -x.to(DEV), table, lengths)
     c, s = rows8(x)
-    assert torch.equal(cache.k[0, 0].cpu(), c[:, 0]) and torch.equal(cache.v[0, 0].cpu(), -c[:, 0])
-    assert torch.equal(cache.k_scale[0, 0].cpu().nan_to_num(-1.0), s[:, 0].nan_to_num(-1.0))
+    assert torch.equal(cache.k[0, 0, :8].cpu(), c[:, 0]) and torch.equal(cache.v[0, 0, :8].cpu(), -c[:, 0])
+    assert torch.equal(cache.k_scale[0, 0, :8].cpu().nan_to_num(-1.0), s[:, 0].nan_to_num(-1.0))
     k, v = paged.read(cache, table, lengths, 8, out_dtype=dtype)
     assert torch.isnan(k[0, 1:4]).all() and torch.isnan(v[0, 1:4]).all() and torch.isfinite(k[0, 4:]).all()
     # a value is within half a step of its row, and half a step of the type
@@ -190,14 +190,14 @@ def test_views_of_a_fused_projection_and_far_pages():
     g = torch.Generator().manual_seed(6)
     fused = torch.randn(5, 6, 64, generator=g).half()
     dev = fused.to(DEV)
-    store = torch.empty(2, 2 * 8 * 64, dtype=torch.int8, device=DEV)
+    store = torch.empty(2, 2 * 16 * 64, dtype=torch.int8, device=DEV)
     far = torch.empty((1 << 31) + 4096, dtype=torch.int8, device=DEV)
-    k = far.as_strided((2, 2, 8, 64), (1 << 31, 512, 64, 1))
-    scale = torch.empty(2, 2, 8, device=DEV)
-    cache = paged.Cache(k, store.view(2, 2, 8, 64), scale, torch.empty_like(scale))
-    table, lengths = torch.tensor([[1, 0]], dtype=torch.int32, device=DEV), torch.tensor([10], dtype=torch.int32, device=DEV)
+    k = far.as_strided((2, 2, 16, 64), (1 << 31, 1024, 64, 1))
+    scale = torch.empty(2, 2, 16, device=DEV)
+    cache = paged.Cache(k, store.view(2, 2, 16, 64), scale, torch.empty_like(scale))
+    table, lengths = torch.tensor([[1, 0]], dtype=torch.int32, device=DEV), torch.tensor([19], dtype=torch.int32, device=DEV)
     paged.write(cache, dev[:, 2:4], dev[:, 4:], table, lengths)
-    got = paged.read(cache, table, lengths, 5, starts=torch.tensor([5], dtype=torch.int32, device=DEV))
+    got = paged.read(cache, table, lengths, 5, starts=torch.tensor([14], dtype=torch.int32, device=DEV))
     for x, y in ((fused[:, 2:4], got[0][0]), (fused[:, 4:], got[1][0])):
         c, s = rows8(x)
         assert torch.equal(y.cpu(), c.float() * s[..., None])
@@ -229,18 +229,18 @@ def test_captured_calls_follow_the_lengths():
         assert torch.equal(out[0][1, n - last:n].cpu(), c.float() * s[..., None])
 
 
-def cpu_cache(pages=3, heads=2, size=8, d=32):
+def cpu_cache(pages=3, heads=2, size=16, d=32):
     return paged.Cache.empty(pages, size, heads, d, "cpu")
 
 
 def test_cache_refusals():
-    i, s = torch.zeros(3, 2, 8, 32, dtype=torch.int8), torch.zeros(3, 2, 8)
+    i, s = torch.zeros(3, 2, 16, 32, dtype=torch.int8), torch.zeros(3, 2, 16)
     paged.Cache(i, i.clone(), s, s.clone())
     for bad in (lambda: paged.Cache(i.float(), i.clone(), s, s.clone()), lambda: paged.Cache(i, i[:2], s, s.clone()), lambda: paged.Cache(i[0], i[0].clone(), s, s.clone()),
                 lambda: paged.Cache(i, i.clone(), s.half(), s.clone()), lambda: paged.Cache(i, i.clone(), s, s[:2]), lambda: paged.Cache(i, i, s, s.clone()),
                 lambda: paged.Cache(i, i.clone(), s, s), lambda: paged.Cache(i[:1].expand(3, -1, -1, -1), i.clone(), s, s.clone()),
                 lambda: paged.Cache(i.transpose(2, 3), i.clone().transpose(2, 3), torch.zeros(3, 2, 32), torch.ones(3, 2, 32)),
-                lambda: paged.Cache(i, i.clone(), s[:1].expand(3, -1, -1), s.clone()), lambda: cpu_cache(size=12), lambda: cpu_cache(size=4),
+                lambda: paged.Cache(i, i.clone(), s[:1].expand(3, -1, -1), s.clone()), lambda: cpu_cache(size=12), lambda: cpu_cache(size=8),
                 lambda: cpu_cache(size=2048), lambda: cpu_cache(d=24), lambda: cpu_cache(d=272), lambda: cpu_cache(heads=0)):
         with pytest.raises(ValueError):
             bad()
@@ -270,18 +270,18 @@ def test_call_refusals():
 
 def test_library_refusals():
     L, one, odd = _hip.lib(), 16, 8
-    heads, pages = _hip.Heads(one, 0, 64, 32), _hip.Pages(one, one, 512, 256, 32, 16, 8, 1)
-    paging = lambda **kw: _hip.Paging(*{**dict(table=one, kv_lengths=one, q_offsets=one, table_stride=3, table_width=3, batch=2, pages=3, page_size=8,  # noqa: E731
+    heads, pages = _hip.Heads(one, 0, 64, 32), _hip.Pages(one, one, 1024, 512, 32, 32, 16, 1)
+    paging = lambda **kw: _hip.Paging(*{**dict(table=one, kv_lengths=one, q_offsets=one, table_stride=3, table_width=3, batch=2, pages=3, page_size=16,  # noqa: E731
                                                tokens=4), **kw}.values())
     write = lambda k=heads, t=0, hk=2, d=32, p=pages, g=None: L.kea_paged_write(k, k, t, hk, d, p, p, g or paging(), None)  # noqa: E731
     read = lambda p=pages, g=None, n=4, k=one, t=0, s=None: L.kea_paged_read(p, p, g or paging(), s, n, 2, 32, k, k, t, None)  # noqa: E731
     for rc in (write(t=3), write(hk=0), write(d=24), write(d=272), write(g=paging(batch=-1)), write(g=paging(tokens=-1)), write(g=paging(page_size=12)),
-               write(g=paging(page_size=4)), write(g=paging(page_size=2048)), write(g=paging(table_width=1 << 28)), write(g=paging(q_offsets=None, tokens=3)),
-               write(g=paging(kv_lengths=None)), write(g=paging(table=None)), write(p=_hip.Pages(None, one, 512, 256, 32, 16, 8, 1)),
+               write(g=paging(page_size=8)), write(g=paging(page_size=2048)), write(g=paging(table_width=1 << 28)), write(g=paging(q_offsets=None, tokens=3)),
+               write(g=paging(kv_lengths=None)), write(g=paging(table=None)), write(p=_hip.Pages(None, one, 1024, 512, 32, 32, 16, 1)),
                write(k=_hip.Heads(None, 0, 64, 32)), read(t=5), read(n=-1), read(n=(1 << 30) + 1), read(k=None)):
         assert rc == -1
     for rc in (write(k=_hip.Heads(odd, 0, 64, 32)), write(k=_hip.Heads(one, 0, 66, 32)), write(k=_hip.Heads(one, 0, -64, 32)),
-               write(p=_hip.Pages(odd, one, 512, 256, 32, 16, 8, 1)), write(p=_hip.Pages(one, 18, 512, 256, 32, 16, 8, 1)),
-               write(p=_hip.Pages(one, one, 520, 256, 32, 16, 8, 1)), write(g=paging(table=18)), read(k=odd), read(s=ctypes.c_void_p(18))):
+               write(p=_hip.Pages(odd, one, 1024, 512, 32, 32, 16, 1)), write(p=_hip.Pages(one, 18, 1024, 512, 32, 32, 16, 1)),
+               write(p=_hip.Pages(one, one, 1032, 512, 32, 16, 8, 1)), write(g=paging(table=18)), read(k=odd), read(s=ctypes.c_void_p(18))):
         assert rc == -2
     assert write(g=paging(tokens=0)) == 0 and read(n=0) == 0 and write(g=paging(batch=0, tokens=0)) == 0
