@@ -1,8 +1,7 @@
 // The host side of an operator call in one native call: argument checks on the tensors' own fields, the output and
 // workspace allocations and the library's launch, without the Python objects (shape tuples, dictionary keys, ctypes
-// conversions) that cost a call more than its two kernel launches. The module extends kea_kernels.lowbit, int8, norms and
-// window: everything it does
-// not take (tensor subclasses and transforms, arguments that would raise) it declines by returning None / False, and the
+// conversions) that cost a call more than its two kernel launches. The module extends kea_kernels.lowbit, int8, norms,
+// window, int4 and paged: everything it does not take (tensor subclasses and transforms, arguments that would raise) it declines by returning None / False, and the
 // caller's Python path, which holds the full checks and their messages, runs instead.
 //
 // Calls in a row, host bound: Int8MmaLayer.linear at M = 128, N = 4096, K = 1024 (fp16 in and out) 13.2 -> 9.3 us, at one
@@ -41,6 +40,10 @@ struct Library {
     decltype(&kea_window_attention) window = nullptr;
     decltype(&kea_window_attention_workspace) window_workspace = nullptr;
     decltype(&kea_int4_gemm) int4_gemm = nullptr;
+    decltype(&kea_paged_write) paged_write = nullptr;
+    decltype(&kea_paged_read) paged_read = nullptr;
+    decltype(&kea_paged_attention) paged_attention = nullptr;
+    decltype(&kea_paged_attention_workspace) paged_workspace = nullptr;
 } lib;
 
 // The tensor behind an exact torch.Tensor whose memory a kernel may read as it is: on a GPU, strided, no transform
@@ -665,11 +668,154 @@ PyObject *native_int4_gemm(PyObject *, PyObject *const *args, Py_ssize_t count) 
     Py_RETURN_NONE;
 }
 
-// bind_decode(int4_gemm)
+// The cache's tensors (args[0 .. 3]: k, v and their scales) as kea_pages; false where they are not what paged.Cache holds.
+struct PagedCache {
+    const at::Tensor *t[4];
+    kea_pages k, v;
+    int64_t pages, heads, size, d;
+};
+bool cache_of(PyObject *const *args, PagedCache *c) {
+    for (int i = 0; i < 4; ++i)
+        if (!(c->t[i] = plain(args[i])) || c->t[i]->device() != c->t[0]->device()) return false;
+    const at::Tensor &k = *c->t[0];
+    if (k.dim() != 4) return false;
+    c->pages = k.size(0), c->heads = k.size(1), c->size = k.size(2), c->d = k.size(3);
+    for (int i = 0; i < 2; ++i) {
+        const at::Tensor &t = *c->t[i], &s = *c->t[2 + i];
+        if (t.scalar_type() != at::kChar || t.sizes() != k.sizes() || t.stride(3) != 1 || (uintptr_t)t.const_data_ptr() % 16 || s.scalar_type() != at::kFloat ||
+            s.dim() != 3 || s.size(0) != c->pages || s.size(1) != c->heads || s.size(2) != c->size)
+            return false;
+        int64_t st[6];
+        for (int j = 0; j < 3; ++j) {
+            st[j] = t.size(j) > 1 ? t.stride(j) : 0;
+            st[3 + j] = s.size(j) > 1 ? s.stride(j) : 0;
+            if (st[j] % 16) return false;
+        }
+        (i ? c->v : c->k) = kea_pages{(int8_t *)const_cast<void *>(t.const_data_ptr()), (float *)const_cast<void *>(s.const_data_ptr()), st[0], st[1], st[2], st[3], st[4], st[5]};
+    }
+    return true;
+}
+
+bool index_of(const at::Tensor *t, int64_t n) { return t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == n && t->is_contiguous(); }
+
+// The table, lengths and offsets (args[0 .. 2]; offsets may be None) for `tokens` new tokens.
+bool paging_of(PyObject *const *args, const PagedCache &c, int64_t tokens, const at::Tensor **t, kea_paging *g) {
+    const auto device = c.t[0]->device();
+    t[0] = plain(args[0]), t[1] = plain(args[1]);
+    if (!t[0] || !t[1] || t[0]->device() != device || t[1]->device() != device || !optional(args[2], device, &t[2])) return false;
+    const at::Tensor &table = *t[0];
+    if (table.scalar_type() != at::kInt || table.dim() != 2 || (table.size(1) > 1 && table.stride(1) != 1)) return false;
+    const int64_t batch = table.size(0), width = table.size(1);
+    if (batch < 1 || width * c.size > (1 << 30) || !index_of(t[1], batch) || (t[2] ? !index_of(t[2], batch + 1) : tokens % batch != 0)) return false;
+    *g = kea_paging{(const int32_t *)table.const_data_ptr(), (const int32_t *)t[1]->const_data_ptr(), t[2] ? (const int32_t *)t[2]->const_data_ptr() : nullptr,
+                    batch > 1 ? table.stride(0) : 0, width, batch, c.pages, c.size, tokens};
+    return true;
+}
+
+// [tokens][heads][d] of a float type; heads 0: any number.
+bool tokens_of(const at::Tensor &t, int64_t heads, int64_t d, kea_heads *h) {
+    if (code_of(t.scalar_type()) < 0 || t.dim() != 3 || t.size(0) < 1 || (heads && t.size(1) != heads) || t.size(2) != d || t.stride(2) != 1 || (uintptr_t)t.const_data_ptr() % 16)
+        return false;
+    const int64_t unit = 16 / (int64_t)t.element_size();
+    int64_t s[2];
+    for (int i = 0; i < 2; ++i) {
+        s[i] = t.size(i) > 1 ? t.stride(i) : 0;
+        if (s[i] % unit) return false;
+    }
+    *h = kea_heads{const_cast<void *>(t.const_data_ptr()), 0, s[0], s[1]};
+    return true;
+}
+
+// paged_write(cache x 4, k, v, table, kv_lengths, q_offsets) -> True, or None
+PyObject *native_paged_write(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    PagedCache c;
+    const at::Tensor *g[3], *x[2];
+    kea_heads h[2];
+    kea_paging paging;
+    if (count != 9 || modes_active() || !cache_of(args, &c)) Py_RETURN_NONE;
+    const auto device = c.t[0]->device();
+    if (!current(device) || !optional(args[4], device, &x[0]) || !optional(args[5], device, &x[1]) || !x[0] || !x[1] || x[0]->scalar_type() != x[1]->scalar_type() ||
+        x[0]->sizes() != x[1]->sizes() || !tokens_of(*x[0], c.heads, c.d, &h[0]) || !tokens_of(*x[1], c.heads, c.d, &h[1]) ||
+        !paging_of(args + 6, c, x[0]->size(0), g, &paging))
+        Py_RETURN_NONE;
+    for (const at::Tensor *to : c.t)
+        for (const at::Tensor *t : {x[0], x[1], g[0], g[1], g[2]})
+            if (t && to->numel() && t->numel() && meet(*to, *t)) Py_RETURN_NONE;
+    try {
+        if (lib.paged_write(&h[0], &h[1], code_of(x[0]->scalar_type()), c.heads, c.d, &c.k, &c.v, &paging, stream_of(device)) == 0) Py_RETURN_TRUE;
+    } catch (const std::exception &) {
+    }
+    Py_RETURN_NONE;
+}
+
+// paged_read(cache x 4, table, kv_lengths, length, starts, out_dtype) -> (k, v), or None
+PyObject *native_paged_read(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    PagedCache c;
+    const at::Tensor *g[3], *starts;
+    kea_paging paging;
+    int64_t length;
+    if (count != 9 || modes_active() || !cache_of(args, &c)) Py_RETURN_NONE;
+    const auto device = c.t[0]->device();
+    PyObject *const index[3] = {args[4], args[5], Py_None};
+    if (!current(device) || !paging_of(index, c, 0, g, &paging) || !PyLong_CheckExact(args[6]) || !as_int(args[6], &length) || length < 1 || length > (1 << 30) ||
+        !optional(args[7], device, &starts) || (starts && !index_of(starts, paging.batch)) || !THPDtype_Check(args[8]))
+        Py_RETURN_NONE;
+    const auto type = ((THPDtype *)args[8])->scalar_type;
+    if (code_of(type) < 0) Py_RETURN_NONE;
+    try {
+        const auto options = at::TensorOptions().device(device).dtype(type);
+        at::Tensor k = at::empty({paging.batch, length, c.heads, c.d}, options), v = at::empty({paging.batch, length, c.heads, c.d}, options);
+        if (lib.paged_read(&c.k, &c.v, &paging, starts ? (const int32_t *)starts->const_data_ptr() : nullptr, length, c.heads, c.d, k.mutable_data_ptr(),
+                           v.mutable_data_ptr(), code_of(type), stream_of(device)) != 0)
+            Py_RETURN_NONE;
+        const THPObjectPtr ko(THPVariable_Wrap(std::move(k))), vo(THPVariable_Wrap(std::move(v)));
+        return PyTuple_Pack(2, ko.get(), vo.get());
+    } catch (const std::exception &) {
+        Py_RETURN_NONE;
+    }
+}
+
+// paged_attention(cache x 4, q, table, kv_lengths, q_offsets, left, scale) -> the output, or None. left: None or int.
+PyObject *native_paged_attention(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    PagedCache c;
+    const at::Tensor *g[3], *q;
+    kea_heads h;
+    kea_paging paging;
+    int64_t left = 1 << 30;
+    double scale;
+    if (count != 10 || modes_active() || !cache_of(args, &c)) Py_RETURN_NONE;
+    const auto device = c.t[0]->device();
+    if (!current(device) || !optional(args[4], device, &q) || !q || !tokens_of(*q, 0, c.d, &h) || q->size(1) < 1 || q->size(1) % c.heads ||
+        !paging_of(args + 5, c, q->size(0), g, &paging) || (args[8] != Py_None && (!PyLong_CheckExact(args[8]) || !as_int(args[8], &left) || left < 0)))
+        Py_RETURN_NONE;
+    if (args[9] == Py_None) scale = 1.0 / std::sqrt((double)c.d);
+    else if (!as_float(args[9], &scale)) Py_RETURN_NONE;
+    if (left > 1 << 30) left = 1 << 30;
+    try {
+        const int64_t tokens = q->size(0), heads = q->size(1);
+        const int code = code_of(q->scalar_type());
+        at::Tensor y = at::empty({tokens, heads, c.d}, at::TensorOptions().device(device).dtype(q->scalar_type())), space;
+        const kea_heads yh{y.mutable_data_ptr(), 0, heads * c.d, c.d};
+        const int64_t need = lib.paged_workspace(code, paging.batch, tokens, paging.table_width * c.size, heads, c.heads, c.d, left, g[2] != nullptr);
+        if (need < 0) Py_RETURN_NONE;
+        if (need > 0) space = at::empty({need}, at::TensorOptions().device(device).dtype(at::kByte));
+        if (lib.paged_attention(&h, &yh, code, heads, c.heads, c.d, &c.k, &c.v, &paging, left, (float)scale, 1, need > 0 ? space.mutable_data_ptr() : nullptr, need,
+                                stream_of(device)) == 0)
+            return THPVariable_Wrap(std::move(y));
+    } catch (const std::exception &) {
+    }
+    Py_RETURN_NONE;
+}
+
+// bind_decode(int4_gemm, paged_write, paged_read, paged_attention, paged_attention_workspace)
 PyObject *native_bind_decode(PyObject *, PyObject *args) {
-    unsigned long long g;
-    if (!PyArg_ParseTuple(args, "K", &g)) return nullptr;
+    unsigned long long g, w, r, a, s;
+    if (!PyArg_ParseTuple(args, "KKKKK", &g, &w, &r, &a, &s)) return nullptr;
     lib.int4_gemm = (decltype(lib.int4_gemm))g;
+    lib.paged_write = (decltype(lib.paged_write))w;
+    lib.paged_read = (decltype(lib.paged_read))r;
+    lib.paged_attention = (decltype(lib.paged_attention))a;
+    lib.paged_workspace = (decltype(lib.paged_workspace))s;
     Py_RETURN_NONE;
 }
 
@@ -700,6 +846,9 @@ PyMethodDef module_methods[] = {
     {"bind_block", native_bind_block, METH_VARARGS, nullptr},
     {"bind_decode", native_bind_decode, METH_VARARGS, nullptr},
     {"int4_gemm", (PyCFunction)(void (*)())native_int4_gemm, METH_FASTCALL, nullptr},
+    {"paged_write", (PyCFunction)(void (*)())native_paged_write, METH_FASTCALL, nullptr},
+    {"paged_read", (PyCFunction)(void (*)())native_paged_read, METH_FASTCALL, nullptr},
+    {"paged_attention", (PyCFunction)(void (*)())native_paged_attention, METH_FASTCALL, nullptr},
     {"int8_gemm", (PyCFunction)(void (*)())native_int8_gemm, METH_FASTCALL, nullptr},
     {"block_norm", (PyCFunction)(void (*)())native_block_norm, METH_FASTCALL, nullptr},
     {"window_attention", (PyCFunction)(void (*)())native_window, METH_FASTCALL, nullptr},

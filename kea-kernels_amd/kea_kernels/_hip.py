@@ -175,7 +175,7 @@ def native():
                 module.bind_block(*(ctypes.cast(getattr(library, name), ctypes.c_void_p).value for name in (
                     "kea_int8_gemm", "kea_block_norm", "kea_window_attention", "kea_window_attention_workspace")))
                 module.bind_decode(*(ctypes.cast(getattr(library, name), ctypes.c_void_p).value for name in (
-                    "kea_int4_gemm",)))
+                    "kea_int4_gemm", "kea_paged_write", "kea_paged_read", "kea_paged_attention", "kea_paged_attention_workspace")))
                 _native = module
     return _native
 
