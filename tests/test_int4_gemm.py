@@ -137,6 +137,32 @@ def test_epilogue(m, n, k, group, dtype):
 
 @pytest.mark.gpu
 @torch.inference_mode()
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("m,n,k", [(2000, 2050, 900), (3000, 700, 130), (500, 1050, 4097), (260, 4001, 4000), (300, 700, 1111), (1300, 130, 6000), (800, 1550, 506)])
+def test_tiles_of_many_rows(m, n, k, group):
+    """Sizes that take tiles of 32 x 64 to 128 x 128, by one, two or four groups of waves, stages past the end among them."""
+    q, qs, w, ws = make(m, n, k, group, m + n + k, torch.float32 if group > 64 else torch.float16)
+    qg, qsg, wg = on_gpu(q, qs, w, ws, group)
+    bias = torch.linspace(-3, 3, n)
+    got = int4.gemm(qg, qsg, wg, bias.to(DEV), silu=True, out_dtype=torch.float16)
+    for rows in (slice(0, 150), slice(m - 150, m)):
+        check(got[rows], *expected(q[:, rows], qs[:, rows], w, ws, group, bias, True, None, 1.0, torch.float16))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+def test_rows_far_apart():
+    """Rows of q 2^23 bytes and more apart, past 32 bits in all."""
+    q, qs, w, ws = make(300, 40, 200, 64, 17)
+    _, qsg, wg = on_gpu(q, qs, w, ws, 64)
+    store = torch.empty(299 * (1 << 24) + 256, dtype=torch.int8, device=DEV)
+    far = store.as_strided((300, 208), (1 << 24, 1))
+    far.copy_(q[0])
+    check(int4.gemm(far, qsg, wg), *expected(q, qs, w, ws, 64, None, False, None, 1.0, torch.float32))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("m,n,k", [(1, 17, 40), (5, 130, 200), (33, 100, 640), (300, 131, 150)])
 def test_outputs_inside_larger_ones(m, n, k, dtype):
