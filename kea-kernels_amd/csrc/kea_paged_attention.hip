@@ -37,6 +37,7 @@ typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) v2i *ltr8_t;
@@ -140,13 +141,16 @@ __device__ __forceinline__ v16f mma(v8h a, v8h b, v16f c) { return __builtin_amd
 __device__ __forceinline__ int exponent(float v) { return __builtin_amdgcn_frexp_expf(v); }
 __device__ __forceinline__ bool finite(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) != 0x7F800000u; }
 
-// The largest of 32 lanes' numbers (both halves of the wave hold the same ones).
-__device__ __forceinline__ int max32(int v) {
+// The largest number of each 16 lanes, in all of them; of 32 lanes (both halves of the wave hold the same ones).
+__device__ __forceinline__ int row_max(int v) {
     auto dpp = [](int v, auto ctrl) { return __builtin_amdgcn_update_dpp(v, v, decltype(ctrl)::value, 0xF, 0xF, false); };
     v = max(v, dpp(v, std::integral_constant<int, 0xB1>{}));
     v = max(v, dpp(v, std::integral_constant<int, 0x4E>{}));
     v = max(v, dpp(v, std::integral_constant<int, 0x141>{}));
-    v = max(v, dpp(v, std::integral_constant<int, 0x140>{}));
+    return max(v, dpp(v, std::integral_constant<int, 0x140>{}));
+}
+__device__ __forceinline__ int max32(int v) {
+    v = row_max(v);
     return max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
 }
 
@@ -207,10 +211,28 @@ struct Sums {
     float ref, l;
 };
 
+// A block that some of a wave's rows do not see as a whole: what this lane's query does not see becomes -infinity. valid: the block's
+// keys that have a page; hi, lo: the last and first key that the query sees, counted from the block's first.
+__device__ __forceinline__ void mask(v16f &s, const v4f *v, uint32_t valid, int hi, int lo, int h, int *v_exponent) {
+    asm volatile("");  // (a branch: not done for every block)
+    const int hx = hi - 4 * h, lx = lo - 4 * h;
+    const uint32_t bits = valid >> (4 * h);
+    float most = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int at = 8 * (e / 4) + e % 4;
+        const bool seen = at <= hx && at >= lx && (bits >> at & 1);
+        if (!seen) s[e] = -INFINITY;
+        most = fmaxf(most, seen ? fabsf(v[e / 4][e % 4]) : 0.0f);
+    }
+    most = other_half_max(most);
+    *v_exponent = most != 0.0f ? max(exponent(most), kLeast) : kLeast;  // (of what this query sees)
+}
+
 // A block's scores s (16 keys of one query) become weights: p in the sum, w = p v as operands of the second product. v: the keys'
 // value scales, v_exponent: the exponent of the largest of them; by: what the scores are multiplied by.
 template <int PARTS, int DB>
-__device__ __forceinline__ void weigh(v16f s, const v4f *v, float by, int v_exponent, Sums *m, v16f (&o)[DB], v8h (&w)[2 * PARTS]) {
+__device__ __forceinline__ void weigh(const v16f &s, const v4f *v, float by, int v_exponent, Sums *m, v16f (&o)[DB], v4u (&w)[2 * PARTS]) {
     float top = s[0];
 #pragma unroll
     for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
@@ -228,15 +250,16 @@ __device__ __forceinline__ void weigh(v16f s, const v4f *v, float by, int v_expo
     const float ref = m->ref == -INFINITY ? 0.0f : m->ref;
     float sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], by, -ref));
-        float x = p * v[e / 4][e % 4];
+    for (int e = 0; e < 16; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], by, -ref)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], by, -ref));
+        float x0 = p0 * v[e / 4][e % 4], x1 = p1 * v[e / 4][e % 4 + 1];
         // (of two parts both are made from the FP32 product: the compiler may round the exact one to FP16 for the first)
-        if constexpr (PARTS == 2) asm("" : "+v"(x));
-        sum += p;
-        const _Float16 hi = (_Float16)x;
-        w[e / 8 * PARTS][e % 8] = hi;
-        if constexpr (PARTS == 2) w[e / 8 * PARTS + 1][e % 8] = (_Float16)(x - (float)hi);
+        if constexpr (PARTS == 2) asm("" : "+v"(x0), "+v"(x1));
+        sum += p0;
+        sum += p1;
+        const v2h hi = {(_Float16)x0, (_Float16)x1};
+        w[e / 8 * PARTS][e % 8 / 2] = __builtin_bit_cast(uint32_t, hi);
+        if constexpr (PARTS == 2) w[e / 8 * PARTS + 1][e % 8 / 2] = __builtin_bit_cast(uint32_t, v2h{(_Float16)(x0 - (float)hi[0]), (_Float16)(x1 - (float)hi[1])});
     }
     m->l += sum;
 }
@@ -271,7 +294,7 @@ struct Ring {
 };
 
 template <typename T, int DP, int NS>
-__global__ void __launch_bounds__(256, 1) token_kernel(Args a) {
+__global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) token_kernel(Args a) {
     using R = Ring<DP, NS>;
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, UNITS = R::UNITS, COPIES = R::COPIES, DB = DP / 32, QN = DP / 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -426,21 +449,8 @@ __global__ void __launch_bounds__(256, 1) token_kernel(Args a) {
         for (int e = 0; e < 4; ++e) kx[e] = *(const v4f *)(scales + 8 * e + 4 * h), vx[e] = *(const v4f *)(scales + 32 + 8 * e + 4 * h);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] *= kx[e / 4][e % 4];
-        if (!(valid == 0xFFFFFFFFu && k0 + 31 <= p0 && k0 >= p1 - a.left)) {  // not seen as a whole by every row
-            const int hx = hi - k0 - 4 * h, lx = lo - k0 - 4 * h;
-            const uint32_t bits = valid >> (4 * h);
-            float most = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int at = 8 * (e / 4) + e % 4;
-                const bool seen = at <= hx && at >= lx && (bits >> at & 1);
-                if (!seen) s[e] = -INFINITY;
-                most = fmaxf(most, seen ? fabsf(vx[e / 4][e % 4]) : 0.0f);
-            }
-            most = other_half_max(most);
-            v_exponent = most != 0.0f ? max(exponent(most), kLeast) : kLeast;  // (of what this query sees)
-        }
-        v8h w[2 * PARTS];
+        if (!(valid == 0xFFFFFFFFu && k0 + 31 <= p0 && k0 >= p1 - a.left)) mask(s, vx, valid, hi - k0, lo - k0, h, &v_exponent);  // not seen as a whole by every row
+        v4u w[2 * PARTS];
         weigh<PARTS, DB>(s, vx, by, v_exponent, &m, o, w);
 #pragma unroll
         for (int z = 0; z < 2; ++z)
@@ -449,7 +459,7 @@ __global__ void __launch_bounds__(256, 1) token_kernel(Args a) {
                 const v2i codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32((ltr8_t)(slot + R::KEYS + (va ^ 32 * d) + 16 * z * DP));
                 const v8h v = numbers((uint32_t)codes[0], (uint32_t)codes[1]);
 #pragma unroll
-                for (int u = 0; u < PARTS; ++u) o[d] = mma(v, w[z * PARTS + u], o[d]);
+                for (int u = 0; u < PARTS; ++u) o[d] = mma(v, __builtin_bit_cast(v8h, w[z * PARTS + u]), o[d]);
             }
 #pragma unroll
         for (int s1 = 0; s1 + 1 < NS; ++s1) page[s1] = page[s1 + 1];
@@ -500,6 +510,227 @@ __global__ void __launch_bounds__(256, 1) token_kernel(Args a) {
     }
 }
 
+// ---- many rows -------------------------------------------------------------------------------------------------------------------
+
+// A workgroup takes 256 rows (128 of heads up to 64), 32 a wave, which share tiles of 64 keys: each thread loads codes of the next tile
+// into registers while the present one is worked on, and writes them to the other of two buffers as FP16 numbers, so that they are
+// unpacked once for all rows. Wave 0 does the same with the scales.
+//
+// The place of unit c (eight numbers) of a key's row is c ^ place: rows that are read together lie in different banks. Keys: eight
+// (16) rows at one unit. Values: four rows at two neighbouring pairs of units, which stay pairs.
+template <int UNITS>
+__device__ __forceinline__ int place_k(int key) {
+    return UNITS == 8 ? key >> 1 & 7 : key & 15;
+}
+template <int UNITS>
+__device__ __forceinline__ int place_v(int key) {
+    return UNITS == 8 ? (key >> 1 & 1) * 4 : (key & 3) * 4;
+}
+
+template <int DP>
+struct Tiles {
+    static constexpr int WQ = DP == 128 ? 8 : 4, NT = 64 * WQ, ROWS = 32 * WQ, KB = 2, KT = 32 * KB, ROW = 2 * DP, UNITS = DP / 8;
+    static constexpr int KEYS = KT * ROW, BUF = 2 * KEYS + 2 * KT * 4 + 16, LDS = 2 * BUF;  // keys, values, scales of both, exponents of blocks
+    static constexpr int LOADS = KT * (DP / 16) / NT;  // of 16 codes, by each thread, of keys and of values
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(Tiles<DP>::NT, 2) rows_kernel(Args a) {
+    using S = Tiles<DP>;
+    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, KB = S::KB, KT = S::KT, ROW = S::ROW, UNITS = S::UNITS, LOADS = S::LOADS, DB = DP / 32, QN = DP / 16;
+    constexpr int GRANULES = KT / 16, NT = S::NT, ROWS = S::ROWS;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, h = lane >> 5;
+    const int hk = blockIdx.x % a.kv_heads, split = blockIdx.y;
+    Tile t;
+    if (!find_tile<ROWS>(a, blockIdx.x / a.kv_heads, &t)) {
+        if (a.fill && split == 0 && (int)blockIdx.x / a.kv_heads == a.tiles) fill_rest<T>(a, hk, NT);
+        return;
+    }
+    const int count = min(ROWS, t.rows - t.r0), w0 = min(t.r0 + 32 * wave, t.rows - 1), w1 = min(t.r0 + 32 * wave + 31, t.rows - 1);
+    const bool real = 32 * wave + n < count;
+    const int row = min(t.r0 + 32 * wave + n, t.rows - 1), token = row / a.group, head = hk * a.group + row - token * a.group;
+    const int p = t.start + token, hi = p, lo = max(0, p - a.left);
+    const int p0 = t.start + w0 / a.group, p1 = t.start + w1 / a.group;  // of the wave's rows
+    const int first_p = t.start + t.r0 / a.group, last_p = t.start + (t.r0 + count - 1) / a.group;
+    const int wave_first = max(0, p0 - a.left);
+
+    // the tiles of keys that some row sees, and this split's share of them
+    const int first_key = max(0, first_p - a.left), start = first_key / KT, all = last_p < 0 ? 0 : last_p / KT + 1 - start;
+    const int share = (all + a.splits - 1) / a.splits, from = start + min(all, split * share), to = start + min(all, (split + 1) * share);
+    if (to <= from && a.splits > 1) {  // nothing for this split
+        if (tid < count) {
+            const long long slot = ((long long)split * a.at.tokens + t.first + (t.r0 + tid) / a.group) * (a.kv_heads * a.group) + hk * a.group + (t.r0 + tid) % a.group;
+            *(float2 *)(a.stats + 2 * slot) = make_float2(-INFINITY, 0.0f);
+        }
+        return;
+    }
+
+    const int8_t *const kd = a.kp.data_dev + (long long)hk * a.kp.head_stride, *const vd = a.vp.data_dev + (long long)hk * a.vp.head_stride;
+    const float *const ks = a.kp.scale_dev + (long long)hk * a.kp.scale_head_stride, *const vs = a.vp.scale_dev + (long long)hk * a.vp.scale_head_stride;
+    const int32_t *const table = a.at.table + (long long)t.b * a.at.table_stride;
+    const int last_entry = a.at.width - 1, page_mask = (1 << a.at.shift) - 1;
+    // The pages of a tile's granules of 16 keys (uniform: read through the scalar cache).
+    typedef int pages_t __attribute__((ext_vector_type(GRANULES)));
+    auto entries = [&](int tile) {
+        typedef const __attribute__((address_space(4))) int32_t *uniform_t;
+        const uniform_t u = (uniform_t)(uintptr_t)table;
+        pages_t e;
+#pragma unroll
+        for (int i = 0; i < GRANULES; ++i) e[i] = u[min((KT * tile + 16 * i) >> a.at.shift, last_entry)];
+        return e;
+    };
+    auto page_ok = [&](int page) { return (unsigned)page < (unsigned)a.at.pages; };
+    // this thread's codes: unit `unit` of the keys key0 + u STEP, which lie in one granule for a wave
+    constexpr int PER = DP / 16, STEP = NT / PER;
+    const int key0 = tid / PER, unit = tid % PER;
+    const bool some = 16 * unit < a.d;
+    v4u k_codes[LOADS], v_codes[LOADS];
+    float k_scale = 0.0f, v_scale = 0.0f;
+    auto load = [&](int tile, pages_t e) {
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int granule = __builtin_amdgcn_readfirstlane((u * STEP + key0) / 16);
+            int page = e[0];
+#pragma unroll
+            for (int i = 1; i < GRANULES; ++i) page = granule == i ? e[i] : page;
+            if (!page_ok(page)) page = 0;  // (read, and masked)
+            const int r0 = (KT * tile + 16 * granule) & page_mask;
+            const uint32_t in = (uint32_t)(u * STEP + key0) % 16;
+            const int8_t *const k_from = kd + (page * a.kp.page_stride + r0 * a.kp.row_stride), *const v_from = vd + (page * a.vp.page_stride + r0 * a.vp.row_stride);
+            k_codes[u] = v_codes[u] = v4u{0, 0, 0, 0};
+            if (some) {
+                k_codes[u] = *(const v4u *)(k_from + (in * (uint32_t)a.kp.row_stride + 16u * (uint32_t)unit));
+                v_codes[u] = *(const v4u *)(v_from + (in * (uint32_t)a.vp.row_stride + 16u * (uint32_t)unit));
+            }
+        }
+        if (wave == 0) {
+            const int key = lane % KT, granule = key / 16;
+            int page = e[0];
+#pragma unroll
+            for (int i = 1; i < GRANULES; ++i) page = granule == i ? e[i] : page;
+            if (!page_ok(page)) page = 0;
+            const long long r = (KT * tile + key) & page_mask;
+            k_scale = ks[page * a.kp.scale_page_stride + r * a.kp.scale_row_stride];
+            v_scale = vs[page * a.vp.scale_page_stride + r * a.vp.scale_row_stride];
+        }
+    };
+    // the keys of a tile that have a page and that some row of the workgroup may see
+    auto valid_keys = [&](int tile, pages_t e) {
+        uint64_t valid = 0;
+#pragma unroll
+        for (int i = 0; i < GRANULES; ++i) valid |= page_ok(e[i]) ? 0xFFFFULL << (16 * i) : 0;
+        const int ahead = last_p - KT * tile, behind = first_key - KT * tile;  // the last and first key seen, in the tile
+        return valid & (ahead >= 63 ? ~0ULL : (2ULL << ahead) - 1) & (behind > 0 ? ~0ULL << behind : ~0ULL);
+    };
+    const float scale = a.scale * kLog2e;
+    auto put = [&](int buf, uint64_t valid) {
+        char *const to = lds + buf * S::BUF;
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int key = u * STEP + key0;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                *(v8h *)(to + key * ROW + ((2 * unit + half) ^ place_k<UNITS>(key)) * 16) = numbers(k_codes[u][2 * half], k_codes[u][2 * half + 1]);
+                *(v8h *)(to + S::KEYS + key * ROW + ((2 * unit + half) ^ place_v<UNITS>(key)) * 16) = numbers(v_codes[u][2 * half], v_codes[u][2 * half + 1]);
+            }
+        }
+        if (wave == 0) {
+            float *const scales = (float *)(to + 2 * S::KEYS);
+            const int key = lane % KT;
+            const bool there = valid >> key & 1, number = finite(v_scale);
+            scales[key] = !there ? 0.0f : number ? k_scale * scale : __builtin_nanf("");
+            const float y = there && number ? v_scale : 0.0f;
+            scales[KT + key] = y;
+            const int e = y != 0.0f ? max(exponent(y), kLeast) : kLeast, most = row_max(e);  // of 16 keys
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const int block = max(__builtin_amdgcn_readlane(most, 32 * kb), __builtin_amdgcn_readlane(most, 32 * kb + 16));
+                if (lane == 0) ((int *)scales)[2 * KT + kb] = block;
+            }
+        }
+    };
+
+    v8h q[QN * PARTS];
+    float by;
+    load_queries<T, QN>((const T *)a.q.data_dev + (long long)(t.first + token) * a.q.t_stride + (long long)head * a.q.head_stride, a.d, p >= 0,
+                        [&](int i) { return 16 * i + 8 * h; }, q, &by);
+    v16f o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    Sums m{-INFINITY, 0.0f};
+    // operand addresses: unit 2 c + h of key n at ka ^ 32 c, units 4 d .. of the values' rows at va ^ 64 d
+    const int ka = n * ROW + (h ^ place_k<UNITS>(n)) * 16;
+    const int vkey = 4 * h + (lane & 15) / 4, va = vkey * ROW + ((2 * (lane >> 4 & 1) + (lane & 3) / 2) ^ place_v<UNITS>(vkey)) * 16 + (lane & 1) * 8;
+
+    pages_t pages = entries(from);
+    uint64_t valid = 0, next_valid = 0;
+    if (from < to) {
+        load(from, pages);
+        valid = valid_keys(from, pages);
+        put(0, valid);
+        if (from + 1 < to) pages = entries(from + 1);
+    }
+    for (int tile = from; tile < to; ++tile) {
+        __syncthreads();
+        const int buf = (tile - from) & 1;
+        if (tile + 1 < to) {
+            load(tile + 1, pages);
+            next_valid = valid_keys(tile + 1, pages);
+            if (tile + 2 < to) pages = entries(tile + 2);
+        }
+        const char *const kt = lds + buf * S::BUF, *const vt = kt + S::KEYS;
+        const float *const scales = (const float *)(vt + S::KEYS);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            const int k0 = KT * tile + 32 * kb;
+            if (k0 > p1 || k0 + 31 < wave_first) continue;  // seen by none of the wave's rows
+            v16f s = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < QN; ++c) {
+                const v8h k = *(const v8h *)(kt + 32 * kb * ROW + (ka ^ 32 * c));
+#pragma unroll
+                for (int u = 0; u < PARTS; ++u) s = mma(k, q[c * PARTS + u], s);
+            }
+            v4f kx[4], vx[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) kx[e] = *(const v4f *)(scales + 32 * kb + 8 * e + 4 * h), vx[e] = *(const v4f *)(scales + KT + 32 * kb + 8 * e + 4 * h);
+            int v_exponent = __builtin_amdgcn_readfirstlane(((const int *)scales)[2 * KT + kb]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] *= kx[e / 4][e % 4];
+            const uint32_t here = (uint32_t)(valid >> (32 * kb));
+            if (!(here == 0xFFFFFFFFu && k0 + 31 <= p0 && k0 >= p1 - a.left)) mask(s, vx, here, hi - k0, lo - k0, h, &v_exponent);  // not seen as a whole by every row
+            v4u w[2 * PARTS];
+            weigh<PARTS, DB>(s, vx, by, v_exponent, &m, o, w);
+#pragma unroll
+            for (int i = 0; i < 2 * DB; ++i) {
+                const char *const at = vt + (va ^ 64 * (i % DB)) + (32 * kb + 16 * (i / DB)) * ROW;
+                const v4s x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr16_t)at), x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr16_t)(at + 8 * ROW));
+                const v8h v = __builtin_bit_cast(v8h, v8s{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]});
+#pragma unroll
+                for (int u = 0; u < PARTS; ++u) o[i % DB] = mma(v, __builtin_bit_cast(v8h, w[i / DB * PARTS + u]), o[i % DB]);
+            }
+        }
+        if (tile + 1 < to) put(buf ^ 1, next_valid);
+        valid = next_valid;
+    }
+    m.l = both_halves(m.l);
+    if (!real) return;
+    const float inv = m.l != 0.0f ? 1.0f / m.l : 0.0f;
+    const long long slot = ((long long)split * a.at.tokens + t.first + token) * (a.kv_heads * a.group) + head;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int c = 32 * d + 2 * e + 4 * h;
+            if (c >= a.d) continue;
+            const v4f v = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]} * inv;
+            if (a.splits > 1) *(v4f *)(a.part + slot * a.d + c) = v;
+            else store4((T *)a.out.data_dev + (long long)(t.first + token) * a.out.t_stride + (long long)head * a.out.head_stride + c, v);
+        }
+    if (a.splits > 1 && h == 0) *(float2 *)(a.stats + 2 * slot) = make_float2(m.ref, m.l);
+}
+
 // Joins the splits: out = sum_s f_s mean_s, f_s = l_s 2^(ref_s - ref) over their sum; four elements a thread, eight splits at a time.
 template <typename T>
 __global__ void __launch_bounds__(64) join_kernel(Args a) {
@@ -544,24 +775,42 @@ __global__ void __launch_bounds__(64) join_kernel(Args a) {
 // ---- host ----------------------------------------------------------------------------------------------------------------------
 
 struct Plan {
+    bool few;  // tiles of 32 rows
     int64_t tiles, tiles_each, splits, part_bytes, stats_bytes;
 };
 
 int plan_of(int64_t batch, int64_t tokens, int64_t positions, int64_t heads, int64_t kv_heads, int64_t d, int64_t left, bool offsets, Plan *out) {
-    const int64_t group = heads / kv_heads;
+    const int64_t group = heads / kv_heads, each = batch > 0 ? tokens / batch : 0;
     Plan p{};
-    const int64_t each = batch > 0 ? tokens / batch : 0;
-    p.tiles_each = (each * group + 31) / 32;
-    p.tiles = offsets ? tokens * group / 32 + batch : p.tiles_each * batch;
+    // The keys that a token may meet: the positions that there is room for (lengths are not known here), less what causality hides.
+    const int64_t room = positions - each / 2, keys = left < room ? left + 1 : room;
+    // Tiles of 32 rows walk their keys without a wait between waves, tiles of 256 unpack the codes for eight times as many rows: they
+    // are ahead where there are many rows and long walks. F16, heads of 128, 16 on 4, us (32 rows, 256 rows): 2048 tokens of 16000
+    // 469 and 333, 1000 of 16000 240 and 179, 8 x 512 of 4000 187 and 143, 1000 of 4000 74 and 66, 2048 of 4000 105 and 104, 4000 of
+    // 4000 133 and 125, 2048 of 2048 45 and 67, 1000 of 1000 21 and 36; 512 of 4000 (FP32) 59 and 61. Heads of 129 to 256 are faster in 32
+    // rows throughout (1000 of 4000 142 and 160: the outputs of a row alone take half of a wave's registers).
+    p.few = d > 128 || tokens * heads < 16000 || keys < 3000;
+    const int64_t per = p.few ? 32 : d <= 64 ? Tiles<64>::ROWS : Tiles<128>::ROWS;
+    p.tiles_each = (each * group + per - 1) / per;
+    p.tiles = offsets ? tokens * group / per + batch : p.tiles_each * batch;
     if (tokens * group > INT32_MAX / 4 || p.tiles > INT32_MAX / 4) return -1;
     const int64_t wgs = p.tiles * kv_heads;
-    const int64_t span = left < positions ? left + 32 / group + 64 : positions, keys = span < positions ? span : positions;
     p.splits = 1;
-    if (wgs > 0 && wgs < 512) {
-        int64_t s = 1024 / wgs;
-        const int64_t most = (keys + 255) / 256;
+    if (wgs > 0 && p.few) {
+        // Two workgroups on every CU where each part has 700 keys and more, one otherwise; 128 keys at least. BF16, one token of 16 streams
+        // of 16000 keys (64 workgroups): 189, 104, 60, 48 and 53 us in 1, 2, 4, 8 and 16 parts; 64 tokens of 4000 (32) 51, 32, 22, 18 and 22;
+        // 8 x 64 of 1000 (256) 19 and 26 in 1 and 2.
+        const int64_t span = keys + per / group;
+        int64_t s = wgs < 512 ? 512 / wgs : 1;
+        if (span / s < 700) s = wgs < 256 ? 256 / wgs : 1;
+        const int64_t most = (span + 127) / 128;
         s = s < most ? s : most;
         p.splits = s < 1 ? 1 : s < 64 ? s : 64;
+    } else if (wgs > 0) {
+        // One workgroup on every CU, or two rounds of them, whose parts even out what causality leaves to the tiles: 4000 of 4000 (256
+        // workgroups) 161 us in one, 125 in two, 144 in four parts; 2048 of 16000 (128) 333 in two, 422 in three.
+        const int64_t s = wgs <= 128 ? 256 / wgs : wgs < 384 ? 2 : 1;
+        p.splits = s < 16 ? s : 16;
     }
     if (p.splits > 1) {
         p.part_bytes = p.splits * tokens * heads * d * 4;
@@ -576,28 +825,39 @@ int launched() {
     return e == hipSuccess ? KEA_OK : kea::fail((int)e, std::string("kea_paged_attention: ") + hipGetErrorString(e));
 }
 
-template <typename T, int DP, int NS>
-int run_shape(const Args &a, hipStream_t stream) {
-    using R = Ring<DP, NS>;
-    static_assert(R::LDS <= 160 * 1024, "LDS");
+// One of the two kernels, then the join of its parts.
+int launch(void (*kernel)(Args), void (*join)(Args), int threads, int lds, const Args &a, hipStream_t stream) {
     const int64_t tiles = ((int64_t)a.tiles + a.fill) * a.kv_heads;
-    const int64_t join = ((int64_t)a.at.tokens * a.kv_heads * a.group * (a.d / 4) + 63) / 64;
-    if (!kea::fits_dispatch(tiles, 256) || !kea::fits_dispatch(join, 64)) return kea::fail(KEA_EINVAL, "kea_paged_attention: too large for one launch");
-    const auto kernel = token_kernel<T, DP, NS>;
-    if (R::LDS > 65536) {
-        const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, R::LDS);
+    const int64_t joins = ((int64_t)a.at.tokens * a.kv_heads * a.group * (a.d / 4) + 63) / 64;
+    if (!kea::fits_dispatch(tiles, threads) || !kea::fits_dispatch(joins, 64)) return kea::fail(KEA_EINVAL, "kea_paged_attention: too large for one launch");
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return kea::fail((int)e, std::string("kea_paged_attention: ") + hipGetErrorString(e));
     }
-    kernel<<<dim3((unsigned)tiles, (unsigned)a.splits), 256, R::LDS, stream>>>(a);
+    kernel<<<dim3((unsigned)tiles, (unsigned)a.splits), threads, lds, stream>>>(a);
     const int rc = launched();
     if (rc || a.splits == 1) return rc;
-    join_kernel<T><<<dim3((unsigned)join), 64, 0, stream>>>(a);
+    join<<<dim3((unsigned)joins), 64, 0, stream>>>(a);
     return launched();
 }
 
+template <typename T, int DP, int NS>
+int run_few(const Args &a, hipStream_t stream) {
+    static_assert(Ring<DP, NS>::LDS <= 160 * 1024, "LDS");
+    return launch(token_kernel<T, DP, NS>, join_kernel<T>, 256, Ring<DP, NS>::LDS, a, stream);
+}
+
+template <typename T, int DP>
+int run_rows(const Args &a, hipStream_t stream) {
+    using S = Tiles<DP>;
+    static_assert(S::LDS <= 160 * 1024 && S::LOADS * S::NT == S::KT * (DP / 16) && S::LOADS > 0, "LDS and loads");
+    return launch(rows_kernel<T, DP>, join_kernel<T>, S::NT, S::LDS, a, stream);
+}
+
 template <typename T>
-int run(const Args &a, hipStream_t stream) {
-    return a.d <= 64 ? run_shape<T, 64, 4>(a, stream) : a.d <= 128 ? run_shape<T, 128, 3>(a, stream) : run_shape<T, 256, 2>(a, stream);
+int run(const Args &a, bool few, hipStream_t stream) {
+    if (!few) return a.d <= 64 ? run_rows<T, 64>(a, stream) : run_rows<T, 128>(a, stream);
+    return a.d <= 64 ? run_few<T, 64, 4>(a, stream) : a.d <= 128 ? run_few<T, 128, 2>(a, stream) : run_few<T, 256, 2>(a, stream);
 }
 
 bool rows_ok(const kea_heads *t, int64_t unit) {
@@ -651,7 +911,7 @@ int kea_paged_attention(const kea_heads *q, const kea_heads *out, int dtype, int
     a.splits = (int)p.splits, a.tiles_each = (int)p.tiles_each, a.tiles = (int)p.tiles, a.scale = scale;
     a.fill = fill && paging->q_offsets_dev ? 1 : 0;
     const hipStream_t s = (hipStream_t)stream;
-    return dtype == KEA_F32 ? run<float>(a, s) : dtype == KEA_F16 ? run<_Float16>(a, s) : run<__bf16>(a, s);
+    return dtype == KEA_F32 ? run<float>(a, p.few, s) : dtype == KEA_F16 ? run<_Float16>(a, p.few, s) : run<__bf16>(a, p.few, s);
 }
 
 }  // extern "C"

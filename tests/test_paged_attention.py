@@ -135,6 +135,50 @@ def test_as_many_tokens_for_every_sequence(batch, new, length, heads, hk, d, dty
 @pytest.mark.gpu
 @torch.inference_mode()
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("news,lengths,heads,hk,d", [([700, 3, 333], [1500, 900, 333], 16, 4, 128), ([1200], [3500], 16, 2, 64), ([1100, 0, 1, 64], [1100, 40, 3300, 2000], 16, 16, 80),
+                                                      ([257, 256, 255, 600], [500, 256, 3100, 700], 12, 3, 112)])
+def test_many_rows(news, lengths, heads, hk, d, dtype):
+    """Enough rows, and room for enough keys, for tiles of 128 and 256 rows."""
+    g = torch.Generator().manual_seed(d)
+    q, cache, table, ln, offsets = make(news, lengths, heads, hk, d, 16, dtype, g)
+    wide = torch.full((len(news), 300), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    wide[0, 5] = -1  # (an entry without a page in front of every row)
+    for left in (None, 3000) if d == 128 else (None,):
+        check(run(q, cache, wide, ln, offsets, left=left), *expected(q, cache, wide, ln, offsets, left=left))
+    if len(news) == 1:
+        check(run(q, cache, wide, ln, None), *expected(q, cache, wide, ln, offsets))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows_beside_scales_that_are_no_numbers(dtype):
+    """Tiles of 256 rows: the last keys hold NaN or the largest scales; rows in front of them keep their bits, those behind are NaN."""
+    g = torch.Generator().manual_seed(12)
+    q, cache, table, ln, offsets = make([1100], [3400], 16, 4, 128, 16, dtype, g)
+    clean = run(q, cache, table, ln, offsets)
+    out = torch.full_like(clean, 7.0)
+    tail = torch.cat([q, q[:20]])
+    got = paged.attention(tail.to(DEV), on_gpu(cache), table.to(DEV), ln.to(DEV), offsets.to(DEV))
+    assert torch.equal(got[:1100], clean) and not got[1100:].any()
+    paged.attention(q.to(DEV), on_gpu(cache), table.to(DEV), ln.to(DEV), offsets.to(DEV), out=out)
+    assert torch.equal(out, clean)
+    for bad in (float("nan"), float("inf"), 3e38):
+        k_scale, v_scale = cache.k_scale.clone(), cache.v_scale.clone()
+        for p in (3390, 3399):
+            k_scale[int(table[0, p // 16]), :, p % 16], v_scale[int(table[0, p // 16]), :, p % 16] = bad, bad
+        for p in range(3400, -(-3400 // 16) * 16):
+            k_scale[int(table[0, p // 16]), :, p % 16], v_scale[int(table[0, p // 16]), :, p % 16] = bad, bad
+        got = run(q, paged.Cache(cache.k, cache.v, k_scale, v_scale), table, ln, offsets)
+        assert torch.equal(got[:1090], clean[:1090]), bad
+        if bad != 3e38:
+            assert torch.isnan(got[1090:]).all()
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
 def test_tables_lengths_and_offsets_that_leave_rows_empty(dtype):
     """Entries without a page (all of a sequence's, the last, some), lengths of zero, below the new tokens and past the table, rows in
     front of and behind all sequences: zeros in a new tensor, left as they are in out."""
