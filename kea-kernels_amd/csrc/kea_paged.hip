@@ -2,8 +2,8 @@
 //
 //   s = max(max|x| / 127, 1e-30), held to where 127 s is finite, c = rint(x / s) for each row x of d elements;   x' = c s
 //
-// Either moves bytes and little else: a wave takes one token or position, whose sequence and page are then uniform, and runs
-// through its 2 kv_heads rows, L = 8, 16 or 32 lanes of eight elements to a row.
+// Either moves bytes and little else. L = 4, 8 or 16 lanes of sixteen elements take a row, one head of a token or position; keys and
+// values are two halves of the grid.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -16,11 +16,11 @@
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint16_t v8u __attribute__((ext_vector_type(8)));
 
 constexpr float kMostScale = 0x1.0204060000000p+121f;  // the largest s of which 127 s is a finite number
-constexpr int kWaves = 4;  // tokens or positions of a workgroup
+constexpr int kThreads = 256;
 
 template <typename T>
 __device__ __forceinline__ void load8(const T *p, float *v) {
@@ -56,9 +56,8 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
     auto dpp = [](uint32_t v, auto ctrl) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xF, 0xF, false); };
     v = max(v, dpp(v, std::integral_constant<int, 0xB1>{}));   // l ^ 1
     v = max(v, dpp(v, std::integral_constant<int, 0x4E>{}));   // l ^ 2
-    v = max(v, dpp(v, std::integral_constant<int, 0x141>{}));  // the other four of eight
+    if constexpr (L >= 8) v = max(v, dpp(v, std::integral_constant<int, 0x141>{}));   // the other four of eight
     if constexpr (L >= 16) v = max(v, dpp(v, std::integral_constant<int, 0x140>{}));  // the other eight of 16
-    if constexpr (L >= 32) v = max(v, (uint32_t)__shfl_xor((int)v, 16));
     return v;
 }
 
@@ -69,55 +68,47 @@ struct WriteArgs {
     int kv_heads, d;
 };
 
-// U passes of 64 / L rows each are loaded at once.
-template <typename T, int L, int U>
-__global__ void __launch_bounds__(64 * kWaves) write_kernel(WriteArgs a) {
-    const int lane = threadIdx.x & 63, t = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
-    if (t >= a.at.tokens) return;
-    const int b = a.at.sequence(t);
-    if (b < 0) return;
-    const int2 rows = a.at.rows(b);
-    const int p = a.at.length(b) - rows.y + t;  // len - n + i
-    if (p < 0) return;
-    const int page = __builtin_amdgcn_readfirstlane(a.at.page(b, p));
-    if (page < 0) return;
-    const int row = p & ((1 << a.at.shift) - 1), at = lane % L * 8;
-    for (int r0 = 0; r0 < 2 * a.kv_heads; r0 += U * (64 / L)) {
-        float x[U][8];
+template <typename T, int L>
+__global__ void __launch_bounds__(kThreads) write_kernel(WriteArgs a) {
+    const long long r = (long long)blockIdx.x * (kThreads / L) + threadIdx.x / L;
+    if (r >= (long long)a.at.tokens * a.kv_heads) return;
+    const int t = (int)(r / a.kv_heads), h = (int)(r - (long long)t * a.kv_heads), at = threadIdx.x % L * 16;
+    const kea_heads &from = blockIdx.y ? a.v : a.k;
+    const kea_pages &to = blockIdx.y ? a.vp : a.kp;
+    float x[16];
+    uint32_t most = 0;  // (as whole numbers the sizes keep their order, with infinities and NaN on top)
+    const T *const src = (const T *)from.data_dev + (long long)t * from.t_stride + (long long)h * from.head_stride + at;
+    if (at < a.d) {
+        load8(src, x);
+        load8(src + 8, x + 8);
+    } else {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * (64 / L) + lane / L, h = r >> 1;
-            const kea_heads &from = r & 1 ? a.v : a.k;
-            if (h < a.kv_heads && at < a.d) load8((const T *)from.data_dev + (long long)t * from.t_stride + (long long)h * from.head_stride + at, x[u]);
-            else
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[u][e] = 0.0f;
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * (64 / L) + lane / L, h = r >> 1;
-            const kea_pages &to = r & 1 ? a.vp : a.kp;
-            uint32_t most = 0;  // (as whole numbers the sizes keep their order, with infinities and NaN on top)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) most = max(most, __builtin_bit_cast(uint32_t, x[u][e]) & 0x7FFFFFFFu);
-            most = lanes_max<L>(most);
-            const bool number = most < 0x7F800000u;
-            const float s = number ? fminf(fmaxf(__builtin_bit_cast(float, most) / 127.0f, 1e-30f), kMostScale) : __builtin_nanf(""), inv = 1.0f / s;
-            uint32_t code[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float z = x[u][e];
-                code[e] = number ? kea::quantize_code(z, s, inv) : 0u;
-            }
-            if (h < a.kv_heads && at < a.d) {
-                v2u w;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) w[i] = code[4 * i] | code[4 * i + 1] << 8 | code[4 * i + 2] << 16 | code[4 * i + 3] << 24;
-                *(v2u *)(to.data_dev + page * to.page_stride + h * to.head_stride + row * to.row_stride + at) = w;
-                if (at == 0) to.scale_dev[page * to.scale_page_stride + h * to.scale_head_stride + row * to.scale_row_stride] = s;
-            }
-        }
+        for (int e = 0; e < 16; ++e) x[e] = 0.0f;
     }
+    // where the token stands, while its elements are on their way
+    const int b = a.at.sequence(t);
+    int p = -1, page = -1;
+    if (b >= 0) {
+        p = a.at.length(b) - a.at.rows(b).y + t;  // len - n + i
+        if (p >= 0) page = a.at.page(b, p);
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) most = max(most, __builtin_bit_cast(uint32_t, x[e]) & 0x7FFFFFFFu);
+    most = lanes_max<L>(most);
+    const bool number = most < 0x7F800000u;
+    const float s = number ? fminf(fmaxf(__builtin_bit_cast(float, most) / 127.0f, 1e-30f), kMostScale) : __builtin_nanf(""), inv = 1.0f / s;
+    if (page < 0 || at >= a.d) return;
+    v4u w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t code[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) code[e] = number ? kea::quantize_code(x[4 * i + e], s, inv) : 0u;
+        w[i] = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
+    }
+    const int row = p & ((1 << a.at.shift) - 1);
+    *(v4u *)(to.data_dev + page * to.page_stride + h * to.head_stride + row * to.row_stride + at) = w;
+    if (at == 0) to.scale_dev[page * to.scale_page_stride + h * to.scale_head_stride + row * to.scale_row_stride] = s;
 }
 
 struct ReadArgs {
@@ -128,37 +119,28 @@ struct ReadArgs {
     int kv_heads, d, length;
 };
 
-template <typename T, int L, int U>
-__global__ void __launch_bounds__(64 * kWaves) read_kernel(ReadArgs a) {
-    const int lane = threadIdx.x & 63, i = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6)), b = blockIdx.y;
-    if (i >= a.length) return;
+template <typename T, int L>
+__global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
+    const int r = blockIdx.x * (kThreads / L) + threadIdx.x / L, b = blockIdx.y, at = threadIdx.x % L * 16;
+    if (r >= a.length * a.kv_heads || at >= a.d) return;
+    const int i = r / a.kv_heads, h = r - i * a.kv_heads;
+    const kea_pages &from = blockIdx.z ? a.vp : a.kp;
     const long long p = (a.starts ? (long long)a.starts[b] : 0) + i;
-    const int page = __builtin_amdgcn_readfirstlane(p >= 0 && p < a.at.length(b) ? a.at.page(b, (int)p) : -1);
-    const int row = (int)p & ((1 << a.at.shift) - 1), at = lane % L * 8;
-    const long long out = ((long long)b * a.length + i) * a.kv_heads * a.d;
-    for (int r0 = 0; r0 < 2 * a.kv_heads; r0 += U * (64 / L)) {
-        v2u c[U];
-        float s[U];
+    const int page = p >= 0 && p < a.at.length(b) ? a.at.page(b, (int)p) : -1;
+    v4u c = {0, 0, 0, 0};
+    float s = 0.0f;
+    if (page >= 0) {
+        const int row = (int)p & ((1 << a.at.shift) - 1);
+        c = *(const v4u *)(from.data_dev + page * from.page_stride + h * from.head_stride + row * from.row_stride + at);
+        s = from.scale_dev[page * from.scale_page_stride + h * from.scale_head_stride + row * from.scale_row_stride];
+    }
+    T *const to = (T *)(blockIdx.z ? a.v : a.k) + ((long long)b * a.length * a.kv_heads + r) * a.d + at;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * (64 / L) + lane / L, h = r >> 1;
-            const kea_pages &from = r & 1 ? a.vp : a.kp;
-            c[u] = v2u{0, 0};
-            s[u] = 0.0f;
-            if (page >= 0 && h < a.kv_heads && at < a.d) {
-                c[u] = *(const v2u *)(from.data_dev + page * from.page_stride + h * from.head_stride + row * from.row_stride + at);
-                s[u] = from.scale_dev[page * from.scale_page_stride + h * from.scale_head_stride + row * from.scale_row_stride];
-            }
-        }
+    for (int half = 0; half < 2; ++half) {
+        float x[8];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * (64 / L) + lane / L, h = r >> 1;
-            if (h >= a.kv_heads || at >= a.d) continue;
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (float)(int8_t)(c[u][e / 4] >> (8 * (e % 4))) * s[u];
-            store8((T *)(r & 1 ? a.v : a.k) + out + (long long)h * a.d + at, x);
-        }
+        for (int e = 0; e < 8; ++e) x[e] = (float)(int8_t)(c[2 * half + e / 4] >> (8 * (e % 4))) * s;
+        store8(to + 8 * half, x);
     }
 }
 
@@ -177,21 +159,26 @@ bool rows_ok(const kea_heads *t, int64_t unit) {
 
 template <typename T>
 int run_write(const WriteArgs &a, hipStream_t stream) {
-    const dim3 grid((unsigned)((a.at.tokens + kWaves - 1) / kWaves));
-    if (!kea::fits_dispatch(grid.x, 64 * kWaves)) return kea::fail(KEA_EINVAL, "kea_paged_write: too large for one launch");
-    if (a.d <= 64) write_kernel<T, 8, 2><<<grid, 64 * kWaves, 0, stream>>>(a);
-    else if (a.d <= 128) write_kernel<T, 16, 2><<<grid, 64 * kWaves, 0, stream>>>(a);
-    else write_kernel<T, 32, 2><<<grid, 64 * kWaves, 0, stream>>>(a);
+    const int lanes = a.d <= 64 ? 4 : a.d <= 128 ? 8 : 16;
+    const int64_t rows = (int64_t)a.at.tokens * a.kv_heads, blocks = (rows + kThreads / lanes - 1) / (kThreads / lanes);
+    if (!kea::fits_dispatch(blocks, kThreads)) return kea::fail(KEA_EINVAL, "kea_paged_write: too large for one launch");
+    const dim3 grid((unsigned)blocks, 2);
+    if (lanes == 4) write_kernel<T, 4><<<grid, kThreads, 0, stream>>>(a);
+    else if (lanes == 8) write_kernel<T, 8><<<grid, kThreads, 0, stream>>>(a);
+    else write_kernel<T, 16><<<grid, kThreads, 0, stream>>>(a);
     return launched("kea_paged_write");
 }
 
 template <typename T>
 int run_read(const ReadArgs &a, hipStream_t stream) {
-    const dim3 grid((unsigned)((a.length + kWaves - 1) / kWaves), (unsigned)a.at.batch);
-    if (!kea::fits_dispatch(grid.x, 64 * kWaves) || a.at.batch > 65535) return kea::fail(KEA_EINVAL, "kea_paged_read: too large for one launch");
-    if (a.d <= 64) read_kernel<T, 8, 2><<<grid, 64 * kWaves, 0, stream>>>(a);
-    else if (a.d <= 128) read_kernel<T, 16, 2><<<grid, 64 * kWaves, 0, stream>>>(a);
-    else read_kernel<T, 32, 2><<<grid, 64 * kWaves, 0, stream>>>(a);
+    const int lanes = a.d <= 64 ? 4 : a.d <= 128 ? 8 : 16;
+    const int64_t rows = (int64_t)a.length * a.kv_heads, blocks = (rows + kThreads / lanes - 1) / (kThreads / lanes);
+    if (rows > INT32_MAX - kThreads || !kea::fits_dispatch(blocks, kThreads) || a.at.batch > 65535)
+        return kea::fail(KEA_EINVAL, "kea_paged_read: too large for one launch");
+    const dim3 grid((unsigned)blocks, (unsigned)a.at.batch, 2);
+    if (lanes == 4) read_kernel<T, 4><<<grid, kThreads, 0, stream>>>(a);
+    else if (lanes == 8) read_kernel<T, 8><<<grid, kThreads, 0, stream>>>(a);
+    else read_kernel<T, 16><<<grid, kThreads, 0, stream>>>(a);
     return launched("kea_paged_read");
 }
 

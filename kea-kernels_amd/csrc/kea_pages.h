@@ -25,15 +25,16 @@ struct Paging {
         const int from = min(max(offsets[b], 0), tokens);
         return make_int2(from, min(max(offsets[b + 1], from), tokens));
     }
-    // The sequence that has row t (uniform in the wave), -1 for none: as many offsets behind the first as are not above t.
+    // The sequence that has row t, -1 for none: as many offsets behind the first as are not above t, found by halving.
     __device__ __forceinline__ int sequence(int t) const {
         if (!offsets) return t / each;
-        int b = 0;
-        for (int j = 0; j < batch; j += 64) {
-            const int lane = __lane_id();
-            b += __builtin_popcountll(__ballot(j + lane < batch && offsets[min(j + lane, batch - 1) + 1] <= t));
+        int b = 0, n = batch;
+        while (n > 0) {
+            const int half = n / 2;
+            const bool past = offsets[b + half + 1] <= t;
+            b = past ? b + half + 1 : b;
+            n = past ? n - half - 1 : half;
         }
-        b = __builtin_amdgcn_readfirstlane(b);
         return b < batch && t >= offsets[b] && t < offsets[b + 1] ? b : -1;
     }
     // The page of position p (0 <= p < width << shift) of sequence b, -1 for none.
