@@ -39,9 +39,8 @@ SOURCES = ["kea_gemm_ring_w1.hip", "kea_gemm_ring_w2.hip", "kea_gemm_wsplit_p1.h
 ARCH = "gfx950"
 # Per-source flags. The probe's loop keeps eight MFMA accumulators live across iterations; in the accumulator
 # (AGPR) form the register allocator shuffles them with accvgpr moves every iteration, which would be measured as
-# matrix-core time, so it selects the VGPR form of the MFMAs; the int4 product's sums are read by vector instructions as soon as
-# they are made.
-SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("kea_probe.hip", "kea_int4.hip")}
+# matrix-core time, so it selects the VGPR form of the MFMAs.
+SOURCE_FLAGS = {"kea_probe.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 # The wave-split kernels take their load operands as ten leading scalar arguments (4 pointers, 6 ints: 14 SGPRs) that
 # the dispatch preloads into SGPRs, so the first loads issue without a kernel-argument round trip.
 for _p in (1, 2, 3):

@@ -397,7 +397,6 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) token_kernel(Args a) {
     float by;
     load_queries<T, QN>((const T *)a.q.data_dev + (long long)(t.first + token) * a.q.t_stride + (long long)head * a.q.head_stride, a.d, p >= 0,
                         [&](int i) { return 16 * (2 * (i / 2) + h) + 8 * (i % 2); }, q, &by);
-    const float scale = a.scale * kLog2e;
 
     v16f o[DB];
 #pragma unroll
@@ -427,7 +426,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) token_kernel(Args a) {
         const uint32_t valid = paged & (ahead >= 31 ? ~0u : (2u << ahead) - 1u) & (behind > 0 ? ~0u << behind : ~0u);
         const float k_scale = scales[n], v_scale = scales[32 + n];
         const bool there = valid >> n & 1, number = finite(v_scale);
-        const float x = !there ? 0.0f : number ? k_scale * scale : __builtin_nanf(""), y = there && number ? v_scale : 0.0f;
+        const float x = !there ? 0.0f : number ? k_scale * a.scale * kLog2e : __builtin_nanf(""), y = there && number ? v_scale : 0.0f;
         int v_exponent = max32(y != 0.0f ? max(exponent(y), kLeast) : kLeast);
         asm volatile("" ::: "memory");
         scales[lane] = h ? y : x;
@@ -623,7 +622,6 @@ __global__ void __launch_bounds__(Tiles<DP>::NT, 2) rows_kernel(Args a) {
         const int ahead = last_p - KT * tile, behind = first_key - KT * tile;  // the last and first key seen, in the tile
         return valid & (ahead >= 63 ? ~0ULL : (2ULL << ahead) - 1) & (behind > 0 ? ~0ULL << behind : ~0ULL);
     };
-    const float scale = a.scale * kLog2e;
     auto put = [&](int buf, uint64_t valid) {
         char *const to = lds + buf * S::BUF;
 #pragma unroll
@@ -639,7 +637,7 @@ __global__ void __launch_bounds__(Tiles<DP>::NT, 2) rows_kernel(Args a) {
             float *const scales = (float *)(to + 2 * S::KEYS);
             const int key = lane % KT;
             const bool there = valid >> key & 1, number = finite(v_scale);
-            scales[key] = !there ? 0.0f : number ? k_scale * scale : __builtin_nanf("");
+            scales[key] = !there ? 0.0f : number ? k_scale * a.scale * kLog2e : __builtin_nanf("");
             const float y = there && number ? v_scale : 0.0f;
             scales[KT + key] = y;
             const int e = y != 0.0f ? max(exponent(y), kLeast) : kLeast, most = row_max(e);  // of 16 keys
@@ -663,9 +661,10 @@ __global__ void __launch_bounds__(Tiles<DP>::NT, 2) rows_kernel(Args a) {
     const int ka = n * ROW + (h ^ place_k<UNITS>(n)) * 16;
     const int vkey = 4 * h + (lane & 15) / 4, va = vkey * ROW + ((2 * (lane >> 4 & 1) + (lane & 3) / 2) ^ place_v<UNITS>(vkey)) * 16 + (lane & 1) * 8;
 
-    pages_t pages = entries(from);
+    pages_t pages{};
     uint64_t valid = 0, next_valid = 0;
     if (from < to) {
+        pages = entries(from);
         load(from, pages);
         valid = valid_keys(from, pages);
         put(0, valid);

@@ -66,7 +66,8 @@ inline int check_paging(const char *what, const kea_pages *k, const kea_pages *v
         return fail(KEA_EINVAL, name + ": a pointer is missing");
     int shift = 0;
     while ((1 << shift) < g->page_size) ++shift;
-    *out = Paging{g->table_dev, g->kv_lengths_dev, g->q_offsets_dev, g->table_stride, (int)g->batch, (int)g->table_width, (int)g->pages, shift,
+    // (no pages: no positions)
+    *out = Paging{g->table_dev, g->kv_lengths_dev, g->q_offsets_dev, g->table_stride, (int)g->batch, g->pages > 0 ? (int)g->table_width : 0, (int)g->pages, shift,
                   (int)g->tokens, g->batch > 0 ? (int)(g->tokens / g->batch) : 0};
     return KEA_OK;
 }

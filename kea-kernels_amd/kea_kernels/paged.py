@@ -21,8 +21,16 @@ from kea_kernels.window import _bound, _span
 _MOST = 1 << 30  # positions of a sequence, tokens of a call
 
 
-def _distinct(name: str, t: Tensor) -> None:
-    steps = sorted((t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] > 1)
+def _distinct(name: str, t: Tensor, other: Tensor | None = None) -> None:
+    """ValueError where two elements of t, or of t and `other` of its shape, share memory."""
+    steps = [(t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] > 1]
+    if other is not None:  # one tensor of both, where they lie in each other's span
+        if not t.numel() or _span(t)[0] >= _span(other)[1] or _span(other)[0] >= _span(t)[1]:
+            return
+        if any(n > 1 and a != b for a, b, n in zip(t.stride(), other.stride(), t.shape)):
+            raise ValueError(f"{name} lie in the same memory in different orders")
+        steps.append((abs(t.data_ptr() - other.data_ptr()) // t.element_size(), 2))
+    steps.sort()
     if any(s < 1 for s, _ in steps) or any(s < reach for (s, _), reach in zip(steps[1:], (1 + sum((n - 1) * s for s, n in steps[:i + 1])
                                                                                           for i in range(len(steps))))):
         raise ValueError(f"{name} has elements that share memory: shape {tuple(t.shape)}, strides {t.stride()}")
@@ -52,8 +60,12 @@ class Cache:
             _distinct(name, t)
         if any(t.device != k.device for t in (v, k_scale, v_scale)):
             raise ValueError("the cache's tensors are on different devices")
-        if k.numel() and (k.data_ptr() == v.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr()):
-            raise ValueError("keys and values share memory")
+        _distinct("k and v", k, v)
+        _distinct("k_scale and v_scale", k_scale, v_scale)
+        for t in (k, v):
+            for s in (k_scale, v_scale):
+                if t.numel() and _span(t)[0] < _span(s)[1] and _span(s)[0] < _span(t)[1]:
+                    raise ValueError("codes and scales lie in the same memory")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
 
     @classmethod

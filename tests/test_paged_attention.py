@@ -241,7 +241,7 @@ def test_values_of_any_size(dtype):
     for new, length in ((1, 700), (20, 333)):
         q, cache, table, lengths, offsets = make([new], [length], 4, 2, 64, 16, dtype, g, spread=2.0)
         check(run(q, cache, table, lengths, offsets), *expected(q, cache, table, lengths, offsets))
-        for scale in (0.0, -0.3, 1.0, 1e-20, -0.0):
+        for scale in (0.0, -0.3, 1.0, 1e-20, -0.0, 1e-45):
             check(run(q, cache, table, lengths, offsets, scale=scale), *expected(q, cache, table, lengths, offsets, scale=scale))
         for size in (1e-30, 1e-12, 1e4) if dtype == F16 else (1e-30, 1e-12, 1e4, 1e25):  # all values alike, and zeros among them
             values = torch.full_like(cache.v_scale, size)

@@ -157,6 +157,11 @@ def test_bad_entries_lengths_and_offsets_are_left_out():
     assert not paged.read(cache, table[:, :0].to(DEV), lengths.to(DEV), 4)[0].any()
     assert paged.read(cache, table[:0].to(DEV), lengths[:0].to(DEV), 4)[0].shape == (0, 4, 2, 32)
     assert paged.read(cache, table.to(DEV), lengths.to(DEV), 0)[1].shape == (3, 0, 2, 32)
+    none = paged.Cache.empty(0, 16, 2, 32, DEV)
+    paged.write(none, k.to(DEV), v.to(DEV), table.to(DEV), lengths.to(DEV), offsets.to(DEV))
+    assert not paged.read(none, table.to(DEV), lengths.to(DEV), 30)[0].any()
+    assert not paged.attention(k.to(DEV), none, table.to(DEV), lengths.to(DEV), offsets.to(DEV)).any()
+    assert not paged.attention(k.to(DEV), cache, table[:, :0].to(DEV), lengths.to(DEV), offsets.to(DEV)).any()
 
 
 @pytest.mark.gpu
@@ -244,6 +249,17 @@ def test_cache_refusals():
                 lambda: cpu_cache(size=2048), lambda: cpu_cache(d=24), lambda: cpu_cache(d=272), lambda: cpu_cache(heads=0)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_keys_and_values_that_share_memory_are_refused():
+    b, s = torch.zeros(6, 2, 16, 32, dtype=torch.int8), torch.zeros(6, 2, 16)
+    for k, v in ((b[::2], b[1::2]), (b[:3], b[3:]), (b.view(3, 2, 2, 16, 32)[:, 0], b.view(3, 2, 2, 16, 32)[:, 1])):
+        paged.Cache(k, v, s[:3], s[3:])
+    paged.Cache(b[:3], b[3:], s[::2], s[1::2])
+    for k, v, ks, vs in ((b[:3], b[2:5], s[:3], s[3:]), (b[:3], b[3:], s[:3], s[1:4]), (b[:3], b[::2], s[:3], s[3:]),
+                         (b[:3].transpose(1, 2).reshape(3, 2, 16, 32), b[3:], b.view(-1)[:3 * 2 * 16 * 4].view(torch.float32).view(3, 2, 16), b.view(-1)[3072:3072 + 384].view(torch.float32).view(3, 2, 16))):
+        with pytest.raises(ValueError):
+            paged.Cache(k, v, ks, vs)
 
 
 def test_call_refusals():
