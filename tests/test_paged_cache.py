@@ -257,7 +257,7 @@ def test_keys_and_values_that_share_memory_are_refused():
         paged.Cache(k, v, s[:3], s[3:])
     paged.Cache(b[:3], b[3:], s[::2], s[1::2])
     for k, v, ks, vs in ((b[:3], b[2:5], s[:3], s[3:]), (b[:3], b[3:], s[:3], s[1:4]), (b[:3], b[::2], s[:3], s[3:]),
-                         (b[:3].transpose(1, 2).reshape(3, 2, 16, 32), b[3:], b.view(-1)[:3 * 2 * 16 * 4].view(torch.float32).view(3, 2, 16), b.view(-1)[3072:3072 + 384].view(torch.float32).view(3, 2, 16))):
+                         (b[:3].transpose(1, 2).reshape(3, 2, 16, 32), b[3:], b.view(-1)[:3 * 2 * 16 * 4].view(torch.float32).view(3, 2, 16), b[3:].view(-1)[:3 * 2 * 16 * 4].view(torch.float32).view(3, 2, 16))):
         with pytest.raises(ValueError):
             paged.Cache(k, v, ks, vs)
 
