@@ -9,6 +9,13 @@
 //
 // An integer sum is scaled after 128 k (groups of 128 and more), 64, or 32, for which the instruction runs twice, each time with
 // the other half of q's k set to zero.
+//
+// What bounds it: a token reads n k / 2 bytes of weights once (1 x 16384 x 4096: 33.6 MB, 6.5 us at the rate of a large copy; 7.7 us,
+// 82 % of it), and below some 8 MB the launch and one walk of k by one workgroup (1 x 2560 x 640 4.7 us; 13 x 1024 x 4096,
+// groups of 32, 5.5).
+// Many rows are bound by instruction issue: scaling takes eight vector instructions for two products (a conversion and a
+// multiply-add for each of four sums), unpacking six for an operand, and little of that hides behind the products of the other wave of a SIMD (4000 x 4096 x 4096: 88 us, 1.5
+// POP/s, of 4.1 that the instruction alone reaches here).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -126,7 +133,8 @@ __device__ __forceinline__ void store4(const Args &p, int row, int n0, v4f acc, 
 // ---- few rows ------------------------------------------------------------------------------------------------------------------
 
 // A workgroup owns 16 RM rows of 16 columns; its NW waves share out the blocks of k, each loading its operands straight into
-// registers, U blocks at once, and their sums meet in LDS, added in the waves' order.
+// registers, U blocks at once, and their sums meet in LDS, added in the waves' order. With 16 columns to a workgroup 1024 outputs
+// are 64 of them, whose waves have a few blocks each: a token is two memory round trips.
 template <int RM, int SCALES, typename ST, int NW, int U>
 __global__ void __launch_bounds__(NW * 64) split_kernel(Args p, int tiles_n) {
     static_assert(RM <= NW, "a wave finishes one block at most");
@@ -200,7 +208,9 @@ __device__ __forceinline__ void barrier() {
 // LDS. Stages of such a block for each group stream into LDS by direct copies, NS - 1 ahead: rows of q (unit c of 16 bytes of row r at
 // place c ^ r % 8, so that eight rows read together lie in different banks), the weights' tiles and their scales as they are stored.
 // A wave unpacks the weights of a stage once for all of its rows; the sums of a block of rows are scaled behind the products of the
-// next one.
+// next one. 128 x 128 of eight waves, two workgroups on a CU, are 1.5 POP/s at 4000 x 4096 x 4096; 256 x 256, one on a CU, unpack half as
+// much but have nobody to fill the scaling's time (95 us against 88 there), and groups of 32 do not fit their registers. Smaller tiles and
+// groups of waves are for outputs that would leave CUs without work.
 template <int BM, int BN, int WM, int WN, int KG, int NS, int SCALES, typename ST>
 __global__ void __launch_bounds__(WM *WN *KG * 64) tile_kernel(Args p, int tiles_m, int tiles_n) {
     constexpr int NT = WM * WN * 64, RM = BM / WM / 16, RN = BN / WN / 16;

@@ -2,8 +2,11 @@
 //
 //   s = max(max|x| / 127, 1e-30), held to where 127 s is finite, c = rint(x / s) for each row x of d elements;   x' = c s
 //
-// Either moves bytes and little else. L = 4, 8 or 16 lanes of sixteen elements take a row, one head of a token or position; keys and
-// values are two halves of the grid.
+// Either moves bytes and little else: L = 4, 8 or 16 lanes of sixteen elements take a row, one head of a token or position; keys and
+// values are two halves of the grid. Memory bounds both (16000 F16 tokens, 8 heads of 128: 99 MB written in 24.6 us, 4.0 TB/s, read back
+// in 21.1, 4.7; eight sequences of up to 4000, 5.8 TB/s; a large copy's two directions together make 5.3), for few tokens a launch and
+// three loads in line (length, page, row): 3.8 us for 16. A wave for each token or position, its heads in line, took 76 us for
+// both where these two launches take 50 (calls in a row).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
