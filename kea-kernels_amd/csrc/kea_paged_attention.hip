@@ -65,7 +65,7 @@ struct Tile {
     int b, r0, rows, first, start, len;
 };
 
-// Tile `at` of PER rows; false where there are no more. All values are uniform.
+// Tile `at` of PER rows; false where there are no more, with t->b the number that there are (with offsets). All values are uniform.
 template <int PER>
 __device__ __forceinline__ bool find_tile(const Args &a, int at, Tile *t) {
     int tile;
@@ -95,8 +95,8 @@ __device__ __forceinline__ bool find_tile(const Args &a, int at, Tile *t) {
             }
             before += __builtin_amdgcn_readlane(sum, 63);
         }
+        t->b = found < 0 ? before : found;
         if (found < 0) return false;
-        t->b = found;
     }
     t->b = __builtin_amdgcn_readfirstlane(t->b);
     const int2 r = a.at.rows(t->b);
@@ -111,15 +111,17 @@ __device__ __forceinline__ bool find_tile(const Args &a, int at, Tile *t) {
     return true;
 }
 
-// Zeros for the rows of no sequence, of the heads of one key head.
+// Zeros for the rows of no sequence, of the heads of one key head: what workgroup `part` of the `parts` that found no tile does of it
+// (4096 padded rows of 16 heads of 128 beside 8 tokens of 4000 keys: 93 us in all, 1072 with one workgroup for each key head's).
 template <typename T>
-__device__ void fill_rest(const Args &a, int hk, int threads) {
+__device__ void fill_rest(const Args &a, int hk, int threads, int part, int parts) {
     const int from = min(max(a.at.offsets[0], 0), a.at.tokens), to = min(max(a.at.offsets[a.at.batch], from), a.at.tokens);
-    const int per = a.group * a.d;
+    constexpr int E = 16 / sizeof(T);
+    const int units = a.d / E, per = a.group * units;  // (vectors of a head, of a row)
     const long long all = (long long)(a.at.tokens - (to - from)) * per;
-    for (long long i = threadIdx.x; i < all; i += threads) {
+    for (long long i = (long long)part * threads + threadIdx.x; i < all; i += (long long)parts * threads) {
         const int row = (int)(i / per), e = (int)(i - (long long)row * per), t = row < from ? row : row + (to - from);
-        ((T *)a.out.data_dev)[(long long)t * a.out.t_stride + (long long)(hk * a.group + e / a.d) * a.out.head_stride + e % a.d] = (T)0.0f;
+        *(v4f *)((T *)a.out.data_dev + (long long)t * a.out.t_stride + (long long)(hk * a.group + e / units) * a.out.head_stride + e % units * E) = v4f{0, 0, 0, 0};
     }
 }
 
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) token_kernel(Args a) {
     const int hk = blockIdx.x % a.kv_heads, split = blockIdx.y;
     Tile t;
     if (!find_tile<32>(a, blockIdx.x / a.kv_heads, &t)) {
-        if (a.fill && split == 0 && (int)blockIdx.x / a.kv_heads == a.tiles) fill_rest<T>(a, hk, 256);
+        if (a.fill && split == 0) fill_rest<T>(a, hk, 256, blockIdx.x / a.kv_heads - t.b, a.tiles + 1 - t.b);
         return;
     }
     const int count = min(32, t.rows - t.r0), row = min(t.r0 + n, t.rows - 1), token = row / a.group, head = hk * a.group + row - token * a.group;
@@ -553,7 +555,7 @@ __global__ void __launch_bounds__(Tiles<DP>::NT, 2) rows_kernel(Args a) {
     const int hk = blockIdx.x % a.kv_heads, split = blockIdx.y;
     Tile t;
     if (!find_tile<ROWS>(a, blockIdx.x / a.kv_heads, &t)) {
-        if (a.fill && split == 0 && (int)blockIdx.x / a.kv_heads == a.tiles) fill_rest<T>(a, hk, NT);
+        if (a.fill && split == 0) fill_rest<T>(a, hk, NT, blockIdx.x / a.kv_heads - t.b, a.tiles + 1 - t.b);
         return;
     }
     const int count = min(ROWS, t.rows - t.r0), w0 = min(t.r0 + 32 * wave, t.rows - 1), w1 = min(t.r0 + 32 * wave + 31, t.rows - 1);

@@ -58,7 +58,7 @@ inline int check_paging(const char *what, const kea_pages *k, const kea_pages *v
     if (g->page_size < 16 || g->page_size > 1024 || (g->page_size & (g->page_size - 1))) return fail(KEA_EINVAL, name + ": a page holds a power of two of 16 to 1024 positions");
     if (g->table_width > (1 << 30) / g->page_size) return fail(KEA_EINVAL, name + ": more than 2^30 positions");
     if (kv_heads < 1 || kv_heads > 65535 || d < 16 || d > 256 || d % 16) return fail(KEA_EINVAL, name + ": 1 to 65535 heads of a multiple of 16, 16 to 256, elements");
-    if (!g->q_offsets_dev && g->batch > 0 && g->tokens % g->batch) return fail(KEA_EINVAL, name + ": without offsets every sequence has as many tokens");
+    if (!g->q_offsets_dev && (g->batch > 0 ? g->tokens % g->batch : g->tokens)) return fail(KEA_EINVAL, name + ": without offsets every sequence has as many tokens");
     if (!pages_ok(k) || !pages_ok(v)) return fail(KEA_EALIGN, name + ": pages and their strides are multiples of 16 bytes, strides not negative");
     if ((uintptr_t)g->table_dev % 4 || (uintptr_t)g->kv_lengths_dev % 4 || (uintptr_t)g->q_offsets_dev % 4)
         return fail(KEA_EALIGN, name + ": the table, lengths and offsets are aligned to four bytes");

@@ -204,6 +204,32 @@ def test_tables_lengths_and_offsets_that_leave_rows_empty(dtype):
 
 @pytest.mark.gpu
 @torch.inference_mode()
+@pytest.mark.parametrize("rows,first,news,lengths,heads,hk,d,dtype", [
+    (700, 5, (1, 3, 0, 3), (40, 70, 30, 9), 16, 4, 128, BF16), (300, 0, (2,), (33,), 5, 5, 80, F32), (400, 390, (1, 9), (100, 9), 6, 2, 48, F16),
+    (64, 64, (0, 0), (20, 0), 4, 1, 256, F32), (1100, 1, (3, 2), (3200, 3000), 16, 4, 128, F16), (600, 599, (1,), (3100,), 32, 2, 64, F32)])
+def test_rows_of_no_sequence_become_zeros(rows, first, news, lengths, heads, hk, d, dtype):
+    """Padded batches: rows before the first sequence's and behind the last one's, in tiles of 32 rows and of more."""
+    g = torch.Generator().manual_seed(rows)
+    q, cache, table, lens, offsets = make(news, lengths, heads, hk, d, 16, dtype, g)
+    padded = torch.full((rows, heads, d), math.nan, dtype=dtype)
+    padded[first:first + len(q)] = q
+    offsets = offsets + first
+    want, err = expected(padded, cache, table, lens, offsets)
+    old = torch.full((rows, heads, d), math.nan, dtype=dtype, device=DEV)
+    args = padded.to(DEV), on_gpu(cache), table.to(DEV), lens.to(DEV), offsets.to(DEV)
+    del old  # (its memory may become the output's)
+    got = paged.attention(*args)
+    outside = torch.ones(rows, dtype=torch.bool)
+    outside[first:first + len(q)] = False
+    assert (got.cpu()[outside] == 0).all()
+    check(got, want, err)
+    kept = torch.full_like(got, 7.0)
+    paged.attention(*args, out=kept)
+    assert (kept.cpu()[outside] == 7).all() and torch.equal(kept.cpu()[~outside], got.cpu()[~outside])
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("new,length", [(1, 900), (5, 400), (150, 300)])
 def test_unseen_keys_have_no_part(new, length, dtype):
