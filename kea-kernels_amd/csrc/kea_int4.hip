@@ -12,7 +12,7 @@
 //
 // What bounds it: a token reads n k / 2 bytes of weights once (1 x 16384 x 4096: 33.6 MB, 6.5 us at the rate of a large copy; 7.7 us,
 // 82 % of it), and below some 8 MB the launch and one walk of k by one workgroup (1 x 2560 x 640 4.7 us; 13 x 1024 x 4096,
-// groups of 32, 5.5).
+// groups of 32, 5.2).
 // Many rows are bound by instruction issue: scaling takes eight vector instructions for two products (a conversion and a
 // multiply-add for each of four sums), unpacking six for an operand, and little of that hides behind the products of the other wave of a SIMD (4000 x 4096 x 4096: 88 us, 1.5
 // POP/s, of 4.1 that the instruction alone reaches here).
@@ -419,9 +419,8 @@ int choose(int m, int n, int blocks, int scales) {
     return best;
 }
 
-template <int RM, int SCALES, typename ST>
+template <int RM, int SCALES, typename ST, int NW>
 int run_split(const Args &a, hipStream_t stream) {
-    constexpr int NW = 4;
     const int tn = (a.n + 15) / 16;
     const long long tiles = (long long)((a.m + 16 * RM - 1) / (16 * RM)) * tn;
     if (tiles > INT32_MAX / 2 || !kea::fits_dispatch(tiles, NW * 64)) return kea::fail(KEA_EINVAL, "kea_int4_gemm: too large for one launch");
@@ -448,9 +447,12 @@ template <int SCALES, typename ST>
 int run(const Args &a, hipStream_t stream) {
     // (the tile forms address a tile's rows with 32 bits)
     switch (a.ldq < (1 << 23) ? choose(a.m, a.n, a.blocks, SCALES) : 2) {
-        case 0: return run_split<1, SCALES, ST>(a, stream);
-        case 1: return run_split<2, SCALES, ST>(a, stream);
-        case 2: return run_split<4, SCALES, ST>(a, stream);
+        // (eight waves where four would load their blocks of k in more than one turn, and no more than two workgroups meet on a CU: 1 x
+        // 1024 x 16384 6.2 us and 7.3 with four, 13 x 1024 x 4096 5.2 and 5.5 from cold weights; 1 x 4096 x 1024 3.2 and 2.7, 1 x 16384 x
+        // 4096 8.0 and 7.6 from cold weights)
+        case 0: return a.blocks > 16 && (long long)((a.m + 15) / 16) * ((a.n + 15) / 16) <= 512 ? run_split<1, SCALES, ST, 8>(a, stream) : run_split<1, SCALES, ST, 4>(a, stream);
+        case 1: return run_split<2, SCALES, ST, 4>(a, stream);
+        case 2: return run_split<4, SCALES, ST, 4>(a, stream);
         case 3: return run_tiles<32, 64, 1, 4, 4, 3, SCALES, ST>(a, stream);
         case 4: return run_tiles<64, 64, 2, 2, 4, 2, SCALES, ST>(a, stream);
         case 5: return run_tiles<64, 64, 2, 2, 2, 3, SCALES, ST>(a, stream);
