@@ -151,6 +151,19 @@ def test_tiles_of_many_rows(m, n, k, group):
 
 @pytest.mark.gpu
 @torch.inference_mode()
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("m,n,k", [(1, 30, 2048), (1, 30, 2049), (13, 50, 2177), (16, 1024, 4096), (2, 8193, 2100), (1, 8192, 2200)])
+def test_tokens_of_wide_layers(m, n, k, group):
+    """Four and eight waves to a workgroup, with and without a block of k for each of them."""
+    q, qs, w, ws = make(m, n, k, group, m + n + k, torch.float32 if group > 64 else torch.float16)
+    qg, qsg, wg = on_gpu(q, qs, w, ws, group)
+    bias = torch.linspace(-3, 3, n)
+    got = int4.gemm(qg, qsg, wg, bias.to(DEV), silu=True, out_dtype=torch.float16)
+    check(got, *expected(q, qs, w, ws, group, bias, True, None, 1.0, torch.float16))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
 def test_rows_far_apart():
     """Rows of q 2^23 bytes and more apart, past 32 bits in all."""
     q, qs, w, ws = make(300, 40, 200, 64, 17)
