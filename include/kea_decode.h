@@ -78,7 +78,7 @@ int kea_paged_read(const kea_pages *k_pages, const kea_pages *v_pages, const kea
  *   out = sum_j softmax_j(scale * q . k_j) v_j over what it sees, zeros where it sees nothing or p is below 0.
  * Head h reads key head h / (heads / kv_heads). A position that a token does not see has no part in its output, whatever its scales
  * and codes are. Sums, maxima and scores are FP32; the weights exp(s - max) v_scale are rounded to FP16 (to two parts of it, 22
- * bits, with KEA_F32), and the elements of a row of q, with KEA_BF16 and KEA_F32, to 2^-28 of the row's largest (KEA_F32: 22 bits).
+ * bits, with KEA_F32), small ones to multiples of 2^-30 of the row's largest such weight, and the elements of a row of q, with KEA_BF16 and KEA_F32, to 2^-28 of the row's largest (KEA_F32: 22 bits).
  *   dtype        of q and out: KEA_F32, KEA_F16 or KEA_BF16; pointers and strides multiples of 16 bytes, strides not negative
  *                (batch_stride is not used). out overlaps no input, and no two of its rows share memory.
  *   left         >= 0; 2^30 and above: without bound.  scale: finite.  Rows of a page less than 2^26 bytes apart.

@@ -8,9 +8,11 @@
 //   p = 2^(s - ref)    l += p;   w = p v_scale, rounded to FP16;   O^T += V^T w^T;   out = O / l
 // The queries are FP16 numbers: F16 as they are, BF16 by a power of two of their row (an element below 2^-28 of the row's largest is
 // rounded to a multiple of 2^-28 of it), F32 the same in two parts, 22 bits of each element. The weights of F32 are in two parts too.
-// The reference is such that w is at most 2^15: it is raised, and l and O rescaled, only where a block's largest s, with the
-// exponent of the block's largest v_scale, passes it by more than 8 (base 2). Weights below 2^-14 lose digits of FP16: they are
-// 2^-21 and less of the largest at that time.
+// The reference is such that w is at most 2^15: it is raised, and l and O rescaled, only where a block's largest s + (exponent of that
+// key's v_scale) passes it by more than 5 (base 2), and then stands where the largest w is 2^6 at least. Weights below 2^-14 lose digits of
+// FP16: they are 2^-20 and less of the largest. Where the exponents of a block's v_scales are at most 3 apart, the largest s and the
+// largest exponent are taken for it, of whichever keys they are; where they lie further apart, a key of no weight with a large
+// v_scale would push the others' weights out of FP16's range, and each key's own sum is formed.
 //
 // Keys that a query does not see have p = 0, whatever scales they have: a scale of a key that no query sees is taken as 0, one that is
 // no number makes the scores of its key NaN, for the queries that see it.
@@ -44,8 +46,9 @@ typedef __attribute__((address_space(3))) v2i *ltr8_t;
 typedef __attribute__((address_space(3))) v4s *ltr16_t;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLazy = 8.0f;   // what a block may pass the reference by (base 2) before it is raised
-constexpr int kTop = 7;         // the exponent of the largest weight where the reference has just been raised
+constexpr float kLazy = 5.0f;   // what a block may pass the reference by (base 2) before it is raised
+constexpr int kTop = 10;        // the exponent of the largest weight where the reference has just been raised; kTop + kLazy <= 15
+constexpr int kWide = 3;        // exponents of a block's value scales that are further apart are taken key by key
 constexpr int kLeast = -85;     // scales of values below 2^-85 count as that for the reference, so that sums of 2^33 weights are finite
 
 struct Args {
@@ -141,6 +144,8 @@ __device__ __forceinline__ v16f mma(v8h a, v8h b, v16f c) { return __builtin_amd
 
 // The exponent e with 2^(e - 1) <= |v| < 2^e; 0 for 0, infinities and NaN.
 __device__ __forceinline__ int exponent(float v) { return __builtin_amdgcn_frexp_expf(v); }
+// That of a value scale, as the reference takes it.
+__device__ __forceinline__ int scale_exponent(float v) { return v != 0.0f ? max(exponent(v), kLeast) : kLeast; }
 __device__ __forceinline__ bool finite(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) != 0x7F800000u; }
 
 // The largest number of each 16 lanes, in all of them; of 32 lanes (both halves of the wave hold the same ones).
@@ -214,31 +219,43 @@ struct Sums {
 };
 
 // A block that some of a wave's rows do not see as a whole: what this lane's query does not see becomes -infinity. valid: the block's
-// keys that have a page; hi, lo: the last and first key that the query sees, counted from the block's first.
-__device__ __forceinline__ void mask(v16f &s, const v4f *v, uint32_t valid, int hi, int lo, int h, int *v_exponent) {
+// keys that have a page; hi, lo: the last and first key that the query sees, counted from the block's first. *v_exponent, *wide: as
+// weigh takes them, of what this query sees.
+__device__ __forceinline__ void mask(v16f &s, const v4f *v, uint32_t valid, int hi, int lo, int h, int *v_exponent, bool *wide) {
     asm volatile("");  // (a branch: not done for every block)
     const int hx = hi - 4 * h, lx = lo - 4 * h;
     const uint32_t bits = valid >> (4 * h);
-    float most = 0.0f;
+    float most = 0.0f, less = -INFINITY;  // (the smallest as a largest: of the numbers below zero)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         const int at = 8 * (e / 4) + e % 4;
         const bool seen = at <= hx && at >= lx && (bits >> at & 1);
         if (!seen) s[e] = -INFINITY;
         most = fmaxf(most, seen ? fabsf(v[e / 4][e % 4]) : 0.0f);
+        less = fmaxf(less, seen ? -fabsf(v[e / 4][e % 4]) : -INFINITY);
     }
-    most = other_half_max(most);
-    *v_exponent = most != 0.0f ? max(exponent(most), kLeast) : kLeast;  // (of what this query sees)
+    most = other_half_max(most), less = other_half_max(less);
+    *v_exponent = scale_exponent(most);
+    *wide = less != -INFINITY && scale_exponent(less) < *v_exponent - kWide;
 }
 
 // A block's scores s (16 keys of one query) become weights: p in the sum, w = p v as operands of the second product. v: the keys'
-// value scales, v_exponent: the exponent of the largest of them; by: what the scores are multiplied by.
+// value scales, v_exponent: the exponent of the largest of them, wide: some are more than kWide below it; by: what the scores are
+// multiplied by.
 template <int PARTS, int DB>
-__device__ __forceinline__ void weigh(const v16f &s, const v4f *v, float by, int v_exponent, Sums *m, v16f (&o)[DB], v4u (&w)[2 * PARTS]) {
+__device__ __forceinline__ void weigh(const v16f &s, const v4f *v, float by, int v_exponent, bool wide, Sums *m, v16f (&o)[DB], v4u (&w)[2 * PARTS]) {
     float top = s[0];
 #pragma unroll
     for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
     top = other_half_max(top) * by + (float)(v_exponent - kTop);
+    if (__any(wide)) {
+        asm volatile("");  // (a branch: not done for every block)
+        float own = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) own = fmaxf(own, __builtin_fmaf(s[e], by, (float)scale_exponent(v[e / 4][e % 4])));
+        own = other_half_max(own) - (float)kTop;
+        top = wide ? own : top;
+    }
     if (__any(top > m->ref + kLazy)) {
         const float next = top > m->ref + kLazy ? top : m->ref;
         if (__any(m->ref != -INFINITY)) {  // (nothing is there to rescale at first)
@@ -434,7 +451,9 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) token_kernel(Args a) {
         const float k_scale = scales[n], v_scale = scales[32 + n];
         const bool there = valid >> n & 1, number = finite(v_scale);
         const float x = !there ? 0.0f : number ? k_scale * a.scale * kLog2e : __builtin_nanf(""), y = there && number ? v_scale : 0.0f;
-        int v_exponent = max32(y != 0.0f ? max(exponent(y), kLeast) : kLeast);
+        const int own_exponent = scale_exponent(y);
+        int v_exponent = max32(own_exponent);
+        bool wide = __any(own_exponent < v_exponent - kWide);
         asm volatile("" ::: "memory");
         scales[lane] = h ? y : x;
 
@@ -455,9 +474,9 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) token_kernel(Args a) {
         for (int e = 0; e < 4; ++e) kx[e] = *(const v4f *)(scales + 8 * e + 4 * h), vx[e] = *(const v4f *)(scales + 32 + 8 * e + 4 * h);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] *= kx[e / 4][e % 4];
-        if (!(valid == 0xFFFFFFFFu && k0 + 31 <= p0 && k0 >= p1 - a.left)) mask(s, vx, valid, hi - k0, lo - k0, h, &v_exponent);  // not seen as a whole by every row
+        if (!(valid == 0xFFFFFFFFu && k0 + 31 <= p0 && k0 >= p1 - a.left)) mask(s, vx, valid, hi - k0, lo - k0, h, &v_exponent, &wide);  // not seen as a whole by every row
         v4u w[2 * PARTS];
-        weigh<PARTS, DB>(s, vx, by, v_exponent, &m, o, w);
+        weigh<PARTS, DB>(s, vx, by, v_exponent, wide, &m, o, w);
 #pragma unroll
         for (int z = 0; z < 2; ++z)
 #pragma unroll
@@ -541,7 +560,7 @@ __device__ __forceinline__ int place_v(int key) {
 template <int DP>
 struct Tiles {
     static constexpr int WQ = DP == 128 ? 8 : 4, NT = 64 * WQ, ROWS = 32 * WQ, KB = 2, KT = 32 * KB, ROW = 2 * DP, UNITS = DP / 8;
-    static constexpr int KEYS = KT * ROW, BUF = 2 * KEYS + 2 * KT * 4 + 16, LDS = 2 * BUF;  // keys, values, scales of both, exponents of blocks
+    static constexpr int KEYS = KT * ROW, BUF = 2 * KEYS + 2 * KT * 4 + 16, LDS = 2 * BUF;  // keys, values, scales of both, 2 (exponent) + wide of blocks
     static constexpr int LOADS = KT * (DP / 16) / NT;  // of 16 codes, by each thread, of keys and of values
 };
 
@@ -652,11 +671,12 @@ __global__ void __launch_bounds__(Tiles<DP>::NT, 2) rows_kernel(Args a) {
             scales[key] = !there ? 0.0f : number ? k_scale * a.scale * kLog2e : __builtin_nanf("");
             const float y = there && number ? v_scale : 0.0f;
             scales[KT + key] = y;
-            const int e = y != 0.0f ? max(exponent(y), kLeast) : kLeast, most = row_max(e);  // of 16 keys
+            const int e = scale_exponent(y), most = row_max(e);  // of 16 keys
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 const int block = max(__builtin_amdgcn_readlane(most, 32 * kb), __builtin_amdgcn_readlane(most, 32 * kb + 16));
-                if (lane == 0) ((int *)scales)[2 * KT + kb] = block;
+                const bool apart = (uint32_t)(__ballot(e < block - kWide) >> (32 * kb)) != 0;
+                if (lane == 0) ((int *)scales)[2 * KT + kb] = 2 * block + apart;
             }
         }
     };
@@ -706,13 +726,15 @@ __global__ void __launch_bounds__(Tiles<DP>::NT, 2) rows_kernel(Args a) {
             v4f kx[4], vx[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) kx[e] = *(const v4f *)(scales + 32 * kb + 8 * e + 4 * h), vx[e] = *(const v4f *)(scales + KT + 32 * kb + 8 * e + 4 * h);
-            int v_exponent = __builtin_amdgcn_readfirstlane(((const int *)scales)[2 * KT + kb]);
+            const int block = __builtin_amdgcn_readfirstlane(((const int *)scales)[2 * KT + kb]);
+            int v_exponent = block >> 1;
+            bool wide = block & 1;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] *= kx[e / 4][e % 4];
             const uint32_t here = (uint32_t)(valid >> (32 * kb));
-            if (!(here == 0xFFFFFFFFu && k0 + 31 <= p0 && k0 >= p1 - a.left)) mask(s, vx, here, hi - k0, lo - k0, h, &v_exponent);  // not seen as a whole by every row
+            if (!(here == 0xFFFFFFFFu && k0 + 31 <= p0 && k0 >= p1 - a.left)) mask(s, vx, here, hi - k0, lo - k0, h, &v_exponent, &wide);  // not seen as a whole by every row
             v4u w[2 * PARTS];
-            weigh<PARTS, DB>(s, vx, by, v_exponent, &m, o, w);
+            weigh<PARTS, DB>(s, vx, by, v_exponent, wide, &m, o, w);
 #pragma unroll
             for (int i = 0; i < 2 * DB; ++i) {
                 const char *const at = vt + (va ^ 64 * (i % DB)) + (32 * kb + 16 * (i / DB)) * ROW;

@@ -207,7 +207,7 @@ def attention(q: Tensor, cache: Cache, table: Tensor, kv_lengths: Tensor, q_offs
     output, whatever it holds. scale: 1 / sqrt(D) unless given, any finite FP32 number. out must not overlap an input.
 
     Scores, maxima and sums are FP32 and the codes enter the products exactly; the softmax's weights times the values' scales are
-    rounded to FP16 (f32: to two parts, 22 bits), and so are bf16 and f32 queries, after a power of two of each row's own (what is
+    rounded to FP16 (f32: to two parts, 22 bits; small ones to multiples of 2^-30 of the row's largest), and so are bf16 and f32 queries, after a power of two of each row's own (what is
     below 2^-28 of a row's largest element is lost; f32 keeps 22 bits)."""
     if out is None and (hit := _native("paged_attention", cache, q, table, kv_lengths, q_offsets, left, scale)) is not None:
         return hit

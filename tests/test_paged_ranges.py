@@ -1,0 +1,106 @@
+"""paged.attention where scales, queries and scores lie far apart, against a softmax in 64 bits.
+
+Bounds as in test_paged_attention, but for what FP16 takes from the weights: the reference of a row's weights stands where the largest
+product of a weight and its own key's value scale that the row sees is at least 2^6, and half of FP16's smallest step is 2^-25:
+2^-31 max_j(w_j |v_scale_j|) a code. No key enters it by its value scale alone."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from kea_kernels import paged
+from test_paged_attention import BF16, DEV, F16, F32, HALF_STEP, TYPES, U, on_gpu
+
+ROUNDED = {F32: 2.0**-22, F16: 2.0**-11, BF16: 2.0**-11}
+
+
+def one_sequence(n, length, heads, hk, d, dtype, g, room=None):
+    """q of n new tokens, a cache of `length` positions, its table with room for `room`, and the lengths."""
+    pages = -(-length // 16)
+    table = torch.full((1, -(-(room or length) // 16)), -1, dtype=torch.int32)
+    table[0, :pages] = torch.randperm(pages, generator=g).int()
+    ints = [torch.randint(-127, 128, (pages, hk, 16, d), generator=g, dtype=torch.int8) for _ in range(2)]
+    scales = [torch.full((pages, hk, 16), 0.01) for _ in range(2)]
+    return torch.randn(n, heads, d, generator=g).to(dtype), paged.Cache(*ints, *scales), table, torch.tensor([length], dtype=torch.int32)
+
+
+def place(table, p):
+    """Where position p's rows are: the first three indices of a cache's tensors."""
+    return table[0].long()[p // 16], slice(None), p % 16
+
+
+def expected(q, cache, table, lengths, scale=None, exact_scores=False):
+    """(the output in 64 bits, how far the kernel's may be from it). exact_scores: the softmax is one key's but for nothing, whatever
+    the rounding of scores."""
+    (n, heads, d), hk, length = q.shape, cache.kv_heads, int(lengths[0])
+    scale = 1 / math.sqrt(d) if scale is None else scale
+    at = place(table, torch.arange(length))
+    kc, vc, ks, vs = (t[at].double() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale))  # [length, hk, ...]
+    seen = torch.arange(length) <= torch.arange(length - n, length)[:, None]
+    out, err = torch.zeros(n, heads, d, dtype=torch.float64), torch.zeros(n, heads, d, dtype=torch.float64)
+    for x in range(heads):
+        y = x * hk // heads
+        qd, k, v = q[:, x].double(), kc[:, y] * ks[:, y, None], vc[:, y] * vs[:, y, None]
+        s, mag = (qd @ k.t()) * scale, (qd.abs() @ k.abs().t()) * abs(scale)
+        es = (d + 4) * U * mag + 3 * U * s.abs() + (2.0**-22 * mag if q.dtype == F32 else 0)
+        if q.dtype != F16:
+            es = es + abs(scale) * 2.0**-29 * qd.abs().amax(1, keepdim=True) * k.abs().sum(1)
+        es = torch.zeros(n, 1, dtype=torch.float64) if exact_scores else torch.where(seen, es, 0.0).amax(1, keepdim=True)
+        w = torch.softmax(torch.where(seen, s, -math.inf), 1)
+        out[:, x] = w @ v
+        e = (w @ v.abs()) * (4 * es + (length + 40) * U + ROUNDED[q.dtype]) * 1.05
+        err[:, x] = e + 2.0**-31 * (w * vs[:, y].abs()).amax(1, keepdim=True) * (seen.double() @ vc[:, y].abs())
+    return out, err + (out.abs() + err) * HALF_STEP[q.dtype] + (2.0**-25 if q.dtype == F16 else 1e-37)
+
+
+def check(got, want, err):
+    got = got.cpu().double()
+    assert torch.isfinite(got).all()
+    worst = ((got - want).abs() / err).max().item()
+    assert worst <= 1, f"{worst:.3g} times the bound"
+
+
+def run(q, cache, table, lengths, **kw):
+    return paged.attention(q.to(DEV), on_gpu(cache), table.to(DEV), lengths.to(DEV), **kw)
+
+
+# (new tokens, length, room of the table): tiles of 32 rows, and of 128 and 256
+KERNELS = [(1, 96, None), (5, 200, None), (1000, 1100, 4800)]
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,length,room", KERNELS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_values_without_weight_take_no_digits(d, n, length, room, dtype):
+    """One key has all the weight; its neighbours, 2^65 times lighter, have value scales up to 2^34 times its own."""
+    g = torch.Generator().manual_seed(d + n)
+    q, cache, table, lengths = one_sequence(n, length, 16, 4, d, dtype, g, room)
+    q = (torch.randint(0, 2, (1, 1, d), generator=g) * 2.0 - 1).expand(n, 16, d).contiguous().to(dtype)
+    cache.k.zero_()
+    cache.k[place(table, 40)] = (100 * q[0, :1]).to(torch.int8)
+    cache.k_scale.fill_(45 / (100 * math.sqrt(d)))  # (the score is 45, e^45 = 2^65)
+    cache.v_scale.fill_(2.0**-10)
+    for ratio in (12, 16, 20, 24, 28, 31, 34):
+        for p in range(32, 64):
+            cache.v_scale[place(table, p)] = 2.0 ** (-10 if p == 40 else ratio - 10 - p % 3)
+        check(run(q, cache, table, lengths), *expected(q, cache, table, lengths, exact_scores=True))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,length,room", KERNELS)
+@pytest.mark.parametrize("spread", [4, 24, 60])
+def test_value_scales_of_every_size_side_by_side(spread, n, length, room, dtype):
+    """Each key has a scale of its own, powers of two `spread` apart, zeros among them, and scores that are within some 2^20."""
+    g = torch.Generator().manual_seed(spread + n)
+    q, cache, table, lengths = one_sequence(n, length, 16, 4, 80, dtype, g, room)
+    top = 6 if dtype == F16 else spread / 2
+    cache.v_scale.copy_(torch.exp2(top - spread * torch.rand(cache.v_scale.shape, generator=g)))
+    check(run(q, cache, table, lengths), *expected(q, cache, table, lengths))
+    cache.v_scale[torch.rand(cache.v_scale.shape, generator=g) < 0.2] = 0.0
+    check(run(q, cache, table, lengths), *expected(q, cache, table, lengths))
