@@ -5,14 +5,17 @@
 //   S^T = K Q^T        keys are the matrix instruction's rows, queries its columns, keys and values their codes -127 .. 127, exact in
 //                      FP16: a lane holds 16 keys' sums of one query (its column)
 //   s = S^T a          a = scale log2(e) k_scale, a number for each key
-//   p = 2^(s - ref)    l += p;   w = p v_scale, rounded to FP16;   O^T += V^T w^T;   out = O / l
+//   w = 2^(s - ref) v_scale, rounded to FP16;   O^T += V^T w^T;   l += 2^(s - top);   out = O 2^(ref - top) / l
 // The queries are FP16 numbers: F16 as they are, BF16 by a power of two of their row (an element below 2^-28 of the row's largest is
 // rounded to a multiple of 2^-28 of it), F32 the same in two parts, 22 bits of each element. The weights of F32 are in two parts too.
-// The reference is such that w is at most 2^15: it is raised, and l and O rescaled, only where a block's largest s + (exponent of that
+// The reference ref is such that w is at most 2^15: it is raised, and O rescaled, only where a block's largest s + (exponent of that
 // key's v_scale) passes it by more than 5 (base 2), and then stands where the largest w is 2^6 at least. Weights below 2^-14 lose digits of
 // FP16: they are 2^-20 and less of the largest. Where the exponents of a block's v_scales are at most 3 apart, the largest s and the
 // largest exponent are taken for it, of whichever keys they are; where they lie further apart, a key of no weight with a large
 // v_scale would push the others' weights out of FP16's range, and each key's own sum is formed.
+// The sum l has a reference of its own, the largest s so far, passed by 5 at most. Both are whole numbers: 2^(ref - top) is exact. One
+// exponential serves both, 2^(s - ref), its sum times 2^(ref - top), while that factor is from 2^-100 to 2^60; beyond (values above some
+// 2^70 or below 2^-90, and scores above 2^20) it would pass FP32's range or digits, and each has its own.
 //
 // Keys that a query does not see have p = 0, whatever scales they have: a scale of a key that no query sees is taken as 0, one that is
 // no number makes the scores of its key NaN, for the queries that see it.
@@ -49,7 +52,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 5.0f;   // what a block may pass the reference by (base 2) before it is raised
 constexpr int kTop = 10;        // the exponent of the largest weight where the reference has just been raised; kTop + kLazy <= 15
 constexpr int kWide = 3;        // exponents of a block's value scales that are further apart are taken key by key
-constexpr int kLeast = -85;     // scales of values below 2^-85 count as that for the reference, so that sums of 2^33 weights are finite
+constexpr int kLeast = -149;    // the exponent that a value scale of zero counts as: below that of all others
+constexpr float kNone = -0x1.fffffep127f;       // no reference yet: the lowest number
+constexpr float kLarge = 0x1p20f;               // the largest reference that whole numbers up to some 2^8 are added to
+constexpr int kFar = 60, kNear = -100;  // the largest and smallest ref - top with which one exponential serves both
 
 struct Args {
     kea_heads q, out;
@@ -145,7 +151,7 @@ __device__ __forceinline__ v16f mma(v8h a, v8h b, v16f c) { return __builtin_amd
 // The exponent e with 2^(e - 1) <= |v| < 2^e; 0 for 0, infinities and NaN.
 __device__ __forceinline__ int exponent(float v) { return __builtin_amdgcn_frexp_expf(v); }
 // That of a value scale, as the reference takes it.
-__device__ __forceinline__ int scale_exponent(float v) { return v != 0.0f ? max(exponent(v), kLeast) : kLeast; }
+__device__ __forceinline__ int scale_exponent(float v) { return v != 0.0f ? exponent(v) : kLeast; }
 __device__ __forceinline__ bool finite(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) != 0x7F800000u; }
 
 // The largest number of each 16 lanes, in all of them; of 32 lanes (both halves of the wave hold the same ones).
@@ -213,10 +219,32 @@ __device__ __forceinline__ void load_queries(const T *row, int d, bool inside, A
     }
 }
 
-// The running sums of a lane's query: the weights' reference and sum (of this half's keys).
+// a - b of two references, whole numbers; so far down where they are far apart that nothing is left of a product with its power.
+__device__ __forceinline__ int difference(float a, float b) { return (int)fmaxf(a - b, -1000.0f); }
+
+// The running references of a lane's query, its sum (of this half's keys) and what a block's sum of 2^(s - ref) takes part in it by.
 struct Sums {
-    float ref, l;
+    float top = kNone, ref = kNone, l = 0.0f, unit = 1.0f;
+    int up = 0;        // ref is top + up (to FP32: where that is not exact, the query is far)
+    bool far = false;  // up is beyond kNear .. kFar, or top beyond kLarge: the sum and the weights have an exponential each
 };
+
+// What the sums make of a product: out = O 2^(ref - top) / l.
+__device__ __forceinline__ v4f mean(v4f o, const Sums &m) {
+    const float inv = m.l != 0.0f ? 1.0f / m.l : 0.0f;
+    v4f v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_ldexpf(o[e] * inv, m.up);
+    return v;
+}
+// Of several means: mean[s] 2^(top[s] - top) by (l[s] / the sum of l 2^(top[s] - top)), `by` the latter. (In this order neither a large value
+// of next to no weight is lost nor anything passes FP32's range.)
+__device__ __forceinline__ v4f portion(v4f mean, int down, float by) {
+    v4f v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_ldexpf(mean[e], down) * by;
+    return v;
+}
 
 // A block that some of a wave's rows do not see as a whole: what this lane's query does not see becomes -infinity. valid: the block's
 // keys that have a page; hi, lo: the last and first key that the query sees, counted from the block's first. *v_exponent, *wide: as
@@ -239,34 +267,55 @@ __device__ __forceinline__ void mask(v16f &s, const v4f *v, uint32_t valid, int 
     *wide = less != -INFINITY && scale_exponent(less) < *v_exponent - kWide;
 }
 
-// A block's scores s (16 keys of one query) become weights: p in the sum, w = p v as operands of the second product. v: the keys'
+// A block's scores s (16 keys of one query) become weights: in the sum, and times v as operands of the second product. v: the keys'
 // value scales, v_exponent: the exponent of the largest of them, wide: some are more than kWide below it; by: what the scores are
-// multiplied by.
+// multiplied by. (s and v may be changed.)
 template <int PARTS, int DB>
-__device__ __forceinline__ void weigh(const v16f &s, const v4f *v, float by, int v_exponent, bool wide, Sums *m, v16f (&o)[DB], v4u (&w)[2 * PARTS]) {
+__device__ __forceinline__ void weigh(v16f &s, v4f *v, float by, int v_exponent, bool wide, Sums *m, v16f (&o)[DB], v4u (&w)[2 * PARTS]) {
     float top = s[0];
 #pragma unroll
     for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-    top = other_half_max(top) * by + (float)(v_exponent - kTop);
-    if (__any(wide)) {
-        asm volatile("");  // (a branch: not done for every block)
-        float own = -INFINITY;
+    top = other_half_max(top) * by;
+    const float less = (float)(v_exponent - kTop);
+    bool passed = top + less > m->ref + kLazy || top > m->top + kLazy;
+    float ref = m->ref;
+    // (what few blocks need lies behind the loop: in line it took 10 % more for many rows)
+    if (__builtin_expect(__any(passed || wide || m->far), 0)) {
+        passed = passed || wide || m->far;
+        const float next = passed ? floorf(fmaxf(m->top, top)) : m->top;
+        const int down = difference(m->top, next);
+        float own = top - next + (float)v_exponent;
+        if (__any(wide)) {  // the largest over each key's own score and exponent
+            float most = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) own = fmaxf(own, __builtin_fmaf(s[e], by, (float)scale_exponent(v[e / 4][e % 4])));
-        own = other_half_max(own) - (float)kTop;
-        top = wide ? own : top;
-    }
-    if (__any(top > m->ref + kLazy)) {
-        const float next = top > m->ref + kLazy ? top : m->ref;
-        if (__any(m->ref != -INFINITY)) {  // (nothing is there to rescale at first)
-            const float half = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m->ref - next) * 0.5f), all = half * half;
-            m->l = m->l * half * half;  // (the sum may be as large as 2^100 where the values are small)
+            for (int e = 0; e < 16; ++e) most = fmaxf(most, __builtin_fmaf(s[e], by, -next) + (float)scale_exponent(v[e / 4][e % 4]));
+            most = other_half_max(most);
+            own = wide ? most : own;
+        }
+        const int up = passed ? max(m->up + down, (int)fmaxf(floorf(own), -1000.0f) - kTop) : m->up;
+        if (__any(m->top != kNone)) {  // (nothing is there to rescale at first)
+            const float all = __builtin_amdgcn_ldexpf(1.0f, m->up + down - up);
+            m->l = __builtin_amdgcn_ldexpf(m->l, down);
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[d] *= all;
         }
-        m->ref = next;
+        m->top = next, m->up = up, m->ref = ref = next + (float)up;
+        m->far = up > kFar || up < kNear || (fabsf(next) > kLarge && next != kNone);
+        m->unit = m->far ? 0.0f : __builtin_amdgcn_ldexpf(1.0f, up);
     }
-    const float ref = m->ref == -INFINITY ? 0.0f : m->ref;
+    if (__builtin_expect(__any(m->far), 0)) {  // their weights take the values' mantissas, with the values' exponents in the exponential
+        float apart = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float x = v[e / 4][e % 4], t = __builtin_fmaf(s[e], by, -m->top);
+            const int of_x = scale_exponent(x);
+            apart += __builtin_amdgcn_exp2f(t);
+            s[e] = m->far ? t + (float)(of_x - m->up) : s[e];
+            v[e / 4][e % 4] = m->far ? __builtin_amdgcn_ldexpf(x, -of_x) : x;
+        }
+        by = m->far ? 1.0f : by, ref = m->far ? 0.0f : ref;
+        m->l += m->far ? apart : 0.0f;
+    }
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
@@ -280,7 +329,7 @@ __device__ __forceinline__ void weigh(const v16f &s, const v4f *v, float by, int
         w[e / 8 * PARTS][e % 8 / 2] = __builtin_bit_cast(uint32_t, hi);
         if constexpr (PARTS == 2) w[e / 8 * PARTS + 1][e % 8 / 2] = __builtin_bit_cast(uint32_t, v2h{(_Float16)(x0 - (float)hi[0]), (_Float16)(x1 - (float)hi[1])});
     }
-    m->l += sum;
+    m->l = __builtin_fmaf(sum, m->unit, m->l);
 }
 
 template <typename T>
@@ -425,7 +474,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) token_kernel(Args a) {
     v16f o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-    Sums m{-INFINITY, 0.0f};
+    Sums m;
     // operand addresses: unit 2 c + h of key n at ka ^ 32 c; eight keys' values of unit 2 d + (lane / 16) % 2, for the lanes' d
     const int ka = n * DP + (h ^ place<UNITS>(n)) * 16;
     const int vr = (lane & 15) >> 1, vkey = vr % 4 + 8 * (vr / 4) + 4 * h;
@@ -491,20 +540,19 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) token_kernel(Args a) {
     }
     m.l = both_halves(m.l);
 
-    // the waves' means, references and sums meet in LDS: [wave][32][DP], then [wave][32][2]
+    // the waves' means, their sums and those's references meet in LDS: [wave][32][DP], then [wave][32][2]
     float *const po = (float *)lds, *const ps = po + 4 * 32 * DP;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __syncthreads();
     if (n < count) {
-        const float inv = m.l != 0.0f ? 1.0f / m.l : 0.0f;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const int c = 8 * d + e / 2 + h;  // (units of four elements, moved by the row: 32 rows are written at once)
-                *(v4f *)(po + ((wave * 32 + n) * (DP / 4) + (c ^ (n & 7))) * 4) = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]} * inv;
+                *(v4f *)(po + ((wave * 32 + n) * (DP / 4) + (c ^ (n & 7))) * 4) = mean(v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]}, m);
             }
-        if (h == 0) *(float2 *)(ps + 2 * (wave * 32 + n)) = make_float2(m.ref, m.l);
+        if (h == 0) *(float2 *)(ps + 2 * (wave * 32 + n)) = make_float2(m.top, m.l);
     }
     __syncthreads();
     for (int at = tid; at < count * (DP / 4); at += 256) {
@@ -515,15 +563,15 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) token_kernel(Args a) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) st[w] = *(const float2 *)(ps + 2 * (w * 32 + r)), top = fmaxf(top, st[w].x);
         v4f v = {0, 0, 0, 0};
-        float part[4];
+        int down[4];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            part[w] = st[w].y * (st[w].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st[w].x - top));  // (a NaN stays one)
-            all += part[w];
+            down[w] = difference(st[w].x, top);
+            all += __builtin_amdgcn_ldexpf(st[w].y, down[w]);  // (a NaN stays one)
         }
         const float inv = all != 0.0f ? 1.0f / all : 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) v += *(const v4f *)(po + ((w * 32 + r) * (DP / 4) + (c ^ (r & 7))) * 4) * (part[w] * inv);
+        for (int w = 0; w < 4; ++w) v += portion(*(const v4f *)(po + ((w * 32 + r) * (DP / 4) + (c ^ (r & 7))) * 4), down[w], st[w].y * inv);
         const int tt = (t.r0 + r) / a.group, hh = hk * a.group + (t.r0 + r) - tt * a.group;
         if (a.splits > 1) {
             const long long slot = ((long long)split * a.at.tokens + t.first + tt) * (a.kv_heads * a.group) + hh;
@@ -688,7 +736,7 @@ __global__ void __launch_bounds__(Tiles<DP>::NT, 2) rows_kernel(Args a) {
     v16f o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-    Sums m{-INFINITY, 0.0f};
+    Sums m;
     // operand addresses: unit 2 c + h of key n at ka ^ 32 c, units 4 d .. of the values' rows at va ^ 64 d
     const int ka = n * ROW + (h ^ place_k<UNITS>(n)) * 16;
     const int vkey = 4 * h + (lane & 15) / 4, va = vkey * ROW + ((2 * (lane >> 4 & 1) + (lane & 3) / 2) ^ place_v<UNITS>(vkey)) * 16 + (lane & 1) * 8;
@@ -749,7 +797,6 @@ __global__ void __launch_bounds__(Tiles<DP>::NT, 2) rows_kernel(Args a) {
     }
     m.l = both_halves(m.l);
     if (!real) return;
-    const float inv = m.l != 0.0f ? 1.0f / m.l : 0.0f;
     const long long slot = ((long long)split * a.at.tokens + t.first + token) * (a.kv_heads * a.group) + head;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -757,14 +804,14 @@ __global__ void __launch_bounds__(Tiles<DP>::NT, 2) rows_kernel(Args a) {
         for (int e = 0; e < 16; e += 4) {
             const int c = 32 * d + 2 * e + 4 * h;
             if (c >= a.d) continue;
-            const v4f v = v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]} * inv;
+            const v4f v = mean(v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]}, m);
             if (a.splits > 1) *(v4f *)(a.part + slot * a.d + c) = v;
             else store4((T *)a.out.data_dev + (long long)(t.first + token) * a.out.t_stride + (long long)head * a.out.head_stride + c, v);
         }
-    if (a.splits > 1 && h == 0) *(float2 *)(a.stats + 2 * slot) = make_float2(m.ref, m.l);
+    if (a.splits > 1 && h == 0) *(float2 *)(a.stats + 2 * slot) = make_float2(m.top, m.l);
 }
 
-// Joins the splits: out = sum_s f_s mean_s, f_s = l_s 2^(ref_s - ref) over their sum; four elements a thread, eight splits at a time.
+// Joins the splits: out = sum_s f_s mean_s, f_s = l_s 2^(top_s - top) over their sum; four elements a thread, eight splits at a time.
 template <typename T>
 __global__ void __launch_bounds__(64) join_kernel(Args a) {
     const int heads = a.kv_heads * a.group, per = a.d / 4;
@@ -772,7 +819,7 @@ __global__ void __launch_bounds__(64) join_kernel(Args a) {
     if (slot0 >= all_rows) return;
     const int c = (int)(at - slot0 * per), t = (int)(slot0 / heads), head = (int)(slot0 - (long long)t * heads);
     if (a.at.offsets && !(t >= a.at.offsets[0] && t < a.at.offsets[a.at.batch])) return;
-    float ref = -INFINITY, all = 0.0f;
+    float top = -INFINITY, all = 0.0f;
     v4f v = {0, 0, 0, 0};
     for (int s0 = 0; s0 < a.splits; s0 += 8) {
         float2 st[8];
@@ -782,24 +829,20 @@ __global__ void __launch_bounds__(64) join_kernel(Args a) {
             const long long slot = min(s0 + s, a.splits - 1) * all_rows + slot0;
             st[s] = *(const float2 *)(a.stats + 2 * slot);
             part[s] = *(const v4f *)(a.part + slot * a.d + 4 * c);
+            if (s0 + s >= a.splits) st[s].y = 0.0f;
         }
-        float top = ref;
+        const float old = top;
 #pragma unroll
         for (int s = 0; s < 8; ++s) top = fmaxf(top, st[s].x);
-        const float old = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - top);
-        ref = top;
-        float f[8], sum = all * old;
+        float sum = __builtin_amdgcn_ldexpf(all, difference(old, top));
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            f[s] = s0 + s < a.splits ? st[s].y * (st[s].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st[s].x - top)) : 0.0f;
-            sum += f[s];
-        }
+        for (int s = 0; s < 8; ++s) sum += __builtin_amdgcn_ldexpf(st[s].y, difference(st[s].x, top));
         // (the sum so far is kept as a mean: it neither overflows nor loses digits that the mean has)
         const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-        v *= all * old * inv;
+        v = portion(v, difference(old, top), all * inv);
 #pragma unroll
         for (int s = 0; s < 8; ++s)
-            if (f[s] != 0.0f) v += part[s] * (f[s] * inv);  // (a part that saw nothing was not written)
+            if (st[s].y != 0.0f) v += portion(part[s], difference(st[s].x, top), st[s].y * inv);  // (a part that saw nothing was not written)
         all = sum;
     }
     store4((T *)a.out.data_dev + (long long)t * a.out.t_stride + (long long)head * a.out.head_stride + 4 * c, v);

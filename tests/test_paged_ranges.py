@@ -104,3 +104,74 @@ def test_value_scales_of_every_size_side_by_side(spread, n, length, room, dtype)
     check(run(q, cache, table, lengths), *expected(q, cache, table, lengths))
     cache.v_scale[torch.rand(cache.v_scale.shape, generator=g) < 0.2] = 0.0
     check(run(q, cache, table, lengths), *expected(q, cache, table, lengths))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,length,room", [(1, 2500, None), (5, 3000, None), (1000, 1100, 4800)])
+def test_values_near_the_largest_numbers(n, length, room, dtype):
+    """Values up to 2^127: the light keys, 2^-16 of the heaviest one each, keep their part in the sum; beside them, and in other parts of
+    the keys, rows of zeros with the smallest scale; a weight of 2^-130 with a value of 2^127."""
+    g = torch.Generator().manual_seed(n)
+    q, cache, table, lengths = one_sequence(n, length, 16, 4, 64, dtype, g, room)
+    q = (torch.randint(0, 2, (1, 1, 64), generator=g) * 2.0 - 1).expand(n, 16, 64).contiguous().to(dtype)
+    towards = (100 * q[0, :1]).to(torch.int8)
+    cache.k.zero_()
+    cache.k[place(table, 40)] = towards
+    cache.k_scale.fill_(11.1 / 800)  # (e^11.1 = 2^16)
+    cache.v_scale.fill_(2.0**120)
+    check(run(q, cache, table, lengths), *expected(q, cache, table, lengths))
+    cache.v_scale.fill_(1e-30)
+    check(run(q, cache, table, lengths), *expected(q, cache, table, lengths))
+    cache.k.zero_()
+    cache.v[:, :, 8:] = 0
+    for p in range(32):
+        cache.v_scale[place(table, p)] = 2.0**120
+    check(run(q, cache, table, lengths), *expected(q, cache, table, lengths))
+    cache.v_scale.fill_(2.0**-10)
+    cache.k[:] = towards[0]
+    cache.k_scale.fill_(90.0 / 800)  # (e^90 = 2^130)
+    for p in range(32):
+        cache.k[place(table, p)] = 0
+        cache.v_scale[place(table, p)] = 2.0**120
+    check(run(q, cache, table, lengths), *expected(q, cache, table, lengths))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+def test_a_sum_of_2_to_the_30_weights():
+    """One token of 2^30 positions that share two pages, with the smallest value scale: the first page of every part has the weights 1, all
+    others 2^4.5."""
+    cache = paged.Cache(*(torch.zeros(2, 1, 1024, 16, dtype=torch.int8, device=DEV) for _ in range(2)), torch.full((2, 1, 1024), 4.5 * math.log(2) / 100, device=DEV),
+                        torch.full((2, 1, 1024), 1e-30, device=DEV))
+    cache.k[1, ..., 0], cache.v[0], cache.v[1] = 100, 50, 100
+    table = torch.ones(1, 1 << 20, dtype=torch.int32, device=DEV)
+    table[0, ::1 << 14] = 0
+    q = torch.zeros(1, 1, 16, device=DEV)
+    q[..., 0] = 1.0
+    out = paged.attention(q, cache, table, torch.tensor([1 << 30], dtype=torch.int32, device=DEV), scale=1.0)
+    first = 64 / (1 << 20)
+    want = 1e-30 * (50 * first + 100 * 2**4.5 * (1 - first)) / (first + 2**4.5 * (1 - first))
+    # FP32 sums of equal numbers: of 2^18 blocks a wave, off by half a step each; products and sum, of 16 (32) weights a block
+    assert bool(((out.double() - want).abs() <= want * 2 * (2**18 + 40) * U).all())
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,length,room", KERNELS)
+def test_scores_of_any_size(n, length, room, dtype):
+    """Scores of up to 2^100, one of them the largest by far: its value comes out, whatever its scale and the others' are."""
+    g = torch.Generator().manual_seed(n)
+    q, cache, table, lengths = one_sequence(n, length, 16, 4, 64, dtype, g, room)
+    q = (torch.randint(0, 2, (1, 1, 64), generator=g) * 2.0 - 1).expand(n, 16, 64).contiguous().to(dtype)
+    cache.k[:] = (60 * q[0, :1]).to(torch.int8)
+    cache.k[place(table, 70)] = (100 * q[0, :1]).to(torch.int8)
+    for own, others in ((-10, -10), (-10, 8), (8, -20), (-20, 20), (100, -100), (-90, 100)):
+        if dtype == F16 and abs(own) > 10:
+            continue
+        cache.v_scale.fill_(2.0**others)
+        cache.v_scale[place(table, 70)] = 2.0**own
+        for scale in (1.0, 2.0**14, 2.0**20, 2.0**30, 2.0**97):
+            check(run(q, cache, table, lengths, scale=scale), *expected(q, cache, table, lengths, scale=scale, exact_scores=True))
