@@ -4,7 +4,7 @@
 // r % group of the group. Keys are walked once, 32 at a time, in products of 16-bit floats on whole numbers:
 //   S^T = K Q^T        keys are the matrix instruction's rows, queries its columns, keys and values their codes -127 .. 127, exact in
 //                      FP16: a lane holds 16 keys' sums of one query (its column)
-//   s = S^T a          a = scale log2(e) k_scale, a number for each key
+//   s = S^T a          a = scale log2(e) k_scale, a number for each key (but for powers of two)
 //   w = 2^(s - ref) v_scale, rounded to FP16;   O^T += V^T w^T;   l += 2^(s - top);   out = O 2^(ref - top) / l
 // The queries are FP16 numbers: F16 as they are, BF16 by a power of two of their row (an element below 2^-28 of the row's largest is
 // rounded to a multiple of 2^-28 of it), F32 the same in two parts, 22 bits of each element. The weights of F32 are in two parts too.
@@ -21,6 +21,7 @@
 // no number makes the scores of its key NaN, for the queries that see it.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <string>
@@ -64,7 +65,8 @@ struct Args {
     float *part, *stats;  // splits > 1: [splits][tokens][heads][d], [splits][tokens][heads][2]
     int kv_heads, group, d, left, splits, tiles_each, tiles;  // tiles_each: of a sequence, without offsets; tiles: the most there can be
     int fill;  // rows of no sequence become zeros
-    float scale;
+    float scale;  // times 2^by of each score
+    int by;
 };
 
 // ---- what both kernels do --------------------------------------------------------------------------------------------------------
@@ -168,9 +170,10 @@ __device__ __forceinline__ int max32(int v) {
 }
 
 // A row of queries as the product's second operand, eight elements at a time; `at(i)` is the first element of operand i of this
-// lane. *by: what a sum with it is multiplied by (a power of two).
+// lane. *by: what a sum with it is multiplied by, a power of two: that of the row, and 2^up. (Rows whose power would not be a
+// normal number with that are scaled by less: none of it is lost.)
 template <typename T, int N, typename At>
-__device__ __forceinline__ void load_queries(const T *row, int d, bool inside, At at, v8h (&q)[N * (sizeof(T) == 4 ? 2 : 1)], float *by) {
+__device__ __forceinline__ void load_queries(const T *row, int d, bool inside, At at, int up, v8h (&q)[N * (sizeof(T) == 4 ? 2 : 1)], float *by) {
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
     auto load = [&](int i, float *v) {
         typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
@@ -182,7 +185,6 @@ __device__ __forceinline__ void load_queries(const T *row, int d, bool inside, A
             for (int e = 0; e < E; ++e) v[u * E + e] = (float)x[e];
         }
     };
-    *by = 1.0f;
     int less = 0;
     if constexpr (!__is_same(T, _Float16)) {
         float most = 0.0f;
@@ -194,9 +196,9 @@ __device__ __forceinline__ void load_queries(const T *row, int d, bool inside, A
 #pragma unroll
             for (int e = 0; e < 8; ++e) most = fmaxf(most, finite(v[e]) ? fabsf(v[e]) : 0.0f);
         }
-        less = exponent(other_half_max(most)) - 5;
-        *by = __builtin_amdgcn_ldexpf(1.0f, max(less, -126));
+        less = min(max(exponent(other_half_max(most)) - 5, -126 - up), 127 - up);
     }
+    *by = __builtin_amdgcn_ldexpf(1.0f, less + up);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         if (!inside || at(i) >= d) {
@@ -469,7 +471,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) token_kernel(Args a) {
     v8h q[QN * PARTS];
     float by;
     load_queries<T, QN>((const T *)a.q.data_dev + (long long)(t.first + token) * a.q.t_stride + (long long)head * a.q.head_stride, a.d, p >= 0,
-                        [&](int i) { return 16 * (2 * (i / 2) + h) + 8 * (i % 2); }, q, &by);
+                        [&](int i) { return 16 * (2 * (i / 2) + h) + 8 * (i % 2); }, a.by, q, &by);
 
     v16f o[DB];
 #pragma unroll
@@ -732,7 +734,7 @@ __global__ void __launch_bounds__(Tiles<DP>::NT, 2) rows_kernel(Args a) {
     v8h q[QN * PARTS];
     float by;
     load_queries<T, QN>((const T *)a.q.data_dev + (long long)(t.first + token) * a.q.t_stride + (long long)head * a.q.head_stride, a.d, p >= 0,
-                        [&](int i) { return 16 * i + 8 * h; }, q, &by);
+                        [&](int i) { return 16 * i + 8 * h; }, a.by, q, &by);
     v16f o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -984,7 +986,14 @@ int kea_paged_attention(const kea_heads *q, const kea_heads *out, int dtype, int
     a.q = *q, a.out = *out, a.kp = *k_pages, a.vp = *v_pages;
     a.part = (float *)workspace, a.stats = workspace ? (float *)((char *)workspace + p.part_bytes) : nullptr;
     a.kv_heads = (int)kv_heads, a.group = (int)(heads / kv_heads), a.d = (int)d, a.left = (int)(left < (1 << 30) ? left : 1 << 30);
-    a.splits = (int)p.splits, a.tiles_each = (int)p.tiles_each, a.tiles = (int)p.tiles, a.scale = scale;
+    a.splits = (int)p.splits, a.tiles_each = (int)p.tiles_each, a.tiles = (int)p.tiles;
+    // A score is (sum of codes and queries) (k_scale scale log2(e)) 2^by: the sum is below 2^20 (FP16 queries, which have no power of two
+    // of their own, 2^31) and k_scale below 2^122, so that 2^-16 (2^-27) of the scale's power are left with them and the rest goes with the
+    // queries'.
+    int power = 0;
+    std::frexp(scale, &power);
+    a.by = std::min(std::max(power + (dtype == KEA_F16 ? 27 : 16), -126), 127);
+    a.scale = std::ldexp(scale, -a.by);
     a.fill = fill && paging->q_offsets_dev ? 1 : 0;
     const hipStream_t s = (hipStream_t)stream;
     return dtype == KEA_F32 ? run<float>(a, p.few, s) : dtype == KEA_F16 ? run<_Float16>(a, p.few, s) : run<__bf16>(a, p.few, s);

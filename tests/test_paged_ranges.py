@@ -175,3 +175,20 @@ def test_scores_of_any_size(n, length, room, dtype):
         cache.v_scale[place(table, 70)] = 2.0**own
         for scale in (1.0, 2.0**14, 2.0**20, 2.0**30, 2.0**97):
             check(run(q, cache, table, lengths, scale=scale), *expected(q, cache, table, lengths, scale=scale, exact_scores=True))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,length,room", KERNELS)
+def test_queries_keys_and_scales_of_every_size(n, length, room, dtype):
+    """Powers of two on the queries, the keys' scales and `scale` that cancel: the same scores."""
+    g = torch.Generator().manual_seed(n)
+    q, cache, table, lengths = one_sequence(n, length, 16, 4, 64, dtype, g, room)
+    k_scale = cache.k_scale * torch.exp(0.3 * torch.randn(cache.k_scale.shape, generator=g))
+    for of_q, of_k, of_scale in ([(0, 0, 0), (-8, -90, 98), (8, 110, -118), (0, -95, 95), (4, 117, -121), (-6, 8, -2), (0, -64, 64)] if dtype == F16 else
+                                 [(0, 0, 0), (-126, 0, 126), (-120, 0, 120), (-138, 120, 18), (-124, 122, 2), (-100, 100, 0), (120, -90, -30), (125, 0, -125),
+                                  (100, -96, -4), (90, 30, -120)]):
+        cache.k_scale.copy_(k_scale * 2.0**of_k)
+        scaled, scale = (q.double() * 2.0**of_q).to(dtype), 2.0 ** (of_scale - 3)
+        check(run(scaled, cache, table, lengths, scale=scale), *expected(scaled, cache, table, lengths, scale=scale))
