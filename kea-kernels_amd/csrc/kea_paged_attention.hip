@@ -995,6 +995,7 @@ int kea_paged_attention(const kea_heads *q, const kea_heads *out, int dtype, int
     a.by = std::min(std::max(power + (dtype == KEA_F16 ? 27 : 16), -126), 127);
     a.scale = std::ldexp(scale, -a.by);
     a.fill = fill && paging->q_offsets_dev ? 1 : 0;
+    if (a.at.batch == 0 && !a.fill) return KEA_OK;  // (no tiles, and the rows of no sequence stay as they are)
     const hipStream_t s = (hipStream_t)stream;
     return dtype == KEA_F32 ? run<float>(a, p.few, s) : dtype == KEA_F16 ? run<_Float16>(a, p.few, s) : run<__bf16>(a, p.few, s);
 }
