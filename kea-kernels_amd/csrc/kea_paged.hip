@@ -124,10 +124,12 @@ struct ReadArgs {
 
 template <typename T, int L>
 __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
-    const int r = blockIdx.x * (kThreads / L) + threadIdx.x / L, b = blockIdx.y, at = threadIdx.x % L * 16;
-    if (r >= a.length * a.kv_heads || at >= a.d) return;
+    // (a grid has at most 65535 rows: more sequences lie behind each other in z, keys and values in turn)
+    const int r = blockIdx.x * (kThreads / L) + threadIdx.x / L, b = blockIdx.z / 2 * gridDim.y + blockIdx.y, at = threadIdx.x % L * 16;
+    const bool values = blockIdx.z % 2;
+    if (b >= a.at.batch || r >= a.length * a.kv_heads || at >= a.d) return;
     const int i = r / a.kv_heads, h = r - i * a.kv_heads;
-    const kea_pages &from = blockIdx.z ? a.vp : a.kp;
+    const kea_pages &from = values ? a.vp : a.kp;
     const long long p = (a.starts ? (long long)a.starts[b] : 0) + i;
     const int page = p >= 0 && p < a.at.length(b) ? a.at.page(b, (int)p) : -1;
     v4u c = {0, 0, 0, 0};
@@ -137,7 +139,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
         c = *(const v4u *)(from.data_dev + page * from.page_stride + h * from.head_stride + row * from.row_stride + at);
         s = from.scale_dev[page * from.scale_page_stride + h * from.scale_head_stride + row * from.scale_row_stride];
     }
-    T *const to = (T *)(blockIdx.z ? a.v : a.k) + ((long long)b * a.length * a.kv_heads + r) * a.d + at;
+    T *const to = (T *)(values ? a.v : a.k) + ((long long)b * a.length * a.kv_heads + r) * a.d + at;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         float x[8];
@@ -176,9 +178,9 @@ template <typename T>
 int run_read(const ReadArgs &a, hipStream_t stream) {
     const int lanes = a.d <= 64 ? 4 : a.d <= 128 ? 8 : 16;
     const int64_t rows = (int64_t)a.length * a.kv_heads, blocks = (rows + kThreads / lanes - 1) / (kThreads / lanes);
-    if (rows > INT32_MAX - kThreads || !kea::fits_dispatch(blocks, kThreads) || a.at.batch > 65535)
-        return kea::fail(KEA_EINVAL, "kea_paged_read: too large for one launch");
-    const dim3 grid((unsigned)blocks, (unsigned)a.at.batch, 2);
+    if (rows > INT32_MAX - kThreads || !kea::fits_dispatch(blocks, kThreads)) return kea::fail(KEA_EINVAL, "kea_paged_read: too large for one launch");
+    const int64_t layers = (a.at.batch + 65534LL) / 65535;
+    const dim3 grid((unsigned)blocks, (unsigned)((a.at.batch + layers - 1) / layers), (unsigned)(2 * layers));
     if (lanes == 4) read_kernel<T, 4><<<grid, kThreads, 0, stream>>>(a);
     else if (lanes == 8) read_kernel<T, 8><<<grid, kThreads, 0, stream>>>(a);
     else read_kernel<T, 16><<<grid, kThreads, 0, stream>>>(a);
