@@ -27,7 +27,8 @@ extern "C" {
  *   words    w as two's complement nibbles in tiles of 16 rows and 128 k, 1024 bytes each, [ceil(n / 16)][ceil(k / 128)]: 16 bytes
  *            for each lane 16 j + i (i: the row in the tile): byte 8 h + 4 u + b holds in its low nibble k = 64 h + 16 j + 8 u + b
  *            and in its high nibble the k 4 further on. Rows and k behind the matrix are zero. 16-byte aligned.
- *   wscale   [ceil(n / 16)][ceil(k / group)][16], KEA_F32 or KEA_F16, 16-byte aligned; rows behind the matrix are zero.
+ *   wscale   [ceil(n / 16)][ceil(k / group)][16], KEA_F32 or KEA_F16, 16-byte aligned; rows behind the matrix are zero. A sum is held
+ *            as 16 acc: scales up to 2^113 / k in size keep it below FP32's largest number.
  *   group    a power of two, 32 or more.
  *   qs, bias KEA_F32 or KEA_F16 (bias may be NULL), aligned to their element size.
  *   residual NULL or FP32 [m][ldr]; y may be the residual itself (y_dtype KEA_F32, ldy == ldr) and overlaps no other operand.

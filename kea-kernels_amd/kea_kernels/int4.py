@@ -56,8 +56,8 @@ def _groups(k: int, group: int) -> int:
 
 
 def pack(weight: Tensor, scale: Tensor, group: int) -> Weight:
-    """int8 weight [N, K] of values from -8 to 7 and their scales [N, ceil(K / group)] (f32 or f16, finite, up to 2^100 in size), on
-    the tensors' device. Copies; reads the values back once to check them."""
+    """int8 weight [N, K] of values from -8 to 7 and their scales [N, ceil(K / group)] (f32 or f16, finite, up to 2^100 in size, from K =
+    8192 on up to 2^113 / K: no sum passes FP32's range), on the tensors' device. Copies; reads the values back once to check them."""
     if weight.dtype != torch.int8 or weight.dim() != 2 or not 1 <= weight.shape[1] <= MAX_K or weight.shape[0] < 1:
         raise ValueError(f"weight must be int8 [N, K], 1 <= K <= {MAX_K}, got {weight.dtype} {tuple(weight.shape)}")
     n, k = weight.shape
@@ -69,8 +69,10 @@ def pack(weight: Tensor, scale: Tensor, group: int) -> Weight:
         weight, scale = weight.detach(), scale.detach()
         if int(weight.min()) < -8 or int(weight.max()) > 7:
             raise ValueError("weight has values outside -8 .. 7")
-        if not bool((scale.float().abs() <= MOST_SCALE).all()):
-            raise ValueError("scale must be finite values of at most 2^100")
+        # (the kernel holds 16 times a sum of up to 128 * 8 k products and scales)
+        most = min(MOST_SCALE, 2.0**113 / k)
+        if not bool((scale.double().abs() <= most).all()):
+            raise ValueError(f"scale must be finite values of at most {most:.6g}")
         tiles, blocks = -(-n // 16), -(-k // 128)
         full = torch.zeros(16 * tiles, 128 * blocks, dtype=torch.int8, device=weight.device)
         full[:n, :k] = weight
