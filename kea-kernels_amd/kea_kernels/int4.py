@@ -43,7 +43,7 @@ class Weight:
         v = torch.stack((b & 15, b >> 4), 6).to(torch.int8)               # [tile, block, j, i, h, u, nibble, b]
         v = torch.where(v > 7, v - 16, v).permute(0, 3, 1, 4, 2, 5, 6, 7).reshape(16 * tiles, -1)[:n, :k]
         s = self.scales.float().transpose(1, 2).reshape(16 * tiles, -1)[:n]
-        return v.float() * s.repeat_interleave(self.group, 1)[:, :k]
+        return v.float() * s.repeat_interleave(min(self.group, k), 1)[:, :k]  # (a longer group is all of a row)
 
     def nbytes(self) -> int:
         return self.words.numel() * 4 + self.scales.numel() * self.scales.element_size()
@@ -199,9 +199,10 @@ class Int4Linear:
         with torch.no_grad():
             n, k = weight.shape
             groups = _groups(k, group)
-            w = torch.zeros(n, groups * group, device=weight.device)
+            span = min(group, k)  # (a longer group is all of a row)
+            w = torch.zeros(n, groups * span, device=weight.device)
             w[:, :k] = weight.detach()
-            w = w.view(n, groups, group)
+            w = w.view(n, groups, span)
             scale = (w.abs().amax(2) / 7).clamp_min(1e-30)
             q = torch.round(w / scale[:, :, None]).clamp_(-7, 7).to(torch.int8).view(n, -1)[:, :k]
         return cls.prepare(q, scale, bias, group, device)

@@ -37,3 +37,19 @@ def test_the_largest_sums(m, n, k, group):
     p = int4.pack(w, torch.full((n, -(-k // group)), most, device=DEV), group)
     got = int4.gemm(q, torch.full((1, m), 2.0**-100, device=DEV), p)
     assert torch.equal(got, torch.full((m, n), 1024.0 * k * most * 2.0**-100, device=DEV))  # (powers of two: every sum is exact)
+
+
+def test_groups_far_longer_than_a_row_take_no_memory():
+    """A group is any power of two up to 2^30: what a row of 100 does not have is not made."""
+    g = torch.Generator().manual_seed(1)
+    w, s = torch.randint(-8, 8, (40, 100), generator=g, dtype=torch.int8), torch.rand(40, 1, generator=g)
+    assert torch.equal(int4.pack(w, s, 1 << 30).dense(), w.float() * s)
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+def test_layers_of_groups_far_longer_than_a_row():
+    g = torch.Generator().manual_seed(2)
+    w, x = torch.randn(70, 100, generator=g), torch.randn(5, 100, generator=g).to(DEV)
+    long, short = (int4.Int4Linear.from_dense(w, group=group, device=DEV) for group in (1 << 30, 128))
+    assert torch.equal(long.weight.dense(), short.weight.dense()) and torch.equal(long.linear(x), short.linear(x))
