@@ -62,14 +62,16 @@ typedef struct {
 
 /* Writes new tokens' keys and values, [tokens][kv_heads][d] of `dtype` (KEA_F32, KEA_F16, KEA_BF16; batch_stride is not used), to
  * their places: a row x becomes s = max(max|x| / 127, 1e-30) and rint(x / s), as kea_quantize makes one part (s is held to the
- * largest number of which 127 s is finite); a row with an infinity or NaN becomes s = NaN and zeros. Tokens that stand at no position (rows of no sequence, positions below 0, entries that name no
- * page) are left out; nothing else is written. Tokens of one call that stand at the same place are not ordered: what is written
- * there is not defined. d: a multiple of 16 up to 256; k, v and their strides multiples of 16 bytes, not negative. */
+ * largest number of which 127 s is finite); a row with an infinity or NaN becomes s = NaN and zeros. Tokens that stand at no position
+ * (rows of no sequence, positions below 0, entries that name no page) are left out; nothing else is written. Tokens of one call that
+ * stand at the same place are not ordered: what is written there is not defined. d: a multiple of 16 up to 256; k, v and their strides
+ * multiples of 16 bytes, not negative. */
 int kea_paged_write(const kea_heads *k, const kea_heads *v, int dtype, int64_t kv_heads, int64_t d, const kea_pages *k_pages,
                     const kea_pages *v_pages, const kea_paging *paging, void *stream);
 
 /* Reads positions starts_dev[b] + i (starts_dev NULL: i), 0 <= i < length, of every sequence as values: k_dev, v_dev
- * [batch][length][kv_heads][d] of `dtype`, contiguous and 16-byte aligned, data * scale rounded once; zeros for positions
+ * [batch][length][kv_heads][d] of `dtype`, contiguous and 16-byte aligned: data * scale rounded to FP32, and from there to the 16-bit
+ * types (so that a 16-bit result may lie a step of FP32 more than half a step of its type from the product); zeros for positions
  * outside 0 .. len-1 and for entries that name no page. paging->tokens and q_offsets_dev are not used. */
 int kea_paged_read(const kea_pages *k_pages, const kea_pages *v_pages, const kea_paging *paging, const int32_t *starts_dev,
                    int64_t length, int64_t kv_heads, int64_t d, void *k_dev, void *v_dev, int dtype, void *stream);
@@ -79,7 +81,8 @@ int kea_paged_read(const kea_pages *k_pages, const kea_pages *v_pages, const kea
  *   out = sum_j softmax_j(scale * q . k_j) v_j over what it sees, zeros where it sees nothing or p is below 0.
  * Head h reads key head h / (heads / kv_heads). A position that a token does not see has no part in its output, whatever its scales
  * and codes are. Sums, maxima and scores are FP32; the weights exp(s - max) v_scale are rounded to FP16 (to two parts of it, 22
- * bits, with KEA_F32), small ones to multiples of 2^-30 of the row's largest such weight, and the elements of a row of q, with KEA_BF16 and KEA_F32, to 2^-28 of the row's largest (KEA_F32: 22 bits).
+ * bits, with KEA_F32), small ones to multiples of 2^-30 of the row's largest such weight, and the elements of a row of q, with KEA_BF16
+ * and KEA_F32, to 2^-28 of the row's largest (KEA_F32: 22 bits).
  *   dtype        of q and out: KEA_F32, KEA_F16 or KEA_BF16; pointers and strides multiples of 16 bytes, strides not negative
  *                (batch_stride is not used). out overlaps no input, and no two of its rows share memory.
  *   left         >= 0; 2^30 and above: without bound.  scale: finite.  Rows of a page less than 2^26 bytes apart.

@@ -174,8 +174,8 @@ def write(cache: Cache, k: Tensor, v: Tensor, table: Tensor, kv_lengths: Tensor,
 def read(cache: Cache, table: Tensor, kv_lengths: Tensor, length: int, *, starts: Tensor | None = None,
          out_dtype: torch.dtype = torch.float32) -> tuple[Tensor, Tensor]:
     """(k, v), each [B, length, kv_heads, D] of out_dtype (f32, f16, bf16): the values of positions starts[b] + i, 0 <= i < length, of
-    every sequence (starts int32 [B], None: 0), integers times scales rounded once; zeros for positions outside 0 .. kv_lengths[b] - 1
-    and for table entries outside 0 .. pages - 1."""
+    every sequence (starts int32 [B], None: 0), integers times scales in FP32, f16 and bf16 rounded from there; zeros for positions
+    outside 0 .. kv_lengths[b] - 1 and for table entries outside 0 .. pages - 1."""
     if (hit := _native("paged_read", cache, table, kv_lengths, length, starts, out_dtype)) is not None:
         return hit
     if out_dtype not in _hip.DTYPES:
