@@ -102,7 +102,6 @@ __device__ __forceinline__ int swizzle_v(int key) {
 
 using kea::both_halves;
 using kea::copy16;
-using kea::halves;
 using kea::other_half_max;
 
 template <typename T>
