@@ -192,3 +192,48 @@ def test_queries_keys_and_scales_of_every_size(n, length, room, dtype):
         cache.k_scale.copy_(k_scale * 2.0**of_k)
         scaled, scale = (q.double() * 2.0**of_q).to(dtype), 2.0 ** (of_scale - 3)
         check(run(scaled, cache, table, lengths, scale=scale), *expected(scaled, cache, table, lengths, scale=scale))
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,length,room", [(6, 200, None), (33, 97, None), (1000, 1100, 4800)])
+@pytest.mark.parametrize("spread", [1, 24, 200])
+def test_rows_keep_their_bits_beside_keys_that_they_do_not_see(spread, n, length, room, dtype):
+    """The last four keys, which the last tokens see, hold NaN, infinities, the largest, smallest and ordinary scales: nothing changes for
+    the tokens before them, whatever the other keys' scales are."""
+    g = torch.Generator().manual_seed(spread + n)
+    q, cache, table, lengths = one_sequence(n, length, 16, 4, 64, dtype, g, room)
+    top = 6 if dtype == F16 else min(spread / 2, 100)
+    cache.v_scale.copy_(torch.exp2(top - spread * torch.rand(cache.v_scale.shape, generator=g)))
+    clean = run(q, cache, table, lengths)
+    check(clean, *expected(q, cache, table, lengths))
+    for bad in (math.nan, math.inf, 3e38, 2.0**120, 1e-30, 0.0, 1e-45):
+        k_scale, v_scale = cache.k_scale.clone(), cache.v_scale.clone()
+        for p in range(length - 4, length):
+            v_scale[place(table, p)] = bad
+            if not 0 < bad < 1e30:
+                k_scale[place(table, p)] = bad
+        assert torch.equal(run(q, paged.Cache(cache.k, cache.v, k_scale, v_scale), table, lengths)[:-4], clean[:-4]), bad
+
+
+@pytest.mark.gpu
+@torch.inference_mode()
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("seed", range(12))
+def test_mixtures(seed, dtype):
+    """Heads of 16 to 256, value scales of several sizes in runs and alone, scores of several sizes."""
+    g = torch.Generator().manual_seed(100 + seed)
+    pick = lambda *c: c[int(torch.randint(0, len(c), (1,), generator=g))]  # noqa: E731
+    n, length = pick((1, 40), (1, 3000), (7, 700), (40, 333), (1000, 1100))
+    room, d = pick(None, 4800), pick(16, 64, 128, 128, 208, 256)
+    q, cache, table, lengths = one_sequence(n, length, 16, pick(1, 4, 16), d, dtype, g, room)
+    at = place(table, torch.arange(length))
+    low, high = (-16, 6) if dtype == F16 else (-140, 118)
+    run_of = pick(1, 5, 40, 300)
+    power = torch.randint(low, high, (-(-length // run_of), cache.kv_heads), generator=g).repeat_interleave(run_of, 0)[:length]
+    if pick(0, 1):  # (most keys alike)
+        power = torch.where(torch.rand(power.shape, generator=g) < 0.9, -5, power)
+    cache.v_scale[at] = torch.exp2(power.float() + torch.rand(power.shape, generator=g))
+    scale = pick(1.0, 0.125, 8.0)
+    check(run(q, cache, table, lengths, scale=scale), *expected(q, cache, table, lengths, scale=scale))
