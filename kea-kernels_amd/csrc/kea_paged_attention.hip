@@ -8,12 +8,12 @@
 //   w = 2^(s - ref) v_scale, rounded to FP16;   O^T += V^T w^T;   l += 2^(s - top);   out = O 2^(ref - top) / l
 // The queries are FP16 numbers: F16 as they are, BF16 by a power of two of their row (an element below 2^-28 of the row's largest is
 // rounded to a multiple of 2^-28 of it), F32 the same in two parts, 22 bits of each element. The weights of F32 are in two parts too.
-// The reference ref is such that w is at most 2^15: it is raised, and O rescaled, only where a block's largest s + (exponent of that
-// key's v_scale) passes it by more than 5 (base 2), and then stands where the largest w is 2^6 at least. Weights below 2^-14 lose digits of
+// The reference ref is such that w is below 2^15.94: it is raised, and O rescaled, only where a block's largest s + (exponent of that
+// key's v_scale) passes it by more than 5.94 (base 2), and then stands where the largest w is 2^6 at least. Weights below 2^-14 lose digits of
 // FP16: they are 2^-20 and less of the largest. Where the exponents of a block's v_scales are at most 3 apart, the largest s and the
 // largest exponent are taken for it, of whichever keys they are; where they lie further apart, a key of no weight with a large
 // v_scale would push the others' weights out of FP16's range, and each key's own sum is formed.
-// The sum l has a reference of its own, the largest s so far, passed by 5 at most. Both are whole numbers: 2^(ref - top) is exact. One
+// The sum l has a reference of its own, the largest s so far, passed by 5.94 at most. Both are whole numbers: 2^(ref - top) is exact. One
 // exponential serves both, 2^(s - ref), its sum times 2^(ref - top), while that factor is from 2^-100 to 2^60; beyond (values above some
 // 2^70 or below 2^-90, and scores above 2^20) it would pass FP32's range or digits, and each has its own.
 //
@@ -50,8 +50,8 @@ typedef __attribute__((address_space(3))) v2i *ltr8_t;
 typedef __attribute__((address_space(3))) v4s *ltr16_t;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLazy = 5.0f;   // what a block may pass the reference by (base 2) before it is raised
-constexpr int kTop = 10;        // the exponent of the largest weight where the reference has just been raised; kTop + kLazy <= 15
+constexpr float kLazy = 5.9375f;  // what a block may pass the reference by (base 2) before it is raised
+constexpr int kTop = 10;        // the exponent of the largest weight where the reference has just been raised: 2^(kTop + kLazy) < 65504
 constexpr int kWide = 3;        // exponents of a block's value scales that are further apart are taken key by key
 constexpr int kLeast = -149;    // the exponent that a value scale of zero counts as: below that of all others
 constexpr float kNone = -0x1.fffffep127f;       // no reference yet: the lowest number
@@ -352,9 +352,9 @@ __device__ __forceinline__ void store4(T *y, v4f v) {
 // that neither the eight keys at one unit that eight lanes read as scores' operands, nor the eight keys at one unit that a
 // transposing read takes, share banks.
 //
-// One token is bound by memory: 16 streams of up to 16000 BF16 keys of 4 heads of 128 are 176 MB of codes and scales, read in 47 us
-// with the join (3.7 TB/s; a large copy takes 33). For that 2 x 4 waves a CU have two blocks each under way; three or four blocks a
-// wave leave room for one workgroup and take 66. Without a barrier between them the waves drift apart, so that some load while others
+// One token is bound by memory: 16 streams of up to 16000 BF16 keys of 4 heads of 128 are 176 MB of codes and scales, read in 50 us
+// with the join as a graph of calls, 53 from call to call (3.5 and 3.3 TB/s; a large copy takes 33). For that 2 x 4 waves a CU have two
+// blocks each under way; three or four blocks a wave leave room for one workgroup and take a third more (66 where two took 50). Without a barrier between them the waves drift apart, so that some load while others
 // multiply.
 template <int UNITS>
 __device__ __forceinline__ int place(int key) {
@@ -596,8 +596,8 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) token_kernel(Args a) {
 //
 // Instruction issue bounds it: for 32 x 32 scores 16 matrix instructions and some 200 vector ones (the scale, the mask's test, the
 // largest, exponential, sum, v_scale and conversion of 16 scores a lane, and unpacking's share), of which little runs beside them. 2048
-// tokens of 16000, 16 heads of 128 on 4: 329 us, 760 TFLOP/s where a large product of 16-bit floats makes 1220, at 1.8 to 1.9 GHz under
-// this load. With 128 rows the unpacking has a second wave's share (367 us).
+// tokens of 16000, 16 heads of 128 on 4: 344 us, 730 TFLOP/s where a large product of 16-bit floats makes 1220, at 1.8 to 1.9 GHz under
+// this load. With 128 rows the unpacking has a second wave's share (11 % more).
 template <int UNITS>
 __device__ __forceinline__ int place_k(int key) {
     return UNITS == 8 ? key >> 1 & 7 : key & 15;
@@ -864,9 +864,10 @@ int plan_of(int64_t batch, int64_t tokens, int64_t positions, int64_t heads, int
     const int64_t room = positions - each / 2, keys = left < room ? left + 1 : room;
     // Tiles of 32 rows walk their keys without a wait between waves, tiles of 256 unpack the codes for eight times as many rows: they
     // are ahead where there are many rows and long walks. F16, heads of 128, 16 on 4, us (32 rows, 256 rows): 2048 tokens of 16000
-    // 469 and 333, 1000 of 16000 240 and 179, 8 x 512 of 4000 187 and 143, 1000 of 4000 74 and 66, 2048 of 4000 105 and 104, 4000 of
-    // 4000 133 and 125, 2048 of 2048 45 and 67, 1000 of 1000 21 and 36; 512 of 4000 (FP32) 59 and 61. Heads of 129 to 256 are faster in 32
-    // rows throughout (1000 of 4000 142 and 160: the outputs of a row alone take half of a wave's registers).
+    // 502 and 346, 1000 of 16000 253 and 187, 8 x 512 of 4000 247 and 205, 1000 of 4000 67 and 66, 2048 of 4000 105 and 106, 4000 of
+    // 4000 139 and 130, 2048 of 2048 47 and 68, 1000 of 1000 19 and 36; 512 of 4000 (FP32) 63 and 61. (A table with room for more keys
+    // than its sequences hold counts as they would: a prompt of 2048 in a table of 16000 takes 256 rows.) Heads of 129 to 256 are faster
+    // in 32 rows throughout (a tenth: the outputs of a row alone take half of a wave's registers).
     p.few = d > 128 || tokens * heads < 16000 || keys < 3000;
     const int64_t per = p.few ? 32 : d <= 64 ? Tiles<64>::ROWS : Tiles<128>::ROWS;
     p.tiles_each = (each * group + per - 1) / per;
@@ -876,8 +877,8 @@ int plan_of(int64_t batch, int64_t tokens, int64_t positions, int64_t heads, int
     p.splits = 1;
     if (wgs > 0 && p.few) {
         // Two workgroups on every CU where each part has 700 keys and more, one otherwise; 128 keys at least. BF16, one token of 16 streams
-        // of 16000 keys (64 workgroups): 189, 104, 60, 48 and 53 us in 1, 2, 4, 8 and 16 parts; 64 tokens of 4000 (32) 51, 32, 22, 18 and 22;
-        // 8 x 64 of 1000 (256) 19 and 26 in 1 and 2.
+        // of 16000 keys (64 workgroups): 182, 102, 61, 56 and 59 us in 1, 2, 4, 8 and 16 parts; 64 tokens of 4000 (32) 52, 34, 25, 21 and 25;
+        // 8 x 64 of 1000 (256) 22 and 30 in 1 and 2.
         const int64_t span = keys + per / group;
         int64_t s = wgs < 512 ? 512 / wgs : 1;
         if (span / s < 700) s = wgs < 256 ? 256 / wgs : 1;
@@ -886,7 +887,7 @@ int plan_of(int64_t batch, int64_t tokens, int64_t positions, int64_t heads, int
         p.splits = s < 1 ? 1 : s < 64 ? s : 64;
     } else if (wgs > 0) {
         // One workgroup on every CU, or two rounds of them, whose parts even out what causality leaves to the tiles: 4000 of 4000 (256
-        // workgroups) 161 us in one, 125 in two, 144 in four parts; 2048 of 16000 (128) 333 in two, 422 in three.
+        // workgroups) 170 us in one, 135 in two, 151 in four parts; 2048 of 16000 (128) 347 in two, 436 in three.
         const int64_t s = wgs <= 128 ? 256 / wgs : wgs < 384 ? 2 : 1;
         p.splits = s < 16 ? s : 16;
     }
