@@ -71,7 +71,7 @@ int kea_paged_write(const kea_heads *k, const kea_heads *v, int dtype, int64_t k
 
 /* Reads positions starts_dev[b] + i (starts_dev NULL: i), 0 <= i < length, of every sequence as values: k_dev, v_dev
  * [batch][length][kv_heads][d] of `dtype`, contiguous and 16-byte aligned: data * scale rounded to FP32, and from there to the 16-bit
- * types (so that a 16-bit result may lie a step of FP32 more than half a step of its type from the product); zeros for positions
+ * types (a 16-bit result may lie half a step of FP32 more than half a step of its type from the product); zeros for positions
  * outside 0 .. len-1 and for entries that name no page. paging->tokens and q_offsets_dev are not used. */
 int kea_paged_read(const kea_pages *k_pages, const kea_pages *v_pages, const kea_paging *paging, const int32_t *starts_dev,
                    int64_t length, int64_t kv_heads, int64_t d, void *k_dev, void *v_dev, int dtype, void *stream);
