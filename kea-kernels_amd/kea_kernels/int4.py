@@ -166,7 +166,8 @@ def gemm(q: Tensor, qs: Tensor, weight: Weight, bias: Tensor | None = None, *, o
 
 class Int4Linear:
     """One layer with 4-bit weights and a scale for each group of a row's weights, resident on the GPU, with an FP32 bias. A call
-    makes one int8 part of its input's rows (lowbit.quantize, with the LayerNorm and SiLU that it fuses) and runs gemm."""
+    makes one int8 part of its input's rows (lowbit.quantize, with the LayerNorm and SiLU that it fuses) and runs gemm. Rows are f32 or
+    f16 and up to 8192 wide, as lowbit.quantize takes them; norms.block_norm makes int8 rows of bf16 and wider ones, which gemm takes."""
 
     def __init__(self, weight: Weight, bias: Tensor | None):
         self.weight, self.bias = weight, bias

@@ -39,8 +39,9 @@ def _distinct(name: str, t: Tensor, other: Tensor | None = None) -> None:
 class Cache:
     """Keys and values as int8 `k`, `v` [pages, kv_heads, page_size, D] with FP32 scales `k_scale`, `v_scale` [pages, kv_heads,
     page_size]: element e of a row stands for k[..., e] * k_scale[...]. page_size is a power of two from 16 to 1024, D a multiple of 16
-    up to 256; rows of D are contiguous and start at multiples of 16 bytes, the other dimensions may have any order in memory. The
-    tensors are the caller's (no copies are made); pages need no initial values."""
+    up to 256; rows of D are contiguous and start at multiples of 16 bytes, the other dimensions may have any order in memory. Keys and
+    values may lie between each other, the codes' memory and the scales' may not. The tensors are the caller's (no copies are made);
+    pages need no initial values."""
 
     def __init__(self, k: Tensor, v: Tensor, k_scale: Tensor, v_scale: Tensor):
         if k.dim() != 4 or k.dtype != torch.int8 or k.shape != v.shape or v.dtype != torch.int8:
@@ -151,9 +152,9 @@ def write(cache: Cache, k: Tensor, v: Tensor, table: Tensor, kv_lengths: Tensor,
     goes to row p % page_size of page table[b, p // page_size]. len is held to 0 .. table.shape[1] * page_size.
 
     A row x of D elements becomes s = max(max|x| / 127, 1e-30), held to the largest number of which 127 s is finite, and rint(x / s);
-    one that holds an infinity or NaN becomes s = NaN and zeros, and reads as NaN. Rows of no sequence, positions below 0 and table entries outside 0 .. pages - 1 are left out, and
-    no other byte of the cache is written. No two tokens of a call may stand at the same place (what is there then is not
-    defined)."""
+    one that holds an infinity or NaN becomes s = NaN and zeros, and reads as NaN. Rows of no sequence, positions below 0 and table
+    entries outside 0 .. pages - 1 are left out, and no other byte of the cache is written. No two tokens of a call may stand at the same
+    place (what is there then is not defined)."""
     if (_native("paged_write", cache, k, v, table, kv_lengths, q_offsets)) is not None:
         return
     heads = cache.kv_heads
